@@ -99,18 +99,19 @@ def torch_ops_tag() -> str:
 
 
 def build_torch_ops(force: bool = False) -> Path:
-    """csrc/kernels/torch_ops.cpp -> lib/_b200torch.so: the differentiable layers, linked against torch
+    """csrc/kernels/torch_*.cpp -> lib/_b200torch.so: the differentiable layers, linked against torch
     and against libb200ops.so next to it. Built for one torch and one Python, which the stamp beside it names."""
-    src, out = CSRC / "kernels" / "torch_ops.cpp", LIB / "_b200torch.so"
+    srcs, out = sorted((CSRC / "kernels").glob("torch_*.cpp")), LIB / "_b200torch.so"
+    hdrs = [CSRC / "kernels" / "b200ops.h", CSRC / "kernels" / "torch_layer.h"]
     stamp, tag = LIB / "_b200torch.stamp", torch_ops_tag()
-    if force or _stale(out, [src, src.parent / "b200ops.h"]) or not stamp.exists() or stamp.read_text() != tag:
+    if force or _stale(out, srcs + hdrs) or not stamp.exists() or stamp.read_text() != tag:
         import torch
 
         root = Path(torch.__file__).resolve().parent
         _run([CXX, "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-DTORCH_EXTENSION_NAME=_b200torch",
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(root / "include"),
               "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-I", sysconfig.get_paths()["include"],
-              "-I", f"{CUDA_HOME}/include", str(src), "-o", str(out), "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10",
+              "-I", f"{CUDA_HOME}/include", *map(str, srcs), "-o", str(out), "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10",
               "-lc10_cuda", "-ltorch_python", "-L", str(LIB), "-lb200ops", "-Wl,-rpath,$ORIGIN"])
         stamp.write_text(tag)
     return out

@@ -34,4 +34,30 @@ int b200_gemm_swiglu_bwd_launches(const void* dy, const void* w, int M, int F, i
 int b200_rope_qkv(void* qkv, long long pitch, void* q, void* k, void* v, const long long* strides, const float* cs,
                   const float* sn, long long T, int nq, int nkv, int hd, int seq, int backward, void* stream);
 
+// RMSNorm with its output in 8 bits; see norm_fp8.cu.
+int b200_rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldres, void* h_out, const void* w, void* q, float* scale, long long T,
+                     int H, float eps, int group, void* stream);
+
+// Tokens sorted by expert and back; see moe_sort.cu.
+int b200_expert_order(const void* idx, int idx64, long long n, int experts, int* row_of, int* offsets, void* stream);
+int b200_permute_rows(const void* x, long long pitch, void* rows, const int* row_of, const float* scale, float* row_scale, int groups, long long tokens,
+                      int k, long long row_bytes, int elem, void* stream);
+int b200_unpermute_rows(const void* rows, long long pitch, const float* w, const int* row_of, void* out, long long tokens, int k, int H, int fp32,
+                        void* stream);
+int b200_unpermute_rows_bwd(const void* dout, const void* rows, long long pitch, const float* w, const int* row_of, void* drows, float* dw,
+                            long long tokens, int k, int H, int fp32, void* stream);
+
+// One tensor of an AdamW step: p and g are bf16 unless the flags say otherwise; m and v are e4m3 codes with a scale for every 256 elements, or fp32;
+// master is null, or an fp32 copy of a bf16 p. keep = 1 - lr * weight_decay.
+struct B200AdamwTensor {
+  void *p, *g, *m, *v;
+  float *m_scale, *v_scale, *master;
+  long long n;
+  float keep;
+  unsigned char p_fp32, g_fp32;
+};
+// *launches (unless null): kernels launched; see adamw_many.cu.
+int b200_adamw_many(const B200AdamwTensor* list, int count, int bits, double lr, double beta1, double beta2, double eps, long long step, double grad_scale,
+                    int zero_grad, int* launches, void* stream);
+
 }  // extern "C"

@@ -8,61 +8,18 @@
 // Weight gradients follow the convention of the Python side: a parameter that carries `main_grad` (a
 // view of the flat gradient buffer) has its gradient written there, `grad_written` is set, and the
 // parameter's `grad_ready` hook is called; other parameters receive an ordinary gradient.
-#include <torch/extension.h>
-
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/library.h>
-
-#include <atomic>
 #include <climits>
 
-#include "b200ops.h"
+#include "torch_layer.h"
+
+namespace b200torch {
+std::atomic<int64_t> g_launches{0};
+PyObject* g_error = nullptr;
+}  // namespace b200torch
 
 namespace {
 
-namespace py = pybind11;
-using torch::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Function;
-using torch::autograd::variable_list;
-
-std::atomic<int64_t> g_launches{0};
-PyObject* g_error = nullptr;   // the package's B200OpsError (a RuntimeError), looked up when the module is loaded
-
-// Raises a Python exception with or without the interpreter lock: with it as error_already_set, without (in a
-// layer's body, forward or on an autograd thread) in torch's own carrier.
-[[noreturn]] void raise(PyObject* type, const std::string& what) {
-  if (PyGILState_Check()) {
-    PyErr_SetString(type, what.c_str());
-    throw py::error_already_set();
-  }
-  py::gil_scoped_acquire gil;
-  PyErr_SetString(type, what.c_str());
-  python_error err;
-  err.persist();
-  throw err;
-}
-void require(bool ok, const char* what) {
-  if (!ok) raise(PyExc_AssertionError, what);
-}
-// Rows of `width` elements; an empty row is the error that the division is in Python, not a signal.
-int64_t rows_of(const Tensor& t, int64_t width) {
-  if (width == 0) raise(PyExc_ZeroDivisionError, "the last dimension holds no element of a row");
-  return t.numel() / width;
-}
-void check(int rc, const char* what) {
-  if (rc != 0) raise(g_error, std::string(what) + " failed with code " + std::to_string(rc));
-}
-bool bf16_cuda(const Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kBFloat16; }
-// An incoming gradient as the kernels read it: contiguous and on a 16-byte boundary, whatever view it is.
-Tensor rows16(const Tensor& g) {
-  const Tensor c = g.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
-}
-void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+using namespace b200torch;
 
 // C[M,N] (+)= op(A) op(B); the checks of ops.gemm.gemm
 void gemm(const Tensor& a, const Tensor& b, bool a_mn, bool b_mn, const Tensor& out, bool accumulate) {
@@ -150,20 +107,6 @@ Tensor write_param_grad(const Tensor& weight, Produce produce) {
   const py::object ready = attribute(w, kReady);
   if (ready && !ready.is_none()) ready(w);
   return {};
-}
-
-// pybind's exception cannot cross the autograd engine's threads; torch's carrier can.
-template <class F>
-auto on_engine_thread(F f) {
-  try {
-    return f();
-  } catch (py::error_already_set& e) {
-    py::gil_scoped_acquire gil;
-    e.restore();
-    python_error err;
-    err.persist();
-    throw err;
-  }
 }
 
 // y = x W^T
@@ -479,14 +422,6 @@ variable_list rope_qkv(const Tensor& qkv, const Tensor& cos, const Tensor& sin, 
   return RopeQKV::apply(qkv, cos, sin, B, S, nq, nkv, hd);
 }
 
-// The call itself, or under torch.jit.trace the operator of the same name: the tracer records operators,
-// and of the bodies above it would see nothing but the allocation of their outputs.
-template <class R, class... A, class... Args>
-R traced_or_direct(const char* name, R (*fn)(A...), const Args&... args) {
-  if (!torch::jit::tracer::isTracing()) return fn(args...);
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<R(A...)>().call(args...);
-}
-
 }  // namespace
 
 TORCH_LIBRARY(b200ops, m) {
@@ -522,5 +457,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           return traced_or_direct("b200ops::rope_qkv", rope_qkv, qkv, cos, sin, B, S, nq, nkv, hd);
         }));
   m.def("cross_entropy", torch::wrap_pybind_function_no_gil(cross_entropy));
+  bind_moe(m);
   m.def("launches", [] { return g_launches.load(std::memory_order_relaxed); });
 }

@@ -1,30 +1,42 @@
-"""Expert-parallel mixture-of-experts layer: softmax top-k router, device-initiated dispatch of the
+"""Mixture-of-experts layer: softmax top-k router, device-initiated dispatch of the
 token rows to the ranks that own their experts (optionally as block-scaled fp8), SwiGLU experts
-on the tcgen05 GEMM, gate-weighted combine back to token order."""
+on the tcgen05 GEMM, gate-weighted combine back to token order.  Without a communicator all experts
+are on one GPU: rows are sorted by expert and summed back without a window, any number of tokens at a time."""
 from __future__ import annotations
 
 import torch
 
 from ..ops.gemm import linear
 from ..ops.llm import swiglu
+from ..ops.moe import expert_order, permute_tokens, unpermute_tokens
 from ..parallel.expert_parallel import ExpertParallel
 from ..parallel.symm import Communicator
 
 
 class MoELayer(torch.nn.Module):
-    def __init__(self, comm: Communicator, tokens: int, hidden: int, ffn: int, experts: int, topk: int, *,
-                 fp8_dispatch: bool = False, capacity_factor: float = 2.0, window_offset: int = 0, seed: int = 0):
+    def __init__(self, comm: Communicator | None, tokens: int, hidden: int, ffn: int, experts: int, topk: int, *,
+                 fp8_dispatch: bool = False, capacity_factor: float = 2.0, window_offset: int = 0, seed: int = 0,
+                 device: torch.device | str | None = None):
+        """comm None: all experts on ``device`` (default: the current GPU); ``tokens`` and the window's arguments then mean nothing."""
         super().__init__()
-        self.ep = ExpertParallel(comm, tokens, hidden, experts, topk, capacity_factor=capacity_factor,
-                                 window_offset=window_offset)
+        if comm is None:
+            if fp8_dispatch:
+                raise ValueError("fp8_dispatch is for rows that travel between ranks: it needs a communicator")
+            self.ep, world, rank = None, 1, 0
+            dev = torch.device(device if device is not None else "cuda")
+        else:
+            if device is not None and torch.device(device) != torch.device(comm.device):
+                raise ValueError("the communicator has the layer's device")
+            self.ep = ExpertParallel(comm, tokens, hidden, experts, topk, capacity_factor=capacity_factor,
+                                     window_offset=window_offset)
+            world, rank, dev = comm.world, comm.rank, comm.device
         self.hidden, self.ffn, self.experts, self.topk, self.fp8 = hidden, ffn, experts, topk, fp8_dispatch
-        el = experts // comm.world
+        el = experts // world
         g = torch.Generator(device="cpu").manual_seed(seed)
         router = torch.randn(experts, hidden, generator=g) * hidden ** -0.5
         w_gu = torch.randn(experts, 2 * ffn, hidden, generator=g) * hidden ** -0.5
         w_dn = torch.randn(experts, hidden, ffn, generator=g) * ffn ** -0.5
-        lo = comm.rank * el
-        dev = comm.device
+        lo = rank * el
         self.router = torch.nn.Parameter(router.to(dev))   # fp32, replicated
         self.w_gate_up = torch.nn.ParameterList(
             [torch.nn.Parameter(w_gu[lo + e].to(dev, torch.bfloat16)) for e in range(el)])
@@ -39,10 +51,14 @@ class MoELayer(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         idx, w = self.route(x)
-        rows = self.ep.dispatch(x, idx, w, self.fp8)
+        if self.ep is None:
+            order = expert_order(idx, self.experts)
+            rows, offsets = permute_tokens(x, order), order.offsets
+        else:
+            rows, offsets = self.ep.dispatch(x, idx, w, self.fp8), self.ep.expert_offsets
         # The per-expert row ranges live on the device; slicing the rows for the per-expert GEMM
         # calls needs them on the host.
-        off = self.ep.expert_offsets.tolist()
+        off = offsets.tolist()
         outs = []
         for e in range(len(self.w_gate_up)):
             if off[e + 1] > off[e]:
@@ -52,4 +68,4 @@ class MoELayer(torch.nn.Module):
             y = torch.cat(outs, dim=0)
         else:
             y = rows[:0]
-        return self.ep.combine(y, w)
+        return self.ep.combine(y, w) if self.ep is not None else unpermute_tokens(y, order, w)

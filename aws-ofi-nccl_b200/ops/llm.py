@@ -13,6 +13,17 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: 
     return out[0], (out[1] if residual is not None else x)
 
 
+def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: torch.Tensor | None = None,
+                group: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``rmsnorm`` with its output in 8 bits: (q, scale, h) with normed ~= q * scale, q e4m3 of x's shape and h as
+    ``rmsnorm`` returns it.  ``group`` 0: one fp32 scale per row, of x's shape without the last dimension, as ``gemm_fp8``
+    takes them; 128: one per 128 columns, as the expert exchange moves its rows.  The norm is rounded once, where
+    ``quantize_rows_fp8(rmsnorm(x))`` rounds it to bf16 first.  Rows may be strided (last dim contiguous); they hold a
+    multiple of 8 elements, at most 16384.  A row that holds a NaN or an infinity has a NaN as its scale.  There is no gradient: inputs that
+    require one are refused unless gradients are off."""
+    return tuple(_lib.native().rmsnorm_fp8(x, residual, weight, eps, group))
+
+
 def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up for a fused [..., 2F] tensor laid out as gate | up."""
     return _lib.native().swiglu(gate_up)
@@ -122,6 +133,46 @@ def adamw_step(p: torch.Tensor, g: torch.Tensor, m: torch.Tensor, v: torch.Tenso
                                 master.data_ptr() if master is not None else None, n, lr, beta1, beta2, eps,
                                 weight_decay, step, grad_scale, int(zero_grad), _lib.stream_ptr())
     _lib.check(rc, "b200_adamw")
+
+
+ADAMW_BLOCK = 256   # elements of a tensor that share a scale of its 8-bit moments
+
+
+def adamw_states(params, *, bits: int = 32, master: bool = False) -> dict:
+    """The state of ``adamw_step_many`` before its first step, by the names of its arguments: zero moments, in 8 bits the scales
+    too, and with ``master`` fp32 copies of the bf16 parameters."""
+    if bits not in (8, 32):
+        raise ValueError(f"moments are held in 8 or 32 bits, not {bits}")
+    params = list(params)
+
+    def zeros():
+        if bits == 32:
+            return [torch.zeros_like(p, dtype=torch.float32, requires_grad=False, memory_format=torch.contiguous_format) for p in params]
+        return [torch.zeros(p.shape, device=p.device, dtype=torch.uint8).view(torch.float8_e4m3fn) for p in params]
+
+    def scales():
+        if bits == 32:
+            return None
+        return [torch.zeros(-(-p.numel() // ADAMW_BLOCK), device=p.device, dtype=torch.float32) for p in params]
+
+    copies = [p.detach().float() if p.dtype == torch.bfloat16 else None for p in params] if master else None
+    return dict(m=zeros(), v=zeros(), m_scale=scales(), v_scale=scales(), master=copies)
+
+
+def adamw_step_many(params, grads, m, v, m_scale=None, v_scale=None, master=None, *, lr: float, beta1: float, beta2: float,
+                    eps: float, weight_decay, step: int, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
+    """One AdamW update of many tensors at once, in place: the step of ``adamw_step`` for parameters that share no flat buffer.
+
+    Parameters and gradients are lists of contiguous bf16 or fp32 tensors; a gradient that is None leaves its parameter and
+    its state as they are.  ``m`` and ``v`` are lists of fp32 tensors, or of e4m3 ones: then every 256 elements of a tensor
+    share an fp32 scale in ``m_scale`` and ``v_scale``, m is code * scale and v the square of that (its root is what is held).  8-bit
+    moments are rounded by a dither of element and step, so that small changes move them in the mean; what is not finite is held as NaN, and
+    a root that is not zero as no less than the least code. ``master`` holds fp32 copies (or None) of bf16 parameters: they are updated, the parameters
+    are their roundings.  ``weight_decay`` is a number, or a list of one per parameter.  ``step`` counts from one and is a host
+    number like the others: a captured call repeats the step that it was captured with."""
+    params = list(params)
+    decay = [float(d) for d in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * len(params)
+    _lib.native().adamw_step_many(params, grads, m, v, m_scale, v_scale, master, decay, lr, beta1, beta2, eps, step, grad_scale, zero_grad)
 
 
 def sumsq(x: torch.Tensor) -> torch.Tensor:

@@ -14,8 +14,8 @@
 //   d = element * 0xC13FA9A9 + step * 0x91E10DA5 mod 2^32     up where fraction + (d >> 12) / 2^20 >= 1 for m, with ~d for the root
 // Scaled by 2^-120 a float has its exponent and upper mantissa where e4m3 has them, denormals included, so the code is the top of a sum of integers.
 //
-// The update takes the moments of 32 bits, before they are rounded. Each operation on what is held is rounded by itself (no fused multiply-adds, a root
-// and a quotient of IEEE's), so that codes do not depend on how the compiler contracts: a neighbouring code is 12 % away.
+// The update takes the moments of 32 bits, before they are rounded. Each operation on what is held is rounded by itself (no fused multiply-adds, IEEE's
+// root and reciprocal), so that a step's codes do not depend on how a compiler contracts: a neighbouring code is 12 % away.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -23,28 +23,35 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "b200ops.h"
 #include "dependent_launch.cuh"
 #include "host_util.h"
 
 namespace b200 {
 
-constexpr int ADAMW_THREADS = 256;
-constexpr int ADAMW_BLOCK = 256;                                        // elements of a warp's pass, eight of a lane
-constexpr int ADAMW_PASS = ADAMW_THREADS / 32 * ADAMW_BLOCK;            // of a CTA's
+constexpr int ADAMW_BLOCK = 256;   // elements of a warp's pass, eight of a lane
+// With 8-bit moments it is instructions that memory waits for, 380 of a warp for a block, and their latencies: small CTAs, which end and start one by one,
+// and registers for sixteen of them on an SM. Medians of 218 M bf16 parameters, of 101 M with a master copy: 384 and 272 us; in CTAs of 128 threads 440
+// and 298, with 14 CTAs (72 registers) 403 and 281, with blocks copied ahead into shared memory 449 and 346, with nothing ahead 415 and 285.
+constexpr int adamw_threads(int bits) { return bits == 8 ? 64 : 256; }
+constexpr int adamw_ctas(int bits) { return bits == 8 ? 16 : 3; }        // of an SM at least
+constexpr int adamw_pass(int bits) { return adamw_threads(bits) * 8; }   // elements of a CTA's pass
 constexpr uint32_t DITHER_ELEMENT = 0xC13FA9A9u, DITHER_STEP = 0x91E10DA5u;
-
-enum : uint32_t { ADAMW_P32 = 1, ADAMW_G32 = 2, ADAMW_VECTORS = 4 };
 
 struct AdamwEntry {
   B200AdamwTensor t;
-  uint32_t first;   // the tensor's first CTA
-  uint32_t flags;
+  uint32_t first;          // the tensor's first CTA
+  uint32_t places;         // how a lane's elements lie (Places)
 };
+// The step's numbers, those of the float units twice: an instruction that works on two elements takes both.
 struct AdamwNumbers {
-  float beta1, rest1, beta2, rest2, lr1, root2, eps, grad_scale;   // rest: 1 - beta; lr1 = lr / (1 - b1^t); root2 = 1 / sqrt(1 - b2^t)
+  float2 beta1, rest1, minus_beta2, minus_rest2, minus_lr1, minus_root2, eps, grad_scale;   // rest: 1 - beta; lr1 = lr / (1 - b1^t); root2 = 1 / sqrt(1 - b2^t)
+  float2 one;    // products are added as multiples of it: a product and an addition the assembler makes a fused multiply-add of, whatever their roundings are called
   uint32_t dither;
   int zero_grad;
+  int careful;   // eps is so small that roots of denormal numbers count beside it
 };
 // A launch's parameters are 32764 bytes at most.
 template <int N>
@@ -52,187 +59,435 @@ struct AdamwTable {
   AdamwEntry e[N];
   AdamwNumbers a;
   int count;
-  int chunk;        // elements of a CTA, a multiple of ADAMW_PASS
+  int chunk;        // elements of a CTA, a multiple of its pass
 };
 constexpr int ADAMW_MOST = 400;
 static_assert(sizeof(AdamwTable<ADAMW_MOST>) <= 32764, "parameters of a launch");
 
-// Eight elements from i on, or as many as are left of n, zeros behind them.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int64_t i, int64_t n, bool vectors, float (&f)[8]) {
-  if (vectors && i + 8 <= n) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p + i);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+// A lane's eight elements of a block of 256:
+//  ALIGNED  eight in a row, where all that the step reads and writes of a tensor lies on 16-byte boundaries (8 for codes); they move as vectors.
+//  STRIDED  every 32nd, whatever the tensors start at: a warp's access is one piece of memory. 40 M bf16 parameters and 8-bit moments in buffers
+//           without padding take 125 us so, 70 aligned; 184 with eight in a row read one by one, 164 with vectors between a block's two ends.
+//  LAST     the same in a tensor's last block, with zeros beyond its end.
+enum Places { ALIGNED, STRIDED, LAST };
+template <Places HOW>
+struct Lane {
+  uint32_t first, n;      // its first element, from the chunk's beginning, and the chunk's elements
+  __device__ __forceinline__ Lane(uint32_t block, uint32_t n_) {
+    const uint32_t lane = threadIdx.x & 31;
+    n = n_;
+    first = HOW == ALIGNED ? block + 8 * lane : block + lane;
+  }
+  // element j: how far behind the first
+  __device__ __forceinline__ uint32_t step(int j) const { return HOW == ALIGNED ? j : 32 * j; }
+  __device__ __forceinline__ bool has(int j) const { return HOW != LAST || first + 32 * j < n; }
+  __device__ __forceinline__ bool row() const { return HOW == ALIGNED; }
+};
+
+template <typename T>
+struct Raw8 {   // eight elements as they come from memory
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void to(float (&f)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(q);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[2 * j] = __low2float(h[j]), f[2 * j + 1] = __high2float(h[j]);
+      for (int j = 0; j < 4; ++j) f[2 * j] = __low2float(h[j]), f[2 * j + 1] = __high2float(h[j]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 w = q[h % (sizeof(T) / 2)];
+        f[4 * h] = __uint_as_float(w.x), f[4 * h + 1] = __uint_as_float(w.y), f[4 * h + 2] = __uint_as_float(w.z), f[4 * h + 3] = __uint_as_float(w.w);
+      }
+    }
+  }
+  __device__ __forceinline__ void from(const float (&f)[8]) {
+    if constexpr (sizeof(T) == 2) {
+      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        q[h % (sizeof(T) / 2)] = make_uint4(__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]), __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3]));
+    }
+  }
+};
+template <>
+struct Raw8<uint8_t> {
+  uint2 q;
+};
+
+template <typename T, Places HOW>
+__device__ __forceinline__ void load(Raw8<T>& raw, const T* p, const Lane<HOW>& l) {
+  using Element = std::conditional_t<sizeof(T) == 4, uint32_t, std::conditional_t<sizeof(T) == 2, uint16_t, uint8_t>>;
+  using Vector = std::conditional_t<sizeof(T) == 1, uint2, uint4>;
+  if (l.row()) {
+#pragma unroll
+    for (int h = 0; h < static_cast<int>(sizeof(raw) / sizeof(Vector)); ++h) reinterpret_cast<Vector*>(&raw)[h] = reinterpret_cast<const Vector*>(p + l.first)[h];
   } else {
+    const Element* const from = reinterpret_cast<const Element*>(p + l.first);
+    uint32_t* const words = reinterpret_cast<uint32_t*>(&raw);
+    constexpr int PER = 4 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = i + j < n ? __bfloat162float(p[i + j]) : 0.f;
+    for (int w = 0; w < 8 / PER; ++w) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = w * PER; j < (w + 1) * PER; ++j)
+        if (l.has(j)) bits |= static_cast<uint32_t>(from[l.step(j)]) << (8 * sizeof(T) * (j % PER) % 32);
+      words[w] = bits;
+    }
   }
 }
-__device__ __forceinline__ void load8(const float* p, int64_t i, int64_t n, bool vectors, float (&f)[8]) {
-  if (vectors && i + 8 <= n) {
-    const float4 a = reinterpret_cast<const float4*>(p + i)[0], b = reinterpret_cast<const float4*>(p + i)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
+template <typename T, Places HOW>
+__device__ __forceinline__ void store(const Raw8<T>& raw, T* p, const Lane<HOW>& l) {
+  using Element = std::conditional_t<sizeof(T) == 4, uint32_t, std::conditional_t<sizeof(T) == 2, uint16_t, uint8_t>>;
+  using Vector = std::conditional_t<sizeof(T) == 1, uint2, uint4>;
+  if (l.row()) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = i + j < n ? p[i + j] : 0.f;
-  }
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int64_t i, int64_t n, bool vectors, const float (&f)[8]) {
-  if (vectors && i + 8 <= n) {
-    uint4 q;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-    *reinterpret_cast<uint4*>(p + i) = q;
+    for (int h = 0; h < static_cast<int>(sizeof(raw) / sizeof(Vector)); ++h) reinterpret_cast<Vector*>(p + l.first)[h] = reinterpret_cast<const Vector*>(&raw)[h];
   } else {
+    Element* const to = reinterpret_cast<Element*>(p + l.first);
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(&raw);
+    constexpr int PER = 4 / sizeof(T);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (i + j < n) p[i + j] = __float2bfloat16_rn(f[j]);
+      if (l.has(j)) to[l.step(j)] = static_cast<Element>(words[j / PER] >> (8 * sizeof(T) * (j % PER) % 32));
   }
 }
-__device__ __forceinline__ void store8(float* p, int64_t i, int64_t n, bool vectors, const float (&f)[8]) {
-  if (vectors && i + 8 <= n) {
-    reinterpret_cast<float4*>(p + i)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p + i)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j < n) p[i + j] = f[j];
-  }
+template <typename T, Places HOW>
+__device__ __forceinline__ void store8(const float (&f)[8], T* p, const Lane<HOW>& l) {
+  Raw8<T> raw;
+  raw.from(f);
+  store(raw, p, l);
 }
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int64_t i, int64_t n, bool vectors) {
-  if (vectors && i + 8 <= n) return *reinterpret_cast<const uint2*>(p + i);
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (i + j < n) w[j / 4] |= static_cast<uint32_t>(p[i + j]) << (8 * (j % 4));
-  return make_uint2(w[0], w[1]);
+
+// Two floats in a register pair: an instruction of the float units works on both, each rounded as by itself.
+struct Pair {
+  unsigned long long bits;
+  Pair() = default;
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void to(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+};
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int64_t i, int64_t n, bool vectors, const uint32_t (&code)[8]) {
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) w[h] = code[4 * h] | code[4 * h + 1] << 8 | code[4 * h + 2] << 16 | code[4 * h + 3] << 24;
-  if (vectors && i + 8 <= n) {
-    *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j < n) p[i + j] = static_cast<uint8_t>(code[j]);
-  }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
 }
-__device__ __forceinline__ void decode8(uint2 q, float scale, float (&f)[8]) {
+__device__ __forceinline__ Pair both(float a) { return Pair(a, a); }
+__device__ __forceinline__ Pair both(float2 a) { return Pair(a.x, a.y); }
+
+__device__ __forceinline__ void decode8(uint2 q, float scale, Pair (&f)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t w = j < 2 ? q.x : q.y;
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * (j & 1))), __NV_E4M3);
     const float2 v = __half22float2(__half2(h));
-    f[2 * j] = __fmul_rn(v.x, scale);
-    f[2 * j + 1] = __fmul_rn(v.y, scale);
+    f[j] = Pair(v.x, v.y) * both(scale);
   }
+}
+
+__device__ __forceinline__ float reciprocal_root(float v) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
+  return y;
+}
+__device__ __forceinline__ float reciprocal(float v) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
+  return y;
+}
+// 1 / v for 2^-110 < v < 2^120, rounded as IEEE's: one Newton step from the unit's reciprocal (as roots8; of all mantissas none differs)
+__device__ __forceinline__ float inverse(float v) {
+  const float y = reciprocal(v);
+  return fmaf(fmaf(-v, y, 1.f), y, y);
 }
 
 constexpr uint32_t E4M3_MOST = 0x7E, E4M3_NAN = 0x7F, INF_BITS = 0x7f800000u;
 
-// Magnitudes' bits -> the scale of a warp's block and the codes. What is not finite is held as NaN and counts for no scale.
-__device__ __forceinline__ float hold8(const float (&f)[8], const uint32_t (&dither)[8], uint32_t (&code)[8]) {
-  uint32_t most = 0;
+__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
+
+// The largest of three magnitudes, a NaN if there is one
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+// The largest magnitude of a warp's block, as bits; `finite` whether all are numbers, which it counts alone.
+__device__ __forceinline__ uint32_t block_most(const float (&f)[8], bool& finite) {
+  float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
-  most = __reduce_max_sync(0xffffffffu, most);
-  const bool finite = most < INF_BITS;   // the same in every lane
+  for (int j = 0; j < 8; j += 2) top = largest(top, f[j], f[j + 1]);
+  uint32_t most = __reduce_max_sync(0xffffffffu, magnitude(top));   // a NaN's bits are above all others'
+  finite = most < INF_BITS;   // the same in every lane
   if (!finite) {
     most = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
-      most = max(most, b < INF_BITS ? b : 0u);
-    }
+    for (int j = 0; j < 8; ++j) most = max(most, magnitude(f[j]) < INF_BITS ? magnitude(f[j]) : 0u);
     most = __reduce_max_sync(0xffffffffu, most);
   }
-  const float scale = __fmul_rn(fmaxf(__uint_as_float(most), 1e-30f), 1.f / 448.f);
-  const float inv = __fdiv_rn(1.f, scale);
+  return most;
+}
+
+// Four words with a code in bits 20 to 27 each -> the four codes, the first lowest
+__device__ __forceinline__ uint32_t pack_codes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t even = __byte_perm(a, c, 0x7632), odd = __byte_perm(b, d, 0x7632);   // upper halves
+  return (even >> 4 & 0x00ff00ffu) | (odd << 4 & 0xff00ff00u);
+}
+
+// Values -> their block's scale and codes; `dither` is 20 bits for each. ROOTS: they are all negative or zero, held without the sign, and what is not
+// zero is not held as zero.
+template <bool ROOTS>
+__device__ __forceinline__ uint2 hold8(const float (&f)[8], const uint32_t (&dither)[8], uint32_t most, bool finite, float& scale) {
+  scale = __fmul_rn(fmaxf(__uint_as_float(most), 1e-30f), 1.f / 448.f);
+  const float inv = inverse(scale);
+  Pair share[4];
+  auto shares = [&](float by) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float share = __fmul_rn(__fmul_rn(fabsf(f[j]), inv), 0x1p-120f);
-    code[j] = min((__float_as_uint(share) + dither[j]) >> 20, E4M3_MOST);
+    for (int j = 0; j < 4; ++j)
+      share[j] = ROOTS ? fma2(Pair(f[2 * j], f[2 * j + 1]), both(-by), both(0.f)) :   // of zeros of either sign the positive one
+                  Pair(__fmul_rn(fabsf(f[2 * j]), by), __fmul_rn(fabsf(f[2 * j + 1]), by));
+  };
+  if (scale < 32.f) {
+    shares(inv * 0x1p-120f);
+  } else {   // a factor that is denormal itself would not be exact
+    shares(inv);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) share[j] = share[j] * both(0x1p-120f);
+  }
+  uint32_t word[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float s[2];
+    share[j / 2].to(s[0], s[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      word[j + h] = min(__float_as_uint(s[h]) + (ROOTS ? 0xfffffu - dither[j + h] : dither[j + h]), E4M3_MOST << 20 | 0xfffffu);
   }
   if (!finite) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if ((__float_as_uint(f[j]) & 0x7fffffffu) >= INF_BITS) code[j] = E4M3_NAN;
+      if (magnitude(f[j]) >= INF_BITS) word[j] = E4M3_NAN << 20;
   }
-  return scale;
+  uint2 q = make_uint2(pack_codes(word[0], word[1], word[2], word[3]), pack_codes(word[4], word[5], word[6], word[7]));
+  if constexpr (ROOTS) {
+    auto zeros = [](uint32_t w) { return (w - 0x01010101u) & ~w & 0x80808080u; };   // whether one of four bytes is
+    if (zeros(q.x) | zeros(q.y)) {
+      uint32_t least[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) least[j] = word[j] >> 20 == 0 && f[j] < 0.f ? 1u << 20 : 0u;
+      q.x |= pack_codes(least[0], least[1], least[2], least[3]);
+      q.y |= pack_codes(least[4], least[5], least[6], least[7]);
+    }
+  } else {
+    auto signs = [&](int j) {   // the top bytes of four values
+      const uint32_t lo = __byte_perm(__float_as_uint(f[j]), __float_as_uint(f[j + 1]), 0x0073);
+      const uint32_t hi = __byte_perm(__float_as_uint(f[j + 2]), __float_as_uint(f[j + 3]), 0x0073);
+      return __byte_perm(lo, hi, 0x5410) & 0x80808080u;
+    };
+    q.x |= signs(0);
+    q.y |= signs(4);
+  }
+  return q;
+}
+
+// The negative roots of pairs of numbers, given as -v: one Newton step from the unit's reciprocal root y, v y + (v - (v y)^2) y / 2, whose residual a fused
+// multiply-add has exactly (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), with the sign of v
+// so that nothing has to be negated. What is left of y's error is its square, 2^-44 of the root: of all floats from 2^-100 on none differs from IEEE's
+// root, of those from 2^-126 on none by more than an ulp.
+__device__ __forceinline__ Pair minus_roots(Pair minus_v) {
+  float a, b;   // 2^-126 is nothing to what is above 2^-100, and zero gets a reciprocal root that is finite
+  fma2(minus_v, both(1.f), both(-0x1p-126f)).to(a, b);
+  const Pair y(reciprocal_root(fabsf(a)), reciprocal_root(fabsf(b))), g = minus_v * y;
+  return fma2(fma2(g, g, minus_v), y * both(0.5f), g);
+}
+// The same for any number: small ones are scaled by 2^100.
+__device__ __forceinline__ Pair any_minus_roots(Pair minus_v, Pair plain) {
+  float a, b, lo, hi, x, y;
+  minus_v.to(a, b);
+  plain.to(x, y);
+  (minus_roots(minus_v * both(0x1p100f)) * both(0x1p-50f)).to(lo, hi);
+  x = a == -INFINITY ? -INFINITY : a > -0x1p-100f ? lo : x;
+  y = b == -INFINITY ? -INFINITY : b > -0x1p-100f ? hi : y;
+  return Pair(x, y);
+}
+
+// The moments of a lane's eight elements behind the step, v with its sign turned.
+__device__ __forceinline__ void moments8(const float (&gr)[8], Pair (&m)[4], Pair (&v)[4], const AdamwNumbers& a) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const Pair d = Pair(gr[2 * j], gr[2 * j + 1]) * both(a.grad_scale);
+    m[j] = fma2(m[j] * both(a.beta1), both(a.one), d * both(a.rest1));
+    v[j] = fma2(v[j] * both(a.minus_beta2), both(a.one), d * d * both(a.minus_rest2));
+  }
+}
+__device__ __forceinline__ void update8(float (&x)[8], const Pair (&m)[4], const Pair (&minus_root)[4], const AdamwNumbers& a, float keep) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float lo, hi;
+    fma2(minus_root[j], both(a.minus_root2), both(a.eps)).to(lo, hi);
+    const Pair update = m[j] * both(a.minus_lr1) * Pair(reciprocal(lo), reciprocal(hi));
+    fma2(Pair(x[2 * j], x[2 * j + 1]), both(keep), update).to(x[2 * j], x[2 * j + 1]);
+  }
+}
+
+constexpr uint32_t CAREFUL_BELOW = 0x2b800000u;   // 2^-40: beside larger roots those of denormal numbers have the least code whatever their last bits
+
+// What a CTA has of a tensor: pointers to its first element, so that places are numbers of 32 bits. X: what the step reads the parameter from.
+template <int BITS, typename P, typename G, bool MASTER>
+struct Chunk {
+  using X = std::conditional_t<MASTER, float, P>;
+  using M = std::conditional_t<BITS == 8, uint8_t, float>;
+  P* p;
+  G* g;
+  X* x;
+  M *m, *v;
+  float *m_scale, *v_scale;
+  uint32_t n;        // elements
+  uint32_t dither;   // of the first
+  float keep;
+  __device__ __forceinline__ Chunk(const B200AdamwTensor& t, const AdamwNumbers& a, int64_t begin, int64_t end) {
+    p = static_cast<P*>(t.p) + begin;
+    g = static_cast<G*>(t.g) + begin;
+    x = MASTER ? reinterpret_cast<X*>(t.master) + begin : reinterpret_cast<X*>(p);
+    m = static_cast<M*>(t.m) + begin;
+    v = static_cast<M*>(t.v) + begin;
+    if constexpr (BITS == 8) {
+      m_scale = t.m_scale + begin / ADAMW_BLOCK;
+      v_scale = t.v_scale + begin / ADAMW_BLOCK;
+    }
+    n = static_cast<uint32_t>(end - begin);
+    dither = static_cast<uint32_t>(begin) * DITHER_ELEMENT + a.dither;
+    keep = t.keep;
+  }
+};
+
+// A lane's part of a block as it is in memory
+template <typename C>
+struct Held {
+  Raw8<typename std::remove_pointer_t<decltype(C::g)>> g;
+  Raw8<typename C::X> x;
+  Raw8<typename C::M> m, v;
+  float m_scale, v_scale;
+  template <Places HOW>
+  __device__ __forceinline__ void load_from(const C& c, const Lane<HOW>& l, uint32_t block) {
+    load(g, c.g, l);
+    load(x, c.x, l);
+    load(m, c.m, l);
+    load(v, c.v, l);
+    if constexpr (sizeof(typename C::M) == 1) {
+      m_scale = c.m_scale[block];
+      v_scale = c.v_scale[block];
+    }
+  }
+};
+
+template <Places HOW, int BITS, typename P, typename G, bool MASTER, typename Next>
+__device__ __forceinline__ void step8(const Chunk<BITS, P, G, MASTER>& c, const AdamwNumbers& a, const Lane<HOW>& l, uint32_t block,
+                                      const Held<Chunk<BITS, P, G, MASTER>>& held, Next&& next) {
+  float gr[8], x[8];
+  Pair m[4], v[4], root[4];
+  float mf[8], rf[8];
+  held.g.to(gr);
+  held.x.to(x);
+  if constexpr (BITS == 8) {
+    decode8(held.m.q, held.m_scale, m);
+    decode8(held.v.q, held.v_scale, v);
+  } else {
+    held.m.to(mf);
+    held.v.to(rf);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = Pair(mf[2 * j], mf[2 * j + 1]), v[j] = Pair(rf[2 * j], rf[2 * j + 1]);
+  }
+  next();   // what was held is in registers of its own now: the next block's loads
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = v[j] * v[j];
+  }
+  moments8(gr, m, v, a);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    root[j] = minus_roots(v[j]);
+    if constexpr (BITS == 32) root[j] = any_minus_roots(v[j], root[j]);
+    root[j].to(rf[2 * j], rf[2 * j + 1]);
+    m[j].to(mf[2 * j], mf[2 * j + 1]);
+  }
+  if constexpr (BITS == 8) {
+    bool v_finite, m_finite;
+    uint32_t v_most = block_most(rf, v_finite);
+    if (a.careful || !v_finite || (v_most < CAREFUL_BELOW && v_most > 0)) {   // the same for the warp
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        root[j] = any_minus_roots(v[j], root[j]);
+        root[j].to(rf[2 * j], rf[2 * j + 1]);
+      }
+      v_most = block_most(rf, v_finite);
+    }
+    update8(x, m, root, a, c.keep);
+    const uint32_t m_most = block_most(mf, m_finite), d0 = l.first * DITHER_ELEMENT + c.dither;
+    uint32_t dither[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dither[j] = (d0 + l.step(j) * DITHER_ELEMENT) >> 12;
+    float ms, vs;
+    Raw8<uint8_t> code;
+    code.q = hold8<false>(mf, dither, m_most, m_finite, ms);
+    store(code, c.m, l);
+    code.q = hold8<true>(rf, dither, v_most, v_finite, vs);
+    store(code, c.v, l);
+    if ((threadIdx.x & 31) == 0) {
+      c.m_scale[block] = ms;
+      c.v_scale[block] = vs;
+    }
+  } else {
+    update8(x, m, root, a, c.keep);
+    store8(mf, c.m, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) (v[j] * both(-1.f)).to(rf[2 * j], rf[2 * j + 1]);
+    store8(rf, c.v, l);
+  }
+  if constexpr (MASTER) store8(x, c.x, l);
+  store8(x, c.p, l);
+  if (a.zero_grad) {
+    const float zero[8] = {};
+    store8(zero, c.g, l);
+  }
 }
 
 template <int BITS, typename P, typename G, bool MASTER>
-__device__ __forceinline__ void adamw_chunk(const B200AdamwTensor& t, const AdamwNumbers& a, bool vectors, int64_t begin, int64_t end) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  P* const p = static_cast<P*>(t.p);
-  G* const g = static_cast<G*>(t.g);
-  const int64_t n = t.n;
-  const float keep = t.keep;
-  for (int64_t b = begin + warp * ADAMW_BLOCK; b < end; b += ADAMW_PASS) {
-    const int64_t i = b + lane * 8, block = b / ADAMW_BLOCK;
-    float x[8], gr[8], m[8], v[8], root[8];
-    load8(g, i, n, vectors, gr);
-    if constexpr (MASTER)
-      load8(t.master, i, n, vectors, x);
-    else
-      load8(p, i, n, vectors, x);
-    if constexpr (BITS == 8) {
-      const uint2 mc = load_codes(static_cast<const uint8_t*>(t.m), i, n, vectors), vc = load_codes(static_cast<const uint8_t*>(t.v), i, n, vectors);
-      const float ms = t.m_scale[block], vs = t.v_scale[block];
-      decode8(mc, ms, m);
-      decode8(vc, vs, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], v[j]);
-    } else {
-      load8(static_cast<const float*>(t.m), i, n, vectors, m);
-      load8(static_cast<const float*>(t.v), i, n, vectors, v);
+__device__ __forceinline__ void adamw_chunk(const AdamwEntry& e, const AdamwNumbers& a, int64_t begin, int64_t end) {
+  const Chunk<BITS, P, G, MASTER> c(e.t, a, begin, end);
+  Held<Chunk<BITS, P, G, MASTER>> held;
+  constexpr uint32_t PASS = adamw_pass(BITS);
+  uint32_t b = (threadIdx.x >> 5) * ADAMW_BLOCK;
+  // Whole blocks: with moments in 8 bits each is loaded while the one before it is worked on, which takes as long.
+  auto whole = [&](auto how) {
+    constexpr Places HOW = decltype(how)::value;
+    if (BITS == 8 && b + ADAMW_BLOCK <= c.n) held.load_from(c, Lane<HOW>(b, c.n), b / ADAMW_BLOCK);
+    for (; b + ADAMW_BLOCK <= c.n; b += PASS) {
+      const Lane<HOW> l(b, c.n);
+      if (BITS == 32) held.load_from(c, l, b / ADAMW_BLOCK);
+      step8(c, a, l, b / ADAMW_BLOCK, held, [&] {
+        if (BITS == 8 && b + PASS + ADAMW_BLOCK <= c.n) held.load_from(c, Lane<HOW>(b + PASS, c.n), (b + PASS) / ADAMW_BLOCK);
+      });
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = __fmul_rn(gr[j], a.grad_scale);
-      m[j] = __fadd_rn(__fmul_rn(m[j], a.beta1), __fmul_rn(d, a.rest1));
-      v[j] = __fadd_rn(__fmul_rn(v[j], a.beta2), __fmul_rn(__fmul_rn(d, d), a.rest2));
-      root[j] = __fsqrt_rn(v[j]);
-      x[j] = fmaf(x[j], keep, -__fdividef(m[j] * a.lr1, fmaf(root[j], a.root2, a.eps)));
-    }
-    if constexpr (BITS == 8) {
-      uint32_t dither[8], code[8];
-      const uint32_t d0 = static_cast<uint32_t>(i) * DITHER_ELEMENT + a.dither;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dither[j] = (d0 + j * DITHER_ELEMENT) >> 12;
-      const float ms = hold8(m, dither, code);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) code[j] |= __float_as_uint(m[j]) >> 24 & 0x80u;
-      store_codes(static_cast<uint8_t*>(t.m), i, n, vectors, code);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dither[j] = ~(d0 + j * DITHER_ELEMENT) >> 12;
-      const float vs = hold8(root, dither, code);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) code[j] = max(code[j], root[j] > 0.f ? 1u : 0u);
-      store_codes(static_cast<uint8_t*>(t.v), i, n, vectors, code);
-      if (lane == 0) {
-        t.m_scale[block] = ms;
-        t.v_scale[block] = vs;
-      }
-    } else {
-      store8(static_cast<float*>(t.m), i, n, vectors, m);
-      store8(static_cast<float*>(t.v), i, n, vectors, v);
-    }
-    if constexpr (MASTER) store8(t.master, i, n, vectors, x);
-    store8(p, i, n, vectors, x);
-    if (a.zero_grad) {
-      const float zero[8] = {};
-      store8(g, i, n, vectors, zero);
-    }
+  };
+  if (e.places == ALIGNED)
+    whole(std::integral_constant<Places, ALIGNED>{});
+  else
+    whole(std::integral_constant<Places, STRIDED>{});
+  for (; b < c.n; b += PASS) {
+    const Lane<LAST> l(b, c.n);
+    held.load_from(c, l, b / ADAMW_BLOCK);
+    step8(c, a, l, b / ADAMW_BLOCK, held, [] {});
   }
 }
 
 template <int BITS, int N>
-__global__ void __launch_bounds__(ADAMW_THREADS) adamw_many_kernel(const __grid_constant__ AdamwTable<N> table) {
+__global__ void __launch_bounds__(adamw_threads(BITS), adamw_ctas(BITS)) adamw_many_kernel(const __grid_constant__ AdamwTable<N> table) {
   int lo = 0, hi = table.count - 1;   // the last entry whose first CTA is not behind this one
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -244,34 +499,34 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_many_kernel(const __grid_
   const AdamwEntry& e = table.e[lo];
   const int64_t begin = static_cast<int64_t>(blockIdx.x - e.first) * table.chunk;
   const int64_t end = begin + table.chunk < e.t.n ? begin + table.chunk : e.t.n;
-  const bool vectors = e.flags & ADAMW_VECTORS;
   grid_wait();
   grid_release();
   using bf16 = __nv_bfloat16;
-  if (e.flags & ADAMW_P32) {
-    if (e.flags & ADAMW_G32)
-      adamw_chunk<BITS, float, float, false>(e.t, table.a, vectors, begin, end);
+  if (e.t.p_fp32) {
+    if (e.t.g_fp32)
+      adamw_chunk<BITS, float, float, false>(e, table.a, begin, end);
     else
-      adamw_chunk<BITS, float, bf16, false>(e.t, table.a, vectors, begin, end);
+      adamw_chunk<BITS, float, bf16, false>(e, table.a, begin, end);
   } else if (e.t.master) {
-    if (e.flags & ADAMW_G32)
-      adamw_chunk<BITS, bf16, float, true>(e.t, table.a, vectors, begin, end);
+    if (e.t.g_fp32)
+      adamw_chunk<BITS, bf16, float, true>(e, table.a, begin, end);
     else
-      adamw_chunk<BITS, bf16, bf16, true>(e.t, table.a, vectors, begin, end);
+      adamw_chunk<BITS, bf16, bf16, true>(e, table.a, begin, end);
   } else {
-    if (e.flags & ADAMW_G32)
-      adamw_chunk<BITS, bf16, float, false>(e.t, table.a, vectors, begin, end);
+    if (e.t.g_fp32)
+      adamw_chunk<BITS, bf16, float, false>(e, table.a, begin, end);
     else
-      adamw_chunk<BITS, bf16, bf16, false>(e.t, table.a, vectors, begin, end);
+      adamw_chunk<BITS, bf16, bf16, false>(e, table.a, begin, end);
   }
 }
 
 static bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// Elements of a CTA: as few as fill the chip, up to four passes of it.
-static int adamw_chunk_elements(int64_t total) {
-  const int64_t per_sm = total / (static_cast<int64_t>(sm_count()) * 8 * ADAMW_PASS);
-  return ADAMW_PASS * static_cast<int>(per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+// Elements of a CTA: as few as fill the chip, up to some passes of it.
+static int adamw_chunk_elements(int64_t total, int bits) {
+  const int most = bits == 8 ? 8 : 4;
+  const int64_t passes = total / (static_cast<int64_t>(sm_count()) * 2048 * 8);
+  return adamw_pass(bits) * static_cast<int>(passes < 1 ? 1 : passes > most ? most : passes);
 }
 
 template <int N>
@@ -283,15 +538,14 @@ static int launch_adamw(const B200AdamwTensor* list, int count, int bits, const 
     e.t = list[i];
     e.first = static_cast<uint32_t>(ctas);
     const int state = bits == 8 ? 8 : 16;
-    const bool vectors = on(e.t.p, 16) && on(e.t.g, 16) && on(e.t.master, 16) && on(e.t.m, state) && on(e.t.v, state);
-    e.flags = (e.t.p_fp32 ? ADAMW_P32 : 0) | (e.t.g_fp32 ? ADAMW_G32 : 0) | (vectors ? ADAMW_VECTORS : 0);
+    e.places = on(e.t.p, 16) && on(e.t.g, 16) && on(e.t.master, 16) && on(e.t.m, state) && on(e.t.v, state) ? ALIGNED : STRIDED;
     ctas += (e.t.n + chunk - 1) / chunk;
   }
   if (ctas > INT_MAX) return B200_ERR_TOO_LARGE;
   table.a = a;
   table.count = count;
   table.chunk = chunk;
-  launch_dependent(bits == 8 ? adamw_many_kernel<8, N> : adamw_many_kernel<32, N>, static_cast<int>(ctas), ADAMW_THREADS, 0, stream, table);
+  launch_dependent(bits == 8 ? adamw_many_kernel<8, N> : adamw_many_kernel<32, N>, static_cast<int>(ctas), adamw_threads(bits), 0, stream, table);
   B200_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -316,18 +570,21 @@ int b200_adamw_many(const B200AdamwTensor* list, int count, int bits, double lr,
     total += t.n;
   }
   const double c1 = 1.0 - pow(beta1, static_cast<double>(step)), c2 = 1.0 - pow(beta2, static_cast<double>(step));
+  auto twice = [](double v) { return make_float2(static_cast<float>(v), static_cast<float>(v)); };
   AdamwNumbers a{};
-  a.beta1 = static_cast<float>(beta1);
-  a.rest1 = static_cast<float>(1.0 - beta1);
-  a.beta2 = static_cast<float>(beta2);
-  a.rest2 = static_cast<float>(1.0 - beta2);
-  a.lr1 = static_cast<float>(lr / c1);
-  a.root2 = static_cast<float>(1.0 / sqrt(c2));
-  a.eps = static_cast<float>(eps);
-  a.grad_scale = static_cast<float>(grad_scale);
+  a.one = twice(1.0);
+  a.beta1 = twice(beta1);
+  a.rest1 = twice(1.0 - beta1);
+  a.minus_beta2 = twice(-beta2);
+  a.minus_rest2 = twice(beta2 - 1.0);
+  a.minus_lr1 = twice(-lr / c1);
+  a.minus_root2 = twice(-1.0 / sqrt(c2));
+  a.eps = twice(eps);
+  a.grad_scale = twice(grad_scale);
+  a.careful = eps < 1e-12;
   a.dither = static_cast<uint32_t>(step) * DITHER_STEP;
   a.zero_grad = zero_grad;
-  const int chunk = adamw_chunk_elements(total);
+  const int chunk = adamw_chunk_elements(total, bits);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   for (int at = 0; at < count; at += ADAMW_MOST) {
     const int some = count - at < ADAMW_MOST ? count - at : ADAMW_MOST;

@@ -177,29 +177,60 @@ Tensor unpermute_tokens(const Tensor& rows, const Tensor& row_of, const c10::opt
 
 // ------------------------------------------------------------------ AdamW over many tensors
 using Range = std::pair<uintptr_t, uintptr_t>;
-// Whether no two of the written ranges share a byte. Lists of tensors mostly lie in order, which needs no sorting.
-bool apart(std::vector<Range>& r) {
-  if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
-  for (size_t i = 1; i < r.size(); ++i)
-    if (r[i].first < r[i - 1].second) return false;
+// Whether no two of the written ranges share a byte. A list of tensors mostly lies in order, so lists are sorted by themselves, if at all, and merged.
+bool apart(std::initializer_list<std::vector<Range>*> lists) {
+  std::vector<Range> all;
+  for (std::vector<Range>* r : lists) {
+    if (!std::is_sorted(r->begin(), r->end())) std::sort(r->begin(), r->end());
+    const size_t before = all.size();
+    all.insert(all.end(), r->begin(), r->end());
+    if (before && !r->empty() && all[before] < all[before - 1]) std::inplace_merge(all.begin(), all.begin() + before, all.end());
+  }
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].first < all[i - 1].second) return false;
   return true;
 }
 
-void adamw_step_many(const std::vector<Tensor>& params, const std::vector<c10::optional<Tensor>>& grads, const std::vector<Tensor>& m,
-                     const std::vector<Tensor>& v, const c10::optional<std::vector<Tensor>>& m_scale, const c10::optional<std::vector<Tensor>>& v_scale,
-                     const c10::optional<std::vector<c10::optional<Tensor>>>& master, const std::vector<double>& decay, double lr, double beta1,
-                     double beta2, double eps, int64_t step, double grad_scale, bool zero_grad) {
+// A sequence of tensors, read as they lie in a tuple, which keeps them: converted to a vector they take 50 ns each, and a step has up to seven for
+// every parameter. Needs the interpreter lock.
+class Tensors {
+ public:
+  Tensors(const py::object& sequence, const char* what, bool may_lack) {
+    if (sequence.is_none()) return;
+    items_ = py::reinterpret_steal<py::object>(PySequence_Tuple(sequence.ptr()));
+    if (!items_) throw py::error_already_set();
+    for (size_t i = 0; i < size(); ++i) {
+      PyObject* const item = PyTuple_GET_ITEM(items_.ptr(), i);
+      if (!(may_lack && item == Py_None) && !THPVariable_Check(item)) raise(PyExc_TypeError, what);
+    }
+  }
+  explicit operator bool() const { return static_cast<bool>(items_); }
+  size_t size() const { return items_ ? PyTuple_GET_SIZE(items_.ptr()) : 0; }
+  bool has(size_t i) const { return PyTuple_GET_ITEM(items_.ptr(), i) != Py_None; }
+  const Tensor& operator[](size_t i) const { return THPVariable_Unpack(PyTuple_GET_ITEM(items_.ptr(), i)); }
+
+ private:
+  py::object items_;
+};
+
+void adamw_step_many(const py::object& param_list, const py::object& grad_list, const py::object& m_list, const py::object& v_list,
+                     const py::object& m_scale_list, const py::object& v_scale_list, const py::object& master_list, const std::vector<double>& decay,
+                     double lr, double beta1, double beta2, double eps, int64_t step, double grad_scale, bool zero_grad) {
+  const Tensors params(param_list, "parameters are tensors", false), grads(grad_list, "gradients are tensors or None", true);
+  const Tensors m(m_list, "moments are tensors", false), v(v_list, "moments are tensors", false);
+  const Tensors m_scale(m_scale_list, "scales are tensors", false), v_scale(v_scale_list, "scales are tensors", false);
+  const Tensors master(master_list, "master copies are tensors or None", true);
   const size_t count = params.size();
-  require(grads.size() == count && m.size() == count && v.size() == count && (!master || master->size() == count),
+  require(grads.size() == count && m.size() == count && v.size() == count && (!master || master.size() == count),
           "gradients, moments and master copies are as many as the parameters");
   require(decay.size() == count, "the weight decay is a number, or one for every parameter");
   require(step >= 1, "steps count from one");
   require(lr >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0, "lr and eps are not negative, the betas lie in [0, 1)");
   if (count == 0) return;
   const bool eight = m[0].scalar_type() == at::kFloat8_e4m3fn;
-  require(eight == (m_scale.has_value() && v_scale.has_value()) && eight == (m_scale.has_value() || v_scale.has_value()),
+  require(eight == static_cast<bool>(m_scale) && eight == static_cast<bool>(v_scale),
           "scales of both moments go with 8-bit moments, and only with those");
-  require(!eight || (m_scale->size() == count && v_scale->size() == count), "scales are as many as the parameters");
+  require(!eight || (m_scale.size() == count && v_scale.size() == count), "scales are as many as the parameters");
   const auto state = eight ? at::kFloat8_e4m3fn : at::kFloat;
   const c10::Device device = params[0].device();
   require(device.is_cuda(), "parameters are CUDA tensors");
@@ -207,16 +238,16 @@ void adamw_step_many(const std::vector<Tensor>& params, const std::vector<c10::o
     return t.scalar_type() == type && t.device() == device && t.numel() == n && t.is_contiguous();
   };
   std::vector<B200AdamwTensor> list;
-  std::vector<Range> written, states;
+  std::vector<Range> of_p, of_g, of_m, of_v, of_ms, of_vs, of_master;   // what is written
   std::vector<const Tensor*> changed;
   list.reserve(count);
-  written.reserve(2 * count);
-  states.reserve(5 * count);
+  changed.reserve(4 * count);
   auto write = [&](std::vector<Range>& to, const Tensor& t) -> void* {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    void* const data = t.data_ptr();
+    const uintptr_t at = reinterpret_cast<uintptr_t>(data);
     to.emplace_back(at, at + t.nbytes());
     changed.push_back(&t);
-    return t.data_ptr();
+    return data;
   };
   for (size_t i = 0; i < count; ++i) {
     const Tensor& p = params[i];
@@ -224,37 +255,38 @@ void adamw_step_many(const std::vector<Tensor>& params, const std::vector<c10::o
     require(of_32_or_bf16(p) && p.device() == device && p.is_contiguous(), "parameters are contiguous bfloat16 or float32 tensors of one device");
     require(fits(m[i], state, n) && fits(v[i], state, n), "moments are contiguous, of their parameter's size and all float32 or all float8_e4m3fn");
     if (eight)
-      require(fits((*m_scale)[i], at::kFloat, (n + 255) / 256) && fits((*v_scale)[i], at::kFloat, (n + 255) / 256),
+      require(fits(m_scale[i], at::kFloat, (n + 255) / 256) && fits(v_scale[i], at::kFloat, (n + 255) / 256),
               "scales are contiguous float32 tensors of one number for every 256 elements");
-    const Tensor* copy = master && (*master)[i] ? &*(*master)[i] : nullptr;
+    const Tensor* copy = master && master.has(i) ? &master[i] : nullptr;
     require(!copy || (p.scalar_type() == at::kBFloat16 && fits(*copy, at::kFloat, n)), "a master copy is a contiguous float32 tensor beside a bfloat16 parameter");
-    if (!grads[i]) continue;   // took no part in this step
-    const Tensor& g = *grads[i];
+    if (!grads.has(i)) continue;   // took no part in this step
+    const Tensor& g = grads[i];
     require(of_32_or_bf16(g) && fits(g, g.scalar_type(), n), "gradients are contiguous bfloat16 or float32 tensors of their parameter's size");
     if (n == 0) continue;
     B200AdamwTensor t{};
-    t.p = write(written, p);
-    t.g = zero_grad ? write(written, g) : g.data_ptr();
-    t.m = write(states, m[i]);
-    t.v = write(states, v[i]);
+    t.p = write(of_p, p);
+    t.g = zero_grad ? write(of_g, g) : g.data_ptr();
+    t.m = write(of_m, m[i]);
+    t.v = write(of_v, v[i]);
     if (eight) {
-      t.m_scale = static_cast<float*>(write(states, (*m_scale)[i]));
-      t.v_scale = static_cast<float*>(write(states, (*v_scale)[i]));
+      t.m_scale = static_cast<float*>(write(of_ms, m_scale[i]));
+      t.v_scale = static_cast<float*>(write(of_vs, v_scale[i]));
     }
-    if (copy) t.master = static_cast<float*>(write(states, *copy));
+    if (copy) t.master = static_cast<float*>(write(of_master, *copy));
     t.n = n;
     t.keep = static_cast<float>(1.0 - lr * decay[i]);
     t.p_fp32 = p.scalar_type() == at::kFloat;
     t.g_fp32 = g.scalar_type() == at::kFloat;
     list.push_back(t);
   }
-  written.insert(written.end(), states.begin(), states.end());
-  require(apart(written), "parameters, moments, scales, master copies and gradients that are zeroed share no memory: is a parameter in the list twice?");
+  require(apart({&of_p, &of_g, &of_m, &of_v, &of_ms, &of_vs, &of_master}), "parameters, moments, scales, master copies and gradients that are zeroed share no memory: is a parameter in the list twice?");
   if (list.empty()) return;
   const CUDAGuard guard(device);
-  int launches = 0;
-  const int rc = b200_adamw_many(list.data(), static_cast<int>(list.size()), eight ? 8 : 32, lr, beta1, beta2, eps, step, grad_scale, zero_grad, &launches,
-                                 stream());
+  int launches = 0, rc;
+  {
+    py::gil_scoped_release other_threads_run;   // while the launch waits for room in the queue
+    rc = b200_adamw_many(list.data(), static_cast<int>(list.size()), eight ? 8 : 32, lr, beta1, beta2, eps, step, grad_scale, zero_grad, &launches, stream());
+  }
   launched(launches);
   for (const Tensor* t : changed)
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();   // a graph that kept the old values is told
@@ -283,5 +315,5 @@ void b200torch::bind_moe(py::module_& m) {
   m.def("unpermute_tokens", torch::wrap_pybind_function_no_gil([](const Tensor& rows, const Tensor& row_of, const c10::optional<Tensor>& w) {
           return traced_or_direct("b200ops::unpermute_tokens", unpermute_tokens, rows, row_of, w);
         }));
-  m.def("adamw_step_many", torch::wrap_pybind_function_no_gil(adamw_step_many));
+  m.def("adamw_step_many", torch::wrap_pybind_function(adamw_step_many));
 }

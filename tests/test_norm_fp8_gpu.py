@@ -34,7 +34,8 @@ def _check(x, w, res, group, eps=1e-5):
 
 # every layout of a row, full, ragged and of one vector; one row, a CTA's rows and one more
 @pytest.mark.parametrize("T,H", [(1, 8), (9, 256), (7, 264), (8, 512), (17, 520), (5, 1024), (6, 1032), (300, 2048), (3, 2056), (299, 4096), (4, 4104),
-                                 (301, 8192), (2, 8200), (3, 16384), (1, 4096)])
+                                 (301, 8192), (2, 8200), (3, 16384), (1, 4096), (11, 768), (5, 776), (9, 1536), (6, 1544), (3, 5120), (4, 5128),
+                                 (5, 6144), (2, 6152), (4, 7168), (3, 7176)])
 @pytest.mark.parametrize("with_res", [False, True])
 def test_row_scales(T, H, with_res):
     g = torch.Generator(device="cuda").manual_seed(T + H)
@@ -42,7 +43,7 @@ def test_row_scales(T, H, with_res):
     _check(x, (1 + 0.3 * torch.randn(H, device="cuda", generator=g)).bfloat16(), r if with_res else None, 0)
 
 
-@pytest.mark.parametrize("T,H", [(1, 128), (9, 256), (7, 384), (17, 640), (300, 2048), (33, 7168), (5, 8192), (3, 16384), (11, 1152)])
+@pytest.mark.parametrize("T,H", [(1, 128), (9, 256), (7, 384), (17, 640), (300, 2048), (33, 7168), (5, 8192), (3, 16384), (11, 1152), (5, 768), (3, 896), (5, 1536), (4, 1664), (3, 5120), (2, 5248), (3, 6144), (4, 6272), (2, 7296)])
 @pytest.mark.parametrize("with_res", [False, True])
 def test_group_scales(T, H, with_res):
     g = torch.Generator(device="cuda").manual_seed(T + H)

@@ -294,6 +294,60 @@ def test_captured_forward_and_backward_pass():
 
 
 @pytest.mark.gpu
+def test_more_than_two_to_the_31st_elements():
+    """Rows, norms and parameters whose last elements lie beyond numbers of 32 bits: the same as of a slice by itself."""
+    from aws_ofi_nccl_b200.ops import llm, moe
+
+    T, k, H = 40001, 8, 8192
+    idx = torch.randint(0, 5, (T, k), device="cuda", dtype=torch.int32)
+    x = torch.randn(T, H, device="cuda", dtype=BF)
+    order = moe.expert_order(idx, 5)
+    rows = moe.permute_tokens(x, order)
+    assert rows.numel() > 2 ** 31
+    at = order.row_of[-3:].reshape(-1).long()
+    assert torch.equal(rows[at], x[-3:].repeat_interleave(k, 0))
+    token = torch.empty(T * k, device="cuda", dtype=torch.long)
+    token[order.row_of.reshape(-1).long()] = torch.arange(T * k, device="cuda") // k
+    assert torch.equal(rows[-5:], x[token[-5:]])
+    w = torch.full((T, k), 0.125, device="cuda", requires_grad=True)
+    out = moe.unpermute_tokens(rows, order, w)
+    assert torch.equal(out.detach(), x)   # eighths of the same number: no rounding
+    rows.requires_grad_(True)
+    drows, dw = torch.autograd.grad(moe.unpermute_tokens(rows, order, w), (rows, w), x)
+    assert torch.equal(drows[at], (x[-3:].float() / 8).to(BF).repeat_interleave(k, 0))
+    want = x[-3:].double().square().sum(-1, keepdim=True)
+    assert ((dw[-3:].double() - want).abs() <= (H + 8) * 2.0 ** -24 * want).all()
+    del rows, drows, out
+    wide = x.repeat(7, 1)
+    assert wide.numel() > 2 ** 31
+    norm = torch.ones(H, device="cuda", dtype=BF)
+    for group in (0, 128):
+        q, s, h = llm.rmsnorm_fp8(wide, norm, residual=wide, group=group)
+        q1, s1, h1 = llm.rmsnorm_fp8(x[-3:], norm, residual=x[-3:], group=group)
+        assert torch.equal(q[-3:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-3:], s1) and torch.equal(h[-3:], h1)
+    del wide, q, h, x
+    n, tail = 2 ** 31 + 2 ** 20 + 77, 2 ** 20 + 77
+    hyper = dict(lr=1e-2, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, zero_grad=False)
+    for bits in (8, 32):
+        p = torch.empty(n, device="cuda", dtype=BF)
+        p[-tail:].normal_()
+        g = torch.empty(n, device="cuda", dtype=BF)
+        g[-tail:].normal_()
+        p[:-tail] = 0
+        g[:-tail] = 0
+        small, gs = p[-tail:].clone(), g[-tail:].clone()
+        state, other = llm.adamw_states([p], bits=bits), llm.adamw_states([small], bits=bits)
+        llm.adamw_step_many([p], [g], **state, **hyper, step=1)
+        llm.adamw_step_many([small], [gs], **other, **hyper, step=1)
+        assert torch.equal(p[-tail:], small) and (p[:1000] == 0).all() and (p[2 ** 31 - 1000:2 ** 31] == 0).all()
+        if bits == 32:
+            assert torch.equal(state["v"][0][-tail:], other["v"][0])
+        else:
+            assert torch.equal(state["v_scale"][0][-(-(-tail // 256)):], other["v_scale"][0])
+        del p, g, state
+
+
+@pytest.mark.gpu
 def test_other_device_than_the_current_one():
     if torch.cuda.device_count() < 2:
         pytest.skip("needs two GPUs")

@@ -32,7 +32,7 @@
 namespace b200 {
 
 constexpr int ADAMW_BLOCK = 256;   // elements of a warp's pass, eight of a lane
-// With 8-bit moments it is instructions that memory waits for, 380 of a warp for a block, and their latencies: small CTAs, which end and start one by one,
+// With 8-bit moments it is instructions that memory waits for, 410 of a warp for a block, and their latencies: small CTAs, which end and start one by one,
 // and registers for sixteen of them on an SM. Medians of 218 M bf16 parameters, of 101 M with a master copy: 384 and 272 us; in CTAs of 128 threads 440
 // and 298, with 14 CTAs (72 registers) 403 and 281, with blocks copied ahead into shared memory 449 and 346, with nothing ahead 415 and 285.
 constexpr int adamw_threads(int bits) { return bits == 8 ? 64 : 256; }
@@ -51,7 +51,7 @@ struct AdamwNumbers {
   float2 one;    // products are added as multiples of it: a product and an addition the assembler makes a fused multiply-add of, whatever their roundings are called
   uint32_t dither;
   int zero_grad;
-  int careful;   // eps is so small that roots of denormal numbers count beside it
+  int careful;   // eps is so small that roots of the least numbers count beside it
 };
 // A launch's parameters are 32764 bytes at most.
 template <int N>
@@ -201,7 +201,7 @@ __device__ __forceinline__ float reciprocal(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
   return y;
 }
-// 1 / v for 2^-110 < v < 2^120, rounded as IEEE's: one Newton step from the unit's reciprocal (as roots8; of all mantissas none differs)
+// 1 / v for 2^-110 < v < 2^120, rounded as IEEE's: one Newton step from the unit's reciprocal (as minus_roots; of all floats of that range none differs)
 __device__ __forceinline__ float inverse(float v) {
   const float y = reciprocal(v);
   return fmaf(fmaf(-v, y, 1.f), y, y);
@@ -298,9 +298,9 @@ __device__ __forceinline__ uint2 hold8(const float (&f)[8], const uint32_t (&dit
 // The negative roots of pairs of numbers, given as -v: one Newton step from the unit's reciprocal root y, v y + (v - (v y)^2) y / 2, whose residual a fused
 // multiply-add has exactly (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), with the sign of v
 // so that nothing has to be negated. What is left of y's error is its square, 2^-44 of the root: of all floats from 2^-100 on none differs from IEEE's
-// root, of those from 2^-126 on none by more than an ulp.
+// root. Below, 2^-126 counts beside them: the root of 2^-115 is off by an ulp, that of 2^-126 by an eighth.
 __device__ __forceinline__ Pair minus_roots(Pair minus_v) {
-  float a, b;   // 2^-126 is nothing to what is above 2^-100, and zero gets a reciprocal root that is finite
+  float a, b;   // zero gets a reciprocal root that is finite
   fma2(minus_v, both(1.f), both(-0x1p-126f)).to(a, b);
   const Pair y(reciprocal_root(fabsf(a)), reciprocal_root(fabsf(b))), g = minus_v * y;
   return fma2(fma2(g, g, minus_v), y * both(0.5f), g);
@@ -335,7 +335,9 @@ __device__ __forceinline__ void update8(float (&x)[8], const Pair (&m)[4], const
   }
 }
 
-constexpr uint32_t CAREFUL_BELOW = 0x2b800000u;   // 2^-40: beside larger roots those of denormal numbers have the least code whatever their last bits
+// 2^-40: beside a largest root of more, a root that is off by 2^-16 of itself or more (that of a number up to 2^-119) has the
+// least code either way, and eps is more than all of it.
+constexpr uint32_t CAREFUL_BELOW = 0x2b800000u;
 
 // What a CTA has of a tensor: pointers to its first element, so that places are numbers of 32 bits. X: what the step reads the parameter from.
 template <int BITS, typename P, typename G, bool MASTER>

@@ -140,10 +140,13 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
 // ------------------------------------------------------------------ there and back
 // Bound by the rows' bytes. Where rows are whole numbers of aligned 16-byte vectors a thread has one of a token, or some, and goes through the token's
 // rows, several of whose loads or stores are under way at once. Other rows go element by element: a warp has a piece of a row, a lane every 32nd
-// element of it, so that an access is one stretch of memory whatever it starts at. Vectors that are put together from the two that they straddle
-// (of which one is read from L1) keep the float units waiting for 120 instructions each: the gradient of 2000 x 7169 x 6 in bf16 132 us, 102 so,
-// of 3001 x 1283 x 3 in fp32 32 and 23.
+// element of it, so that an access is one stretch of memory whatever it starts at. Whole vectors of which each is put together from the two that it
+// straddles cost more in instructions than they save in accesses: the gradient of 2000 x 7169 x 6 in bf16 takes 132 us that way, 102 so, that of
+// 3001 x 1283 x 3 in fp32 32 and 23, writing the rows 48 and 44, 15 and 12.
+// Aligned, 4096 x 7168 x 8 in bf16: there 91 us (5.8 TB/s), back 87 (6.1), its gradient 159 (6.3); 205 with a team of warps for a token, whose parts of
+// the weights' gradient meet behind barriers.
 constexpr int ROWS_THREADS = 256;
+constexpr int MAX_ROW = 1 << 29;   // elements, so that a piece beyond the last is a number of 32 bits too
 
 // The rows of a token are written from one read of it. `scale`: `groups` numbers of a token that go with its rows, or null
 template <typename Index>
@@ -512,7 +515,8 @@ int b200_expert_order(const void* idx, int idx64, long long n, int experts, int*
 int b200_permute_rows(const void* x, long long pitch, void* rows, const int* row_of, const float* scale, float* row_scale, int groups, long long tokens,
                       int k, long long row_bytes, int elem, void* stream) {
   ensure_context();
-  if (bad_slots(tokens, k) || row_bytes <= 0 || row_bytes > INT_MAX || (elem != 1 && elem != 2 && elem != 4) || row_bytes % elem) return B200_ERR_BAD_ARG;
+  if (bad_slots(tokens, k) || row_bytes <= 0 || (elem != 1 && elem != 2 && elem != 4) || row_bytes % elem ||
+      row_bytes / elem > MAX_ROW) return B200_ERR_BAD_ARG;
   if (!scale != !row_scale || (scale ? groups <= 0 : groups != 0)) return B200_ERR_BAD_ARG;
   if (!tokens) return 0;
   if (!x || !rows || !row_of || !on(x, pitch, elem) || !on(rows, 0, elem)) return B200_ERR_BAD_ARG;
@@ -530,7 +534,7 @@ int b200_permute_rows(const void* x, long long pitch, void* rows, const int* row
 int b200_unpermute_rows(const void* rows, long long pitch, const float* w, const int* row_of, void* out, long long tokens, int k, int H, int fp32,
                         void* stream) {
   ensure_context();
-  if (bad_slots(tokens, k) || H <= 0) return B200_ERR_BAD_ARG;
+  if (bad_slots(tokens, k) || H <= 0 || H > MAX_ROW) return B200_ERR_BAD_ARG;
   if (!tokens) return 0;
   const int elem = fp32 ? 4 : 2;
   if (!rows || !row_of || !out || !on(rows, 0, elem) || !on(out, 0, elem)) return B200_ERR_BAD_ARG;
@@ -545,7 +549,7 @@ int b200_unpermute_rows(const void* rows, long long pitch, const float* w, const
 int b200_unpermute_rows_bwd(const void* dout, const void* rows, long long pitch, const float* w, const int* row_of, void* drows, float* dw,
                             long long tokens, int k, int H, int fp32, void* stream) {
   ensure_context();
-  if (bad_slots(tokens, k) || H <= 0) return B200_ERR_BAD_ARG;
+  if (bad_slots(tokens, k) || H <= 0 || H > MAX_ROW) return B200_ERR_BAD_ARG;
   if (!tokens || (!drows && !dw)) return 0;
   const int elem = fp32 ? 4 : 2;
   if (!dout || !w || !row_of || (dw && !rows) || !on(dout, 0, elem) || !on(rows, 0, elem) || !on(drows, 0, elem)) return B200_ERR_BAD_ARG;

@@ -153,7 +153,7 @@ variable_list permute_tokens(const Tensor& x, const Tensor& row_of, const c10::o
   require(x.is_cuda() && x.dim() == 2 && (codes || of_32_or_bf16(x)), "x is a bfloat16, float32 or float8_e4m3fn CUDA matrix");
   check_rows(row_of, x);
   require(x.size(0) == row_of.size(0), "x has a row for every token");
-  require(x.size(1) > 0 && x.size(1) <= INT_MAX / 4, "rows are neither empty nor of more than 2^29 elements");
+  require(x.size(1) > 0 && x.size(1) <= 1 << 29, "rows are neither empty nor of more than 2^29 elements");
   require(!scale || codes, "scales go with 8-bit rows");
   if (!codes) return {Permute::apply(x, row_of)};
   require(!scale || (scale->scalar_type() == at::kFloat && same_device(*scale, x) && scale->is_contiguous() && (scale->dim() == 1 || scale->dim() == 2) &&
@@ -169,7 +169,7 @@ Tensor unpermute_tokens(const Tensor& rows, const Tensor& row_of, const c10::opt
   require(rows.is_cuda() && rows.dim() == 2 && of_32_or_bf16(rows), "the rows are a bfloat16 or float32 CUDA matrix");
   check_rows(row_of, rows);
   require(rows.size(0) == row_of.numel(), "there is a row for every choice");
-  require(rows.size(1) > 0 && rows.size(1) <= INT_MAX / 4, "rows are neither empty nor of more than 2^29 elements");
+  require(rows.size(1) > 0 && rows.size(1) <= 1 << 29, "rows are neither empty nor of more than 2^29 elements");
   require(!w || (w->scalar_type() == at::kFloat && same_device(*w, rows) && w->sizes() == row_of.sizes()),
           "the weights are a float32 CUDA tensor of row_of's shape");
   return Unpermute::apply(rows, row_of, w);

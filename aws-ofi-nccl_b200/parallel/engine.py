@@ -122,7 +122,7 @@ class Trainer:
 
 class AdamW:
     """The optimizer of parameters that are tensors of their own, such as those of ``models.moe.MoELayer``: one launch for up to 400 of them,
-    with the moments in 32 bits or, at a third of a training step's optimizer traffic, in 8.  Parameters without a gradient (experts
+    with the moments in 32 bits or, for less than half of the bytes, in 8.  Parameters without a gradient (experts
     that no token chose) are left as they are."""
 
     def __init__(self, params, optim: OptimConfig | None = None, *, bits: int = 32):

@@ -111,7 +111,7 @@ def build_torch_ops(force: bool = False) -> Path:
         _run([CXX, "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-DTORCH_EXTENSION_NAME=_b200torch",
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(root / "include"),
               "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-I", sysconfig.get_paths()["include"],
-              "-I", f"{CUDA_HOME}/include", *map(str, srcs), "-o", str(out), "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10",
+              "-I", f"{CUDA_HOME}/include", *map(str, srcs), "-o", str(out), "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
               "-lc10_cuda", "-ltorch_python", "-L", str(LIB), "-lb200ops", "-Wl,-rpath,$ORIGIN"])
         stamp.write_text(tag)
     return out

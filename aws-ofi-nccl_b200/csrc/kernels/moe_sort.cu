@@ -10,6 +10,7 @@
 #include <limits.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "b200ops.h"
@@ -109,10 +110,8 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
       if (rank == 0) offsets[b] = static_cast<int32_t>(first);   // the bin behind the experts begins where they end
     }
   }
-  if (CTAS > 1)
-    cluster.sync();   // nobody reads this CTA's counts any more, and `start` is whole
-  else
-    __syncthreads();
+  if (CTAS > 1) cluster.barrier_arrive();   // this CTA has read the others' counts
+  __syncthreads();                          // and `start` is whole
   for (int b = lane; b < bins; b += 32) mine[b] += start[b];
   __syncwarp();
   for (int64_t i0 = begin; i0 < end; i0 += 32 * ORDER_AHEAD) {
@@ -135,6 +134,7 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
       __syncwarp();
     }
   }
+  if (CTAS > 1) cluster.barrier_wait();   // nobody reads this CTA's counts any more
 }
 
 // ------------------------------------------------------------------ there and back
@@ -420,8 +420,9 @@ static int launch_order_on(const void* idx, long long n, int experts, int32_t* r
 // 5.0 on sixteen CTAs.
 template <typename Index>
 static int launch_order(const void* idx, long long n, int experts, int32_t* row_of, int32_t* offsets, cudaStream_t stream) {
-  int warps = 1;
-  while (warps < ORDER_WARPS && warps * 64 < n) warps *= 2;
+  // two batches of slots for a warp, and a thread for each expert
+  const int64_t wanted = std::max((n + 63) / 64, static_cast<long long>(experts + 32) / 32);
+  const int warps = static_cast<int>(std::min<int64_t>(wanted, ORDER_WARPS));
   return n > 1024 ? launch_order_on<Index, ORDER_CTAS>(idx, n, experts, row_of, offsets, warps, stream)
                   : launch_order_on<Index, 1>(idx, n, experts, row_of, offsets, warps, stream);
 }

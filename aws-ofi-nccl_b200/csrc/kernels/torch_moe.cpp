@@ -5,6 +5,7 @@
 #include <utility>
 #include <vector>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "torch_layer.h"
@@ -15,6 +16,10 @@ using namespace b200torch;
 using c10::cuda::CUDAGuard;
 
 void launched(int kernels = 1) { g_launches.fetch_add(kernels, std::memory_order_relaxed); }
+// A new tensor beside `like`, without the dispatcher, which takes as long again as the allocation
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 bool same_device(const Tensor& a, const Tensor& b) { return a.is_cuda() && a.device() == b.device(); }
 void refuse_gradients(std::initializer_list<const Tensor*> inputs, const char* what) {
   if (!at::GradMode::is_enabled()) return;
@@ -41,12 +46,12 @@ variable_list rmsnorm_fp8(const Tensor& x, const c10::optional<Tensor>& res, con
   const CUDAGuard guard(x.device());
   const Tensor xm = matrix(x), rm = res ? matrix(*res) : Tensor(), w = rows16(weight);
   auto shape = x.sizes().vec();
-  Tensor q = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn)), h = res ? at::empty(shape, x.options()) : x;
+  Tensor q = fresh(shape, at::kFloat8_e4m3fn, x), h = res ? fresh(shape, at::kBFloat16, x) : x;
   if (group)
     shape.back() = H / group;
   else
     shape.pop_back();
-  Tensor scale = at::empty(shape, x.options().dtype(at::kFloat));
+  Tensor scale = fresh(shape, at::kFloat, x);
   if (T) launched();
   check(b200_rmsnorm_fp8(xm.data_ptr(), pitch_of(xm), res ? rm.data_ptr() : nullptr, res ? pitch_of(rm) : 0, res ? h.data_ptr() : nullptr, w.data_ptr(),
                          q.data_ptr(), scale.data_ptr<float>(), T, static_cast<int>(H), static_cast<float>(eps), static_cast<int>(group), stream()),
@@ -62,8 +67,7 @@ variable_list expert_order(const Tensor& idx, int64_t experts) {
   require(experts >= 1 && experts <= 1024, "there are 1 to 1024 experts");
   require(idx.numel() <= INT_MAX, "rows are numbers of 32 bits");
   const CUDAGuard guard(idx.device());
-  const auto ints = idx.options().dtype(at::kInt);
-  Tensor row_of = at::empty(idx.sizes(), ints), offsets = at::empty({experts + 1}, ints);
+  Tensor row_of = fresh(idx.sizes(), at::kInt, idx), offsets = fresh({experts + 1}, at::kInt, idx);
   launched();
   check(b200_expert_order(idx.data_ptr(), idx.scalar_type() == at::kLong, idx.numel(), static_cast<int>(experts), row_of.data_ptr<int>(),
                           offsets.data_ptr<int>(), stream()),
@@ -81,13 +85,13 @@ Tensor gather(const Tensor& x, const Tensor& row_of, const Tensor& scale, Tensor
   const CUDAGuard guard(x.device());
   const int64_t T = row_of.size(0), k = row_of.size(1), H = x.size(1), elem = x.element_size();
   const Tensor m = rows_with_pitch(x);
-  Tensor rows = at::empty({T * k, H}, x.options());
+  Tensor rows = fresh({T * k, H}, x.scalar_type(), x);
   int groups = 0;
   if (scale.defined()) {
     groups = static_cast<int>(scale.dim() == 1 ? 1 : scale.size(1));
     auto shape = scale.sizes().vec();
     shape[0] = T * k;
-    *row_scale = at::empty(shape, scale.options());
+    *row_scale = fresh(shape, at::kFloat, scale);
   }
   if (T) launched();
   check(b200_permute_rows(m.data_ptr(), pitch_of(m) * elem, rows.data_ptr(), row_of.data_ptr<int>(), groups ? scale.data_ptr<float>() : nullptr,
@@ -99,7 +103,7 @@ Tensor weighted_sum(const Tensor& rows, const Tensor& row_of, const float* w) {
   const CUDAGuard guard(rows.device());
   const int64_t T = row_of.size(0), k = row_of.size(1), H = rows.size(1);
   const Tensor m = rows_with_pitch(rows);
-  Tensor out = at::empty({T, H}, rows.options());
+  Tensor out = fresh({T, H}, rows.scalar_type(), rows);
   if (T) launched();
   check(b200_unpermute_rows(m.data_ptr(), pitch_of(m), w, row_of.data_ptr<int>(), out.data_ptr(), T, static_cast<int>(k), static_cast<int>(H),
                             rows.scalar_type() == at::kFloat, stream()),
@@ -134,8 +138,8 @@ struct Unpermute : public Function<Unpermute> {
       const int64_t T = row_of.size(0), k = row_of.size(1), H = dout.size(1);
       const Tensor d = dout.contiguous(), rows = saved[2].defined() ? rows_with_pitch(saved[2]) : Tensor();
       Tensor drows, dw;
-      if (ctx->needs_input_grad(0)) drows = at::empty({T * k, H}, dout.options());
-      if (rows.defined()) dw = at::empty({T, k}, w.options());
+      if (ctx->needs_input_grad(0)) drows = fresh({T * k, H}, dout.scalar_type(), dout);
+      if (rows.defined()) dw = fresh({T, k}, at::kFloat, w);
       if (T && (drows.defined() || dw.defined())) launched();
       check(b200_unpermute_rows_bwd(d.data_ptr(), rows.defined() ? rows.data_ptr() : nullptr, rows.defined() ? pitch_of(rows) : H, w.data_ptr<float>(),
                                     row_of.data_ptr<int>(), drows.defined() ? drows.data_ptr() : nullptr, dw.defined() ? dw.data_ptr<float>() : nullptr,
@@ -155,7 +159,7 @@ variable_list permute_tokens(const Tensor& x, const Tensor& row_of, const c10::o
   require(x.size(0) == row_of.size(0), "x has a row for every token");
   require(x.size(1) > 0 && x.size(1) <= 1 << 29, "rows are neither empty nor of more than 2^29 elements");
   require(!scale || codes, "scales go with 8-bit rows");
-  if (!codes) return {Permute::apply(x, row_of)};
+  if (!codes) return {at::GradMode::is_enabled() && x.requires_grad() ? Permute::apply(x, row_of) : gather(x, row_of, Tensor(), nullptr)};
   require(!scale || (scale->scalar_type() == at::kFloat && same_device(*scale, x) && scale->is_contiguous() && (scale->dim() == 1 || scale->dim() == 2) &&
                      scale->size(0) == x.size(0) && (scale->dim() == 1 || (scale->size(1) > 0 && scale->size(1) <= x.size(1)))),
           "scales are a contiguous float32 CUDA tensor of one row, or one number, for every row of x");
@@ -172,7 +176,9 @@ Tensor unpermute_tokens(const Tensor& rows, const Tensor& row_of, const c10::opt
   require(rows.size(1) > 0 && rows.size(1) <= 1 << 29, "rows are neither empty nor of more than 2^29 elements");
   require(!w || (w->scalar_type() == at::kFloat && same_device(*w, rows) && w->sizes() == row_of.sizes()),
           "the weights are a float32 CUDA tensor of row_of's shape");
-  return Unpermute::apply(rows, row_of, w);
+  if (at::GradMode::is_enabled() && (rows.requires_grad() || (w && w->requires_grad()))) return Unpermute::apply(rows, row_of, w);
+  const Tensor weights = w ? w->contiguous() : Tensor();
+  return weighted_sum(rows, row_of, w ? weights.data_ptr<float>() : nullptr);
 }
 
 // ------------------------------------------------------------------ AdamW over many tensors

@@ -111,6 +111,10 @@ Tensor weighted_sum(const Tensor& rows, const Tensor& row_of, const float* w) {
   return out;
 }
 
+// Each one's gradient is the other one, so that both have derivatives of any order (a backward pass that is to be differentiated runs with gradients on).
+Tensor permute(const Tensor& x, const Tensor& row_of);
+Tensor unpermute(const Tensor& rows, const Tensor& row_of, const c10::optional<Tensor>& w);
+
 // rows[row_of[t][j]] = x[t]; its gradient is the sum over a token's rows
 struct Permute : public Function<Permute> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& row_of) {
@@ -118,7 +122,7 @@ struct Permute : public Function<Permute> {
     return gather(x, row_of, Tensor(), nullptr);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return on_engine_thread([&]() -> variable_list { return {weighted_sum(grads[0], ctx->get_saved_variables()[0], nullptr), Tensor()}; });
+    return on_engine_thread([&]() -> variable_list { return {unpermute(grads[0], ctx->get_saved_variables()[0], c10::nullopt), Tensor()}; });
   }
 };
 
@@ -133,7 +137,8 @@ struct Unpermute : public Function<Unpermute> {
     return on_engine_thread([&]() -> variable_list {
       const auto saved = ctx->get_saved_variables();
       const Tensor &row_of = saved[0], &w = saved[1], &dout = grads[0];
-      if (!w.defined()) return {gather(dout, row_of, Tensor(), nullptr), Tensor(), Tensor()};
+      if (!w.defined()) return {permute(dout, row_of), Tensor(), Tensor()};
+      if (at::GradMode::is_enabled()) raise(PyExc_RuntimeError, "a weighted unpermute_tokens has no second derivative");
       const CUDAGuard guard(dout.device());
       const int64_t T = row_of.size(0), k = row_of.size(1), H = dout.size(1);
       const Tensor d = dout.contiguous(), rows = saved[2].defined() ? rows_with_pitch(saved[2]) : Tensor();
@@ -150,6 +155,15 @@ struct Unpermute : public Function<Unpermute> {
   }
 };
 
+Tensor permute(const Tensor& x, const Tensor& row_of) {
+  return at::GradMode::is_enabled() && x.requires_grad() ? Permute::apply(x, row_of) : gather(x, row_of, Tensor(), nullptr);
+}
+Tensor unpermute(const Tensor& rows, const Tensor& row_of, const c10::optional<Tensor>& w) {
+  if (at::GradMode::is_enabled() && (rows.requires_grad() || (w && w->requires_grad()))) return Unpermute::apply(rows, row_of, w);
+  const Tensor weights = w ? w->contiguous() : Tensor();
+  return weighted_sum(rows, row_of, w ? weights.data_ptr<float>() : nullptr);
+}
+
 bool of_32_or_bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 
 variable_list permute_tokens(const Tensor& x, const Tensor& row_of, const c10::optional<Tensor>& scale) {
@@ -159,7 +173,7 @@ variable_list permute_tokens(const Tensor& x, const Tensor& row_of, const c10::o
   require(x.size(0) == row_of.size(0), "x has a row for every token");
   require(x.size(1) > 0 && x.size(1) <= 1 << 29, "rows are neither empty nor of more than 2^29 elements");
   require(!scale || codes, "scales go with 8-bit rows");
-  if (!codes) return {at::GradMode::is_enabled() && x.requires_grad() ? Permute::apply(x, row_of) : gather(x, row_of, Tensor(), nullptr)};
+  if (!codes) return {permute(x, row_of)};
   require(!scale || (scale->scalar_type() == at::kFloat && same_device(*scale, x) && scale->is_contiguous() && (scale->dim() == 1 || scale->dim() == 2) &&
                      scale->size(0) == x.size(0) && (scale->dim() == 1 || (scale->size(1) > 0 && scale->size(1) <= x.size(1)))),
           "scales are a contiguous float32 CUDA tensor of one row, or one number, for every row of x");
@@ -176,9 +190,7 @@ Tensor unpermute_tokens(const Tensor& rows, const Tensor& row_of, const c10::opt
   require(rows.size(1) > 0 && rows.size(1) <= 1 << 29, "rows are neither empty nor of more than 2^29 elements");
   require(!w || (w->scalar_type() == at::kFloat && same_device(*w, rows) && w->sizes() == row_of.sizes()),
           "the weights are a float32 CUDA tensor of row_of's shape");
-  if (at::GradMode::is_enabled() && (rows.requires_grad() || (w && w->requires_grad()))) return Unpermute::apply(rows, row_of, w);
-  const Tensor weights = w ? w->contiguous() : Tensor();
-  return weighted_sum(rows, row_of, w ? weights.data_ptr<float>() : nullptr);
+  return unpermute(rows, row_of, w);
 }
 
 // ------------------------------------------------------------------ AdamW over many tensors

@@ -38,5 +38,6 @@ def permute_tokens(x: torch.Tensor, order: ExpertOrder, scale: torch.Tensor | No
 
 def unpermute_tokens(rows: torch.Tensor, order: ExpertOrder, topk_w: torch.Tensor | None = None) -> torch.Tensor:
     """rows [tokens * k, H] (bf16 or fp32) -> [tokens, H], each token's rows summed in 32 bits, weighted by ``topk_w`` (fp32 [tokens, k])
-    unless that is None.  Choices without an expert add nothing and their rows are not read.  Rows and weights have gradients."""
+    unless that is None.  Choices without an expert add nothing and their rows are not read.  Rows and weights have gradients, of the
+    weighted sum the first ones only."""
     return _lib.native().unpermute_tokens(rows, order.row_of, topk_w)

@@ -259,3 +259,67 @@ def test_two_streams_at_once():
                 got[n].append(moe.permute_tokens(work[n][1], moe.expert_order(work[n][0], 64)))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[n]) for n in range(2) for g in got[n])
+
+
+def test_second_derivatives():
+    """Of the plain sum and of the rows, which are linear; with weights it is refused instead of left out."""
+    from aws_ofi_nccl_b200.ops import moe
+
+    idx = _choices(20, 3, 5)
+    order = moe.expert_order(idx, 5)
+    n = int(order.offsets[-1])
+    x, d = torch.randn(20, 72, device="cuda", requires_grad=True), torch.randn(60, 72, device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(moe.permute_tokens(x, order), x, d, create_graph=True)
+    (dd,) = torch.autograd.grad(dx, d, x.detach())
+    assert torch.equal(dd, moe.permute_tokens(x.detach(), order)) and (dd[n:] == 0).all()
+    (dy,) = torch.autograd.grad(moe.unpermute_tokens(d, order), d, x, create_graph=True)
+    (back,) = torch.autograd.grad(dy, x, d.detach())
+    assert torch.equal(back, moe.unpermute_tokens(d.detach(), order))
+    w = torch.rand(20, 3, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(moe.unpermute_tokens(d, order, w), (d, w), x.detach(), create_graph=True)
+
+
+def test_an_inference_pass_and_changed_inputs():
+    """Without gradients nothing is kept; what a graph keeps is checked when it is used."""
+    from aws_ofi_nccl_b200.ops import moe
+
+    idx = _choices(20, 3, 5)
+    with torch.inference_mode():
+        order = moe.expert_order(idx, 5)
+        rows = moe.permute_tokens(torch.randn(20, 64, device="cuda"), order)
+        assert moe.unpermute_tokens(rows, order, torch.rand(20, 3, device="cuda")).shape == (20, 64)
+    order = moe.expert_order(idx, 5)
+    y, w = torch.randn(60, 64, device="cuda"), torch.rand(20, 3, device="cuda", requires_grad=True)
+    out = moe.unpermute_tokens(y, order, w)
+    y.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_threads_at_once():
+    import threading
+
+    from aws_ofi_nccl_b200.ops import llm, moe
+
+    x, idx, failed = torch.randn(500, 264, device="cuda"), _choices(500, 4, 16), []
+    want = moe.permute_tokens(x, moe.expert_order(idx, 16))
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    p = [torch.zeros(700, device="cuda") for _ in range(20)]
+                    g = [torch.ones(700, device="cuda") for _ in range(20)]
+                    llm.adamw_step_many(p, g, **llm.adamw_states(p, bits=8), lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, step=1)
+                    rows = moe.permute_tokens(x, moe.expert_order(idx, 16))
+                    torch.cuda.current_stream().synchronize()
+                    assert torch.equal(rows, want) and all(torch.equal(q, p[0]) and (q != 0).all() for q in p)
+        except BaseException as e:   # noqa: BLE001  the test's thread raises it
+            failed.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed

@@ -25,10 +25,12 @@ namespace cg = cooperative_groups;
 // A counting sort in one launch: a cluster of CTAs, whose counts meet in distributed shared memory. Every warp has a range of
 // consecutive slots and counters of its own; it counts its range, takes as its start what the experts before, the CTAs before and
 // the warps before it have, and goes over its range again, 32 slots at a time, a slot's place among them being that among the lanes with its expert.
+// Latencies bound it: 32768 slots of 256 experts take 6.2 us, 524288 of 64 33. With the lanes of an expert found by a match of whole numbers they take 6.8 and
+// 39, with both passes that way 7.5 and 69.
 constexpr int ORDER_WARPS = 16;
 constexpr int ORDER_AHEAD = 8;    // indices of a lane that are on their way at once
 constexpr int ORDER_MAX_EXPERTS = 1024;
-constexpr int ORDER_CTAS = 16;    // more than 8 are not portable, but this GPU has room for them: 32768 slots of 256 experts 7.5 us, 9.0 on eight CTAs, 524288 of 64 40 and 73
+constexpr int ORDER_CTAS = 16;    // more than 8 are not portable, but this GPU has room for them: eight take 1.2 and 1.8 times as long at those sizes
 
 constexpr int order_smem(int warps, int experts) { return (warps + 2) * (experts + 1) * 4; }
 
@@ -38,7 +40,8 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
   extern __shared__ uint32_t order_shared[];
   __shared__ uint32_t warp_total[ORDER_WARPS];
   const cg::cluster_group cluster = cg::this_cluster();
-  const int bins = experts + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = threads >> 5;
+  const int bins = experts + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warps = CTAS > 1 ? ORDER_WARPS : blockDim.x >> 5, threads = 32 * warps;
   const unsigned rank = CTAS > 1 ? cluster.block_rank() : 0;
   uint32_t* const mine = order_shared + warp * bins;       // this warp's counts, later the rows that its slots get next
   uint32_t* const total = order_shared + warps * bins;     // the CTA's counts, read by the cluster
@@ -56,20 +59,25 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
     return e >= 0 && e < experts ? static_cast<int>(e) : experts;
   };
   int bin[ORDER_AHEAD];   // of the last batch, which is the only one of most calls
-  for (int64_t i0 = begin; i0 < end; i0 += 32 * ORDER_AHEAD) {
+  auto load = [&](int64_t i0) {
 #pragma unroll
     for (int u = 0; u < ORDER_AHEAD; ++u) bin[u] = i0 + 32 * u + lane < end ? bin_of(i0 + 32 * u + lane) : -1;
+  };
+  for (int64_t i0 = begin; i0 < end; i0 += 32 * ORDER_AHEAD) {
+    load(i0);
 #pragma unroll
     for (int u = 0; u < ORDER_AHEAD; ++u)
       if (bin[u] >= 0) atomicAdd(&mine[bin[u]], 1u);
   }
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += threads) {   // counts -> what the CTA's warps before have
-    uint32_t sum = 0;
-    for (int w = 0; w < warps; ++w) {
-      const uint32_t c = order_shared[w * bins + b];
-      order_shared[w * bins + b] = sum;
-      sum += c;
+    uint32_t sum = 0, c[ORDER_WARPS];
+#pragma unroll
+    for (int w = 0; w < ORDER_WARPS; ++w) c[w] = w < warps ? order_shared[w * bins + b] : 0;
+#pragma unroll
+    for (int w = 0; w < ORDER_WARPS; ++w) {
+      if (w < warps) order_shared[w * bins + b] = sum;
+      sum += c[w];
     }
     total[b] = sum;
   }
@@ -99,8 +107,9 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
     if (lane == 31) warp_total[warp] = sum;
     __syncthreads();
     uint32_t first = carry + sum - all;
-    for (int w = 0; w < warps; ++w) {
-      const uint32_t c = warp_total[w];
+#pragma unroll
+    for (int w = 0; w < ORDER_WARPS; ++w) {
+      const uint32_t c = w < warps ? warp_total[w] : 0;
       first += w < warp ? c : 0;
       carry += c;
     }
@@ -114,15 +123,18 @@ __global__ void __launch_bounds__(32 * ORDER_WARPS)
   __syncthreads();                          // and `start` is whole
   for (int b = lane; b < bins; b += 32) mine[b] += start[b];
   __syncwarp();
+  const int bits = 32 - __clz(experts);   // of the largest number, the dropped slots'
   for (int64_t i0 = begin; i0 < end; i0 += 32 * ORDER_AHEAD) {
-    if (per_warp > 32 * ORDER_AHEAD) {
-#pragma unroll
-      for (int u = 0; u < ORDER_AHEAD; ++u) bin[u] = i0 + 32 * u + lane < end ? bin_of(i0 + 32 * u + lane) : -1;
-    }
+    if (per_warp > 32 * ORDER_AHEAD) load(i0);
 #pragma unroll
     for (int u = 0; u < ORDER_AHEAD; ++u) {
       if (i0 + 32 * u >= end) break;
-      const unsigned same = __match_any_sync(0xffffffffu, bin[u]);
+      unsigned same = __ballot_sync(0xffffffffu, bin[u] >= 0);   // the lanes with this one's expert, by a vote for each bit of its number
+      for (int k = 0; k < bits; ++k) {
+        const bool one = bin[u] >> k & 1;
+        const unsigned ones = __ballot_sync(0xffffffffu, one);
+        same &= one ? ones : ~ones;
+      }
       const int place = __popc(same & ((1u << lane) - 1));
       uint32_t row = 0;
       if (bin[u] >= 0) row = mine[bin[u]] + place;
@@ -416,13 +428,12 @@ static int launch_order_on(const void* idx, long long n, int experts, int32_t* r
   B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, static_cast<const Index*>(idx), static_cast<int64_t>(n), experts, row_of, offsets));
   return 0;
 }
-// One CTA up to 1024 slots (128 take 3.0 to 4.6 us with 64 and 256 experts), where a cluster's barriers cost more than they share out: 4096 slots 6.7 us so,
-// 5.0 on sixteen CTAs.
+// One CTA up to 1024 slots (128 take 2.8 us, 1024 3.8), where a cluster's barriers cost more than they share out: 4096 slots 6.7 us so, 5.0 on sixteen CTAs.
 template <typename Index>
 static int launch_order(const void* idx, long long n, int experts, int32_t* row_of, int32_t* offsets, cudaStream_t stream) {
   // two batches of slots for a warp, and a thread for each expert
   const int64_t wanted = std::max((n + 63) / 64, static_cast<long long>(experts + 32) / 32);
-  const int warps = static_cast<int>(std::min<int64_t>(wanted, ORDER_WARPS));
+  const int warps = n > 1024 ? ORDER_WARPS : static_cast<int>(std::min<int64_t>(wanted, ORDER_WARPS));
   return n > 1024 ? launch_order_on<Index, ORDER_CTAS>(idx, n, experts, row_of, offsets, warps, stream)
                   : launch_order_on<Index, 1>(idx, n, experts, row_of, offsets, warps, stream);
 }

@@ -428,13 +428,14 @@ static int launch_order_on(const void* idx, long long n, int experts, int32_t* r
   B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, static_cast<const Index*>(idx), static_cast<int64_t>(n), experts, row_of, offsets));
   return 0;
 }
-// One CTA up to 1024 slots (128 take 2.8 us, 1024 3.8), where a cluster's barriers cost more than they share out: 4096 slots 6.7 us so, 5.0 on sixteen CTAs.
+// One CTA up to 2048 slots (128 take 2.8 us, 2048 4.6 on one or sixteen), where a cluster's barriers cost as much as they share out: 4096 slots take 5.8 us so,
+// 4.3 on sixteen CTAs.
 template <typename Index>
 static int launch_order(const void* idx, long long n, int experts, int32_t* row_of, int32_t* offsets, cudaStream_t stream) {
   // two batches of slots for a warp, and a thread for each expert
   const int64_t wanted = std::max((n + 63) / 64, static_cast<long long>(experts + 32) / 32);
-  const int warps = n > 1024 ? ORDER_WARPS : static_cast<int>(std::min<int64_t>(wanted, ORDER_WARPS));
-  return n > 1024 ? launch_order_on<Index, ORDER_CTAS>(idx, n, experts, row_of, offsets, warps, stream)
+  const int warps = n > 2048 ? ORDER_WARPS : static_cast<int>(std::min<int64_t>(wanted, ORDER_WARPS));
+  return n > 2048 ? launch_order_on<Index, ORDER_CTAS>(idx, n, experts, row_of, offsets, warps, stream)
                   : launch_order_on<Index, 1>(idx, n, experts, row_of, offsets, warps, stream);
 }
 

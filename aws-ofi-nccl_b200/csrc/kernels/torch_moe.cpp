@@ -40,7 +40,7 @@ variable_list rmsnorm_fp8(const Tensor& x, const c10::optional<Tensor>& res, con
   require(group == 0 || (group == 128 && H % 128 == 0), "a scale is one row's (group 0) or 128 columns' (group 128) of rows that are a multiple of them");
   refuse_gradients({&x, res ? &*res : nullptr, &weight}, "rmsnorm_fp8 has no gradient: call it under torch.no_grad()");
   auto matrix = [&](const Tensor& t) {   // rows of a pitch that the kernel's vectors fit
-    const Tensor m = rows_with_pitch(t.reshape({T, H}));
+    const Tensor m = rows_with_pitch(t.dim() == 2 ? t : t.reshape({T, H}));
     return reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 || pitch_of(m) % 8 ? m.clone(at::MemoryFormat::Contiguous) : m;
   };
   const CUDAGuard guard(x.device());

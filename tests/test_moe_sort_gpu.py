@@ -27,7 +27,7 @@ def _choices(T, k, E, seed=0, lost=0.2):
 
 
 # one warp's part of a batch of loads, whole batches and one more; a CTA, two, four and eight; several batches; the fewest and the most experts
-@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 64), (3, 5, 7), (16, 8, 256), (511, 1, 3), (4096, 1, 60), (4097, 1, 60), (1025, 8, 128),
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 64), (3, 5, 7), (16, 8, 256), (511, 1, 3), (2048, 1, 1000), (2049, 1, 40), (4096, 1, 60), (4097, 1, 60), (1025, 8, 128),
                                    (2731, 3, 1024), (5000, 8, 1023), (20011, 7, 256), (65536, 8, 33), (333, 2, 1024)])
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
 def test_order_is_a_stable_sort(T, k, E, kind):

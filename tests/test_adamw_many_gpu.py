@@ -119,6 +119,52 @@ def test_sizes_types_and_alignments(sizes, bits, dtype, master, packed):
     _run(sizes, bits, dtype, master=master, packed=packed, offset=1 if packed else 0)
 
 
+@pytest.mark.parametrize("offset", range(8))
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype,master", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+def test_every_offset_from_a_boundary(offset, bits, dtype, master):
+    """Parameters, gradients and state off a boundary by as many elements, with neighbours on either side that are not touched"""
+    from aws_ofi_nccl_b200.ops import llm
+
+    sizes, room = (2000, 256, 700, 5), 16
+    total = sum(sizes) + offset + room
+    g = torch.Generator(device="cuda").manual_seed(offset)
+    where = [offset + sum(sizes[:i]) for i in range(len(sizes))]
+    cut = lambda flat: [flat[a:a + n] for a, n in zip(where, sizes)]   # noqa: E731
+
+    def flat(make):
+        t = make(total)
+        return t, t.clone()
+
+    p, p0 = flat(lambda n: (torch.randn(n, device="cuda", generator=g) * 0.05).to(dtype))
+    d, d0 = flat(lambda n: torch.randn(n, device="cuda", generator=g).to(dtype))
+    names = ["m", "v"] + (["master"] if master else [])
+    make = {n: (lambda k: torch.zeros(k, device="cuda")) if bits == 32 or n == "master" else
+            (lambda k: torch.zeros(k, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)) for n in names}
+    buffers = {n: make[n](total) for n in names}
+    if master:
+        buffers["master"].copy_(p.float())
+    scales = {f"{n}_scale": [torch.zeros(-(-k // 256), device="cuda") for k in sizes] if bits == 8 else None for n in "mv"}
+    state = {"master": None, **{n: cut(b) for n, b in buffers.items()}, **scales}
+    other = llm.adamw_states([t.clone() for t in cut(p)], bits=bits, master=master)
+    apart = [t.clone() for t in cut(p)]
+    for step in (1, 2, 3):
+        llm.adamw_step_many(cut(p), cut(d), **state, **HYPER, weight_decay=0.1, step=step, zero_grad=step == 3)
+        llm.adamw_step_many(apart, [t.clone() for t in cut(d0)], **other, **HYPER, weight_decay=0.1, step=step)
+    as_bytes = lambda t: t.contiguous().view(torch.uint8)   # noqa: E731
+    for a, b in zip(cut(p), apart):
+        assert torch.equal(a, b)
+    for n in names:
+        for a, b in zip(state[n], other[n]):
+            assert torch.equal(as_bytes(a), as_bytes(b))
+    assert all((t == 0).all() for t in cut(d))
+    end = where[-1] + sizes[-1]
+    for now, then in ((p, p0), (d, d0)):
+        assert torch.equal(as_bytes(now[:offset]), as_bytes(then[:offset])) and torch.equal(as_bytes(now[end:]), as_bytes(then[end:]))
+    for n in ("m", "v"):
+        assert (as_bytes(buffers[n][:offset]) == 0).all() and (as_bytes(buffers[n][end:]) == 0).all()
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("dtype,grad_dtype", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
 def test_gradients_of_another_type(bits, dtype, grad_dtype):

@@ -24,6 +24,7 @@ class OptimConfig:
     eps: float = 1e-8
     weight_decay: float = 0.1
     master_weights: bool = True
+    state_bits: int = 32   # of the moments: 32, or 8 with a scale for every 256 (six bytes less for each parameter)
 
 
 class Trainer:
@@ -39,8 +40,9 @@ class Trainer:
         # a reducer in "zero" mode leaves each rank the optimizer state of its own shard only
         self.shard = dp.shard_range(n) if getattr(dp, "mode", "") == "zero" else (0, n)
         lo, hi = self.shard
-        self.m = torch.zeros(hi - lo, device=self.device, dtype=torch.float32)
-        self.v = torch.zeros(hi - lo, device=self.device, dtype=torch.float32)
+        moments = llm_ops.adamw_states([self.model.flat_params[lo:hi]], bits=self.optim.state_bits)
+        self.m, self.v = moments["m"][0], moments["v"][0]
+        self.m_scale, self.v_scale = ((moments[k][0] if moments[k] else None) for k in ("m_scale", "v_scale"))
         self.master = self.model.flat_params[lo:hi].float() if self.optim.master_weights else None
         self.step_count = 0
         self.kernel_launches = 0
@@ -67,9 +69,13 @@ class Trainer:
         self.step_count += 1
         lo, hi = self.shard
         grad_scale = float(getattr(self.dp, "grad_scale", 1.0))   # reducers that sum leave the 1/N to the optimizer
-        llm_ops.adamw_step(model.flat_params[lo:hi], model.flat_grads[lo:hi], self.m, self.v, self.master, lr=oc.lr,
-                           beta1=oc.beta1, beta2=oc.beta2, eps=oc.eps, weight_decay=oc.weight_decay,
-                           step=self.step_count, grad_scale=grad_scale, zero_grad=True)
+        hyper = dict(lr=oc.lr, beta1=oc.beta1, beta2=oc.beta2, eps=oc.eps, weight_decay=oc.weight_decay, step=self.step_count,
+                     grad_scale=grad_scale, zero_grad=True)
+        if self.m_scale is None:
+            llm_ops.adamw_step(model.flat_params[lo:hi], model.flat_grads[lo:hi], self.m, self.v, self.master, **hyper)
+        else:
+            llm_ops.adamw_step_many([model.flat_params[lo:hi]], [model.flat_grads[lo:hi]], [self.m], [self.v], [self.m_scale], [self.v_scale],
+                                    [self.master], **hyper)
         if (lo, hi) != (0, model.numel):
             if lo > 0:
                 model.flat_grads[:lo].zero_()
@@ -102,13 +108,19 @@ class Trainer:
 
     # ------------------------------------------------------------------ checkpoint / resume
     def state_dict(self) -> dict:
+        scales = {} if self.m_scale is None else {"m_scale": self.m_scale, "v_scale": self.v_scale}
         return {
-            "params": self.model.flat_params, "m": self.m, "v": self.v, "master": self.master,
+            "params": self.model.flat_params, "m": self.m, "v": self.v, "master": self.master, **scales,
             "step": self.step_count, "rng_cpu": torch.get_rng_state(),
             "rng_cuda": torch.cuda.get_rng_state(self.device) if self.device.type == "cuda" else None,
         }
 
     def load_state_dict(self, sd: dict) -> None:
+        if ("m_scale" in sd) != (self.m_scale is not None):
+            raise ValueError(f"the moments are held in {self.optim.state_bits} bits, the saved ones are not")
+        if self.m_scale is not None:
+            self.m_scale.copy_(sd["m_scale"])
+            self.v_scale.copy_(sd["v_scale"])
         self.model.flat_params.copy_(sd["params"])
         self.m.copy_(sd["m"])
         self.v.copy_(sd["v"])

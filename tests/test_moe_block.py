@@ -193,6 +193,52 @@ def test_training_steps_of_a_layer(bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("master", [False, True])
+def test_trainer_with_moments_in_8_bits(tmp_path, master):
+    """Each step is adamw_step_many on the flat buffers; a checkpoint holds the scales and is none of the trainer with 32 bits."""
+    from aws_ofi_nccl_b200.models.llama import LlamaConfig
+    from aws_ofi_nccl_b200.ops import llm
+    from aws_ofi_nccl_b200.parallel.engine import OptimConfig, Trainer
+
+    cfg = LlamaConfig.tiny()
+    oc = OptimConfig(state_bits=8, master_weights=master)
+    tr = Trainer(cfg, oc, device="cuda")
+    assert tr.m.dtype == tr.v.dtype == torch.float8_e4m3fn and tr.m_scale.numel() == -(-tr.m.numel() // 256)
+    ids, lbl = (torch.randint(0, cfg.vocab_size, (2, 128), device="cuda") for _ in range(2))
+    calls = []
+    step_many = llm.adamw_step_many
+
+    def watched(params, grads, m, v, ms, vs, masters, **hyper):
+        kept = [[t.clone() if t is not None else None for t in x] for x in (params, grads, m, v, ms, vs, masters)]
+        step_many(params, grads, m, v, ms, vs, masters, **hyper)
+        step_many(*kept, **hyper)
+        for now, then in zip((params, grads, m, v, ms, vs, masters), kept):
+            for a, b in zip(now, then):
+                assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        calls.append(hyper["step"])
+
+    llm.adamw_step_many = watched
+    try:
+        for _ in range(2):
+            before = tr.model.flat_params.clone()
+            assert tr.step_device(ids, lbl).isfinite()
+            assert not torch.equal(before, tr.model.flat_params) and (tr.model.flat_grads == 0).all()
+    finally:
+        llm.adamw_step_many = step_many
+    assert calls == [1, 2]
+    path = tmp_path / "ckpt.pt"
+    torch.save(tr.state_dict(), path)
+    other = Trainer(cfg, oc, device="cuda", seed=9)
+    other.load_state_dict(torch.load(path, weights_only=False))
+    for name in ("m", "v", "m_scale", "v_scale"):
+        assert torch.equal(getattr(tr, name).view(torch.uint8), getattr(other, name).view(torch.uint8))
+    assert torch.equal(tr.model.flat_params, other.model.flat_params) and other.step_count == 2
+    for a, b in ((tr, Trainer(cfg, device="cuda")), (Trainer(cfg, device="cuda"), tr)):
+        with pytest.raises(ValueError):
+            b.load_state_dict(a.state_dict())
+
+
+@pytest.mark.gpu
 def test_layer_without_a_communicator_equals_the_one_with_it():
     """The same weights and tokens: expert outputs are the same rows in another order, sums within bf16's rounding."""
     import torch.distributed as dist

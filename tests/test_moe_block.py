@@ -426,3 +426,99 @@ def test_traced():
     traced = torch.jit.trace(block, (x, gate), check_trace=False)
     x, gate = torch.randn(16, 256, device="cuda").to(BF), torch.rand(16, 2, device="cuda")
     assert all(torch.equal(a, b) for a, b in zip(traced(x, gate), block(x, gate)))
+
+
+FIRST_CALLS = """
+import torch
+from aws_ofi_nccl_b200.ops import _lib, llm, moe
+
+idx = torch.randint(0, 50, (4000, 3), device="cuda", dtype=torch.int32)   # a cluster's order
+x, w, norm = torch.randn(4000, 520, device="cuda").bfloat16(), torch.rand(4000, 3, device="cuda"), torch.ones(520, device="cuda").bfloat16()
+p, g = ([torch.full((1000,), v, device="cuda") for _ in range(20)] for v in (0.0, 1.0))
+state = llm.adamw_states(p, bits=8)
+
+
+def step():
+    order = moe.expert_order(idx, 50)
+    rows = moe.permute_tokens(x, order)
+    return (*order, rows, moe.unpermute_tokens(rows, order, w), *llm.rmsnorm_fp8(x, norm, residual=x))
+
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+    llm.adamw_step_many(p, g, **state, lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, step=1, zero_grad=False)
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a.float(), b.float()) for a, b in zip(got, step()))
+assert all(torch.equal(t, p[0]) and (t != 0).all() for t in p) and _lib.read_status() == 0
+"""
+
+
+@pytest.mark.gpu
+def test_a_process_whose_first_calls_are_captured():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_chains_see_what_the_call_before_wrote(captured):
+    """Every operator directly behind the one whose output it takes, over and over: as with the device idle between them."""
+    from aws_ofi_nccl_b200.ops import gemm, llm, moe
+
+    g = torch.Generator(device="cuda").manual_seed(6)
+    T, H, E, k = 900, 512, 12, 3
+    norm, w = torch.ones(H, device="cuda", dtype=BF), torch.rand(T, k, device="cuda", generator=g)
+    weight = (torch.randn(H, H, device="cuda", generator=g) / H ** 0.5).to(BF)
+    wq, ws = gemm.quantize_rows_fp8(weight)
+
+    def run(idx, x, p, state, pause):
+        for step in range(1, 6):
+            q, s, h = llm.rmsnorm_fp8(x, norm, residual=x)
+            pause()
+            y = gemm.gemm_fp8(q, wq, s, ws)
+            pause()
+            order = moe.expert_order(idx, E)
+            pause()
+            rows = moe.permute_tokens(y, order)
+            pause()
+            rows = gemm.linear(rows, weight)
+            pause()
+            x = moe.unpermute_tokens(rows, order, w)
+            pause()
+            llm.adamw_step_many([p], [x], **state, lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, step=step, zero_grad=False)
+            pause()
+            idx = (idx + order.offsets[1]) % E   # of what the order has just written
+            x = (x + p).to(BF)
+            pause()
+        return idx, x, p, state["m"][0].view(torch.uint8), state["v"][0].view(torch.uint8)
+
+    def inputs():
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        p = torch.randn(T, H, device="cuda", generator=gen).to(BF)
+        idx = torch.randint(0, E, (T, k), device="cuda", generator=gen, dtype=torch.int32)
+        return idx, torch.randn(T, H, device="cuda", generator=gen).to(BF), p, llm.adamw_states([p], bits=8)
+
+    want = run(*inputs(), torch.cuda.synchronize)
+    if captured:
+        args = inputs()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*inputs(), lambda: None)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(*args, lambda: None)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    else:
+        for _ in range(20):
+            assert all(torch.equal(a, b) for a, b in zip(run(*inputs(), lambda: None), want))

@@ -25,8 +25,9 @@ class MoELayer(torch.nn.Module):
             self.ep, world, rank = None, 1, 0
             dev = torch.device(device if device is not None else "cuda")
         else:
-            if device is not None and torch.device(device) != torch.device(comm.device):
-                raise ValueError("the communicator has the layer's device")
+            asked = torch.device(device) if device is not None else comm.device
+            if asked.type != comm.device.type or asked.index not in (None, comm.device.index):
+                raise ValueError("the layer is on its communicator's device")
             self.ep = ExpertParallel(comm, tokens, hidden, experts, topk, capacity_factor=capacity_factor,
                                      window_offset=window_offset)
             world, rank, dev = comm.world, comm.rank, comm.device

@@ -6,6 +6,7 @@
 #include <vector>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "torch_layer.h"
@@ -21,7 +22,13 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 bool same_device(const Tensor& a, const Tensor& b) { return a.is_cuda() && a.device() == b.device(); }
+// A dual tensor may require no gradient: its tangent would be lost without a word, and what is lost counts as zero.
+void refuse_tangents(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs)   // torch has one level of them
+    if (t && t->defined() && t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()) raise(PyExc_RuntimeError, what);
+}
 void refuse_gradients(std::initializer_list<const Tensor*> inputs, const char* what) {
+  refuse_tangents(inputs, "8-bit outputs have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : inputs) require(!t || !t->requires_grad(), what);
 }
@@ -112,6 +119,8 @@ Tensor weighted_sum(const Tensor& rows, const Tensor& row_of, const float* w) {
 }
 
 // Each one's gradient is the other one, so that both have derivatives of any order (a backward pass that is to be differentiated runs with gradients on).
+constexpr const char* NO_TANGENTS_THERE = "permute_tokens has no forward-mode derivative";
+constexpr const char* NO_TANGENTS_BACK = "unpermute_tokens has no forward-mode derivative";
 Tensor permute(const Tensor& x, const Tensor& row_of);
 Tensor unpermute(const Tensor& rows, const Tensor& row_of, const c10::optional<Tensor>& w);
 
@@ -137,6 +146,7 @@ struct Unpermute : public Function<Unpermute> {
     return on_engine_thread([&]() -> variable_list {
       const auto saved = ctx->get_saved_variables();
       const Tensor &row_of = saved[0], &w = saved[1], &dout = grads[0];
+      refuse_tangents({&dout, &w, &saved[2]}, NO_TANGENTS_BACK);
       if (!w.defined()) return {permute(dout, row_of), Tensor(), Tensor()};
       if (at::GradMode::is_enabled()) raise(PyExc_RuntimeError, "a weighted unpermute_tokens has no second derivative");
       const CUDAGuard guard(dout.device());
@@ -156,9 +166,11 @@ struct Unpermute : public Function<Unpermute> {
 };
 
 Tensor permute(const Tensor& x, const Tensor& row_of) {
+  refuse_tangents({&x}, NO_TANGENTS_THERE);
   return at::GradMode::is_enabled() && x.requires_grad() ? Permute::apply(x, row_of) : gather(x, row_of, Tensor(), nullptr);
 }
 Tensor unpermute(const Tensor& rows, const Tensor& row_of, const c10::optional<Tensor>& w) {
+  refuse_tangents({&rows, w ? &*w : nullptr}, NO_TANGENTS_BACK);
   if (at::GradMode::is_enabled() && (rows.requires_grad() || (w && w->requires_grad()))) return Unpermute::apply(rows, row_of, w);
   const Tensor weights = w ? w->contiguous() : Tensor();
   return weighted_sum(rows, row_of, w ? weights.data_ptr<float>() : nullptr);

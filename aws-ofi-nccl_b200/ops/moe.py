@@ -2,6 +2,8 @@
 experts are here.  ``parallel.expert_parallel`` moves rows between ranks; these need no communicator and no window, and their order
 is that of a stable sort, the same in every run.
 
+Gradients are of the reverse mode; a tensor with a forward-mode tangent is refused.
+
     order = expert_order(topk_idx, experts)
     rows = permute_tokens(x, order)              # rows [offsets[e], offsets[e + 1]) belong to expert e
     out = unpermute_tokens(y, order, topk_w)     # y: what the experts made of the rows

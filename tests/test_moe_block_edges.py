@@ -1,0 +1,46 @@
+"""What the operators of a mixture-of-experts block say and do at their edges: derivatives that they do not have, experts that sit steps out, and
+moments in 8 bits beyond their first step."""
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+# ------------------------------------------------------------------ forward-mode derivatives
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor requires no gradient, but its tangent would be lost: every operator that takes one says so, in a backward pass too."""
+    import torch.autograd.forward_ad as fwd
+
+    from aws_ofi_nccl_b200.ops import llm, moe
+
+    T, k, E, H = 6, 2, 4, 256
+    x, norm = torch.randn(T, H, device="cuda").to(BF), torch.ones(H, device="cuda", dtype=BF)
+    order = moe.expert_order(torch.randint(0, E, (T, k), device="cuda", dtype=torch.int32), E)
+    rows, w = torch.randn(T * k, H, device="cuda"), torch.rand(T, k, device="cuda")
+    calls = [
+        (lambda t: moe.permute_tokens(t, order), x),
+        (lambda t: moe.unpermute_tokens(t, order, w), rows),
+        (lambda t: moe.unpermute_tokens(t, order), rows),
+        (lambda t: moe.unpermute_tokens(rows, order, t), w),
+        (lambda t: llm.rmsnorm_fp8(t, norm), x),
+        (lambda t: llm.rmsnorm_fp8(x, norm, residual=t), x),
+        (lambda t: llm.rmsnorm_fp8(x, t), norm),
+    ]
+    leaf, gate, d = rows.clone().requires_grad_(True), w.clone().requires_grad_(True), torch.randn(T, H, device="cuda")
+    weighted, plain = moe.unpermute_tokens(leaf, order, gate), moe.unpermute_tokens(leaf, order)
+    xl = x.clone().requires_grad_(True)
+    there = moe.permute_tokens(xl, order)
+    calls += [(lambda t: torch.autograd.grad(weighted, (leaf, gate), t, retain_graph=True), d),
+              (lambda t: torch.autograd.grad(plain, leaf, t, retain_graph=True), d),
+              (lambda t: torch.autograd.grad(there, xl, t, retain_graph=True), torch.ones_like(there))]
+    for fn, t in calls:
+        with fwd.dual_level():
+            dual = fwd.make_dual(t.detach(), torch.ones_like(t))
+            with pytest.raises((RuntimeError, AssertionError, NotImplementedError)):
+                fn(dual)
+            with torch.no_grad(), pytest.raises((RuntimeError, AssertionError, NotImplementedError)):   # which turns backward passes off alone
+                fn(dual)
+            with fwd._set_fwd_grad_enabled(False):   # asked for: the value by itself
+                fn(dual)
+        fn(t.detach())   # outside of the level there is no tangent

@@ -147,9 +147,9 @@ class AdamW:
     def step(self, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
         """Updates the parameters from their ``grad``, which are zeroed on the way unless ``zero_grad`` is false."""
         oc = self.optim
-        self.step_count += 1
         llm_ops.adamw_step_many(self.params, [p.grad for p in self.params], **self.state, lr=oc.lr, beta1=oc.beta1, beta2=oc.beta2,
-                                eps=oc.eps, weight_decay=oc.weight_decay, step=self.step_count, grad_scale=grad_scale, zero_grad=zero_grad)
+                                eps=oc.eps, weight_decay=oc.weight_decay, step=self.step_count + 1, grad_scale=grad_scale, zero_grad=zero_grad)
+        self.step_count += 1   # a step that was refused is none
 
     def state_dict(self) -> dict:
         return {"bits": self.bits, "step": self.step_count, **self.state}

@@ -44,3 +44,16 @@ def test_forward_mode_derivatives_are_refused():
             with fwd._set_fwd_grad_enabled(False):   # asked for: the value by itself
                 fn(dual)
         fn(t.detach())   # outside of the level there is no tangent
+
+
+# ------------------------------------------------------------------ the optimizer's sparse steps
+def test_a_refused_step_counts_for_nothing(built):
+    from aws_ofi_nccl_b200.parallel.engine import AdamW
+
+    p = torch.zeros(64)
+    p.grad = torch.ones(64)
+    opt = AdamW([p])
+    for _ in range(2):
+        with pytest.raises(AssertionError):   # not on a GPU
+            opt.step()
+    assert opt.step_count == 0 and (p.grad == 1).all()

@@ -7,6 +7,7 @@
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "torch_layer.h"
@@ -323,6 +324,14 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
   check(rc, "b200_adamw_many");
 }
 
+// The current stream works on these tensors: memory of theirs that another stream allocated is not handed out again before it has.
+void used_here(const py::object& list) {
+  const Tensors tensors(list, "what is used is tensors or None", true);
+  for (size_t i = 0; i < tensors.size(); ++i)
+    if (tensors.has(i) && tensors[i].is_cuda() && tensors[i].has_storage())
+      c10::cuda::CUDACachingAllocator::recordStream(tensors[i].storage().data_ptr(), c10::cuda::getCurrentCUDAStream(tensors[i].device().index()));
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(b200ops, m) {
@@ -345,5 +354,6 @@ void b200torch::bind_moe(py::module_& m) {
   m.def("unpermute_tokens", torch::wrap_pybind_function_no_gil([](const Tensor& rows, const Tensor& row_of, const c10::optional<Tensor>& w) {
           return traced_or_direct("b200ops::unpermute_tokens", unpermute_tokens, rows, row_of, w);
         }));
+  m.def("used_here", torch::wrap_pybind_function(used_here));
   m.def("adamw_step_many", torch::wrap_pybind_function(adamw_step_many));
 }

@@ -145,11 +145,17 @@ class AdamW:
         self.step_count = 0
 
     def step(self, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
-        """Updates the parameters from their ``grad``, which are zeroed on the way unless ``zero_grad`` is false."""
+        """Updates the parameters from their ``grad``, which is None afterwards unless ``zero_grad`` is false: a tensor of zeros would still be a
+        gradient, whose parameter decays and moves on by its old moments."""
         oc = self.optim
-        llm_ops.adamw_step_many(self.params, [p.grad for p in self.params], **self.state, lr=oc.lr, beta1=oc.beta1, beta2=oc.beta2,
-                                eps=oc.eps, weight_decay=oc.weight_decay, step=self.step_count + 1, grad_scale=grad_scale, zero_grad=zero_grad)
+        grads = [p.grad for p in self.params]
+        llm_ops.adamw_step_many(self.params, grads, **self.state, lr=oc.lr, beta1=oc.beta1, beta2=oc.beta2,
+                                eps=oc.eps, weight_decay=oc.weight_decay, step=self.step_count + 1, grad_scale=grad_scale, zero_grad=False)
         self.step_count += 1   # a step that was refused is none
+        if zero_grad:
+            _lib.native().used_here(grads)
+            for p in self.params:
+                p.grad = None
 
     def state_dict(self) -> dict:
         return {"bits": self.bits, "step": self.step_count, **self.state}

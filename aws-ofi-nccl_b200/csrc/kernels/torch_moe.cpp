@@ -2,6 +2,8 @@
 // and the optimizer's step over many tensors. They run on the tensors' device, whichever is current, and on its current stream.
 #include <algorithm>
 #include <climits>
+#include <functional>
+#include <map>
 #include <utility>
 #include <vector>
 
@@ -246,7 +248,7 @@ class Tensors {
 
 void adamw_step_many(const py::object& param_list, const py::object& grad_list, const py::object& m_list, const py::object& v_list,
                      const py::object& m_scale_list, const py::object& v_scale_list, const py::object& master_list, const std::vector<double>& decay,
-                     double lr, double beta1, double beta2, double eps, int64_t step, double grad_scale, bool zero_grad) {
+                     double lr, double beta1, double beta2, double eps, const py::object& step_or_steps, double grad_scale, bool zero_grad) {
   const Tensors params(param_list, "parameters are tensors", false), grads(grad_list, "gradients are tensors or None", true);
   const Tensors m(m_list, "moments are tensors", false), v(v_list, "moments are tensors", false);
   const Tensors m_scale(m_scale_list, "scales are tensors", false), v_scale(v_scale_list, "scales are tensors", false);
@@ -255,7 +257,19 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
   require(grads.size() == count && m.size() == count && v.size() == count && (!master || master.size() == count),
           "gradients, moments and master copies are as many as the parameters");
   require(decay.size() == count, "the weight decay is a number, or one for every parameter");
-  require(step >= 1, "steps count from one");
+  const bool one_step = PyIndex_Check(step_or_steps.ptr());
+  int64_t step = 1;
+  std::vector<int64_t> steps;
+  try {
+    if (one_step)
+      step = step_or_steps.cast<int64_t>();
+    else
+      steps = step_or_steps.cast<std::vector<int64_t>>();
+  } catch (const py::cast_error&) {
+    raise(PyExc_TypeError, "the step is a whole number, or a list of one for every parameter");
+  }
+  require(one_step || steps.size() == count, "the step is a number, or one for every parameter");
+  require(step >= 1 && std::all_of(steps.begin(), steps.end(), [](int64_t s) { return s >= 1; }), "steps count from one");
   require(lr >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0, "lr and eps are not negative, the betas lie in [0, 1)");
   if (count == 0) return;
   const bool eight = m[0].scalar_type() == at::kFloat8_e4m3fn;
@@ -269,6 +283,7 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
     return t.scalar_type() == type && t.device() == device && t.numel() == n && t.is_contiguous();
   };
   std::vector<B200AdamwTensor> list;
+  std::vector<int64_t> step_of;   // where parameters have steps of their own
   std::vector<Range> of_p, of_g, of_m, of_v, of_ms, of_vs, of_master;   // what is written
   std::vector<const Tensor*> changed;
   list.reserve(count);
@@ -309,14 +324,27 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
     t.p_fp32 = p.scalar_type() == at::kFloat;
     t.g_fp32 = g.scalar_type() == at::kFloat;
     list.push_back(t);
+    if (!one_step) step_of.push_back(steps[i]);
   }
   require(apart({&of_p, &of_g, &of_m, &of_v, &of_ms, &of_vs, &of_master}), "parameters, moments, scales, master copies and gradients that are zeroed share no memory: is a parameter in the list twice?");
   if (list.empty()) return;
   const CUDAGuard guard(device);
-  int launches = 0, rc;
+  int launches = 0, rc = 0;
   {
     py::gil_scoped_release other_threads_run;   // while the launch waits for room in the queue
-    rc = b200_adamw_many(list.data(), static_cast<int>(list.size()), eight ? 8 : 32, lr, beta1, beta2, eps, step, grad_scale, zero_grad, &launches, stream());
+    auto launch = [&](const std::vector<B200AdamwTensor>& some, int64_t s) {
+      int n = 0;
+      rc = b200_adamw_many(some.data(), static_cast<int>(some.size()), eight ? 8 : 32, lr, beta1, beta2, eps, s, grad_scale, zero_grad, &n, stream());
+      launches += n;
+    };
+    if (std::adjacent_find(step_of.begin(), step_of.end(), std::not_equal_to<>()) == step_of.end()) {
+      launch(list, one_step ? step : step_of[0]);
+    } else {
+      std::map<int64_t, std::vector<B200AdamwTensor>> by_step;
+      for (size_t i = 0; i < list.size(); ++i) by_step[step_of[i]].push_back(list[i]);
+      for (const auto& [s, some] : by_step)
+        if (rc == 0) launch(some, s);
+    }
   }
   launched(launches);
   for (const Tensor* t : changed)

@@ -160,7 +160,7 @@ def adamw_states(params, *, bits: int = 32, master: bool = False) -> dict:
 
 
 def adamw_step_many(params, grads, m, v, m_scale=None, v_scale=None, master=None, *, lr: float, beta1: float, beta2: float,
-                    eps: float, weight_decay, step: int, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
+                    eps: float, weight_decay, step, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
     """One AdamW update of many tensors at once, in place: the step of ``adamw_step`` for parameters that share no flat buffer.
 
     Parameters and gradients are lists of contiguous bf16 or fp32 tensors; a gradient that is None leaves its parameter and
@@ -168,8 +168,9 @@ def adamw_step_many(params, grads, m, v, m_scale=None, v_scale=None, master=None
     share an fp32 scale in ``m_scale`` and ``v_scale``, m is code * scale and v the square of that (its root is what is held).  8-bit
     moments are rounded by a dither of element and step, so that small changes move them in the mean; what is not finite is held as NaN, and
     a root that is not zero as no less than the least code. ``master`` holds fp32 copies (or None) of bf16 parameters: they are updated, the parameters
-    are their roundings.  ``weight_decay`` is a number, or a list of one per parameter.  ``step`` counts from one and is a host
-    number like the others: a captured call repeats the step that it was captured with."""
+    are their roundings.  ``weight_decay`` is a number, or a list of one per parameter.  ``step`` counts from one, a number or a list of
+    one per parameter (then there is a launch for every number that differs), and is a host number like the others: a captured call repeats the step
+    that it was captured with."""
     params = list(params)
     decay = [float(d) for d in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * len(params)
     _lib.native().adamw_step_many(params, grads, m, v, m_scale, v_scale, master, decay, lr, beta1, beta2, eps, step, grad_scale, zero_grad)

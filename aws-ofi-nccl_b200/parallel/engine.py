@@ -135,7 +135,8 @@ class Trainer:
 class AdamW:
     """The optimizer of parameters that are tensors of their own, such as those of ``models.moe.MoELayer``: one launch for up to 400 of them,
     with the moments in 32 bits or, for less than half of the bytes, in 8.  Parameters without a gradient (experts
-    that no token chose) are left as they are."""
+    that no token chose) are left as they are, and a step that they sit out does not count in their bias corrections; parameters that have taken
+    part in different numbers of steps are a launch each number."""
 
     def __init__(self, params, optim: OptimConfig | None = None, *, bits: int = 32):
         self.params = list(params)
@@ -143,6 +144,7 @@ class AdamW:
         self.bits = bits
         self.state = llm_ops.adamw_states(self.params, bits=bits, master=self.optim.master_weights)
         self.step_count = 0
+        self.sat_out = [0] * len(self.params)   # steps that a parameter had no gradient in: its bias corrections are those of its own steps
 
     def step(self, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
         """Updates the parameters from their ``grad``, which is None afterwards unless ``zero_grad`` is false: a tensor of zeros would still be a
@@ -150,19 +152,24 @@ class AdamW:
         oc = self.optim
         grads = [p.grad for p in self.params]
         llm_ops.adamw_step_many(self.params, grads, **self.state, lr=oc.lr, beta1=oc.beta1, beta2=oc.beta2,
-                                eps=oc.eps, weight_decay=oc.weight_decay, step=self.step_count + 1, grad_scale=grad_scale, zero_grad=False)
+                                eps=oc.eps, weight_decay=oc.weight_decay, step=[self.step_count + 1 - n for n in self.sat_out],
+                                grad_scale=grad_scale, zero_grad=False)
         self.step_count += 1   # a step that was refused is none
+        self.sat_out = [n + (g is None) for n, g in zip(self.sat_out, grads)]
         if zero_grad:
             _lib.native().used_here(grads)
             for p in self.params:
                 p.grad = None
 
     def state_dict(self) -> dict:
-        return {"bits": self.bits, "step": self.step_count, **self.state}
+        return {"bits": self.bits, "step": self.step_count, "sat_out": list(self.sat_out), **self.state}
 
     def load_state_dict(self, sd: dict) -> None:
         if sd["bits"] != self.bits:
             raise ValueError(f"the moments are held in {self.bits} bits, the saved ones in {sd['bits']}")
+        sat_out = list(sd.get("sat_out") or [0] * len(self.params))
+        if len(sat_out) != len(self.params):
+            raise ValueError("the saved steps are those of other parameters")
         for name, mine in self.state.items():
             saved = sd[name]
             if (mine is None) != (saved is None) or (mine is not None and [t is None or t.shape for t in mine] != [t is None or t.shape for t in saved]):
@@ -171,4 +178,4 @@ class AdamW:
             for to, t in zip(mine or (), sd[name] or ()):
                 if to is not None:
                     to.copy_(t)
-        self.step_count = int(sd["step"])
+        self.step_count, self.sat_out = int(sd["step"]), sat_out

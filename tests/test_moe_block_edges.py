@@ -99,6 +99,77 @@ def test_gradients_that_a_step_drops_are_not_reused_before_it_ran():
     assert (p < 0).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_bias_corrections_count_a_parameters_own_steps(bits):
+    """A first gradient that comes late moves its parameter as the first step does, and a step that a parameter sits out counts for the others alone."""
+    from aws_ofi_nccl_b200.parallel.engine import AdamW, OptimConfig
+
+    oc = OptimConfig(lr=1e-2, weight_decay=0.0)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    grads = [torch.randn(500, device="cuda", generator=g) for _ in range(4)]
+    a, b, alone = (torch.zeros(500, device="cuda") for _ in range(3))
+    opt, other = AdamW([a, b], oc, bits=bits), AdamW([alone], oc, bits=bits)
+    for step, d in enumerate(grads):
+        a.grad = d.clone()
+        b.grad = None if step in (0, 2) else d.clone()
+        opt.step()
+        if step in (1, 3):
+            alone.grad = d.clone()
+            other.step()
+            assert torch.equal(b, alone)
+        if step == 1:   # m / (1 - b1) over the root of v / (1 - b2): lr in the direction of the gradient, whatever its size
+            assert ((b + 1e-2 * grads[1].sign()).abs() <= 1e-2 * (1e-8 / grads[1].abs() + 2.0 ** -20)).all()
+    assert opt.step_count == 4 and other.step_count == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_steps_of_their_own_equal_calls_of_their_own(bits):
+    from aws_ofi_nccl_b200.ops import llm
+
+    hyper = dict(lr=1e-2, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, zero_grad=False)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    sizes, steps = [700, 3, 0, 256, 1000, 5, 90], (4, 1, 1, 4, 2 ** 33, 1, 7)
+    params = [torch.randn(n, device="cuda", generator=g).to(BF) for n in sizes]
+    grads = [torch.randn(n, device="cuda", generator=g).to(BF) for n in sizes]
+    grads[5] = None
+    one, state = [p.clone() for p in params], llm.adamw_states(params, bits=bits, master=True)
+    for wrong in ([1] * 6, [], [1] * 6 + [0], (1, 2)):
+        with pytest.raises(AssertionError):
+            llm.adamw_step_many(params, grads, **state, **hyper, step=wrong)
+    for wrong in (1.5, None, [1.5] * 7, "1", 2 ** 70):
+        with pytest.raises(TypeError):
+            llm.adamw_step_many(params, grads, **state, **hyper, step=wrong)
+    with pytest.raises(AssertionError):   # before any of them is written
+        llm.adamw_step_many(params, [*grads[:6], grads[6].half()], **state, **hyper, step=steps)
+    assert all(torch.equal(a, b) for a, b in zip(params, one))
+    llm.adamw_step_many(params, grads, **state, **hyper, step=steps)
+    for i, p in enumerate(one):
+        s = llm.adamw_states([p], bits=bits, master=True)
+        llm.adamw_step_many([p], [grads[i]], **s, **hyper, step=steps[i])
+        assert torch.equal(p, params[i])
+        for name, tensors in s.items():
+            assert tensors is None or torch.equal(tensors[0].view(torch.uint8), state[name][i].view(torch.uint8))
+
+
+def test_checkpoints_hold_what_was_sat_out():
+    from aws_ofi_nccl_b200.parallel.engine import AdamW
+
+    params = [torch.zeros(300), torch.zeros(7)]
+    a = AdamW(params, bits=8)
+    a.step_count, a.sat_out = 5, [0, 3]
+    b = AdamW(params, bits=8)
+    b.load_state_dict(a.state_dict())
+    assert b.step_count == 5 and b.sat_out == [0, 3] and b.sat_out is not a.sat_out
+    saved = a.state_dict()
+    del saved["sat_out"]   # of a version that had one count for all
+    b.load_state_dict(saved)
+    assert b.step_count == 5 and b.sat_out == [0, 0]
+    with pytest.raises(ValueError):
+        b.load_state_dict({**a.state_dict(), "sat_out": [0]})
+
+
 def test_a_refused_step_counts_for_nothing(built):
     from aws_ofi_nccl_b200.parallel.engine import AdamW
 

@@ -138,11 +138,14 @@ class AdamW:
     that no token chose) are left as they are, and a step that they sit out does not count in their bias corrections; parameters that have taken
     part in different numbers of steps are a launch each number."""
 
-    def __init__(self, params, optim: OptimConfig | None = None, *, bits: int = 32):
+    def __init__(self, params, optim: OptimConfig | None = None, *, bits: int | None = None):
+        """bits: of the moments, by default the configuration's ``state_bits``."""
         self.params = list(params)
         self.optim = optim or OptimConfig()
-        self.bits = bits
-        self.state = llm_ops.adamw_states(self.params, bits=bits, master=self.optim.master_weights)
+        if bits == 32 and self.optim.state_bits == 8:
+            raise ValueError("the configuration asks for moments in 8 bits, the call for 32")
+        self.bits = self.optim.state_bits if bits is None else bits
+        self.state = llm_ops.adamw_states(self.params, bits=self.bits, master=self.optim.master_weights)
         self.step_count = 0
         self.sat_out = [0] * len(self.params)   # steps that a parameter had no gradient in: its bias corrections are those of its own steps
 

@@ -180,3 +180,18 @@ def test_a_refused_step_counts_for_nothing(built):
         with pytest.raises(AssertionError):   # not on a GPU
             opt.step()
     assert opt.step_count == 0 and (p.grad == 1).all()
+
+
+def test_the_configuration_says_the_moments_bits():
+    from aws_ofi_nccl_b200.parallel.engine import AdamW, OptimConfig
+
+    params = [torch.zeros(300, dtype=BF)]
+    for opt, bits in ((AdamW(params), 32), (AdamW(params, OptimConfig(state_bits=8)), 8), (AdamW(params, bits=8), 8),
+                      (AdamW(params, OptimConfig(), bits=8), 8), (AdamW(params, OptimConfig(state_bits=8), bits=8), 8)):
+        assert opt.bits == bits and opt.state["m"][0].dtype == (torch.float8_e4m3fn if bits == 8 else torch.float32)
+        assert opt.state_dict()["bits"] == bits
+    with pytest.raises(ValueError):
+        AdamW(params, OptimConfig(state_bits=8), bits=32)
+    for optim, bits in ((None, 16), (OptimConfig(state_bits=16), None)):
+        with pytest.raises(ValueError):
+            AdamW(params, optim, bits=bits)

@@ -59,11 +59,12 @@ class MoELayer(torch.nn.Module):
             rows, offsets = self.ep.dispatch(x, idx, w, self.fp8), self.ep.expert_offsets
         # The per-expert row ranges live on the device; slicing the rows for the per-expert GEMM
         # calls needs them on the host.
-        off = offsets.tolist()
+        off = [min(n, rows.shape[0]) for n in offsets.tolist()]   # rows beyond the window's capacity have raised its status
+        counts = [b - a for a, b in zip(off, off[1:])]
         outs = []
-        for e in range(len(self.w_gate_up)):
-            if off[e + 1] > off[e]:
-                seg = rows[off[e]:off[e + 1]]
+        # cut at once: the rows' gradient is one concatenation, where that of a slice would be a matrix of all rows for each expert
+        for e, seg in enumerate(rows.split([*counts, rows.shape[0] - off[-1]])[:-1]):
+            if counts[e]:
                 outs.append(linear(swiglu(linear(seg, self.w_gate_up[e])), self.w_down[e]))
         if outs:
             y = torch.cat(outs, dim=0)

@@ -195,3 +195,22 @@ def test_the_configuration_says_the_moments_bits():
     for optim, bits in ((None, 16), (OptimConfig(state_bits=16), None)):
         with pytest.raises(ValueError):
             AdamW(params, optim, bits=bits)
+
+
+# ------------------------------------------------------------------ the layer's backward pass
+@pytest.mark.gpu
+def test_experts_rows_are_cut_and_joined_once():
+    """The rows' gradient is one concatenation, not a matrix of all rows for each expert"""
+    from aws_ofi_nccl_b200.models.moe import MoELayer
+
+    layer = MoELayer(None, 0, 256, 128, 16, 2, seed=1)
+    x = torch.randn(200, 256, device="cuda").to(BF).requires_grad_(True)
+    out = layer(x)
+    seen, todo = {}, [out.grad_fn]
+    while todo:
+        node = todo.pop()
+        if node is not None and node not in seen:
+            seen[node] = node.name()
+            todo += [n for n, _ in node.next_functions]
+    assert not [n for n in seen.values() if "Slice" in n]
+    assert sum("Split" in n for n in seen.values()) == 1

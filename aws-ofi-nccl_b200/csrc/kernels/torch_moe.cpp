@@ -210,17 +210,30 @@ Tensor unpermute_tokens(const Tensor& rows, const Tensor& row_of, const c10::opt
 
 // ------------------------------------------------------------------ AdamW over many tensors
 using Range = std::pair<uintptr_t, uintptr_t>;
-// Whether no two of the written ranges share a byte. A list of tensors mostly lies in order, so lists are sorted by themselves, if at all, and merged.
-bool apart(std::initializer_list<std::vector<Range>*> lists) {
+// Whether no two of the written ranges share a byte, nor one of them with one that is read, which may share theirs. A list of tensors mostly lies in
+// order, so lists are sorted by themselves, if at all, and merged.
+bool apart(std::initializer_list<std::vector<Range>*> lists, std::vector<Range>& read) {
   std::vector<Range> all;
+  size_t total = 0;
+  for (const std::vector<Range>* r : lists) total += r->size();
+  all.reserve(total);
+  auto sort = [](std::vector<Range>& r) {
+    if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
+  };
   for (std::vector<Range>* r : lists) {
-    if (!std::is_sorted(r->begin(), r->end())) std::sort(r->begin(), r->end());
+    sort(*r);
     const size_t before = all.size();
     all.insert(all.end(), r->begin(), r->end());
     if (before && !r->empty() && all[before] < all[before - 1]) std::inplace_merge(all.begin(), all.begin() + before, all.end());
   }
   for (size_t i = 1; i < all.size(); ++i)
     if (all[i].first < all[i - 1].second) return false;
+  sort(read);
+  auto w = all.begin();
+  for (const Range& r : read) {
+    while (w != all.end() && w->second <= r.first) ++w;
+    if (w != all.end() && w->first < r.second) return false;
+  }
   return true;
 }
 
@@ -284,14 +297,19 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
   };
   std::vector<B200AdamwTensor> list;
   std::vector<int64_t> step_of;   // where parameters have steps of their own
-  std::vector<Range> of_p, of_g, of_m, of_v, of_ms, of_vs, of_master;   // what is written
+  std::vector<Range> of_p, of_g, of_m, of_v, of_ms, of_vs, of_master, read;   // all but the last are written
   std::vector<const Tensor*> changed;
   list.reserve(count);
   changed.reserve(4 * count);
-  auto write = [&](std::vector<Range>& to, const Tensor& t) -> void* {
+  auto note = [count](std::vector<Range>& to, const Tensor& t) -> void* {
     void* const data = t.data_ptr();
+    if (to.empty()) to.reserve(count);
     const uintptr_t at = reinterpret_cast<uintptr_t>(data);
     to.emplace_back(at, at + t.nbytes());
+    return data;
+  };
+  auto write = [&](std::vector<Range>& to, const Tensor& t) -> void* {
+    void* const data = note(to, t);
     changed.push_back(&t);
     return data;
   };
@@ -311,7 +329,7 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
     if (n == 0) continue;
     B200AdamwTensor t{};
     t.p = write(of_p, p);
-    t.g = zero_grad ? write(of_g, g) : g.data_ptr();
+    t.g = zero_grad ? write(of_g, g) : note(read, g);
     t.m = write(of_m, m[i]);
     t.v = write(of_v, v[i]);
     if (eight) {
@@ -326,7 +344,9 @@ void adamw_step_many(const py::object& param_list, const py::object& grad_list, 
     list.push_back(t);
     if (!one_step) step_of.push_back(steps[i]);
   }
-  require(apart({&of_p, &of_g, &of_m, &of_v, &of_ms, &of_vs, &of_master}), "parameters, moments, scales, master copies and gradients that are zeroed share no memory: is a parameter in the list twice?");
+  require(apart({&of_p, &of_g, &of_m, &of_v, &of_ms, &of_vs, &of_master}, read),
+          "parameters, moments, scales, master copies and gradients that are zeroed share no memory, with each other or with a gradient that is read: "
+          "is a parameter in the list twice?");
   if (list.empty()) return;
   const CUDAGuard guard(device);
   int launches = 0, rc = 0;

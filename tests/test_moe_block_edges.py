@@ -197,6 +197,30 @@ def test_the_configuration_says_the_moments_bits():
             AdamW(params, optim, bits=bits)
 
 
+@pytest.mark.gpu
+def test_gradients_over_what_is_written_are_refused():
+    """A gradient is read while other CTAs write: it may be shared, but not with a parameter, a moment, a scale or a master copy."""
+    from aws_ofi_nccl_b200.ops import llm
+
+    hyper = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, step=1, zero_grad=False)
+    for bits in (8, 32):
+        buf = torch.ones(4000, device="cuda")
+        p = [buf[:1000], buf[2000:3000]]
+        state = llm.adamw_states(p, bits=bits)
+        inside = [torch.ones(1000, device="cuda"), buf[1500:2500]]
+        before = buf.clone()
+        for grads in (inside, inside[::-1], [buf[1000:2000], buf[2001:3001]], [buf[1:1001], buf[3000:]], [buf[:1000], buf[3000:]]):
+            with pytest.raises(AssertionError):
+                llm.adamw_step_many(p, grads, **state, **hyper)
+        if bits == 32:
+            with pytest.raises(AssertionError):
+                llm.adamw_step_many(p, [state["v"][1], buf[3000:]], **state, **hyper)
+        assert torch.equal(buf, before)
+        llm.adamw_step_many(p, [buf[1000:2000], buf[3000:]], **state, **hyper)   # beside them
+        llm.adamw_step_many(p, [buf[1000:2000]] * 2, **state, **{**hyper, "step": 2})   # one for both
+        assert (buf[:1000] != 1).all() and torch.equal(buf[1000:2000], before[1000:2000]) and torch.equal(buf[:1000], buf[2000:3000])
+
+
 # ------------------------------------------------------------------ the layer's backward pass
 @pytest.mark.gpu
 def test_experts_rows_are_cut_and_joined_once():

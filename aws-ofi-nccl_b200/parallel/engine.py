@@ -8,6 +8,7 @@ Waits in kernels are bounded; where one gave up, the step raises instead.
 from __future__ import annotations
 
 import dataclasses
+import math
 
 import torch
 
@@ -24,7 +25,7 @@ class OptimConfig:
     eps: float = 1e-8
     weight_decay: float = 0.1
     master_weights: bool = True
-    state_bits: int = 32   # of the moments: 32, or 8 with a scale for every 256 (six bytes less for each parameter)
+    state_bits: int = 32   # of the moments: 32, or 8 with a scale for every 256 of a parameter (six bytes less for each parameter)
 
 
 class Trainer:
@@ -40,10 +41,13 @@ class Trainer:
         # a reducer in "zero" mode leaves each rank the optimizer state of its own shard only
         self.shard = dp.shard_range(n) if getattr(dp, "mode", "") == "zero" else (0, n)
         lo, hi = self.shard
-        moments = llm_ops.adamw_states([self.model.flat_params[lo:hi]], bits=self.optim.state_bits)
+        flat = self.model.flat_params[lo:hi]
+        moments = llm_ops.adamw_states([flat], bits=self.optim.state_bits)
         self.m, self.v = moments["m"][0], moments["v"][0]
-        self.m_scale, self.v_scale = ((moments[k][0] if moments[k] else None) for k in ("m_scale", "v_scale"))
-        self.master = self.model.flat_params[lo:hi].float() if self.optim.master_weights else None
+        self.m_scale = self.v_scale = None
+        self.master = flat.float() if self.optim.master_weights else None
+        if self.optim.state_bits == 8:
+            self._by_parameter(lo, hi)
         self.step_count = 0
         self.kernel_launches = 0
         if dp is not None:
@@ -51,9 +55,22 @@ class Trainer:
         self._ids_dev = None
         self._labels_dev = None
 
+    def _by_parameter(self, lo: int, hi: int) -> None:
+        """Moments in 8 bits are stepped parameter by parameter, so that no scale is that of two: a norm's moments are of another size than a matrix's."""
+        spans = [(max(at, lo), min(at + math.prod(shape), hi)) for at, shape in self.model.offsets.values()]
+        spans = [(a, b) for a, b in spans if a < b]
+        blocks = [-(-(b - a) // llm_ops.ADAMW_BLOCK) for a, b in spans]
+        self.m_scale, self.v_scale = (torch.zeros(sum(blocks), device=self.device, dtype=torch.float32) for _ in "mv")
+        of_model = lambda flat: [flat[a:b] for a, b in spans]                 # noqa: E731
+        of_shard = lambda flat: [flat[a - lo:b - lo] for a, b in spans]       # noqa: E731
+        masters = of_shard(self.master) if self.master is not None else [None] * len(spans)
+        self._pieces = (of_model(self.model.flat_params), of_model(self.model.flat_grads), of_shard(self.m), of_shard(self.v),
+                        list(self.m_scale.split(blocks)), list(self.v_scale.split(blocks)), masters)
+        # whether blocks of 256 counted from the shard's beginning would be the same
+        self._blocks_as_flat = all((a - lo) % llm_ops.ADAMW_BLOCK == 0 for a, _ in spans)
+
     @staticmethod
     def _padded_numel(cfg: LlamaConfig) -> int:
-        import math
         return sum((math.prod(s) + 127) // 128 * 128 for _, s in cfg.param_shapes())
 
     # ------------------------------------------------------------------ one optimizer step, device tensors in
@@ -74,8 +91,7 @@ class Trainer:
         if self.m_scale is None:
             llm_ops.adamw_step(model.flat_params[lo:hi], model.flat_grads[lo:hi], self.m, self.v, self.master, **hyper)
         else:
-            llm_ops.adamw_step_many([model.flat_params[lo:hi]], [model.flat_grads[lo:hi]], [self.m], [self.v], [self.m_scale], [self.v_scale],
-                                    [self.master], **hyper)
+            llm_ops.adamw_step_many(*self._pieces, **hyper)
         if (lo, hi) != (0, model.numel):
             if lo > 0:
                 model.flat_grads[:lo].zero_()
@@ -108,7 +124,7 @@ class Trainer:
 
     # ------------------------------------------------------------------ checkpoint / resume
     def state_dict(self) -> dict:
-        scales = {} if self.m_scale is None else {"m_scale": self.m_scale, "v_scale": self.v_scale}
+        scales = {} if self.m_scale is None else {"m_scale": self.m_scale, "v_scale": self.v_scale, "scale_blocks": "parameter"}
         return {
             "params": self.model.flat_params, "m": self.m, "v": self.v, "master": self.master, **scales,
             "step": self.step_count, "rng_cpu": torch.get_rng_state(),
@@ -119,6 +135,8 @@ class Trainer:
         if ("m_scale" in sd) != (self.m_scale is not None):
             raise ValueError(f"the moments are held in {self.optim.state_bits} bits, the saved ones are not")
         if self.m_scale is not None:
+            if sd.get("scale_blocks") != "parameter" and not self._blocks_as_flat:
+                raise ValueError("the saved scales are of blocks that hold more than one parameter")
             self.m_scale.copy_(sd["m_scale"])
             self.v_scale.copy_(sd["v_scale"])
         self.model.flat_params.copy_(sd["params"])

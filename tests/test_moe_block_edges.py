@@ -1,5 +1,7 @@
 """What the operators of a mixture-of-experts block say and do at their edges: derivatives that they do not have, experts that sit steps out, and
 moments in 8 bits beyond their first step."""
+import math
+
 import pytest
 import torch
 
@@ -238,3 +240,107 @@ def test_experts_rows_are_cut_and_joined_once():
             todo += [n for n, _ in node.next_functions]
     assert not [n for n in seen.values() if "Slice" in n]
     assert sum("Split" in n for n in seen.values()) == 1
+
+
+# ------------------------------------------------------------------ moments in 8 bits beyond the first step
+def _odd_config():
+    """Norms of 384 weights: a block of 256 elements of the flat buffer would hold two parameters"""
+    from aws_ofi_nccl_b200.models.llama import LlamaConfig
+
+    return LlamaConfig(vocab_size=512, hidden=384, n_layers=2, n_heads=6, n_kv_heads=2, ffn=640, max_seq=64)
+
+
+def test_blocks_of_the_trainers_moments_are_one_parameters():
+    from aws_ofi_nccl_b200.parallel.engine import OptimConfig, Trainer
+
+    cfg = _odd_config()
+    tr = Trainer(cfg, OptimConfig(state_bits=8), device="cpu")
+    assert tr.m_scale.numel() == tr.v_scale.numel() == sum(-(-math.prod(s) // 256) for _, s in cfg.param_shapes())
+    sd = tr.state_dict()
+    Trainer(cfg, OptimConfig(state_bits=8), device="cpu", seed=3).load_state_dict(sd)
+    # a checkpoint whose blocks went over the parameters' borders
+    flat = {k: v for k, v in sd.items() if k != "scale_blocks"}
+    with pytest.raises(ValueError):
+        tr.load_state_dict(flat)
+    tiny = type(cfg).tiny()   # there the borders of both are the same
+    tr = Trainer(tiny, OptimConfig(state_bits=8), device="cpu")
+    assert tr.m_scale.numel() == -(-tr.m.numel() // 256)
+    tr.load_state_dict({k: v for k, v in tr.state_dict().items() if k != "scale_blocks"})
+
+
+class _Shard:
+    """What the trainer asks of a reducer in "zero" mode, of one rank among others, without the others"""
+    mode, grad_scale = "zero", 0.5
+
+    def __init__(self, lo, hi):
+        self.range = (lo, hi)
+
+    def allocate_grad_buffer(self, n):
+        return torch.zeros(n, device="cuda", dtype=BF)
+
+    def shard_range(self, n):
+        return self.range
+
+    def attach(self, model):
+        pass
+
+    def begin_step(self):
+        pass
+
+    def finish_step(self):
+        pass
+
+    def gather_params(self, flat):
+        pass
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("shard", [None, (100_096, 400_000)])
+def test_trainer_steps_each_parameter_by_itself(master, shard):
+    """Against AdamW's step over the parameters one by one, with the numbers that the configuration names; in a shard, over what it has of each"""
+    from aws_ofi_nccl_b200.ops import llm
+    from aws_ofi_nccl_b200.parallel.engine import OptimConfig, Trainer
+
+    cfg = _odd_config()
+    oc = OptimConfig(lr=2e-3, beta1=0.8, beta2=0.9, eps=1e-6, weight_decay=0.3, state_bits=8, master_weights=master)
+    tr = Trainer(cfg, oc, device="cuda", dp=_Shard(*shard) if shard else None)
+    lo, hi = tr.shard
+    pieces = []
+    for off, shape in tr.model.offsets.values():
+        a, b = max(off, lo), min(off + math.prod(shape), hi)
+        if a < b:
+            pieces.append((a, b))
+    assert len(pieces) >= 3 and any((a - lo) % 256 for a, _ in pieces)
+    params = [tr.model.flat_params[a:b].clone() for a, b in pieces]
+    states = [llm.adamw_states([p], bits=8, master=master) for p in params]
+    outside = torch.cat((tr.model.flat_params[:lo], tr.model.flat_params[hi:])).clone()
+    grads = []
+    step_many = llm.adamw_step_many
+
+    def watched(*args, **kw):
+        grads.append(tr.model.flat_grads.clone())
+        step_many(*args, **kw)
+
+    ids, lbl = (torch.randint(0, cfg.vocab_size, (2, 64), device="cuda") for _ in range(2))
+    llm.adamw_step_many = watched
+    try:
+        for step in (1, 2):
+            tr.step_device(ids, lbl)
+            for (a, b), p, s in zip(pieces, params, states):
+                step_many([p], [grads[-1][a:b].clone()], **s, lr=2e-3, beta1=0.8, beta2=0.9, eps=1e-6, weight_decay=0.3, step=step,
+                          grad_scale=0.5 if shard else 1.0)
+    finally:
+        llm.adamw_step_many = step_many
+    assert len(grads) == 2 and (tr.model.flat_grads == 0).all()
+    at = 0
+    for (a, b), p, s in zip(pieces, params, states):
+        n = s["m_scale"][0].numel()
+        assert torch.equal(tr.model.flat_params[a:b], p)
+        for flat, one in ((tr.m, s["m"][0]), (tr.v, s["v"][0])):
+            assert torch.equal(flat[a - lo:b - lo].view(torch.uint8), one.view(torch.uint8))
+        assert torch.equal(tr.m_scale[at:at + n], s["m_scale"][0]) and torch.equal(tr.v_scale[at:at + n], s["v_scale"][0])
+        assert not master or torch.equal(tr.master[a - lo:b - lo], s["master"][0])
+        at += n
+    assert at == tr.m_scale.numel()
+    assert torch.equal(torch.cat((tr.model.flat_params[:lo], tr.model.flat_params[hi:])), outside)

@@ -19,7 +19,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residu
     ``rmsnorm`` returns it.  ``group`` 0: one fp32 scale per row, of x's shape without the last dimension, as ``gemm_fp8``
     takes them; 128: one per 128 columns, as the expert exchange moves its rows.  The norm is rounded once, where
     ``quantize_rows_fp8(rmsnorm(x))`` rounds it to bf16 first.  Rows may be strided (last dim contiguous); they hold a
-    multiple of 8 elements, at most 16384.  A row that holds a NaN or an infinity has a NaN as its scale.  There is no gradient: inputs that
+    multiple of 8 elements, at most 16384.  A NaN is in every scale of its row.  An infinity makes its own scale a NaN (its row's, or its 128 columns') and
+    the rest of its row zeros, as ``rmsnorm`` does; both leave zeros of a finite row whose squares add up beyond 32 bits.  There is no gradient: inputs that
     require one are refused unless gradients are off, and so are those that have a forward-mode tangent."""
     return tuple(_lib.native().rmsnorm_fp8(x, residual, weight, eps, group))
 

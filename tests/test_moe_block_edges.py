@@ -242,6 +242,34 @@ def test_experts_rows_are_cut_and_joined_once():
     assert sum("Split" in n for n in seen.values()) == 1
 
 
+# ------------------------------------------------------------------ the norm's rows that are not finite
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [256, 1024, 7168])
+def test_scales_of_rows_that_are_not_finite(H):
+    """What the composition of rmsnorm's formula and the scales' makes of them: a NaN is in every scale of its row, an infinity in its own (its row's, or its
+    128 columns'), and the rest of that row is zero times it. A finite row whose squares add up beyond 32 bits is zero, as rmsnorm's is."""
+    from aws_ofi_nccl_b200.ops import llm
+
+    x = torch.randn(4, H, device="cuda").to(BF)
+    x[0, 3], x[1, 130], x[2, 130] = float("nan"), float("inf"), -float("inf")
+    x[3] = 2.0 ** 90
+    w = torch.ones(H, device="cuda", dtype=BF)
+    least = torch.full((), 1e-12, device="cuda") * (1.0 / 448.0)
+    q, scale, _ = llm.rmsnorm_fp8(x, w)
+    assert scale[:3].isnan().all() and scale[3] == least and (q[3].float() == 0).all()
+    q, scale, _ = llm.rmsnorm_fp8(x, w, group=128)
+    assert scale[0].isnan().all()
+    for row in (1, 2):
+        assert scale[row, 1].isnan()
+        others = torch.arange(H // 128, device="cuda") != 1
+        assert (scale[row][others] == least).all() and (q[row].view(-1, 128)[others].float() == 0).all()
+    assert (scale[3] == least).all() and (q[3].float() == 0).all()
+    n, _ = llm.rmsnorm(x, w)
+    assert n[0].isnan().all() and (n[3] == 0).all()
+    for row in (1, 2):
+        assert n[row, 130].isnan() and (n[row, :128] == 0).all() and (n[row, 131:] == 0).all()
+
+
 # ------------------------------------------------------------------ moments in 8 bits beyond the first step
 def _odd_config():
     """Norms of 384 weights: a block of 256 elements of the flat buffer would hold two parameters"""

@@ -271,6 +271,59 @@ def test_scales_of_rows_that_are_not_finite(H):
 
 
 # ------------------------------------------------------------------ moments in 8 bits beyond the first step
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,packed", [((257,), False), ((100003, 7, 4096, 1, 65536), False), ((100003, 7, 4096, 1, 65536), True)])
+@pytest.mark.parametrize("dtype,master", [(BF, False), (BF, True), (torch.float32, False)])
+def test_codes_of_moments_that_are_not_zero_before(sizes, packed, dtype, master):
+    """Element by element: codes and scales of both moments in the second and third step, with the rounding that m's terms leave where they cancel"""
+    from aws_ofi_nccl_b200.ops import llm
+
+    F = 2.0 ** -24
+    b1, b2 = 0.9, 0.95
+    g = torch.Generator(device="cuda").manual_seed(sum(sizes))
+    lay = (lambda t: list(t.split(list(sizes)))) if packed else (lambda t: [s.clone() for s in t.split(list(sizes))])
+    params = lay((torch.randn(sum(sizes), device="cuda", generator=g) * 0.05).to(dtype))
+    state = llm.adamw_states(params, bits=8, master=master)
+    checked = 0
+    for step in (1, 2, 3):
+        grads = lay((torch.randn(sum(sizes), device="cuda", generator=g) * 10.0 ** -step).to(dtype))
+        old = [{n: (state[n][i].double(), state[n + "_scale"][i].double()) for n in "mv"} for i in range(len(sizes))]
+        llm.adamw_step_many(params, grads, **state, lr=1e-3, beta1=b1, beta2=b2, eps=1e-8, weight_decay=0.1, step=step, zero_grad=False)
+        for i, n in enumerate(sizes):
+            block = torch.arange(n, device="cuda") // 256
+            blocks = -(-n // 256)
+            d = grads[i].double()
+            m, v = (old[i][x][0] * old[i][x][1][block] for x in "mv")
+            v = v * v
+            # roundings: m's product and decoding, its scaled gradient, their sum, each of its own size; of the root half of those of v
+            m_off = F * (4 * b1 * m.abs() + 4 * (1 - b1) * d.abs())
+            m = b1 * m + (1 - b1) * d
+            root = (b2 * v + (1 - b2) * d * d).sqrt()
+            word = (torch.arange(n, device="cuda") * 0xC13FA9A9 + step * 0x91E10DA5) & 0xFFFFFFFF
+            for name, z, off, dither in (("m", m, m_off, word), ("v", root, 6 * F * root, word ^ 0xFFFFFFFF)):
+                most = torch.zeros(blocks, device="cuda", dtype=torch.float64).scatter_reduce_(0, block, z.abs(), "amax")
+                top_off = torch.zeros(blocks, device="cuda", dtype=torch.float64).scatter_reduce_(0, block, off, "amax")
+                top = most.clamp_min(1e-30) / 448
+                assert ((state[name + "_scale"][i].double() - top).abs() <= top_off / 448 + 4 * F * top).all()
+                share = z.abs() / top[block]
+                gap = torch.exp2(torch.floor(torch.log2(share.clamp_min(2.0 ** -6))) - 3)
+                place = share / gap + (dither >> 12).double() / 2 ** 20
+                # what the share may be off by: of its own value, of the scale, three roundings, and half of 2^-29 of what is denormal there
+                place_off = (off / top[block] + share * (top_off / most.clamp_min(1e-30))[block] + 6 * F * share) / gap + 2.0 ** -20
+                near = (place - place.round()).abs() <= place_off
+                near |= (share / gap - 8).abs() <= place_off   # the gap itself halves below
+                want = (torch.floor(place) * gap).clamp(max=448)
+                if name == "v":
+                    want = torch.where(z != 0, want.clamp_min(2.0 ** -9), want)
+                got = state[name][i].double()
+                assert torch.equal(got.abs()[~near], want[~near])
+                assert ((got.abs() - want).abs() <= gap * (1 + 1e-9))[near].all()
+                sure = (z.abs() > off) & (got != 0)
+                assert torch.equal(torch.signbit(got)[sure], torch.signbit(z)[sure])
+                checked += int((~near).sum())
+    assert checked >= 0.98 * 6 * sum(sizes)
+
+
 def _odd_config():
     """Norms of 384 weights: a block of 256 elements of the flat buffer would hold two parameters"""
     from aws_ofi_nccl_b200.models.llama import LlamaConfig

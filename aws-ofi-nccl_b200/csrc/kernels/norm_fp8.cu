@@ -8,6 +8,7 @@
 #include "b200ops.h"
 #include "dependent_launch.cuh"
 #include "host_util.h"
+#include "pair_math.cuh"
 
 namespace b200 {
 
@@ -23,22 +24,14 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
          (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
 }
-// The largest of three magnitudes, a NaN if there is one
-__device__ __forceinline__ float largest(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
-  return r;
-}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
-  asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  (both(a) * both(b)).to(r.x, r.y);
   return r;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
-  asm("{.reg .b64 x, y, z, w; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 w, {%6, %7}; fma.rn.f32x2 z, x, y, w; mov.b64 {%0, %1}, z;}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  fma2(both(a), both(b), both(c)).to(r.x, r.y);
   return r;
 }
 

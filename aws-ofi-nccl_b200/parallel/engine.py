@@ -169,15 +169,16 @@ class AdamW:
 
     def step(self, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
         """Updates the parameters from their ``grad``, which is None afterwards unless ``zero_grad`` is false: a tensor of zeros would still be a
-        gradient, whose parameter decays and moves on by its old moments."""
+        gradient, whose parameter decays and moves on by its old moments. While a graph is captured they are zeroed where they are: a replay reads them there."""
         oc = self.optim
         grads = [p.grad for p in self.params]
+        captured = any(g is not None and g.is_cuda for g in grads) and torch.cuda.is_current_stream_capturing()
         llm_ops.adamw_step_many(self.params, grads, **self.state, lr=oc.lr, beta1=oc.beta1, beta2=oc.beta2,
                                 eps=oc.eps, weight_decay=oc.weight_decay, step=[self.step_count + 1 - n for n in self.sat_out],
-                                grad_scale=grad_scale, zero_grad=False)
+                                grad_scale=grad_scale, zero_grad=zero_grad and captured)
         self.step_count += 1   # a step that was refused is none
         self.sat_out = [n + (g is None) for n, g in zip(self.sat_out, grads)]
-        if zero_grad:
+        if zero_grad and not captured:
             _lib.native().used_here(grads)
             for p in self.params:
                 p.grad = None

@@ -102,6 +102,35 @@ def test_gradients_that_a_step_drops_are_not_reused_before_it_ran():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("with_backward", [False, True])
+def test_captured_steps_read_gradients_where_they_were(with_backward):
+    """A replay finds the gradients at their places: those that it was given, or those of its own backward pass"""
+    from aws_ofi_nccl_b200.parallel.engine import AdamW
+
+    p, q = torch.zeros(3000, device="cuda", requires_grad=True), torch.zeros(3000, device="cuda")
+    opt, other = AdamW([p]), AdamW([q])
+    d = torch.randn(3000, device="cuda")
+    if not with_backward:
+        p.grad = torch.zeros_like(d)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        if with_backward:
+            (p * d).sum().backward()
+        opt.step()
+    assert p.grad is not None
+    for _ in range(3):
+        d.normal_()
+        junk = [torch.full((3000,), 7.0, device="cuda") for _ in range(4)]   # in what memory there is
+        if not with_backward:
+            p.grad.copy_(d)
+        graph.replay()
+        q.grad, other.step_count = d.clone(), 0   # a replay repeats the step that was captured
+        other.step()
+        assert torch.equal(p.detach(), q) and (p.grad == 0).all() and all((t == 7).all() for t in junk)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [8, 32])
 def test_bias_corrections_count_a_parameters_own_steps(bits):
     """A first gradient that comes late moves its parameter as the first step does, and a step that a parameter sits out counts for the others alone."""

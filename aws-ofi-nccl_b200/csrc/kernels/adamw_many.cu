@@ -34,9 +34,10 @@ namespace b200 {
 
 constexpr int ADAMW_BLOCK = 256;   // elements of a warp's pass, eight of a lane
 // With 8-bit moments there are 410 instructions of a warp for a block of it, and latencies between them, beside little memory: small CTAs, which end and
-// start one by one, and registers for sixteen of them on an SM. 218 M bf16 parameters, 101 M with a master copy take 388 and 271 us (5.7 and 6.0 TB/s; without
-// rounding to codes at all 1 % less); in CTAs of 128 threads 440 and 298, with 14 CTAs (72 registers) 403 and 281, with blocks copied ahead into
-// shared memory 449 and 346, with nothing ahead 415 and 285. In a loop that keeps float units and memory busy for longer the clock falls, and they take 417 and 266.
+// start one by one, and registers for sixteen of them on an SM. 218 M bf16 parameters take 393 us a pass over some passes (5.6 TB/s; without rounding to codes
+// at all 1 % less), 101 M with a master copy 265 (6.1); over 2000 passes in turn, which draw the clock from 1965 down to 1660 and 1490 MHz, 432 and 270. Each
+// of these beside 388 and 271 of its own run: CTAs of 128 threads 440 and 298, 14 CTAs (72 registers) 403 and 281, blocks copied ahead into
+// shared memory 449 and 346, nothing ahead 415 and 285.
 constexpr int adamw_threads(int bits) { return bits == 8 ? 64 : 256; }
 constexpr int adamw_ctas(int bits) { return bits == 8 ? 16 : 3; }        // of an SM at least
 constexpr int adamw_pass(int bits) { return adamw_threads(bits) * 8; }   // elements of a CTA's pass
@@ -463,7 +464,8 @@ __global__ void __launch_bounds__(adamw_threads(BITS), adamw_ctas(BITS)) adamw_m
 
 static bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// Elements of a CTA: as few as fill the chip, up to some passes of it. With 8-bit moments four take 433 and 270 us in a loop, eight 417 and 266, 32 5 and 10 us more.
+// Elements of a CTA: as few as fill the chip, up to some passes of it. With 8-bit moments, in passes enough to draw the clock down, four take 433 and 270 us, eight
+// 417 and 266, 32 5 and 10 us more.
 static int adamw_chunk_elements(int64_t total, int bits) {
   const int most = bits == 8 ? 8 : 4;
   const int64_t passes = total / (static_cast<int64_t>(sm_count()) * 2048 * 8);

@@ -1,5 +1,6 @@
 // Tokens sorted by expert and back on one GPU: where a mixture-of-experts layer has all its experts here, its rows need no window, no
-// records and no signals (moe.cu), and no atomics: the order is that of a stable sort.
+// records and no signals (moe.cu), and no counters in memory: the order is that of a stable sort. Counts are added up by atomics in shared memory, whose
+// order no sum depends on.
 //
 // A slot n = t * k + j is token t's j-th choice. Its row is the number of slots that go to an earlier expert, or to the same one and stand
 // before it; slots whose expert is none of [0, E) come behind all others, and row_of holds ~row for them. So row_of is a permutation: every

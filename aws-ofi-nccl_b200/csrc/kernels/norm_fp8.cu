@@ -37,9 +37,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // With y = h * r * w the largest |y| of a row is r times the largest |h * w|: it is found together with the sum of squares, in one exchange between the
 // row's threads, and a value's code needs h * w alone, which stays in registers. Maxima are of the numbers' bits, where a NaN is above all others: a row
-// that holds one has it as its scale. A sum of squares beyond 32 bits makes r zero: finite values become zeros, an infinity a NaN of its scale. TPR threads hold a row, VPT 16-byte vectors each, all of whose loads are under way at once; memory bounds it, with
-// what a short kernel takes to come up and run out. 4096 x 4096 with a residual 20.0 us (5.9 TB/s; 22.0 in CTAs of 256 threads that pack and
-// unpack more), without 10.2; 5003 x 7168 in groups 22.6 (4.8 TB/s; 34.8 so). CTAs that stay, with the next row's loads ahead, take 20.4, 10.9 and 22.4: they
+// that holds one has it as its scale. A sum of squares beyond 32 bits makes r zero: finite values become zeros, an infinity a NaN of its scale.
+// Products of two bf16 lie on a tie of e4m3 exactly in 6 of 10000 elements of normal inputs; there the roundings of r and the scale decide between the two codes.
+//
+// TPR threads hold a row, VPT 16-byte vectors each, all of whose loads are under way at once; memory bounds it, with what a short kernel takes to come
+// up and run out. 4096 x 4096 with a residual 20.0 us (5.9 TB/s; 22.0 in CTAs of 256 threads that pack and unpack more), without 10.2; 5003 x 7168 in
+// groups 23.1 (4.7 TB/s; 34.8 in such CTAs). CTAs that stay, with the next row's loads ahead, took 20.4, 10.9 and 22.4 beside 20.0, 10.2 and 22.6: they
 // gain where rows are narrow (60000 x 256 12.7 -> 11.2) and lose with a residual (9000 x 5120 50.9 -> 51.9).
 template <int TPR, int VPT, int THREADS, bool GROUPS, bool RES>
 __global__ void __launch_bounds__(THREADS)
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(THREADS)
     if (c * 8 >= H) continue;
     if constexpr (GROUPS) {
       s = scale_of(group_top[i]);
-      factor = r * __fdividef(1.f, s);
+      factor = r * __fdividef(1.f, s);   // within 2 ulp: a code moves where its share is that near to a tie, as by the products' own roundings
       if (c % (NORM8_GROUP / 8) == 0) scale[row * (H / NORM8_GROUP) + c / (NORM8_GROUP / 8)] = s;
     }
 #pragma unroll

@@ -41,7 +41,8 @@ __device__ __forceinline__ float reciprocal(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
   return y;
 }
-// 1 / v for 2^-110 < v < 2^120, rounded as IEEE's: one Newton step from the unit's reciprocal (as minus_roots; of all floats of that range none differs)
+// 1 / v for 2^-110 < v < 2^120, rounded as IEEE's: one Newton step from the unit's reciprocal (as minus_roots; of all floats of that range none
+// differs: csrc/tests/gpu_pair_math.cu looks at each)
 __device__ __forceinline__ float inverse(float v) {
   const float y = reciprocal(v);
   return fmaf(fmaf(-v, y, 1.f), y, y);
@@ -50,7 +51,7 @@ __device__ __forceinline__ float inverse(float v) {
 // The negative roots of pairs of numbers, given as -v: one Newton step from the unit's reciprocal root y, v y + (v - (v y)^2) y / 2, whose residual a fused
 // multiply-add has exactly (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), with the sign of v
 // so that nothing has to be negated. What is left of y's error is its square, 2^-44 of the root: of all floats from 2^-100 on none differs from IEEE's
-// root. Below, 2^-126 counts beside them: the root of 2^-115 is off by an ulp, that of 2^-126 by an eighth.
+// root (gpu_pair_math.cu). Below, 2^-126 counts beside them: the root of 2^-115 is off by an ulp, that of 2^-126 by an eighth.
 __device__ __forceinline__ Pair minus_roots(Pair minus_v) {
   float a, b;   // zero gets a reciprocal root that is finite
   fma2(minus_v, both(1.f), both(-0x1p-126f)).to(a, b);

@@ -17,7 +17,7 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residu
                 group: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``rmsnorm`` with its output in 8 bits: (q, scale, h) with normed ~= q * scale, q e4m3 of x's shape and h as
     ``rmsnorm`` returns it.  ``group`` 0: one fp32 scale per row, of x's shape without the last dimension, as ``gemm_fp8``
-    takes them; 128: one per 128 columns, as the expert exchange moves its rows.  The norm is rounded once, where
+    takes them (of 256 rows or more); 128: one per 128 columns, the layout of the expert exchange's 8-bit rows, which it makes by itself.  The norm is rounded once, where
     ``quantize_rows_fp8(rmsnorm(x))`` rounds it to bf16 first.  Rows may be strided (last dim contiguous); they hold a
     multiple of 8 elements, at most 16384.  A NaN is in every scale of its row.  An infinity makes its own scale a NaN (its row's, or its 128 columns') and
     the rest of its row zeros, as ``rmsnorm`` does; both leave zeros of a finite row whose squares add up beyond 32 bits.  There is no gradient: inputs that

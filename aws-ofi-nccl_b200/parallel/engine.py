@@ -154,7 +154,8 @@ class AdamW:
     """The optimizer of parameters that are tensors of their own, such as those of ``models.moe.MoELayer``: one launch for up to 400 of them,
     with the moments in 32 bits or, for less than half of the bytes, in 8.  Parameters without a gradient (experts
     that no token chose) are left as they are, and a step that they sit out does not count in their bias corrections; parameters that have taken
-    part in different numbers of steps are a launch each number."""
+    part in different numbers of steps are a launch each number.  Master copies are taken here: load the weights before, or load a state saved with them
+    behind it, since a step overwrites the parameters with their copies."""
 
     def __init__(self, params, optim: OptimConfig | None = None, *, bits: int | None = None):
         """bits: of the moments, by default the configuration's ``state_bits``."""

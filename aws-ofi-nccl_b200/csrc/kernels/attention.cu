@@ -1,0 +1,723 @@
+// Causal attention with a sliding window and first tokens that stay visible, forward and backward, on tcgen05.
+//
+//   S = scale q k^T over visible keys, P = softmax(S), out = P v
+//   delta = sum(dout * out), dS = P * (dout v^T - delta), dq = scale dS k, dk = scale dS^T q, dv = P^T dout
+//
+// Scores never leave the SM: the forward pass keeps a running maximum and sum of each row, the backward pass computes P again from the
+// rows' log-sum (in base 2), which the forward pass stores.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "attention.cuh"
+#include "b200ops.h"
+#include "host_util.h"
+
+namespace b200 {
+
+// ------------------------------------------------------------------ forward
+// A CTA takes two units of 128 queries of one head each that share a head of k and v: two heads of a group for the same tokens, or where the number
+// of heads in a group is odd also neighbouring tokens. So a tile of k and v is loaded once for 256 rows.
+struct AttnUnit {
+  int head, i0, lo, hi;   // rows from i0; key tiles lo to hi of its window (none where lo > hi)
+  bool live;
+};
+__device__ __forceinline__ AttnUnit attn_unit(const AttnShape& s, int kv_head, int u, int len) {
+  AttnUnit r;
+  const int tile = u / s.G;
+  r.head = kv_head * s.G + (u - tile * s.G);
+  r.i0 = tile * ATT_TILE;
+  r.live = r.i0 < len;
+  r.hi = r.live ? (min(r.i0 + ATT_TILE, len) - 1) / ATT_TILE : -1;
+  r.lo = r.live ? (s.window ? max(0, r.i0 - s.window + 1) / ATT_TILE : 0) : 0;
+  return r;
+}
+// The key tiles of a pair of units: those that hold sinks, in front of the windows' tiles, and these.
+struct AttnWalk {
+  int far, lo, n;          // far sink tiles, then tiles from lo; n in all
+  int sink_tiles;
+  __device__ __forceinline__ int tile(int j) const { return j < far ? j : lo + j - far; }
+  __device__ __forceinline__ bool uses(const AttnUnit& u, int t) const { return u.live && t <= u.hi && (t >= u.lo || t < sink_tiles); }
+};
+__device__ __forceinline__ AttnWalk attn_walk(const AttnShape& s, const AttnUnit& a, const AttnUnit& b) {
+  AttnWalk w;
+  w.sink_tiles = s.window ? (s.sinks + ATT_TILE - 1) / ATT_TILE : 0;
+  w.lo = min(a.live ? a.lo : 1 << 30, b.live ? b.lo : 1 << 30);
+  const int hi = max(a.hi, b.hi);
+  w.far = hi < 0 ? 0 : min(w.sink_tiles, w.lo);
+  w.n = hi < 0 ? 0 : w.far + hi - w.lo + 1;
+  return w;
+}
+
+template <int HD>
+struct AttnFwd {
+  static constexpr int TILE = ATT_TILE * HD * 2;
+  static constexpr int STAGES = 4;
+  static constexpr int TILES = (2 + STAGES) * TILE;
+  static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
+  // barriers: stages full and empty; q there; scores there, probabilities there (or their row scaled), sums of a unit done
+  static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, SCORES = Q + 2, PROBS = SCORES + 2, DONE = PROBS + 2, BARS = DONE + 2;
+  // tensor memory: scores of a unit (probabilities as bf16 over their first half), its sums
+  static constexpr int S_COL = 0, O_COL = 256;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(ATT_THREADS, 1)
+    attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                         bf16* out, float* lse, AttnShape s, int* err_word) {
+  using L = AttnFwd<HD>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
+  grid_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the longest walks first
+  const int heads = s.B * s.nkv, units = s.rows / ATT_TILE * s.G;
+  const int pair = (units + 1) / 2 - 1 - static_cast<int>(blockIdx.x) / heads, bh = static_cast<int>(blockIdx.x) % heads;
+  const int b = bh / s.nkv, kv_head = bh - b * s.nkv;
+  const int len = sequence_length(s, b);
+  AttnUnit unit[2] = {attn_unit(s, kv_head, 2 * pair, len), attn_unit(s, kv_head, 2 * pair + 1, len)};
+  if (2 * pair + 1 >= units) unit[1].live = false, unit[1].hi = -1;
+  const AttnWalk walk = attn_walk(s, unit[0], unit[1]);
+  const uint32_t q_tile = cta.smem, stages = cta.smem + 2 * L::TILE;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- loads: q, then k and v in turn
+    if (elect_one_sync()) {
+      for (int u = 0; u < 2; ++u)
+        if (unit[u].live) {
+          mbar_expect_tx(cta.bar(L::Q + u), L::TILE);
+          load_tile<HD, ATT_TILE>(q_tile + u * L::TILE, &tmQ, b, unit[u].head, unit[u].i0, cta.bar(L::Q + u));
+        }
+      for (int i = 0; i < 2 * walk.n; ++i) {
+        const int st = i % L::STAGES;
+        if (!cta.wait(L::EMPTY + st, (i / L::STAGES & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT)) break;
+        mbar_expect_tx(cta.bar(L::FULL + st), L::TILE);
+        load_tile<HD, ATT_TILE>(stages + st * L::TILE, i & 1 ? &tmV : &tmK, b, kv_head, walk.tile(i >> 1) * ATT_TILE, cta.bar(L::FULL + st));
+      }
+      grid_release();
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue: probabilities
+    // are read before the next scores of their unit are written over them
+    constexpr uint32_t idesc_s = make_instr_desc(1, 1, ATT_TILE, ATT_TILE, 0, 0), idesc_o = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
+    auto full = [&](int i) { return cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
+    auto scores = [&](int u, int i) {
+      if (lane == 0) {
+        const uint32_t k_tile = stages + i % L::STAGES * L::TILE;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          umma_f16(cta.tmem + L::S_COL + u * ATT_TILE, desc_rows<ATT_TILE>(q_tile + u * L::TILE, k), desc_rows<ATT_TILE>(k_tile, k), idesc_s, k != 0);
+        umma_commit(cta.bar(L::SCORES + u));
+      }
+      __syncwarp();
+    };
+    auto release = [&](int i) {
+      if (lane == 0) umma_commit(cta.bar(L::EMPTY + i % L::STAGES));
+      __syncwarp();
+    };
+    bool ok = walk.n > 0;
+    uint32_t turns[2] = {0, 0};   // tiles that a unit has taken
+    if (ok && (ok = full(0))) {
+      for (int u = 0; u < 2 && ok; ++u)
+        if (unit[u].live) {
+          ok = cta.wait(L::Q + u, 0, DEV_ERR_FULL_BAR_TIMEOUT);
+          tc_fence_after();
+          if (ok && walk.uses(unit[u], walk.tile(0))) scores(u, 0);
+        }
+      release(0);
+    }
+    for (int j = 0; j < walk.n && ok; ++j) {
+      const int t = walk.tile(j), next = walk.tile(j + 1);
+      const bool more = j + 1 < walk.n;
+      if (!(ok = full(2 * j + 1) && (!more || full(2 * j + 2)))) break;
+      const uint32_t v_tile = stages + (2 * j + 1) % L::STAGES * L::TILE;
+      const int there = len - t * ATT_TILE;
+      if (there < ATT_TILE && len < s.S) zero_rows<HD, ATT_TILE>(v_tile, there);
+      for (int u = 0; u < 2; ++u) {
+        if (walk.uses(unit[u], t)) {
+          if (!(ok = cta.wait(L::PROBS + u, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < ATT_TILE / 16; ++k)
+              umma_f16_ts(cta.tmem + L::O_COL + u * 128, cta.tmem + L::S_COL + u * ATT_TILE + k * 8, desc_cols<ATT_TILE>(v_tile, k), idesc_o,
+                          turns[u] != 0 || k != 0);
+          }
+          __syncwarp();
+          ++turns[u];
+        }
+        if (more && walk.uses(unit[u], next)) scores(u, 2 * j + 2);
+        if (j + 1 == walk.n && lane == 0) umma_commit(cta.bar(L::DONE + u));
+      }
+      if (!ok) break;
+      release(2 * j + 1);
+      if (more) release(2 * j + 2);
+    }
+  } else if (warp < 8) {
+    // ---------------------------------------------------------------- softmax: a thread has a row
+    const int u = warp >> 2;
+    const AttnUnit& me = unit[u];
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_col = cta.tmem + lanes + L::S_COL + u * ATT_TILE, o_col = cta.tmem + lanes + L::O_COL + u * 128;
+    const int i = me.i0 + (warp & 3) * 32 + lane;
+    const float c = s.scale * ATT_LOG2E;
+    float top = -INFINITY, sum = 0.f;   // of the scores times c; the sum is relative to 2^top
+    uint32_t turns = 0;
+    bool ok = true;
+    for (int j = 0; j < walk.n; ++j) {
+      const int t = walk.tile(j);
+      if (!walk.uses(me, t)) continue;
+      if (!(ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+      tc_fence_after();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tmem_ld_32x32(s_col + k * 32, x[k]);
+      tmem_ld_wait();
+      const int j0 = t * ATT_TILE;
+      const bool whole = j0 + ATT_TILE - 1 <= me.i0 &&
+                         (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks);
+      if (!whole) {
+        const int last = i - j0, first = s.window ? last - s.window + 1 : -1, sinks = s.window ? s.sinks - j0 : 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int at = k * 32 + e;
+            if (at > last || (at < first && at >= sinks)) x[k][e] = 0xFF800000u;   // -inf
+          }
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) most = fmaxf(most, __uint_as_float(x[k][e]));
+      most *= c;
+      // The sums are scaled to a new maximum only where it has grown by more than 2^8: probabilities beside the old one stay in range
+      if (__any_sync(0xffffffffu, most > top + 8.f)) {
+        const float now = fmaxf(top, most);
+        const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
+        top = now;
+        sum *= f;
+        if (turns) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            uint32_t o[16];
+            tmem_ld_32x16(o_col + k * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st_32x16(o_col + k * 16, o);
+          }
+        }
+      }
+      const float ref = top == -INFINITY ? 0.f : -top;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t p[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float p0 = exp2_unit(fmaf(__uint_as_float(x[k][e]), c, ref)), p1 = exp2_unit(fmaf(__uint_as_float(x[k][e + 1]), c, ref));
+          part[e & 2] += p0;
+          part[(e & 2) + 1] += p1;
+          p[e / 2] = pack_bf16x2(p0, p1);
+        }
+        tmem_st_32x16(s_col + k * 16, p);   // over scores that all are in registers
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(cta.bar(L::PROBS + u));
+      ++turns;
+    }
+    const bool exists = 2 * pair + u < units;
+    if (exists) {
+      if (ok && turns) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
+      tc_fence_after();
+      const bool mine = i < len;
+      lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? top + log2f(sum) : INFINITY;   // no probability behind the end
+      const float f = 1.f / sum;
+      uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD);
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k) {
+        uint32_t o[32];
+        if (turns && ok) {
+          tmem_ld_32x32(o_col + k * 32, o);
+          tmem_ld_wait();
+        }
+        if (i < s.S) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (mine && turns && ok) {
+              auto two = [&](int at) { return pack_bf16x2(__uint_as_float(o[at]) * f, __uint_as_float(o[at + 1]) * f); };
+              v = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
+            }
+            row[k * 4 + e / 8] = v;
+          }
+        }
+      }
+    }
+  }
+  attn_end(cta);
+}
+
+// ------------------------------------------------------------------ backward
+// delta[b][head][i] = sum over a row of dout * out, 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, float* delta, AttnShape s) {
+  grid_wait();
+  grid_release();
+  constexpr int LANES = HD / 8;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;   // over [B][rows][nq]
+  const int v = threadIdx.x % LANES;
+  const bool there = row < static_cast<int64_t>(s.B) * s.rows * s.nq;
+  const int h = there ? static_cast<int>(row % s.nq) : 0;
+  const int64_t bt = there ? row / s.nq : 0;
+  const int b = static_cast<int>(bt / s.rows), i = static_cast<int>(bt % s.rows);
+  float sum = 0.f;
+  if (there && i < sequence_length(s, b)) {
+    const uint4 a = reinterpret_cast<const uint4*>(dout + b * db + i * dt + h * dh)[v];
+    const uint4 o = reinterpret_cast<const uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + h) * HD)[v];
+    const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162*>(&a), *y = reinterpret_cast<const __nv_bfloat162*>(&o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum = fmaf(__low2float(x[e]), __low2float(y[e]), sum);
+      sum = fmaf(__high2float(x[e]), __high2float(y[e]), sum);
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (there && v == 0) delta[(static_cast<int64_t>(b) * s.nq + h) * s.rows + i] = sum;
+}
+
+// Both gradient kernels hold a tile of 128 rows and walk over tiles of 64 rows of the other side:
+//   KEYS (dk, dv): a tile of k and v; q, dout, lse and delta pass by, over the heads of the group, whose sum is the gradient
+//   else (dq):     a tile of q and dout; k and v pass by
+// First T1 = held1 passing1^T (scores) and T2 = held2 passing2^T (dout v^T), a thread's row of each; then P and dS as bf16 in their place, the first
+// operands of dv += P dout, dk += dS q or dq += dS k. Two groups of warps take every second tile, so that the products of one run while the other's
+// probabilities are computed. Every sum is made in one order: gradients are the same bits in every run.
+template <int HD>
+struct AttnBwd {
+  static constexpr int HELD = ATT_TILE * HD * 2, PASSING = ATT_BOX * HD * 2;
+  static constexpr int STAGE = 2 * PASSING;
+  static constexpr int STAGES = 4;
+  static constexpr int STATS = 2 * ATT_BOX * 4;   // lse and delta of a stage's rows
+  static constexpr int TILES = 2 * HELD + STAGES * (STAGE + STATS);
+  static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
+  static constexpr int FULL = 0, EMPTY = STAGES, THERE = 2 * STAGES, SCORES = THERE + 1, PROBS = SCORES + 2, DONE = PROBS + 2, BARS = DONE + 1;
+  static constexpr int T1_COL = 0, T2_COL = 128, ACC1_COL = 256, ACC2_COL = 384;
+};
+// How the walk of dk and dv over queries that see a tile only through sinks is split: `parts` CTAs take `part_tiles` tiles of 64 queries each, of every
+// head, and their sums and those of the tile's own window are joined in order. parts 0: no tile has any.
+struct AttnSplit {
+  int tiles, parts, part_tiles;
+  float* sums;   // [1 + parts][B * nkv * tiles][dv, dk][128][HD]
+};
+
+template <int HD, bool KEYS>
+__global__ void __launch_bounds__(ATT_THREADS, 1)
+    attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                         const __grid_constant__ CUtensorMap tmD, const float* lse, const float* delta, bf16* grad1, bf16* grad2, AttnShape s,
+                         AttnSplit split, int* err_word) {
+  using L = AttnBwd<HD>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
+  grid_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // this CTA's tile and its walk: `far` tiles from 0, then tiles from `lo` on, `per_head` in all; with KEYS for each head of the group
+  int b, head, tile, part = 0, far = 0, lo = 0, per_head;
+  int index = blockIdx.x;
+  const int heads = s.B * (KEYS ? s.nkv : s.nq), tiles = s.rows / ATT_TILE;
+  const int split_ctas = KEYS ? heads * split.tiles * split.parts : 0;
+  if (index < split_ctas) {
+    part = 1 + index / (heads * split.tiles);
+    index %= heads * split.tiles;
+    tile = index / heads;
+  } else {
+    index -= split_ctas;
+    tile = KEYS ? index / heads : tiles - 1 - index / heads;   // the longest walks first
+  }
+  b = index % heads;
+  head = b % (KEYS ? s.nkv : s.nq);
+  b /= KEYS ? s.nkv : s.nq;
+  const int len = sequence_length(s, b), r0 = tile * ATT_TILE;
+  const bool joined = KEYS && split.parts > 0 && tile < split.tiles;
+  if constexpr (KEYS) {
+    // queries of the window: up to the last key's; of the far parts: behind those
+    const int end = (len + ATT_BOX - 1) / ATT_BOX;
+    const int near = s.window ? static_cast<int>(min(static_cast<int64_t>(end), (static_cast<int64_t>(r0) + ATT_TILE - 1 + s.window - 1) / ATT_BOX + 1)) : end;
+    lo = r0 / ATT_BOX;
+    int hi = near;
+    if (part) {
+      lo = static_cast<int>(min(static_cast<int64_t>(near) + static_cast<int64_t>(part - 1) * split.part_tiles, static_cast<int64_t>(end)));
+      hi = min(lo + split.part_tiles, end);
+    } else if (s.window && !joined && r0 < s.sinks) {
+      hi = end;   // sinks whose walk is not split
+    }
+    per_head = r0 < len ? max(0, hi - lo) : 0;
+  } else {
+    const int last = min(r0 + ATT_TILE, len) - 1;
+    lo = s.window ? max(0, r0 - s.window + 1) / ATT_BOX : 0;
+    far = s.window ? min((s.sinks + ATT_BOX - 1) / ATT_BOX, lo) : 0;
+    per_head = r0 < len ? far + last / ATT_BOX - lo + 1 : 0;
+  }
+  const int group = KEYS ? s.G : 1, n = group * per_head;
+  const int first_head = KEYS ? head * s.G : head / s.G;   // of the passing tensors
+  const uint32_t held = cta.smem, stages = cta.smem + 2 * L::HELD, stats = stages + L::STAGES * L::STAGE;
+  auto row_of = [&](int at) { return (at < far ? at : lo + at - far) * ATT_BOX; };   // the first row of a head's at-th tile
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- loads
+    if (elect_one_sync() && n > 0) {
+      mbar_expect_tx(cta.bar(L::THERE), 2 * L::HELD);
+      load_tile<HD, ATT_TILE>(held, KEYS ? &tmK : &tmQ, b, head, r0, cta.bar(L::THERE));
+      load_tile<HD, ATT_TILE>(held + L::HELD, KEYS ? &tmV : &tmD, b, head, r0, cta.bar(L::THERE));
+      int i = 0;
+      bool ok = true;
+      for (int g = 0; g < group && ok; ++g)
+        for (int at = 0; at < per_head; ++at, ++i) {
+          const int st = i % L::STAGES, row = row_of(at);
+          if (!(ok = cta.wait(L::EMPTY + st, (i / L::STAGES & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
+          const uint32_t dst = stages + st * L::STAGE, bar = cta.bar(L::FULL + st);
+          mbar_expect_tx(bar, L::STAGE + (KEYS ? L::STATS : 0));
+          load_tile<HD, ATT_BOX>(dst, KEYS ? &tmQ : &tmK, b, first_head + g, row, bar);
+          load_tile<HD, ATT_BOX>(dst + L::PASSING, KEYS ? &tmD : &tmV, b, first_head + g, row, bar);
+          if constexpr (KEYS) {
+            const int64_t from = (static_cast<int64_t>(b) * s.nq + first_head + g) * s.rows + row;
+            bulk_load(stats + st * L::STATS, lse + from, ATT_BOX * 4, bar);
+            bulk_load(stats + st * L::STATS + ATT_BOX * 4, delta + from, ATT_BOX * 4, bar);
+          }
+        }
+      grid_release();
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t idesc_t = make_instr_desc(1, 1, ATT_TILE, ATT_BOX, 0, 0), idesc_a = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
+    bool ok = n > 0 && cta.wait(L::THERE, 0, DEV_ERR_FULL_BAR_TIMEOUT);
+    int ahead = 0;   // the place within its head of the next tile whose scores are computed
+    auto scores = [&](int i) {
+      const int st = i % L::STAGES;
+      if (!(ok = cta.wait(L::FULL + st, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+      const uint32_t src = stages + st * L::STAGE;
+      const int there = len - row_of(ahead);
+      if (++ahead == per_head) ahead = 0;
+      if (there < ATT_BOX && len < s.S) {
+        zero_rows<HD, ATT_BOX>(src, there);
+        zero_rows<HD, ATT_BOX>(src + L::PASSING, there);
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t t1 = cta.tmem + L::T1_COL + (i & 1) * ATT_BOX, t2 = cta.tmem + L::T2_COL + (i & 1) * ATT_BOX;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) umma_f16(t1, desc_rows<ATT_TILE>(held, k), desc_rows<ATT_BOX>(src, k), idesc_t, k != 0);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          umma_f16(t2, desc_rows<ATT_TILE>(held + L::HELD, k), desc_rows<ATT_BOX>(src + L::PASSING, k), idesc_t, k != 0);
+        umma_commit(cta.bar(L::SCORES + (i & 1)));
+      }
+      __syncwarp();
+    };
+    if (ok) scores(0);
+    if (ok && n > 1) scores(1);
+    for (int i = 0; i < n && ok; ++i) {
+      if (!(ok = cta.wait(L::PROBS + (i & 1), i / 2 & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t src = stages + i % L::STAGES * L::STAGE;
+        const uint32_t p = cta.tmem + L::T1_COL + (i & 1) * ATT_BOX, ds = cta.tmem + L::T2_COL + (i & 1) * ATT_BOX;
+        if constexpr (KEYS)
+#pragma unroll
+          for (int k = 0; k < ATT_BOX / 16; ++k)
+            umma_f16_ts(cta.tmem + L::ACC1_COL, p + k * 8, desc_cols<ATT_BOX>(src + L::PASSING, k), idesc_a, i != 0 || k != 0);
+#pragma unroll
+        for (int k = 0; k < ATT_BOX / 16; ++k) umma_f16_ts(cta.tmem + L::ACC2_COL, ds + k * 8, desc_cols<ATT_BOX>(src, k), idesc_a, i != 0 || k != 0);
+        umma_commit(cta.bar(L::EMPTY + i % L::STAGES));
+        if (i + 1 == n) umma_commit(cta.bar(L::DONE));
+      }
+      __syncwarp();
+      if (i + 2 < n) scores(i + 2);
+    }
+  } else if (warp < 8) {
+    // ---------------------------------------------------------------- probabilities: a thread has a row of the held tile
+    const int w = warp >> 2;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int r = r0 + (warp & 3) * 32 + lane;
+    const uint32_t t1 = cta.tmem + lanes + L::T1_COL + w * ATT_BOX, t2 = cta.tmem + lanes + L::T2_COL + w * ATT_BOX;
+    const float c = s.scale * ATT_LOG2E;
+    float my_lse = 0.f, my_delta = 0.f;
+    if constexpr (!KEYS) {
+      const int64_t from = (static_cast<int64_t>(b) * s.nq + head) * s.rows + r;
+      my_lse = lse[from];
+      my_delta = delta[from];
+    }
+    bool ok = true;
+    int at = w, times = 0;
+    for (int i = w; i < n; i += 2, ++times) {
+      while (at >= per_head) at -= per_head;
+      const int c0 = row_of(at);
+      at += 2;
+      const int st = i % L::STAGES;
+      if (!(ok = cta.wait(L::SCORES + w, times & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+      if constexpr (KEYS) {   // lse and delta of the stage
+        if (!(ok = cta.wait(L::FULL + st, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
+      }
+      tc_fence_after();
+      // which columns this row's partner sees, as [first, last] and those beyond a border
+      bool whole;
+      int first, last, sinks = 0;
+      if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
+        whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + ATT_BOX - 1 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
+        first = r - c0;
+        last = s.window == 0 || r < s.sinks ? ATT_BOX : static_cast<int>(min(static_cast<int64_t>(first) + s.window - 1, static_cast<int64_t>(ATT_BOX)));
+      } else {                // columns are keys
+        whole = c0 + ATT_BOX - 1 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + ATT_BOX <= s.sinks);
+        last = r - c0;
+        first = s.window ? last - s.window + 1 : 0;
+        sinks = s.window ? s.sinks - c0 : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t x[32], y[32], p[16], ds[16];
+        tmem_ld_32x32(t1 + k * 32, x);
+        tmem_ld_32x32(t2 + k * 32, y);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float pr[4], dp[4], ls[4], de[4];
+          if constexpr (KEYS) {
+            uint32_t v[4];
+            ld_shared_v4(stats + st * L::STATS + (k * 32 + e) * 4, v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) ls[q] = __uint_as_float(v[q]);
+            ld_shared_v4(stats + st * L::STATS + ATT_BOX * 4 + (k * 32 + e) * 4, v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) de[q] = __uint_as_float(v[q]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) ls[q] = my_lse, de[q] = my_delta;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            pr[q] = exp2_unit(fmaf(__uint_as_float(x[e + q]), c, -ls[q]));
+            dp[q] = pr[q] * (__uint_as_float(y[e + q]) - de[q]);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int col = k * 32 + e + q;
+              const bool sees = col <= last && (col >= first || col < sinks);
+              pr[q] = sees ? pr[q] : 0.f;
+              dp[q] = sees ? dp[q] : 0.f;
+            }
+          }
+          p[e / 2] = pack_bf16x2(pr[0], pr[1]);
+          p[e / 2 + 1] = pack_bf16x2(pr[2], pr[3]);
+          ds[e / 2] = pack_bf16x2(dp[0], dp[1]);
+          ds[e / 2 + 1] = pack_bf16x2(dp[2], dp[3]);
+        }
+        // over columns that this warp has read
+        if constexpr (KEYS) tmem_st_32x16(t1 + k * 16, p);
+        tmem_st_32x16(t2 + k * 16, ds);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(cta.bar(L::PROBS + w));
+    }
+    // ---------------------------------------------------------------- what the sums became
+    if (ok && n > 0) ok = cta.wait(L::DONE, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
+    tc_fence_after();
+    const bool full = ok && n > 0, mine = r < len;
+    // KEYS: the first group of warps has dv, the second dk; dq's columns are halved between them
+    constexpr int COLS = KEYS ? HD : HD / 2;
+    const uint32_t acc = cta.tmem + lanes + (KEYS && w == 0 ? L::ACC1_COL : L::ACC2_COL) + (KEYS ? 0 : w * COLS);
+    const float f = KEYS && w == 0 ? 1.f : s.scale;
+    const int out_heads = KEYS ? s.nkv : s.nq;
+    bf16* row = (KEYS && w == 0 ? grad1 : grad2) + ((static_cast<int64_t>(b) * s.S + r) * out_heads + head) * HD + (KEYS ? 0 : w * COLS);
+    float* sums = nullptr;
+    if (joined) sums = split.sums + (((static_cast<int64_t>(part) * heads * split.tiles + static_cast<int64_t>(tile) * heads + b * s.nkv + head) * 2 + w) * ATT_TILE +
+                                     (r - r0)) * HD;
+#pragma unroll
+    for (int k = 0; k < COLS / 32; ++k) {
+      uint32_t o[32];
+      if (full) {
+        tmem_ld_32x32(acc + k * 32, o);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+      if (joined) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) reinterpret_cast<uint4*>(sums)[k * 8 + e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      } else if (r < s.S) {
+        auto two = [&](int a) { return pack_bf16x2(__uint_as_float(o[a]), __uint_as_float(o[a + 1])); };
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) reinterpret_cast<uint4*>(row)[k * 4 + e / 8] = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
+      }
+    }
+  }
+  attn_end(cta);
+}
+
+// The gradients of tiles whose walk was split: their parts' sums, one after the other.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_join_kernel(AttnSplit split, bf16* dv, bf16* dk, AttnShape s) {
+  grid_wait();
+  grid_release();
+  constexpr int VECS = ATT_TILE * HD / 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, tiles = static_cast<int64_t>(s.B) * s.nkv * split.tiles;
+  if (at >= tiles * 2 * VECS) return;
+  const int64_t which = at / VECS;
+  const int v = static_cast<int>(at % VECS), w = static_cast<int>(which & 1);
+  const int64_t place = which >> 1;
+  const int tile = static_cast<int>(place / (s.B * s.nkv)), bh = static_cast<int>(place % (s.B * s.nkv));
+  const int row = tile * ATT_TILE + v / (HD / 4), col = v % (HD / 4) * 4;
+  if (row >= s.S) return;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* from = reinterpret_cast<const float4*>(split.sums) + at;
+#pragma unroll 4
+  for (int p = 0; p <= split.parts; ++p) {
+    const float4 x = from[p * tiles * 2 * VECS];
+    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  }
+  bf16* to = (w ? dk : dv) + ((static_cast<int64_t>(bh / s.nkv) * s.S + row) * s.nkv + bh % s.nkv) * HD + col;
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+}
+
+// [B][S][heads][HD] with element strides {batch, token, head}, boxes of 64 rows x 64 elements of a head
+static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return B200_ERR_NO_DRIVER;
+  auto pitch = [&](int size, long long stride) { return static_cast<cuuint64_t>(size == 1 ? hd : stride) * 2; };   // of a single one any will do
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(B)};
+  const cuuint64_t strides[3] = {pitch(heads, t.head), pitch(S, t.token), pitch(B, t.batch)};
+  const cuuint32_t box[4] = {64, 1, ATT_BOX, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return 0;
+  fprintf(stderr, "[b200ops] cuTensorMapEncodeTiled failed: %d (base=%p, %d x %d x %d x %d)\n", static_cast<int>(r), t.data, B, S, heads, hd);
+  return B200_ERR_TENSORMAP;
+}
+static bool attn_tensor_ok(const B200AttnTensor& t, int B, int S, int heads) {
+  auto fits = [](int size, long long stride) { return size == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+  return t.data && reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && fits(B, t.batch) && fits(S, t.token) && fits(heads, t.head);
+}
+static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
+  if (a.B < 1 || a.S < 1 || a.nkv < 1 || a.nq < 1 || a.nq % a.nkv || (a.hd != 64 && a.hd != 128) || a.window < 0 || a.sinks < 0 || !(a.scale > 0.f)) return false;
+  if (static_cast<int64_t>(a.S) > (1 << 30)) return false;
+  s.B = a.B, s.S = a.S, s.nq = a.nq, s.nkv = a.nkv, s.G = a.nq / a.nkv;
+  s.rows = (a.S + ATT_TILE - 1) / ATT_TILE * ATT_TILE;
+  // a window that holds every key, or sinks that are, is none
+  s.window = a.window >= a.S || (a.window > 0 && a.sinks >= a.S) ? 0 : a.window;
+  s.sinks = s.window ? a.sinks : 0;
+  s.lengths = a.lengths;
+  s.scale = a.scale;
+  // a CTA for each tile and head
+  return static_cast<int64_t>(s.B) * s.nq * (s.rows / ATT_TILE) < (1ll << 30);
+}
+
+template <int HD>
+static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
+  CUtensorMap q, k, v;
+  if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
+  if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
+  if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
+  if (int rc = allow_smem<attention_fwd_kernel<HD>>(AttnFwd<HD>::SMEM)) return rc;
+  const int units = s.rows / ATT_TILE * s.G;
+  launch_dependent(attention_fwd_kernel<HD>, s.B * s.nkv * ((units + 1) / 2), ATT_THREADS, AttnFwd<HD>::SMEM, stream, q, k, v,
+                   static_cast<bf16*>(a.out), a.lse, s, device_status_word());
+  B200_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+// The walk of a sink's tile is split where there is a window: parts as long as a window's walk, but no more CTAs than some waves.
+static AttnSplit attn_split(const AttnShape& s, float* sums) {
+  AttnSplit p{0, 0, 0, sums};
+  if (s.sinks == 0) return p;
+  const int near = (s.window + 2 * ATT_TILE) / ATT_BOX, all = (s.S + ATT_BOX - 1) / ATT_BOX;
+  if (all <= 2 * near) return p;
+  p.tiles = (s.sinks + ATT_TILE - 1) / ATT_TILE;
+  const int64_t most = std::max<int64_t>(1, 4 * 148 / (static_cast<int64_t>(s.B) * s.nkv * p.tiles));
+  p.parts = static_cast<int>(std::min<int64_t>(most, (all - 1) / near));
+  p.part_tiles = (all + p.parts - 1) / p.parts;
+  return p;
+}
+
+template <int HD>
+static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
+  CUtensorMap q, k, v, d;
+  if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
+  if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
+  if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
+  if (int rc = attn_map(&d, a.dout, s.B, s.S, s.nq, HD)) return rc;
+  auto keys = attention_bwd_kernel<HD, true>;
+  auto queries = attention_bwd_kernel<HD, false>;
+  if (int rc = allow_smem<attention_bwd_kernel<HD, true>>(AttnBwd<HD>::SMEM)) return rc;
+  if (int rc = allow_smem<attention_bwd_kernel<HD, false>>(AttnBwd<HD>::SMEM)) return rc;
+  int* err = device_status_word();
+  const int64_t vecs = static_cast<int64_t>(s.B) * s.rows * s.nq * (HD / 8);
+  auto stride = [](int size, long long x) { return size == 1 ? 0 : x; };
+  launch_dependent(attention_delta_kernel<HD>, static_cast<int>((vecs + 255) / 256), 256, 0, stream, static_cast<const bf16*>(a.dout.data),
+                   stride(s.B, a.dout.batch), stride(s.S, a.dout.token), stride(s.nq, a.dout.head), static_cast<const bf16*>(a.out), a.delta, s);
+  const int tiles = s.rows / ATT_TILE;
+  if (a.dk) {
+    const AttnSplit split = attn_split(s, a.sums);
+    launch_dependent(keys, s.B * s.nkv * (tiles + split.tiles * split.parts), ATT_THREADS, AttnBwd<HD>::SMEM, stream, q, k, v, d, a.lse, a.delta,
+                     static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, err);
+    if (split.parts) {
+      const int64_t n = static_cast<int64_t>(s.B) * s.nkv * split.tiles * 2 * (ATT_TILE * HD / 4);
+      launch_dependent(attention_join_kernel<HD>, static_cast<int>((n + 255) / 256), 256, 0, stream, split, static_cast<bf16*>(a.dv),
+                       static_cast<bf16*>(a.dk), s);
+    }
+  }
+  if (a.dq)
+    launch_dependent(queries, s.B * s.nq * tiles, ATT_THREADS, AttnBwd<HD>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
+                     static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, nullptr}, err);
+  B200_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_attention_fwd(const B200AttnArgs* args, void* stream) {
+  ensure_context();
+  const B200AttnArgs& a = *args;
+  AttnShape s;
+  if (!attn_shape(s, a) || !attn_tensor_ok(a.q, a.B, a.S, a.nq) || !attn_tensor_ok(a.k, a.B, a.S, a.nkv) || !attn_tensor_ok(a.v, a.B, a.S, a.nkv) || !a.out ||
+      reinterpret_cast<uintptr_t>(a.out) % 16 || !a.lse)
+    return B200_ERR_BAD_ARG;
+  return a.hd == 128 ? attn_fwd<128>(a, s, static_cast<cudaStream_t>(stream)) : attn_fwd<64>(a, s, static_cast<cudaStream_t>(stream));
+}
+
+long long b200_attention_bwd_workspace(const B200AttnArgs* args) {
+  AttnShape s;
+  if (!attn_shape(s, *args)) return 0;
+  const AttnSplit p = attn_split(s, nullptr);
+  return p.parts ? static_cast<long long>(1 + p.parts) * s.B * s.nkv * p.tiles * 2 * ATT_TILE * args->hd : 0;
+}
+
+int b200_attention_bwd(const B200AttnArgs* args, int* launches, void* stream) {
+  ensure_context();
+  const B200AttnArgs& a = *args;
+  AttnShape s;
+  if (!attn_shape(s, a) || !attn_tensor_ok(a.q, a.B, a.S, a.nq) || !attn_tensor_ok(a.k, a.B, a.S, a.nkv) || !attn_tensor_ok(a.v, a.B, a.S, a.nkv) ||
+      !attn_tensor_ok(a.dout, a.B, a.S, a.nq) || !a.out || reinterpret_cast<uintptr_t>(a.out) % 16 || !a.lse || reinterpret_cast<uintptr_t>(a.lse) % 16 ||
+      !a.delta || reinterpret_cast<uintptr_t>(a.delta) % 16 || !a.dk != !a.dv || reinterpret_cast<uintptr_t>(a.dq) % 16 ||
+      reinterpret_cast<uintptr_t>(a.dk) % 16 || reinterpret_cast<uintptr_t>(a.dv) % 16)
+    return B200_ERR_BAD_ARG;
+  const AttnSplit p = attn_split(s, nullptr);
+  if (a.dk && p.parts && (!a.sums || reinterpret_cast<uintptr_t>(a.sums) % 16)) return B200_ERR_BAD_ARG;
+  if (launches) *launches = 1 + (a.dk ? 1 + (p.parts > 0) : 0) + (a.dq ? 1 : 0);
+  return a.hd == 128 ? attn_bwd<128>(a, s, static_cast<cudaStream_t>(stream)) : attn_bwd<64>(a, s, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

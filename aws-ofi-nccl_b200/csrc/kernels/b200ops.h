@@ -60,4 +60,24 @@ struct B200AdamwTensor {
 int b200_adamw_many(const B200AdamwTensor* list, int count, int bits, double lr, double beta1, double beta2, double eps, long long step, double grad_scale,
                     int zero_grad, int* launches, void* stream);
 
+// Attention with a window and sinks, and its gradients; see attention.cu. Tensors are [batch][token][head][hd] bf16 with element strides (multiples of
+// eight; any for a dimension of one) and contiguous heads; out, dq, dk and dv are contiguous. lse and delta are [B][nq][S rounded up to 128] floats.
+// dq, or dk and dv together, may be null; sums are b200_attention_bwd_workspace's number of floats.
+struct B200AttnTensor {
+  const void* data;
+  long long batch, token, head;
+};
+struct B200AttnArgs {
+  B200AttnTensor q, k, v, dout;
+  void* out;
+  float *lse, *delta, *sums;
+  void *dq, *dk, *dv;
+  const int* lengths;   // [B] or null
+  int B, S, nq, nkv, hd, window, sinks;
+  float scale;
+};
+int b200_attention_fwd(const B200AttnArgs* args, void* stream);
+long long b200_attention_bwd_workspace(const B200AttnArgs* args);
+int b200_attention_bwd(const B200AttnArgs* args, int* launches, void* stream);
+
 }  // extern "C"

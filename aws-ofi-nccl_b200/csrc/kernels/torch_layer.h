@@ -3,6 +3,9 @@
 #pragma once
 #include <torch/extension.h>
 
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -17,6 +20,7 @@
 namespace b200torch {
 
 namespace py = pybind11;
+using c10::cuda::CUDAGuard;
 using torch::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
@@ -58,6 +62,18 @@ inline Tensor rows16(const Tensor& g) {
 }
 inline void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
+inline void launched(int kernels = 1) { g_launches.fetch_add(kernels, std::memory_order_relaxed); }
+// A new tensor beside `like`, without the dispatcher, which takes as long again as the allocation
+inline Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+inline bool same_device(const Tensor& a, const Tensor& b) { return a.is_cuda() && a.device() == b.device(); }
+// A dual tensor may require no gradient: its tangent would be lost without a word, and what is lost counts as zero.
+inline void refuse_tangents(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs)   // torch has one level of them
+    if (t && t->defined() && t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()) raise(PyExc_RuntimeError, what);
+}
+
 // pybind's exception cannot cross the autograd engine's threads; torch's carrier can.
 template <class F>
 auto on_engine_thread(F f) {
@@ -82,5 +98,7 @@ R traced_or_direct(const char* name, R (*fn)(A...), const Args&... args) {
 
 // The layers of a mixture-of-experts block and its optimizer's step (torch_moe.cpp)
 void bind_moe(py::module_& m);
+// Attention (torch_attention.cpp)
+void bind_attention(py::module_& m);
 
 }  // namespace b200torch

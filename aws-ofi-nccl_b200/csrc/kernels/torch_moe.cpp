@@ -7,29 +7,14 @@
 #include <utility>
 #include <vector>
 
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
-#include <c10/cuda/CUDAGuard.h>
 
 #include "torch_layer.h"
 
 namespace {
 
 using namespace b200torch;
-using c10::cuda::CUDAGuard;
 
-void launched(int kernels = 1) { g_launches.fetch_add(kernels, std::memory_order_relaxed); }
-// A new tensor beside `like`, without the dispatcher, which takes as long again as the allocation
-Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
-  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
-}
-bool same_device(const Tensor& a, const Tensor& b) { return a.is_cuda() && a.device() == b.device(); }
-// A dual tensor may require no gradient: its tangent would be lost without a word, and what is lost counts as zero.
-void refuse_tangents(std::initializer_list<const Tensor*> inputs, const char* what) {
-  for (const Tensor* t : inputs)   // torch has one level of them
-    if (t && t->defined() && t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()) raise(PyExc_RuntimeError, what);
-}
 void refuse_gradients(std::initializer_list<const Tensor*> inputs, const char* what) {
   refuse_tangents(inputs, "8-bit outputs have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return;

@@ -458,5 +458,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         }));
   m.def("cross_entropy", torch::wrap_pybind_function_no_gil(cross_entropy));
   bind_moe(m);
+  bind_attention(m);
   m.def("launches", [] { return g_launches.load(std::memory_order_relaxed); });
 }

@@ -4,7 +4,7 @@
 //   delta = sum(dout * out), dS = P * (dout v^T - delta), dq = scale dS k, dk = scale dS^T q, dv = P^T dout
 //
 // Scores never leave the SM: the forward pass keeps a running maximum and sum of each row, the backward pass computes P again from the
-// rows' log-sum (in base 2), which the forward pass stores.
+// rows' log-sum (in base 2), whose negative the forward pass stores.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -66,7 +66,7 @@ struct AttnFwd {
 template <int HD>
 __global__ void __launch_bounds__(ATT_THREADS, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         bf16* out, float* lse, AttnShape s, int* err_word) {
+                         bf16* out, float* minus_lse, AttnShape s, int* err_word) {
   using L = AttnFwd<HD>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
     const uint32_t s_col = cta.tmem + lanes + L::S_COL + u * ATT_TILE, o_col = cta.tmem + lanes + L::O_COL + u * 128;
     const int i = me.i0 + (warp & 3) * 32 + lane;
     const float c = s.scale * ATT_LOG2E;
+    const Pair c2 = both(c);
     float top = -INFINITY, sum = 0.f;   // of the scores times c; the sum is relative to 2^top
     uint32_t turns = 0;
     bool ok = true;
@@ -188,12 +189,14 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
             if (at > last || (at < first && at >= sinks)) x[k][e] = 0xFF800000u;   // -inf
           }
       }
-      float most = -INFINITY;
+      float some[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) some[e] = __uint_as_float(x[0][e]);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) most = fmaxf(most, __uint_as_float(x[k][e]));
-      most *= c;
+        for (int e = k ? 0 : 8; e < 32; e += 2) some[e / 2 & 7] = fmaxf(fmaxf(some[e / 2 & 7], __uint_as_float(x[k][e])), __uint_as_float(x[k][e + 1]));
+      const float most = fmaxf(fmaxf(fmaxf(some[0], some[1]), fmaxf(some[2], some[3])), fmaxf(fmaxf(some[4], some[5]), fmaxf(some[6], some[7]))) * c;
       // The sums are scaled to a new maximum only where it has grown by more than 2^8: probabilities beside the old one stay in range
       if (__any_sync(0xffffffffu, most > top + 8.f)) {
         const float now = fmaxf(top, most);
@@ -212,21 +215,24 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
           }
         }
       }
-      const float ref = top == -INFINITY ? 0.f : -top;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const Pair ref = both(top == -INFINITY ? 0.f : -top);
+      Pair part[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float p0 = exp2_unit(fmaf(__uint_as_float(x[k][e]), c, ref)), p1 = exp2_unit(fmaf(__uint_as_float(x[k][e + 1]), c, ref));
-          part[e & 2] += p0;
-          part[(e & 2) + 1] += p1;
+          float p0, p1;
+          fma2(pair_of(x[k][e], x[k][e + 1]), c2, ref).to(p0, p1);
+          p0 = exp2_unit(p0), p1 = exp2_unit(p1);
+          part[e / 2 & 3] = part[e / 2 & 3] + Pair(p0, p1);
           p[e / 2] = pack_bf16x2(p0, p1);
         }
         tmem_st_32x16(s_col + k * 16, p);   // over scores that all are in registers
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      float a, d;
+      ((part[0] + part[1]) + (part[2] + part[3])).to(a, d);
+      sum += a + d;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -238,7 +244,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       if (ok && turns) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
       tc_fence_after();
       const bool mine = i < len;
-      lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? top + log2f(sum) : INFINITY;   // no probability behind the end
+      minus_lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;   // no probability behind the end
       const float f = 1.f / sum;
       uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD);
 #pragma unroll
@@ -266,9 +272,9 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
 }
 
 // ------------------------------------------------------------------ backward
-// delta[b][head][i] = sum over a row of dout * out, 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes.
+// minus_delta[b][head][i] = -(sum over a row of dout * out), 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes.
 template <int HD>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, float* delta, AttnShape s) {
+__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, float* minus_delta, AttnShape s) {
   grid_wait();
   grid_release();
   constexpr int LANES = HD / 8;
@@ -291,27 +297,33 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, 
   }
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (there && v == 0) delta[(static_cast<int64_t>(b) * s.nq + h) * s.rows + i] = sum;
+  if (there && v == 0) minus_delta[(static_cast<int64_t>(b) * s.nq + h) * s.rows + i] = -sum;
 }
 
-// Both gradient kernels hold a tile of 128 rows and walk over tiles of 64 rows of the other side:
+// Both gradient kernels hold a tile of 128 rows and walk over tiles of 128 rows of the other side:
 //   KEYS (dk, dv): a tile of k and v; q, dout, lse and delta pass by, over the heads of the group, whose sum is the gradient
 //   else (dq):     a tile of q and dout; k and v pass by
-// First T1 = held1 passing1^T (scores) and T2 = held2 passing2^T (dout v^T), a thread's row of each; then P and dS as bf16 in their place, the first
-// operands of dv += P dout, dk += dS q or dq += dS k. Two groups of warps take every second tile, so that the products of one run while the other's
-// probabilities are computed. Every sum is made in one order: gradients are the same bits in every run.
-template <int HD>
+// First T1 = held1 passing1^T (scores) and T2 = held2 passing2^T (dout v^T), then P and dS as bf16 operands in tensor memory of
+// dv += P dout, dk += dS q or dq += dS k. Two groups of warps have 64 columns each, a thread a row of them. Products and probabilities of neighbouring tiles
+// overlap: with KEYS tensor memory is full with T1, T2 and two sums, P lies over T1 and dS over T2; dv's product and the next scores run while dS is
+// computed, dk's and the next T2 while the next probabilities are. dq leaves room for two tiles' scores, and dS lies over those. Every sum is made
+// in one order: gradients are the same bits in every run.
+template <int HD, bool KEYS>
 struct AttnBwd {
-  static constexpr int HELD = ATT_TILE * HD * 2, PASSING = ATT_BOX * HD * 2;
-  static constexpr int STAGE = 2 * PASSING;
-  static constexpr int STAGES = 4;
-  static constexpr int STATS = 2 * ATT_BOX * 4;   // lse and delta of a stage's rows
-  static constexpr int TILES = 2 * HELD + STAGES * (STAGE + STATS);
+  static constexpr int TILE = ATT_TILE * HD * 2;
+  static constexpr int N1 = HD == 64 || !KEYS ? 3 : 2, N2 = 2;   // stages of the passing tensors
+  static constexpr int STATS = 2 * ATT_TILE * 4;                 // lse and delta of a stage's rows
+  static constexpr int PASS1 = 2 * TILE, PASS2 = PASS1 + N1 * TILE, STAT = PASS2 + N2 * TILE;
+  static constexpr int TILES = STAT + (KEYS ? N1 * STATS : 0);
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
-  static constexpr int FULL = 0, EMPTY = STAGES, THERE = 2 * STAGES, SCORES = THERE + 1, PROBS = SCORES + 2, DONE = PROBS + 2, BARS = DONE + 1;
-  static constexpr int T1_COL = 0, T2_COL = 128, ACC1_COL = 256, ACC2_COL = 384;
+  static_assert(SMEM <= 232448, "more than a CTA's shared memory");
+  static constexpr int FULL1 = 0, EMPTY1 = FULL1 + N1, FULL2 = EMPTY1 + N1, EMPTY2 = FULL2 + N2, THERE = EMPTY2 + N2;
+  static constexpr int T1 = THERE + 1, T2 = T1 + (KEYS ? 1 : 2), DONE = T2 + 1;            // T1 and T2 there, sums done
+  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1, BARS = GRADS + 1;  // P and dS there: by eight warps
+  // tensor memory: scores (dq: of two tiles), dout v^T, sums
+  static constexpr int T1_COL = 0, T2_COL = KEYS ? 128 : 256, ACC1_COL = 256, ACC2_COL = 384;
 };
-// How the walk of dk and dv over queries that see a tile only through sinks is split: `parts` CTAs take `part_tiles` tiles of 64 queries each, of every
+// How the walk of dk and dv over queries that see a tile only through sinks is split: `parts` CTAs take `part_tiles` tiles of queries each, of every
 // head, and their sums and those of the tile's own window are joined in order. parts 0: no tile has any.
 struct AttnSplit {
   int tiles, parts, part_tiles;
@@ -321,11 +333,11 @@ struct AttnSplit {
 template <int HD, bool KEYS>
 __global__ void __launch_bounds__(ATT_THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         const __grid_constant__ CUtensorMap tmD, const float* lse, const float* delta, bf16* grad1, bf16* grad2, AttnShape s,
+                         const __grid_constant__ CUtensorMap tmD, const float* minus_lse, const float* minus_delta, bf16* grad1, bf16* grad2, AttnShape s,
                          AttnSplit split, int* err_word) {
-  using L = AttnBwd<HD>;
+  using L = AttnBwd<HD, KEYS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
+  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::READ ? 8 : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -349,12 +361,12 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
   const bool joined = KEYS && split.parts > 0 && tile < split.tiles;
   if constexpr (KEYS) {
     // queries of the window: up to the last key's; of the far parts: behind those
-    const int end = (len + ATT_BOX - 1) / ATT_BOX;
-    const int near = s.window ? static_cast<int>(min(static_cast<int64_t>(end), (static_cast<int64_t>(r0) + ATT_TILE - 1 + s.window - 1) / ATT_BOX + 1)) : end;
-    lo = r0 / ATT_BOX;
+    const int end = (len + ATT_TILE - 1) / ATT_TILE;
+    const int near = s.window ? min(end, (r0 + ATT_TILE - 1 + s.window - 1) / ATT_TILE + 1) : end;
+    lo = tile;
     int hi = near;
     if (part) {
-      lo = static_cast<int>(min(static_cast<int64_t>(near) + static_cast<int64_t>(part - 1) * split.part_tiles, static_cast<int64_t>(end)));
+      lo = min(near + (part - 1) * split.part_tiles, end);
       hi = min(lo + split.part_tiles, end);
     } else if (s.window && !joined && r0 < s.sinks) {
       hi = end;   // sinks whose walk is not split
@@ -362,172 +374,206 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
     per_head = r0 < len ? max(0, hi - lo) : 0;
   } else {
     const int last = min(r0 + ATT_TILE, len) - 1;
-    lo = s.window ? max(0, r0 - s.window + 1) / ATT_BOX : 0;
-    far = s.window ? min((s.sinks + ATT_BOX - 1) / ATT_BOX, lo) : 0;
-    per_head = r0 < len ? far + last / ATT_BOX - lo + 1 : 0;
+    lo = s.window ? max(0, r0 - s.window + 1) / ATT_TILE : 0;
+    far = s.window ? min((s.sinks + ATT_TILE - 1) / ATT_TILE, lo) : 0;
+    per_head = r0 < len ? far + last / ATT_TILE - lo + 1 : 0;
   }
   const int group = KEYS ? s.G : 1, n = group * per_head;
   const int first_head = KEYS ? head * s.G : head / s.G;   // of the passing tensors
-  const uint32_t held = cta.smem, stages = cta.smem + 2 * L::HELD, stats = stages + L::STAGES * L::STAGE;
-  auto row_of = [&](int at) { return (at < far ? at : lo + at - far) * ATT_BOX; };   // the first row of a head's at-th tile
+  auto row_of = [&](int at) { return (at < far ? at : lo + at - far) * ATT_TILE; };   // the first row of a head's at-th tile
+  auto pass1 = [&](int i) { return cta.smem + L::PASS1 + i % L::N1 * L::TILE; };
+  auto pass2 = [&](int i) { return cta.smem + L::PASS2 + i % L::N2 * L::TILE; };
+  auto stats = [&](int i) { return cta.smem + L::STAT + i % L::N1 * L::STATS; };
 
   if (warp == 8) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync() && n > 0) {
-      mbar_expect_tx(cta.bar(L::THERE), 2 * L::HELD);
-      load_tile<HD, ATT_TILE>(held, KEYS ? &tmK : &tmQ, b, head, r0, cta.bar(L::THERE));
-      load_tile<HD, ATT_TILE>(held + L::HELD, KEYS ? &tmV : &tmD, b, head, r0, cta.bar(L::THERE));
+      mbar_expect_tx(cta.bar(L::THERE), 2 * L::TILE);
+      load_tile<HD, ATT_TILE>(cta.smem, KEYS ? &tmK : &tmQ, b, head, r0, cta.bar(L::THERE));
+      load_tile<HD, ATT_TILE>(cta.smem + L::TILE, KEYS ? &tmV : &tmD, b, head, r0, cta.bar(L::THERE));
       int i = 0;
       bool ok = true;
       for (int g = 0; g < group && ok; ++g)
         for (int at = 0; at < per_head; ++at, ++i) {
-          const int st = i % L::STAGES, row = row_of(at);
-          if (!(ok = cta.wait(L::EMPTY + st, (i / L::STAGES & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
-          const uint32_t dst = stages + st * L::STAGE, bar = cta.bar(L::FULL + st);
-          mbar_expect_tx(bar, L::STAGE + (KEYS ? L::STATS : 0));
-          load_tile<HD, ATT_BOX>(dst, KEYS ? &tmQ : &tmK, b, first_head + g, row, bar);
-          load_tile<HD, ATT_BOX>(dst + L::PASSING, KEYS ? &tmD : &tmV, b, first_head + g, row, bar);
+          const int row = row_of(at);
+          const uint32_t full1 = cta.bar(L::FULL1 + i % L::N1), full2 = cta.bar(L::FULL2 + i % L::N2);
+          if (!(ok = cta.wait(L::EMPTY1 + i % L::N1, (i / L::N1 & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
+          mbar_expect_tx(full1, L::TILE + (KEYS ? L::STATS : 0));
+          load_tile<HD, ATT_TILE>(pass1(i), KEYS ? &tmQ : &tmK, b, first_head + g, row, full1);
           if constexpr (KEYS) {
             const int64_t from = (static_cast<int64_t>(b) * s.nq + first_head + g) * s.rows + row;
-            bulk_load(stats + st * L::STATS, lse + from, ATT_BOX * 4, bar);
-            bulk_load(stats + st * L::STATS + ATT_BOX * 4, delta + from, ATT_BOX * 4, bar);
+            bulk_load(stats(i), minus_lse + from, ATT_TILE * 4, full1);
+            bulk_load(stats(i) + ATT_TILE * 4, minus_delta + from, ATT_TILE * 4, full1);
           }
+          if (!(ok = cta.wait(L::EMPTY2 + i % L::N2, (i / L::N2 & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
+          mbar_expect_tx(full2, L::TILE);
+          load_tile<HD, ATT_TILE>(pass2(i), KEYS ? &tmD : &tmV, b, first_head + g, row, full2);
         }
       grid_release();
     }
   } else if (warp == 9) {
-    // ---------------------------------------------------------------- products
-    constexpr uint32_t idesc_t = make_instr_desc(1, 1, ATT_TILE, ATT_BOX, 0, 0), idesc_a = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
+    // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue
+    constexpr uint32_t idesc_t = make_instr_desc(1, 1, ATT_TILE, ATT_TILE, 0, 0), idesc_a = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
     bool ok = n > 0 && cta.wait(L::THERE, 0, DEV_ERR_FULL_BAR_TIMEOUT);
-    int ahead = 0;   // the place within its head of the next tile whose scores are computed
-    auto scores = [&](int i) {
-      const int st = i % L::STAGES;
-      if (!(ok = cta.wait(L::FULL + st, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
-      const uint32_t src = stages + st * L::STAGE;
-      const int there = len - row_of(ahead);
-      if (++ahead == per_head) ahead = 0;
-      if (there < ATT_BOX && len < s.S) {
-        zero_rows<HD, ATT_BOX>(src, there);
-        zero_rows<HD, ATT_BOX>(src + L::PASSING, there);
-      }
+    // how many rows of the i-th tile a sequence has, counted along with the tiles of each kind
+    int at1 = 0, at2 = 0;
+    auto zero_behind = [&](uint32_t tile_at, int& at) {
+      const int there = len - row_of(at);
+      if (++at == per_head) at = 0;
+      if (there < ATT_TILE && len < s.S) zero_rows<HD, ATT_TILE>(tile_at, there);
+    };
+    auto t1 = [&](int i) {
+      if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+      zero_behind(pass1(i), at1);
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t t1 = cta.tmem + L::T1_COL + (i & 1) * ATT_BOX, t2 = cta.tmem + L::T2_COL + (i & 1) * ATT_BOX;
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) umma_f16(t1, desc_rows<ATT_TILE>(held, k), desc_rows<ATT_BOX>(src, k), idesc_t, k != 0);
+        const int two = KEYS ? 0 : i & 1;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          umma_f16(t2, desc_rows<ATT_TILE>(held + L::HELD, k), desc_rows<ATT_BOX>(src + L::PASSING, k), idesc_t, k != 0);
-        umma_commit(cta.bar(L::SCORES + (i & 1)));
+          umma_f16(cta.tmem + L::T1_COL + two * 128, desc_rows<ATT_TILE>(cta.smem, k), desc_rows<ATT_TILE>(pass1(i), k), idesc_t, k != 0);
+        umma_commit(cta.bar(L::T1 + two));
       }
       __syncwarp();
     };
-    if (ok) scores(0);
-    if (ok && n > 1) scores(1);
-    for (int i = 0; i < n && ok; ++i) {
-      if (!(ok = cta.wait(L::PROBS + (i & 1), i / 2 & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+    auto t2 = [&](int i) {
+      if (!(ok = cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+      zero_behind(pass2(i), at2);
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t src = stages + i % L::STAGES * L::STAGE;
-        const uint32_t p = cta.tmem + L::T1_COL + (i & 1) * ATT_BOX, ds = cta.tmem + L::T2_COL + (i & 1) * ATT_BOX;
-        if constexpr (KEYS)
 #pragma unroll
-          for (int k = 0; k < ATT_BOX / 16; ++k)
-            umma_f16_ts(cta.tmem + L::ACC1_COL, p + k * 8, desc_cols<ATT_BOX>(src + L::PASSING, k), idesc_a, i != 0 || k != 0);
-#pragma unroll
-        for (int k = 0; k < ATT_BOX / 16; ++k) umma_f16_ts(cta.tmem + L::ACC2_COL, ds + k * 8, desc_cols<ATT_BOX>(src, k), idesc_a, i != 0 || k != 0);
-        umma_commit(cta.bar(L::EMPTY + i % L::STAGES));
-        if (i + 1 == n) umma_commit(cta.bar(L::DONE));
+        for (int k = 0; k < HD / 16; ++k)
+          umma_f16(cta.tmem + L::T2_COL, desc_rows<ATT_TILE>(cta.smem + L::TILE, k), desc_rows<ATT_TILE>(pass2(i), k), idesc_t, k != 0);
+        umma_commit(cta.bar(L::T2));
+        if constexpr (!KEYS) umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
       }
       __syncwarp();
-      if (i + 2 < n) scores(i + 2);
+    };
+    // sum += operand tile; the operand of each group's 64 columns lies over those columns
+    auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, int i, int freed) {
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < ATT_TILE / 16; ++k)
+          umma_f16_ts(cta.tmem + acc, cta.tmem + operand + (k >> 2) * 64 + (k & 3) * 8, desc_cols<ATT_TILE>(tile_at, k), idesc_a, i != 0 || k != 0);
+        umma_commit(cta.bar(freed));
+      }
+      __syncwarp();
+    };
+    if (ok) t1(0);
+    if (ok) t2(0);
+    if (!KEYS && ok && n > 1) t1(1);
+    for (int i = 0; i < n && ok; ++i) {
+      if constexpr (KEYS) {
+        if (!(ok = cta.wait(L::PROBS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+        tc_fence_after();
+        add(L::ACC1_COL, L::T1_COL, pass2(i), i, L::EMPTY2 + i % L::N2);
+        if (i + 1 < n) t1(i + 1);
+      }
+      if (!ok || !(ok = cta.wait(L::GRADS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+      tc_fence_after();
+      if (!KEYS && i + 1 < n) t2(i + 1);
+      if (!ok) break;
+      add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), i, L::EMPTY1 + i % L::N1);
+      if (KEYS && i + 1 < n) t2(i + 1);
+      if (!KEYS && i + 2 < n) t1(i + 2);
     }
+    if (ok && lane == 0) umma_commit(cta.bar(L::DONE));
   } else if (warp < 8) {
-    // ---------------------------------------------------------------- probabilities: a thread has a row of the held tile
+    // ---------------------------------------------------------------- probabilities: a thread has 64 columns of a row of the held tile
     const int w = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int r = r0 + (warp & 3) * 32 + lane;
-    const uint32_t t1 = cta.tmem + lanes + L::T1_COL + w * ATT_BOX, t2 = cta.tmem + lanes + L::T2_COL + w * ATT_BOX;
-    const float c = s.scale * ATT_LOG2E;
-    float my_lse = 0.f, my_delta = 0.f;
+    const Pair c = both(s.scale * ATT_LOG2E);
+    Pair my_lse, my_delta;
     if constexpr (!KEYS) {
       const int64_t from = (static_cast<int64_t>(b) * s.nq + head) * s.rows + r;
-      my_lse = lse[from];
-      my_delta = delta[from];
+      my_lse = both(minus_lse[from]);
+      my_delta = both(minus_delta[from]);
     }
     bool ok = true;
-    int at = w, times = 0;
-    for (int i = w; i < n; i += 2, ++times) {
-      while (at >= per_head) at -= per_head;
-      const int c0 = row_of(at);
-      at += 2;
-      const int st = i % L::STAGES;
-      if (!(ok = cta.wait(L::SCORES + w, times & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+    int at = 0;
+    for (int i = 0; i < n; ++i) {
+      const int c0 = row_of(at) + w * 64;
+      if (++at == per_head) at = 0;
+      const uint32_t t1 = cta.tmem + lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 64, t2 = cta.tmem + lanes + L::T2_COL + w * 64;
       if constexpr (KEYS) {   // lse and delta of the stage
-        if (!(ok = cta.wait(L::FULL + st, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
+        if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
       }
+      if (!(ok = cta.wait(KEYS ? L::T1 : L::T1 + (i & 1), KEYS ? i & 1 : i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
       tc_fence_after();
-      // which columns this row's partner sees, as [first, last] and those beyond a border
+      // which columns this row's partner sees: those from first to last, and those in front of `sinks`
       bool whole;
       int first, last, sinks = 0;
       if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
-        whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + ATT_BOX - 1 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
+        whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + 63 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
         first = r - c0;
-        last = s.window == 0 || r < s.sinks ? ATT_BOX : static_cast<int>(min(static_cast<int64_t>(first) + s.window - 1, static_cast<int64_t>(ATT_BOX)));
+        last = s.window == 0 || r < s.sinks ? 64 : first + s.window - 1;
       } else {                // columns are keys
-        whole = c0 + ATT_BOX - 1 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + ATT_BOX <= s.sinks);
+        whole = c0 + 63 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + 64 <= s.sinks);
         last = r - c0;
         first = s.window ? last - s.window + 1 : 0;
         sinks = s.window ? s.sinks - c0 : 0;
       }
+      const uint32_t stat = stats(i) + w * 256;
+      uint32_t p[64];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        uint32_t x[32], y[32], p[16], ds[16];
+        uint32_t(&x)[32] = reinterpret_cast<uint32_t(&)[32]>(p[k * 32]);
         tmem_ld_32x32(t1 + k * 32, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          Pair l0 = my_lse, l1 = my_lse;
+          if constexpr (KEYS) ld_shared_pairs(stat + (k * 32 + e) * 4, l0, l1);
+          float a, d;
+          fma2(pair_of(x[e], x[e + 1]), c, l0).to(a, d);
+          x[e] = __float_as_uint(exp2_unit(a)), x[e + 1] = __float_as_uint(exp2_unit(d));
+          fma2(pair_of(x[e + 2], x[e + 3]), c, l1).to(a, d);
+          x[e + 2] = __float_as_uint(exp2_unit(a)), x[e + 3] = __float_as_uint(exp2_unit(d));
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int col = k * 32 + e;
+            if (col > last || (col < first && col >= sinks)) x[e] = 0;
+          }
+        }
+        if constexpr (KEYS) {
+          uint32_t o[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+          tmem_st_32x16(t1 + k * 16, o);   // over columns that this warp has read
+        }
+      }
+      auto arrive = [&](int barrier) {
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(cta.bar(barrier));
+      };
+      if constexpr (KEYS) arrive(L::PROBS);
+      if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t y[32], o[16];
         tmem_ld_32x32(t2 + k * 32, y);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          float pr[4], dp[4], ls[4], de[4];
-          if constexpr (KEYS) {
-            uint32_t v[4];
-            ld_shared_v4(stats + st * L::STATS + (k * 32 + e) * 4, v);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) ls[q] = __uint_as_float(v[q]);
-            ld_shared_v4(stats + st * L::STATS + ATT_BOX * 4 + (k * 32 + e) * 4, v);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) de[q] = __uint_as_float(v[q]);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) ls[q] = my_lse, de[q] = my_delta;
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            pr[q] = exp2_unit(fmaf(__uint_as_float(x[e + q]), c, -ls[q]));
-            dp[q] = pr[q] * (__uint_as_float(y[e + q]) - de[q]);
-          }
-          if (!whole) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int col = k * 32 + e + q;
-              const bool sees = col <= last && (col >= first || col < sinks);
-              pr[q] = sees ? pr[q] : 0.f;
-              dp[q] = sees ? dp[q] : 0.f;
-            }
-          }
-          p[e / 2] = pack_bf16x2(pr[0], pr[1]);
-          p[e / 2 + 1] = pack_bf16x2(pr[2], pr[3]);
-          ds[e / 2] = pack_bf16x2(dp[0], dp[1]);
-          ds[e / 2 + 1] = pack_bf16x2(dp[2], dp[3]);
+          Pair d0 = my_delta, d1 = my_delta;
+          if constexpr (KEYS) ld_shared_pairs(stat + ATT_TILE * 4 + (k * 32 + e) * 4, d0, d1);
+          float a, d;
+          const int at_p = k * 32 + e;
+          (pair_of(p[at_p], p[at_p + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
+          if (!whole) a = p[at_p] ? a : 0.f, d = p[at_p + 1] ? d : 0.f;   // zero times what is not finite
+          o[e / 2] = pack_bf16x2(a, d);
+          (pair_of(p[at_p + 2], p[at_p + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
+          if (!whole) a = p[at_p + 2] ? a : 0.f, d = p[at_p + 3] ? d : 0.f;
+          o[e / 2 + 1] = pack_bf16x2(a, d);
         }
-        // over columns that this warp has read
-        if constexpr (KEYS) tmem_st_32x16(t1 + k * 16, p);
-        tmem_st_32x16(t2 + k * 16, ds);
+        tmem_st_32x16((KEYS ? t2 : t1) + k * 16, o);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(cta.bar(L::PROBS + w));
+      arrive(L::GRADS);
     }
     // ---------------------------------------------------------------- what the sums became
     if (ok && n > 0) ok = cta.wait(L::DONE, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
@@ -639,7 +685,7 @@ static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
 static AttnSplit attn_split(const AttnShape& s, float* sums) {
   AttnSplit p{0, 0, 0, sums};
   if (s.sinks == 0) return p;
-  const int near = (s.window + 2 * ATT_TILE) / ATT_BOX, all = (s.S + ATT_BOX - 1) / ATT_BOX;
+  const int near = s.window / ATT_TILE + 2, all = s.rows / ATT_TILE;
   if (all <= 2 * near) return p;
   p.tiles = (s.sinks + ATT_TILE - 1) / ATT_TILE;
   const int64_t most = std::max<int64_t>(1, 4 * 148 / (static_cast<int64_t>(s.B) * s.nkv * p.tiles));
@@ -657,8 +703,8 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (int rc = attn_map(&d, a.dout, s.B, s.S, s.nq, HD)) return rc;
   auto keys = attention_bwd_kernel<HD, true>;
   auto queries = attention_bwd_kernel<HD, false>;
-  if (int rc = allow_smem<attention_bwd_kernel<HD, true>>(AttnBwd<HD>::SMEM)) return rc;
-  if (int rc = allow_smem<attention_bwd_kernel<HD, false>>(AttnBwd<HD>::SMEM)) return rc;
+  if (int rc = allow_smem<attention_bwd_kernel<HD, true>>(AttnBwd<HD, true>::SMEM)) return rc;
+  if (int rc = allow_smem<attention_bwd_kernel<HD, false>>(AttnBwd<HD, false>::SMEM)) return rc;
   int* err = device_status_word();
   const int64_t vecs = static_cast<int64_t>(s.B) * s.rows * s.nq * (HD / 8);
   auto stride = [](int size, long long x) { return size == 1 ? 0 : x; };
@@ -667,7 +713,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   const int tiles = s.rows / ATT_TILE;
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
-    launch_dependent(keys, s.B * s.nkv * (tiles + split.tiles * split.parts), ATT_THREADS, AttnBwd<HD>::SMEM, stream, q, k, v, d, a.lse, a.delta,
+    launch_dependent(keys, s.B * s.nkv * (tiles + split.tiles * split.parts), ATT_THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, a.lse, a.delta,
                      static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, err);
     if (split.parts) {
       const int64_t n = static_cast<int64_t>(s.B) * s.nkv * split.tiles * 2 * (ATT_TILE * HD / 4);
@@ -676,7 +722,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
     }
   }
   if (a.dq)
-    launch_dependent(queries, s.B * s.nq * tiles, ATT_THREADS, AttnBwd<HD>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
+    launch_dependent(queries, s.B * s.nq * tiles, ATT_THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
                      static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, nullptr}, err);
   B200_CUDA_OK(cudaGetLastError());
   return 0;

@@ -5,6 +5,7 @@
 // and rows behind them are zeros, in the output and in the gradients. Since j <= i, a query in front of the length sees no key behind it.
 #pragma once
 #include "gemm_tcgen05.cuh"
+#include "pair_math.cuh"
 
 namespace b200 {
 
@@ -94,6 +95,11 @@ __device__ __forceinline__ float exp2_unit(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ Pair pair_of(uint32_t a, uint32_t b) { return Pair(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ void ld_shared_pairs(uint32_t addr, Pair& a, Pair& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a.bits), "=l"(b.bits) : "r"(addr) : "memory");
 }
 
 // What all roles of a CTA share: its tensor memory, barriers and the flag that one of its waits has given up.

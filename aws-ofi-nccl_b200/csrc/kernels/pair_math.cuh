@@ -17,6 +17,11 @@ __device__ __forceinline__ Pair operator*(Pair a, Pair b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
   return r;
 }
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
 __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   Pair r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));

@@ -55,11 +55,12 @@ template <int HD>
 struct AttnFwd {
   static constexpr int TILE = ATT_TILE * HD * 2;
   static constexpr int STAGES = 4;
-  static constexpr int TILES = (2 + STAGES) * TILE;
+  static constexpr int ROWS = (2 + STAGES) * TILE;           // a number for each row of each half of a unit's columns
+  static constexpr int TILES = ROWS + 4 * ATT_TILE * 4;
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
   // barriers: stages full and empty; q there; scores there, probabilities there (or their row scaled), sums of a unit done
-  static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, SCORES = Q + 2, PROBS = SCORES + 2, DONE = PROBS + 2, BARS = DONE + 2;
-  // tensor memory: scores of a unit (probabilities as bf16 over their first half), its sums
+  static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, SCORES = Q + 2, PROBS = SCORES + 2, DONE = PROBS + 4, CLEAR = DONE + 2, CLEARED = CLEAR + 1, BARS = CLEARED + 1;
+  // tensor memory: scores of a unit (probabilities as bf16 over each half's first columns), its sums
   static constexpr int S_COL = 0, O_COL = 256;
 };
 
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
                          bf16* out, float* minus_lse, AttnShape s, int* err_word) {
   using L = AttnFwd<HD>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
+  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 8 : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the longest walks first
@@ -81,8 +82,10 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
   if (2 * pair + 1 >= units) unit[1].live = false, unit[1].hi = -1;
   const AttnWalk walk = attn_walk(s, unit[0], unit[1]);
   const uint32_t q_tile = cta.smem, stages = cta.smem + 2 * L::TILE;
+  // from which row on the last tile is not the sequence's: what TMA does not fill with zeros by itself
+  const int clear_from = walk.n > 0 && len < s.S ? len - walk.tile(walk.n - 1) * ATT_TILE : ATT_TILE;
 
-  if (warp == 8) {
+  if (warp == ATT_LOAD) {
     // ---------------------------------------------------------------- loads: q, then k and v in turn
     if (elect_one_sync()) {
       for (int u = 0; u < 2; ++u)
@@ -98,91 +101,98 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       }
       grid_release();
     }
-  } else if (warp == 9) {
+  } else if (warp == ATT_MMA) {
     // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue: probabilities
     // are read before the next scores of their unit are written over them
-    constexpr uint32_t idesc_s = make_instr_desc(1, 1, ATT_TILE, ATT_TILE, 0, 0), idesc_o = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
-    auto full = [&](int i) { return cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
-    auto scores = [&](int u, int i) {
-      if (lane == 0) {
-        const uint32_t k_tile = stages + i % L::STAGES * L::TILE;
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          umma_f16(cta.tmem + L::S_COL + u * ATT_TILE, desc_rows<ATT_TILE>(q_tile + u * L::TILE, k), desc_rows<ATT_TILE>(k_tile, k), idesc_s, k != 0);
+    if (elect_one_sync()) {
+      auto full = [&](int i) { return cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
+      auto scores = [&](int u, int i) {
+        multiply_rows<HD>(L::S_COL + u * ATT_TILE, q_tile + u * L::TILE, stages + i % L::STAGES * L::TILE);
         umma_commit(cta.bar(L::SCORES + u));
-      }
-      __syncwarp();
-    };
-    auto release = [&](int i) {
-      if (lane == 0) umma_commit(cta.bar(L::EMPTY + i % L::STAGES));
-      __syncwarp();
-    };
-    bool ok = walk.n > 0;
-    uint32_t turns[2] = {0, 0};   // tiles that a unit has taken
-    if (ok && (ok = full(0))) {
-      for (int u = 0; u < 2 && ok; ++u)
-        if (unit[u].live) {
-          ok = cta.wait(L::Q + u, 0, DEV_ERR_FULL_BAR_TIMEOUT);
-          tc_fence_after();
-          if (ok && walk.uses(unit[u], walk.tile(0))) scores(u, 0);
-        }
-      release(0);
-    }
-    for (int j = 0; j < walk.n && ok; ++j) {
-      const int t = walk.tile(j), next = walk.tile(j + 1);
-      const bool more = j + 1 < walk.n;
-      if (!(ok = full(2 * j + 1) && (!more || full(2 * j + 2)))) break;
-      const uint32_t v_tile = stages + (2 * j + 1) % L::STAGES * L::TILE;
-      const int there = len - t * ATT_TILE;
-      if (there < ATT_TILE && len < s.S) zero_rows<HD, ATT_TILE>(v_tile, there);
-      for (int u = 0; u < 2; ++u) {
-        if (walk.uses(unit[u], t)) {
-          if (!(ok = cta.wait(L::PROBS + u, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
-          tc_fence_after();
-          if (lane == 0) {
-#pragma unroll
-            for (int k = 0; k < ATT_TILE / 16; ++k)
-              umma_f16_ts(cta.tmem + L::O_COL + u * 128, cta.tmem + L::S_COL + u * ATT_TILE + k * 8, desc_cols<ATT_TILE>(v_tile, k), idesc_o,
-                          turns[u] != 0 || k != 0);
+      };
+      bool ok = walk.n > 0 && full(0);
+      bool first[2] = {true, true};   // a unit's sums are not begun
+      uint32_t turns[2] = {0, 0};     // tiles that a unit has taken
+      if (ok) {
+        for (int u = 0; u < 2 && ok; ++u)
+          if (unit[u].live) {
+            ok = cta.wait(L::Q + u, 0, DEV_ERR_FULL_BAR_TIMEOUT);
+            tc_fence_after();
+            if (ok && walk.uses(unit[u], walk.tile(0))) scores(u, 0);
           }
-          __syncwarp();
-          ++turns[u];
-        }
-        if (more && walk.uses(unit[u], next)) scores(u, 2 * j + 2);
-        if (j + 1 == walk.n && lane == 0) umma_commit(cta.bar(L::DONE + u));
+        umma_commit(cta.bar(L::EMPTY));
       }
-      if (!ok) break;
-      release(2 * j + 1);
-      if (more) release(2 * j + 2);
+      for (int j = 0; j < walk.n && ok; ++j) {
+        const int t = walk.tile(j), next = walk.tile(j + 1);
+        const bool more = j + 1 < walk.n;
+        if (!(ok = full(2 * j + 1) && (!more || full(2 * j + 2)))) break;
+        if (!more && clear_from < ATT_TILE) {
+          mbar_arrive(cta.bar(L::CLEAR));
+          if (!(ok = cta.wait(L::CLEARED, 0, DEV_ERR_FULL_BAR_TIMEOUT))) break;
+        }
+        const uint32_t v_low = TileDesc<ATT_TILE, true>::low(stages + (2 * j + 1) % L::STAGES * L::TILE);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (walk.uses(unit[u], t)) {
+            // in two parts, each of 32 columns of both halves, as they are there
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+              tc_fence_after();
+              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2, part || !first[u]);
+              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 1, true);
+              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 4, true);
+              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 5, true);
+            }
+            if (!ok) break;
+            first[u] = false;
+            ++turns[u];
+          }
+          if (more && walk.uses(unit[u], next)) scores(u, 2 * j + 2);
+          if (!more) umma_commit(cta.bar(L::DONE + u));
+        }
+        if (!ok) break;
+        umma_commit(cta.bar(L::EMPTY + (2 * j + 1) % L::STAGES));
+        if (more) umma_commit(cta.bar(L::EMPTY + (2 * j + 2) % L::STAGES));
+      }
     }
-  } else if (warp < 8) {
-    // ---------------------------------------------------------------- softmax: a thread has a row
-    const int u = warp >> 2;
+  } else if (warp == ATT_ZERO) {
+    // ---------------------------------------------------------------- v behind the sequence's end, in the last tile of the walk
+    const int i = 2 * walk.n - 1;
+    if (clear_from < ATT_TILE && cta.wait(L::CLEAR, 0, DEV_ERR_FULL_BAR_TIMEOUT) && cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))
+      zero_rows<HD, ATT_TILE>(stages + i % L::STAGES * L::TILE, clear_from, cta.bar(L::CLEARED));
+  } else {
+    // ---------------------------------------------------------------- softmax: a thread has half of a row
+    const int u = warp >> 3, half = warp >> 2 & 1, place = (warp & 3) * 32 + lane;
     const AttnUnit& me = unit[u];
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_col = cta.tmem + lanes + L::S_COL + u * ATT_TILE, o_col = cta.tmem + lanes + L::O_COL + u * 128;
-    const int i = me.i0 + (warp & 3) * 32 + lane;
+    const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE + half * 64;
+    const uint32_t o_col = lanes + L::O_COL + u * 128 + half * (HD / 2);
+    // a row's two threads tell each other numbers here
+    volatile float* const told = reinterpret_cast<volatile float*>(smem_raw + (cta.smem - smem_u32(smem_raw)) + L::ROWS) + u * 2 * ATT_TILE + place;
+    const int i = me.i0 + place;
     const float c = s.scale * ATT_LOG2E;
     const Pair c2 = both(c);
-    float top = -INFINITY, sum = 0.f;   // of the scores times c; the sum is relative to 2^top
+    float top = -INFINITY;   // of the scores times c, as far as the sums are scaled to it
+    float sum = 0.f;         // of this half's probabilities, relative to 2^top
     uint32_t turns = 0;
     bool ok = true;
     for (int j = 0; j < walk.n; ++j) {
       const int t = walk.tile(j);
       if (!walk.uses(me, t)) continue;
-      if (!(ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+      // where a wait gives up the walk goes on without its scores: all threads of a unit meet as often
+      ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
       tc_fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) tmem_ld_32x32(s_col + k * 32, x[k]);
+      uint32_t x[2][32];
+      tmem_ld_32x32(s_col, x[0]);
+      tmem_ld_32x32(s_col + 32, x[1]);
       tmem_ld_wait();
-      const int j0 = t * ATT_TILE;
-      const bool whole = j0 + ATT_TILE - 1 <= me.i0 &&
-                         (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks);
+      const int j0 = t * ATT_TILE + half * 64;
+      const bool whole = j0 + 63 <= me.i0 && (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + 64 <= s.sinks);
       if (!whole) {
         const int last = i - j0, first = s.window ? last - s.window + 1 : -1, sinks = s.window ? s.sinks - j0 : 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int at = k * 32 + e;
@@ -193,19 +203,23 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
 #pragma unroll
       for (int e = 0; e < 8; ++e) some[e] = __uint_as_float(x[0][e]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = k ? 0 : 8; e < 32; e += 2) some[e / 2 & 7] = fmaxf(fmaxf(some[e / 2 & 7], __uint_as_float(x[k][e])), __uint_as_float(x[k][e + 1]));
-      const float most = fmaxf(fmaxf(fmaxf(some[0], some[1]), fmaxf(some[2], some[3])), fmaxf(fmaxf(some[4], some[5]), fmaxf(some[6], some[7]))) * c;
-      // The sums are scaled to a new maximum only where it has grown by more than 2^8: probabilities beside the old one stay in range
-      if (__any_sync(0xffffffffu, most > top + 8.f)) {
-        const float now = fmaxf(top, most);
+        for (int e = k ? 0 : 8; e < 32; e += 2)
+          some[e / 2 & 7] = most_of(some[e / 2 & 7], __uint_as_float(x[k][e]), __uint_as_float(x[k][e + 1]));
+      float most = most_of(most_of(some[0], some[1], some[2]), most_of(some[3], some[4], some[5]), most_of(some[6], some[7], some[7])) * c;
+      // The sums are scaled to a new maximum only where one of the unit's rows has grown by more than 2^8: probabilities beside the old one stay in
+      // range. A NaN grows, too, and makes one of everything in its row.
+      if (any_of_256(1 + u, !(most <= top + 8.f))) {
+        told[half * ATT_TILE] = most;
+        meet_256(1 + u);
+        const float now = most_of(top, most, told[(half ^ 1) * ATT_TILE]);
         const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
         top = now;
         sum *= f;
         if (turns) {
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
+          for (int k = 0; k < HD / 32; ++k) {
             uint32_t o[16];
             tmem_ld_32x16(o_col + k * 16, o);
             tmem_ld_wait();
@@ -218,37 +232,40 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       const Pair ref = both(top == -INFINITY ? 0.f : -top);
       Pair part[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float p0, p1;
-          fma2(pair_of(x[k][e], x[k][e + 1]), c2, ref).to(p0, p1);
-          p0 = exp2_unit(p0), p1 = exp2_unit(p1);
+          exp2_pair(e, fma2(pair_of(x[k][e], x[k][e + 1]), c2, ref), p0, p1);
           part[e / 2 & 3] = part[e / 2 & 3] + Pair(p0, p1);
           p[e / 2] = pack_bf16x2(p0, p1);
         }
-        tmem_st_32x16(s_col + k * 16, p);   // over scores that all are in registers
+        tmem_st_32x16(s_col + k * 16, p);   // over this half's scores, which all are in registers
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + k));
       }
       float a, d;
       ((part[0] + part[1]) + (part[2] + part[3])).to(a, d);
       sum += a + d;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(cta.bar(L::PROBS + u));
       ++turns;
     }
-    const bool exists = 2 * pair + u < units;
-    if (exists) {
-      if (ok && turns) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
+    if (2 * pair + u < units) {
+      if (turns) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
       tc_fence_after();
+      meet_256(1 + u);   // maxima told before have been read
+      told[half * ATT_TILE] = sum;
+      meet_256(1 + u);
+      sum = told[0] + told[ATT_TILE];   // in one order
       const bool mine = i < len;
-      minus_lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;   // no probability behind the end
+      if (half == 0)   // no probability behind the end
+        minus_lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
       const float f = 1.f / sum;
-      uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD);
+      uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD + half * (HD / 2));
 #pragma unroll
-      for (int k = 0; k < HD / 32; ++k) {
+      for (int k = 0; k < HD / 64; ++k) {
         uint32_t o[32];
         if (turns && ok) {
           tmem_ld_32x32(o_col + k * 32, o);
@@ -304,7 +321,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, 
 //   KEYS (dk, dv): a tile of k and v; q, dout, lse and delta pass by, over the heads of the group, whose sum is the gradient
 //   else (dq):     a tile of q and dout; k and v pass by
 // First T1 = held1 passing1^T (scores) and T2 = held2 passing2^T (dout v^T), then P and dS as bf16 operands in tensor memory of
-// dv += P dout, dk += dS q or dq += dS k. Two groups of warps have 64 columns each, a thread a row of them. Products and probabilities of neighbouring tiles
+// dv += P dout, dk += dS q or dq += dS k. Four groups of warps have 32 columns each, a thread a row of them. Products and probabilities of neighbouring tiles
 // overlap: with KEYS tensor memory is full with T1, T2 and two sums, P lies over T1 and dS over T2; dv's product and the next scores run while dS is
 // computed, dk's and the next T2 while the next probabilities are. dq leaves room for two tiles' scores, and dS lies over those. Every sum is made
 // in one order: gradients are the same bits in every run.
@@ -319,7 +336,9 @@ struct AttnBwd {
   static_assert(SMEM <= 232448, "more than a CTA's shared memory");
   static constexpr int FULL1 = 0, EMPTY1 = FULL1 + N1, FULL2 = EMPTY1 + N1, EMPTY2 = FULL2 + N2, THERE = EMPTY2 + N2;
   static constexpr int T1 = THERE + 1, T2 = T1 + (KEYS ? 1 : 2), DONE = T2 + 1;            // T1 and T2 there, sums done
-  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1, BARS = GRADS + 1;  // P and dS there: by eight warps
+  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1;
+  // rows behind a sequence's end are to be cleared, are zeros: of both passing tensors
+  static constexpr int CLEAR1 = GRADS + 1, CLEARED1 = CLEAR1 + 1, CLEAR2 = CLEARED1 + 1, CLEARED2 = CLEAR2 + 1, BARS = CLEARED2 + 1;  // P and dS there: by all warps
   // tensor memory: scores (dq: of two tiles), dout v^T, sums
   static constexpr int T1_COL = 0, T2_COL = KEYS ? 128 : 256, ACC1_COL = 256, ACC2_COL = 384;
 };
@@ -337,7 +356,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
                          AttnSplit split, int* err_word) {
   using L = AttnBwd<HD, KEYS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::READ ? 8 : 1; });
+  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::READ && i < L::CLEAR1 ? ATT_COMPUTE : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -381,11 +400,13 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
   const int group = KEYS ? s.G : 1, n = group * per_head;
   const int first_head = KEYS ? head * s.G : head / s.G;   // of the passing tensors
   auto row_of = [&](int at) { return (at < far ? at : lo + at - far) * ATT_TILE; };   // the first row of a head's at-th tile
+  // from which row on a head's last tile is not the sequence's: what TMA does not fill with zeros by itself
+  const int clear_from = n > 0 && len < s.S ? len - row_of(per_head - 1) : ATT_TILE;
   auto pass1 = [&](int i) { return cta.smem + L::PASS1 + i % L::N1 * L::TILE; };
   auto pass2 = [&](int i) { return cta.smem + L::PASS2 + i % L::N2 * L::TILE; };
   auto stats = [&](int i) { return cta.smem + L::STAT + i % L::N1 * L::STATS; };
 
-  if (warp == 8) {
+  if (warp == ATT_LOAD) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync() && n > 0) {
       mbar_expect_tx(cta.bar(L::THERE), 2 * L::TILE);
@@ -411,74 +432,79 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
         }
       grid_release();
     }
-  } else if (warp == 9) {
+  } else if (warp == ATT_MMA) {
     // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue
-    constexpr uint32_t idesc_t = make_instr_desc(1, 1, ATT_TILE, ATT_TILE, 0, 0), idesc_a = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
-    bool ok = n > 0 && cta.wait(L::THERE, 0, DEV_ERR_FULL_BAR_TIMEOUT);
-    // how many rows of the i-th tile a sequence has, counted along with the tiles of each kind
-    int at1 = 0, at2 = 0;
-    auto zero_behind = [&](uint32_t tile_at, int& at) {
-      const int there = len - row_of(at);
-      if (++at == per_head) at = 0;
-      if (there < ATT_TILE && len < s.S) zero_rows<HD, ATT_TILE>(tile_at, there);
-    };
-    auto t1 = [&](int i) {
-      if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
-      zero_behind(pass1(i), at1);
-      tc_fence_after();
-      if (lane == 0) {
+    if (elect_one_sync()) {
+      bool ok = n > 0 && cta.wait(L::THERE, 0, DEV_ERR_FULL_BAR_TIMEOUT);
+      int left1 = per_head, left2 = per_head;   // tiles of a head that are to come, of each of the passing tensors
+      uint32_t cleared1 = 0, cleared2 = 0;
+      auto t1 = [&](int i) {
+        if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+        if (--left1 == 0) {
+          left1 = per_head;
+          if (clear_from < ATT_TILE) {
+            mbar_arrive(cta.bar(L::CLEAR1));
+            if (!(ok = cta.wait(L::CLEARED1, cleared1++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+          }
+        }
+        tc_fence_after();
         const int two = KEYS ? 0 : i & 1;
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          umma_f16(cta.tmem + L::T1_COL + two * 128, desc_rows<ATT_TILE>(cta.smem, k), desc_rows<ATT_TILE>(pass1(i), k), idesc_t, k != 0);
+        multiply_rows<HD>(L::T1_COL + two * 128, cta.smem, pass1(i));
         umma_commit(cta.bar(L::T1 + two));
-      }
-      __syncwarp();
-    };
-    auto t2 = [&](int i) {
-      if (!(ok = cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
-      zero_behind(pass2(i), at2);
-      tc_fence_after();
-      if (lane == 0) {
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          umma_f16(cta.tmem + L::T2_COL, desc_rows<ATT_TILE>(cta.smem + L::TILE, k), desc_rows<ATT_TILE>(pass2(i), k), idesc_t, k != 0);
+      };
+      auto t2 = [&](int i) {
+        if (!(ok = cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+        if (--left2 == 0) {
+          left2 = per_head;
+          if (clear_from < ATT_TILE) {
+            mbar_arrive(cta.bar(L::CLEAR2));
+            if (!(ok = cta.wait(L::CLEARED2, cleared2++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+          }
+        }
+        tc_fence_after();
+        multiply_rows<HD>(L::T2_COL, cta.smem + L::TILE, pass2(i));
         umma_commit(cta.bar(L::T2));
         if constexpr (!KEYS) umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
-      }
-      __syncwarp();
-    };
-    // sum += operand tile; the operand of each group's 64 columns lies over those columns
-    auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, int i, int freed) {
-      if (lane == 0) {
+      };
+      // sum += operand tile; the operand of each group's 32 columns lies over those columns
+      auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, bool begun, int freed) {
+        const uint32_t low = TileDesc<ATT_TILE, true>::low(tile_at);
+        multiply_step<HD, 32>(acc, operand, low, 0, begun);
 #pragma unroll
-        for (int k = 0; k < ATT_TILE / 16; ++k)
-          umma_f16_ts(cta.tmem + acc, cta.tmem + operand + (k >> 2) * 64 + (k & 3) * 8, desc_cols<ATT_TILE>(tile_at, k), idesc_a, i != 0 || k != 0);
+        for (int k = 1; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand, low, k, true);
         umma_commit(cta.bar(freed));
-      }
-      __syncwarp();
-    };
-    if (ok) t1(0);
-    if (ok) t2(0);
-    if (!KEYS && ok && n > 1) t1(1);
-    for (int i = 0; i < n && ok; ++i) {
-      if constexpr (KEYS) {
-        if (!(ok = cta.wait(L::PROBS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+      };
+      if (ok) t1(0);
+      if (ok) t2(0);
+      if (!KEYS && ok && n > 1) t1(1);
+      for (int i = 0; i < n && ok; ++i) {
+        if constexpr (KEYS) {
+          if (!(ok = cta.wait(L::PROBS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+          tc_fence_after();
+          add(L::ACC1_COL, L::T1_COL, pass2(i), i > 0, L::EMPTY2 + i % L::N2);
+          if (i + 1 < n) t1(i + 1);
+        }
+        if (!ok || !(ok = cta.wait(L::GRADS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
         tc_fence_after();
-        add(L::ACC1_COL, L::T1_COL, pass2(i), i, L::EMPTY2 + i % L::N2);
-        if (i + 1 < n) t1(i + 1);
+        if (!KEYS && i + 1 < n) t2(i + 1);
+        if (!ok) break;
+        add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), i > 0, L::EMPTY1 + i % L::N1);
+        if (KEYS && i + 1 < n) t2(i + 1);
+        if (!KEYS && i + 2 < n) t1(i + 2);
       }
-      if (!ok || !(ok = cta.wait(L::GRADS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
-      tc_fence_after();
-      if (!KEYS && i + 1 < n) t2(i + 1);
-      if (!ok) break;
-      add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), i, L::EMPTY1 + i % L::N1);
-      if (KEYS && i + 1 < n) t2(i + 1);
-      if (!KEYS && i + 2 < n) t1(i + 2);
+      if (ok) umma_commit(cta.bar(L::DONE));
     }
-    if (ok && lane == 0) umma_commit(cta.bar(L::DONE));
-  } else if (warp < 8) {
-    // ---------------------------------------------------------------- probabilities: a thread has 64 columns of a row of the held tile
+  } else if (warp == ATT_ZERO) {
+    // ---------------------------------------------------------------- rows behind the sequence's end, in the last tile of each head
+    if (clear_from < ATT_TILE)
+      for (int i = per_head - 1, g = 0; i < n; i += per_head, ++g) {
+        if (!cta.wait(L::CLEAR1, g & 1, DEV_ERR_FULL_BAR_TIMEOUT) || !cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT)) break;
+        zero_rows<HD, ATT_TILE>(pass1(i), clear_from, cta.bar(L::CLEARED1));
+        if (!cta.wait(L::CLEAR2, g & 1, DEV_ERR_FULL_BAR_TIMEOUT) || !cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT)) break;
+        zero_rows<HD, ATT_TILE>(pass2(i), clear_from, cta.bar(L::CLEARED2));
+      }
+  } else {
+    // ---------------------------------------------------------------- probabilities: a thread has 32 columns of a row of the held tile
     const int w = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int r = r0 + (warp & 3) * 32 + lane;
@@ -489,12 +515,13 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       my_lse = both(minus_lse[from]);
       my_delta = both(minus_delta[from]);
     }
+    const uint8_t* const stat_base = smem_raw + (cta.smem - smem_u32(smem_raw)) + L::STAT + w * 128;
     bool ok = true;
     int at = 0;
     for (int i = 0; i < n; ++i) {
-      const int c0 = row_of(at) + w * 64;
+      const int c0 = row_of(at) + w * 32;
       if (++at == per_head) at = 0;
-      const uint32_t t1 = cta.tmem + lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 64, t2 = cta.tmem + lanes + L::T2_COL + w * 64;
+      const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
       if constexpr (KEYS) {   // lse and delta of the stage
         if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
       }
@@ -504,106 +531,103 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       bool whole;
       int first, last, sinks = 0;
       if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
-        whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + 63 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
+        whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + 31 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
         first = r - c0;
-        last = s.window == 0 || r < s.sinks ? 64 : first + s.window - 1;
+        last = s.window == 0 || r < s.sinks ? 32 : first + s.window - 1;
       } else {                // columns are keys
-        whole = c0 + 63 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + 64 <= s.sinks);
+        whole = c0 + 31 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + 32 <= s.sinks);
         last = r - c0;
         first = s.window ? last - s.window + 1 : 0;
         sinks = s.window ? s.sinks - c0 : 0;
       }
-      const uint32_t stat = stats(i) + w * 256;
-      uint32_t p[64];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t(&x)[32] = reinterpret_cast<uint32_t(&)[32]>(p[k * 32]);
-        tmem_ld_32x32(t1 + k * 32, x);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          Pair l0 = my_lse, l1 = my_lse;
-          if constexpr (KEYS) ld_shared_pairs(stat + (k * 32 + e) * 4, l0, l1);
-          float a, d;
-          fma2(pair_of(x[e], x[e + 1]), c, l0).to(a, d);
-          x[e] = __float_as_uint(exp2_unit(a)), x[e + 1] = __float_as_uint(exp2_unit(d));
-          fma2(pair_of(x[e + 2], x[e + 3]), c, l1).to(a, d);
-          x[e + 2] = __float_as_uint(exp2_unit(a)), x[e + 3] = __float_as_uint(exp2_unit(d));
-        }
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int col = k * 32 + e;
-            if (col > last || (col < first && col >= sinks)) x[e] = 0;
-          }
-        }
+      const ulonglong2* const stat = reinterpret_cast<const ulonglong2*>(stat_base + i % L::N1 * L::STATS);
+      auto row_numbers = [&](int of, int e, Pair& p0, Pair& p1) {   // of columns e to e + 3: lse (0), delta (1)
         if constexpr (KEYS) {
-          uint32_t o[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-          tmem_st_32x16(t1 + k * 16, o);   // over columns that this warp has read
+          const ulonglong2 v = stat[of * (ATT_TILE / 4) + e / 4];
+          p0.bits = v.x, p1.bits = v.y;
+        } else {
+          p0 = p1 = of ? my_delta : my_lse;
         }
-      }
+      };
       auto arrive = [&](int barrier) {
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(cta.bar(barrier));
       };
-      if constexpr (KEYS) arrive(L::PROBS);
+      uint32_t p[32], y[32], o[16];
+      tmem_ld_32x32(t1, p);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        Pair l0, l1;
+        row_numbers(0, e, l0, l1);
+        float a, d;
+        exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
+        p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
+        exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
+        p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (e > last || (e < first && e >= sinks)) p[e] = 0;
+      }
+      if constexpr (KEYS) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
+        tmem_st_32x16(t1, o);   // over columns that this warp has read
+        arrive(L::PROBS);
+      }
       if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
       tc_fence_after();
+      tmem_ld_32x32(t2, y);
+      tmem_ld_wait();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t y[32], o[16];
-        tmem_ld_32x32(t2 + k * 32, y);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          Pair d0 = my_delta, d1 = my_delta;
-          if constexpr (KEYS) ld_shared_pairs(stat + ATT_TILE * 4 + (k * 32 + e) * 4, d0, d1);
-          float a, d;
-          const int at_p = k * 32 + e;
-          (pair_of(p[at_p], p[at_p + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
-          if (!whole) a = p[at_p] ? a : 0.f, d = p[at_p + 1] ? d : 0.f;   // zero times what is not finite
-          o[e / 2] = pack_bf16x2(a, d);
-          (pair_of(p[at_p + 2], p[at_p + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
-          if (!whole) a = p[at_p + 2] ? a : 0.f, d = p[at_p + 3] ? d : 0.f;
-          o[e / 2 + 1] = pack_bf16x2(a, d);
-        }
-        tmem_st_32x16((KEYS ? t2 : t1) + k * 16, o);
+      for (int e = 0; e < 32; e += 4) {
+        Pair d0, d1;
+        row_numbers(1, e, d0, d1);
+        float a, d;
+        (pair_of(p[e], p[e + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
+        if (!whole) a = p[e] ? a : 0.f, d = p[e + 1] ? d : 0.f;   // zero times what is not finite
+        o[e / 2] = pack_bf16x2(a, d);
+        (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
+        if (!whole) a = p[e + 2] ? a : 0.f, d = p[e + 3] ? d : 0.f;
+        o[e / 2 + 1] = pack_bf16x2(a, d);
       }
+      tmem_st_32x16(KEYS ? t2 : t1, o);
       arrive(L::GRADS);
     }
     // ---------------------------------------------------------------- what the sums became
     if (ok && n > 0) ok = cta.wait(L::DONE, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
     tc_fence_after();
     const bool full = ok && n > 0, mine = r < len;
-    // KEYS: the first group of warps has dv, the second dk; dq's columns are halved between them
-    constexpr int COLS = KEYS ? HD : HD / 2;
-    const uint32_t acc = cta.tmem + lanes + (KEYS && w == 0 ? L::ACC1_COL : L::ACC2_COL) + (KEYS ? 0 : w * COLS);
-    const float f = KEYS && w == 0 ? 1.f : s.scale;
+    // KEYS: the first two groups of warps have dv, the others dk, half of the columns each; dq's columns are shared by four
+    constexpr int COLS = KEYS ? HD / 2 : HD / 4;
+    const int which = KEYS ? w >> 1 : 1, col = (KEYS ? w & 1 : w) * COLS;
+    const uint32_t acc = lanes + (which ? L::ACC2_COL : L::ACC1_COL) + col;
+    const float f = which ? s.scale : 1.f;
     const int out_heads = KEYS ? s.nkv : s.nq;
-    bf16* row = (KEYS && w == 0 ? grad1 : grad2) + ((static_cast<int64_t>(b) * s.S + r) * out_heads + head) * HD + (KEYS ? 0 : w * COLS);
+    bf16* row = (which ? grad2 : grad1) + ((static_cast<int64_t>(b) * s.S + r) * out_heads + head) * HD + col;
     float* sums = nullptr;
-    if (joined) sums = split.sums + (((static_cast<int64_t>(part) * heads * split.tiles + static_cast<int64_t>(tile) * heads + b * s.nkv + head) * 2 + w) * ATT_TILE +
-                                     (r - r0)) * HD;
+    if (joined) sums = split.sums + (((static_cast<int64_t>(part) * heads * split.tiles + static_cast<int64_t>(tile) * heads + b * s.nkv + head) * 2 + which) *
+                                      ATT_TILE + (r - r0)) * HD + col;
 #pragma unroll
-    for (int k = 0; k < COLS / 32; ++k) {
-      uint32_t o[32];
+    for (int k = 0; k < COLS / 16; ++k) {
+      uint32_t o[16];
       if (full) {
-        tmem_ld_32x32(acc + k * 32, o);
+        tmem_ld_32x16(acc + k * 16, o);
         tmem_ld_wait();
       }
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+      for (int e = 0; e < 16; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
       if (joined) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) reinterpret_cast<uint4*>(sums)[k * 8 + e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        for (int e = 0; e < 16; e += 4) reinterpret_cast<uint4*>(sums)[k * 4 + e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       } else if (r < s.S) {
         auto two = [&](int a) { return pack_bf16x2(__uint_as_float(o[a]), __uint_as_float(o[a + 1])); };
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) reinterpret_cast<uint4*>(row)[k * 4 + e / 8] = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
+        for (int e = 0; e < 16; e += 8) reinterpret_cast<uint4*>(row)[k * 2 + e / 8] = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
       }
     }
   }

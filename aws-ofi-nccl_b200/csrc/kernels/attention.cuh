@@ -13,7 +13,10 @@ using bf16 = __nv_bfloat16;
 
 constexpr int ATT_TILE = 128;                         // rows of a tile that stays, lanes of tensor memory
 constexpr int ATT_BOX = 64;                           // rows of one TMA box
-constexpr int ATT_THREADS = 384;                      // two groups of four warps that compute; warp 8 loads, warp 9 issues products
+constexpr int ATT_COMPUTE = 16;                       // warps that compute: four for each quarter of a tile's rows
+constexpr int ATT_LOAD = 16, ATT_MMA = 17;            // the warps that load and issue products, one thread each
+constexpr int ATT_ZERO = 18;                          // the warp that clears what lies behind a sequence's end
+constexpr int ATT_THREADS = 608;
 constexpr float ATT_LOG2E = 1.4426950408889634f;
 
 struct AttnShape {
@@ -42,38 +45,79 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* m, in
 #pragma unroll
     for (int r = 0; r < ROWS; r += ATT_BOX) tma_load_4d(dst + c * ROWS * 128 + r * 128, m, c * 64, head, row + r, b, bar);
 }
-// Descriptors of such a tile for 16 elements of the reduction: of a row's elements (K-major) ...
-template <int ROWS>
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int k) {
-  return make_smem_desc_sw128(tile + (k >> 2) * ROWS * 128 + (k & 3) * 32, 16, 1024);
-}
-// ... or over its rows (MN-major)
-template <int ROWS>
-__device__ __forceinline__ uint64_t desc_cols(uint32_t tile, int k) {
-  return make_smem_desc_sw128(tile + k * 2048, ROWS * 128, 1024);
-}
+// Descriptors of such a tile: of 16 of a row's elements (K-major), or over 16 of its rows (MN-major). The high word is the same for all tiles; the low
+// one is the address, to which the steps of a reduction are added. One elected thread issues all products of a CTA: beside busy warps, of which its scheduler has four
+// more, its instructions are what products wait for (64 clocks each alone; 114 so beside 16 warps of nothing but multiplications, 860 with descriptors put together
+// for each product, 1460 where a lane is chosen by its number).
+template <int ROWS, bool COLS>
+struct TileDesc {
+  static constexpr uint32_t HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);   // 8 rows to the next group; version; 128-byte swizzle
+  static constexpr uint32_t LEAD = COLS ? ROWS * 128 >> 4 : 1;              // COLS: from 64 columns to the next
+  __device__ static __forceinline__ uint32_t low(uint32_t tile) { return (tile >> 4) | (LEAD << 16); }
+  __device__ static constexpr uint32_t step(int k) { return (COLS ? k * 2048 : (k >> 2) * ROWS * 128 + (k & 3) * 32) >> 4; }
+};
 // Rows from `first` on of a tile become zeros: values that are not finite behind a sequence's end would reach its rows through products with
-// zero. By a whole warp, in front of the products that read the tile.
+// zero. By a whole warp, in front of the products that read the tile, whose issuing thread waits for `done`.
 template <int HD, int ROWS>
-__device__ __forceinline__ void zero_rows(uint32_t tile, int first) {
+__device__ __forceinline__ void zero_rows(uint32_t tile, int first, uint32_t done) {
   const int lane = threadIdx.x & 31;
   for (int i = first * 8 + lane; i < ROWS * 8; i += 32)
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) st_shared_v4(tile + c * ROWS * 128 + i * 16, 0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
+  if (lane == 0) mbar_arrive(done);
 }
 
-// D[tmem] (+)= A[tmem] * B[smem], A as packed pairs of bf16: 16 elements of the reduction are 8 columns.
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem], descriptors in two words
+template <bool ADD>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_low, uint32_t a_high, uint32_t b_low, uint32_t b_high, uint32_t idesc) {
   asm volatile(
       "{\n"
       ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-      "}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      ".reg .b64 a, b;\n"
+      "mov.b64 a, {%1, %2};\n"
+      "mov.b64 b, {%3, %4};\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a_low), "r"(a_high), "r"(b_low), "r"(b_high), "r"(idesc), "n"(ADD)
       : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], A as packed pairs of bf16: 16 elements of the reduction are 8 columns.
+template <bool ADD>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t b_high, uint32_t idesc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 b;\n"
+      "mov.b64 b, {%2, %3};\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "r"(b_low), "r"(b_high), "r"(idesc), "n"(ADD)
+      : "memory");
+}
+// A tile's rows times another's, elements of both reduced
+template <int HD>
+__device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile) {
+  using D = TileDesc<ATT_TILE, false>;
+  constexpr uint32_t idesc = make_instr_desc(1, 1, ATT_TILE, ATT_TILE, 0, 0);
+  const uint32_t a = D::low(a_tile), b = D::low(b_tile);
+  umma_ss<false>(d, a, D::HIGH, b, D::HIGH, idesc);
+#pragma unroll
+  for (int k = 1; k < HD / 16; ++k) umma_ss<true>(d, a + D::step(k), D::HIGH, b + D::step(k), D::HIGH, idesc);
+}
+// d (+)= operand in tensor memory times rows of a tile, 16 rows a step. Its 128 columns are as packed pairs in the first half of each GROUP of columns.
+template <int HD, int GROUP>
+__device__ __forceinline__ void multiply_step(uint32_t d, uint32_t a, uint32_t b_low, int k, bool add) {
+  using D = TileDesc<ATT_TILE, true>;
+  constexpr uint32_t idesc = make_instr_desc(1, 1, ATT_TILE, HD, 0, 1);
+  const uint32_t at = a + k / (GROUP / 16) * GROUP + k % (GROUP / 16) * 8;
+  if (add)
+    umma_ts<true>(d, at, b_low + D::step(k), D::HIGH, idesc);
+  else
+    umma_ts<false>(d, at, b_low + D::step(k), D::HIGH, idesc);
 }
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -102,19 +146,90 @@ __device__ __forceinline__ void ld_shared_pairs(uint32_t addr, Pair& a, Pair& b)
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a.bits), "=l"(b.bits) : "r"(addr) : "memory");
 }
 
-// What all roles of a CTA share: its tensor memory, barriers and the flag that one of its waits has given up.
+// 2^x of both where x <= 120, in float units beside the one for exponentials, which has a quarter of their rate: 2^n p(f) with n the integer nearest to
+// x, f = x - n and p the cubic whose largest relative error on [-1/2, 1/2] is the least (7.5e-5, by Remez' exchange; probabilities are rounded to bf16
+// behind it, 3.9e-3). Below -127 it is zero.
+__device__ __forceinline__ Pair exp2_cubic(Pair x) {
+  constexpr float BIG = 12582912.f;   // 1.5 * 2^23: a sum with it has the integer in its low bits
+  float a, b;
+  x.to(a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+  const Pair y(a, b), t = y + both(BIG), f = fma2(t + both(-BIG), both(-1.f), y);
+  const Pair p = fma2(fma2(fma2(both(0.0551716685f), f, both(0.242611125f)), f, both(0.693260968f)), f, both(0.999928057f));
+  t.to(a, b);
+  return p * pair_of((__float_as_uint(a) << 23) + 0x3F800000u, (__float_as_uint(b) << 23) + 0x3F800000u);
+}
+// The same of x by the unit, or of every fourth pair of a row (number e / 2) in float units: both then have the same to do.
+__device__ __forceinline__ void exp2_pair(int e, Pair x, float& a, float& b) {
+  if (e / 2 % 4 == 3) {
+    exp2_cubic(x).to(a, b);
+  } else {
+    x.to(a, b);
+    a = exp2_unit(a), b = exp2_unit(b);
+  }
+}
+// The largest of three, NaN if there is one
+__device__ __forceinline__ float most_of(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Whether `mine` is true for any thread of 256 that meet at barrier `id`
+__device__ __forceinline__ bool any_of_256(int id, bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %2, 0;\n"
+      "barrier.cta.red.or.pred q, %1, 256, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(id), "r"(static_cast<uint32_t>(mine))
+      : "memory");
+  return r;
+}
+__device__ __forceinline__ void meet_256(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
+
+// What all roles of a CTA share: barriers and the flag that one of its waits has given up. It has all of tensor memory, from column 0 on.
 struct AttnCta {
-  uint32_t smem, bars, tmem;   // aligned tiles; barriers behind them; tensor memory's first column
+  uint32_t smem, bars;   // aligned tiles; barriers behind them
   volatile int* abort_flag;
   int* err_word;
   __device__ __forceinline__ uint32_t bar(int i) const { return bars + 8u * i; }
   __device__ __forceinline__ bool wait(int i, uint32_t parity, int code) const {
-    return mbar_wait_bounded(bar(i), parity, abort_flag, err_word, code, GEMM_WAIT_LIMIT_NS);
+    // Polled: a thread that is suspended for a time comes back later, 5 % of the forward pass and of the gradients
+    const uint32_t at = bar(i);
+    uint64_t t0 = 0;
+    for (uint32_t spins = 0;; ++spins) {
+      uint32_t done;
+      asm volatile(
+          "{\n"
+          ".reg .pred P;\n"
+          "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n"
+          "selp.u32 %0, 1, 0, P;\n"
+          "}\n"
+          : "=r"(done)
+          : "r"(at), "r"(parity)
+          : "memory");
+      if (done) return true;
+      if ((spins & 1023) == 1023) {
+        if (*abort_flag) return false;
+        const uint64_t t = globaltimer_ns();
+        if (!t0) t0 = t;
+        if (t - t0 > GEMM_WAIT_LIMIT_NS) {
+          *abort_flag = 1;
+          if (err_word) atomicCAS(err_word, 0, code);
+          return false;
+        }
+      }
+    }
   }
 };
 constexpr int ATT_BAR_BYTES = 256;   // barriers, the slot of tensor memory's address and the flag
 
-// Barrier i is completed by count(i) arrivals. Tensor memory is the last warp's. Every thread calls this.
+// Barrier i is completed by count(i) arrivals. Tensor memory is the issuing warp's. Every thread calls this.
 template <int TILE_BYTES, int BARS, class Count>
 __device__ __forceinline__ AttnCta attn_begin(uint8_t* smem_raw, int* err_word, Count count) {
   static_assert(BARS * 8 + 16 <= ATT_BAR_BYTES, "more barriers than room");
@@ -129,14 +244,13 @@ __device__ __forceinline__ AttnCta attn_begin(uint8_t* smem_raw, int* err_word, 
     *c.abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x / 32 == ATT_THREADS / 32 - 1) {
+  if (threadIdx.x / 32 == ATT_MMA) {
     tmem_alloc(c.bars + BARS * 8, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  c.tmem = *reinterpret_cast<volatile uint32_t*>(at);
   return c;
 }
 __device__ __forceinline__ void attn_end(const AttnCta& c) {
@@ -146,9 +260,9 @@ __device__ __forceinline__ void attn_end(const AttnCta& c) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
   }
-  if (threadIdx.x / 32 == ATT_THREADS / 32 - 1) {
+  if (threadIdx.x / 32 == ATT_MMA) {
     tc_fence_after();
-    tmem_dealloc(c.tmem, 512);
+    tmem_dealloc(0, 512);
   }
 }
 

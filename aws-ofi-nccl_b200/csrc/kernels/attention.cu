@@ -51,26 +51,27 @@ __device__ __forceinline__ AttnWalk attn_walk(const AttnShape& s, const AttnUnit
   return w;
 }
 
+using AttnFwdRoles = AttnRoles<8>;
 template <int HD>
 struct AttnFwd {
   static constexpr int TILE = ATT_TILE * HD * 2;
   static constexpr int STAGES = 4;
-  static constexpr int ROWS = (2 + STAGES) * TILE;           // a number for each row of each half of a unit's columns
-  static constexpr int TILES = ROWS + 4 * ATT_TILE * 4;
+  static constexpr int TILES = (2 + STAGES) * TILE;
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
   // barriers: stages full and empty; q there; scores there, probabilities there (or their row scaled), sums of a unit done
   static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, SCORES = Q + 2, PROBS = SCORES + 2, DONE = PROBS + 4, CLEAR = DONE + 2, CLEARED = CLEAR + 1, BARS = CLEARED + 1;
-  // tensor memory: scores of a unit (probabilities as bf16 over each half's first columns), its sums
+  // tensor memory: scores of a unit (probabilities as bf16 over their first half), its sums
   static constexpr int S_COL = 0, O_COL = 256;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(ATT_THREADS, 1)
+__global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          bf16* out, float* minus_lse, AttnShape s, int* err_word) {
   using L = AttnFwd<HD>;
+  using R = AttnFwdRoles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 8 : 1; });
+  const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the longest walks first
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
   // from which row on the last tile is not the sequence's: what TMA does not fill with zeros by itself
   const int clear_from = walk.n > 0 && len < s.S ? len - walk.tile(walk.n - 1) * ATT_TILE : ATT_TILE;
 
-  if (warp == ATT_LOAD) {
+  if (warp == R::LOAD) {
     // ---------------------------------------------------------------- loads: q, then k and v in turn
     if (elect_one_sync()) {
       for (int u = 0; u < 2; ++u)
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       }
       grid_release();
     }
-  } else if (warp == ATT_MMA) {
+  } else if (warp == R::MMA) {
     // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue: probabilities
     // are read before the next scores of their unit are written over them
     if (elect_one_sync()) {
@@ -134,15 +135,14 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           if (walk.uses(unit[u], t)) {
-            // in two parts, each of 32 columns of both halves, as they are there
+            // in two parts, as they are there
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
               if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
               tc_fence_after();
-              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2, part || !first[u]);
-              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 1, true);
-              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 4, true);
-              multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 5, true);
+              multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 4, part || !first[u]);
+#pragma unroll
+              for (int k = 1; k < 4; ++k) multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 4 + k, true);
             }
             if (!ok) break;
             first[u] = false;
@@ -156,70 +156,63 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
         if (more) umma_commit(cta.bar(L::EMPTY + (2 * j + 2) % L::STAGES));
       }
     }
-  } else if (warp == ATT_ZERO) {
+  } else if (warp == R::ZERO) {
     // ---------------------------------------------------------------- v behind the sequence's end, in the last tile of the walk
     const int i = 2 * walk.n - 1;
     if (clear_from < ATT_TILE && cta.wait(L::CLEAR, 0, DEV_ERR_FULL_BAR_TIMEOUT) && cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))
       zero_rows<HD, ATT_TILE>(stages + i % L::STAGES * L::TILE, clear_from, cta.bar(L::CLEARED));
   } else {
-    // ---------------------------------------------------------------- softmax: a thread has half of a row
-    const int u = warp >> 3, half = warp >> 2 & 1, place = (warp & 3) * 32 + lane;
-    const AttnUnit& me = unit[u];
+    // ---------------------------------------------------------------- softmax: a thread has a row
+    const int u = warp >> 2;
+    AttnUnit me = attn_unit(s, kv_head, 2 * pair + u, len);
+    if (2 * pair + u >= units) me.live = false;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE + half * 64;
-    const uint32_t o_col = lanes + L::O_COL + u * 128 + half * (HD / 2);
-    // a row's two threads tell each other numbers here
-    volatile float* const told = reinterpret_cast<volatile float*>(smem_raw + (cta.smem - smem_u32(smem_raw)) + L::ROWS) + u * 2 * ATT_TILE + place;
-    const int i = me.i0 + place;
+    const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE, o_col = lanes + L::O_COL + u * 128;
+    const int i = me.i0 + (warp & 3) * 32 + lane;
     const float c = s.scale * ATT_LOG2E;
     const Pair c2 = both(c);
-    float top = -INFINITY;   // of the scores times c, as far as the sums are scaled to it
-    float sum = 0.f;         // of this half's probabilities, relative to 2^top
-    uint32_t turns = 0;
+    // this unit's own tiles of the walk
+    const int far = me.live ? min(walk.sink_tiles, me.lo) : 0, n = me.live ? far + me.hi - me.lo + 1 : 0;
+    float top = -INFINITY, sum = 0.f;   // of the scores times c, as far as the sums are scaled to it; relative to 2^top
     bool ok = true;
-    for (int j = 0; j < walk.n; ++j) {
-      const int t = walk.tile(j);
-      if (!walk.uses(me, t)) continue;
-      // where a wait gives up the walk goes on without its scores: all threads of a unit meet as often
-      ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int j0 = (j < far ? j : me.lo + j - far) * ATT_TILE;
+      if (!(ok = cta.wait(L::SCORES + u, j & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
       tc_fence_after();
-      uint32_t x[2][32];
-      tmem_ld_32x32(s_col, x[0]);
-      tmem_ld_32x32(s_col + 32, x[1]);
+      uint32_t x[4][32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tmem_ld_32x32(s_col + k * 32, x[k]);
       tmem_ld_wait();
-      const int j0 = t * ATT_TILE + half * 64;
-      const bool whole = j0 + 63 <= me.i0 && (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + 64 <= s.sinks);
-      if (!whole) {
+      if (!(j0 + ATT_TILE - 1 <= me.i0 && (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks))) {
         const int last = i - j0, first = s.window ? last - s.window + 1 : -1, sinks = s.window ? s.sinks - j0 : 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int at = k * 32 + e;
             if (at > last || (at < first && at >= sinks)) x[k][e] = 0xFF800000u;   // -inf
           }
       }
-      float some[8];
+      float some[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) some[e] = __uint_as_float(x[0][e]);
+      for (int k = 0; k < 4; ++k) {
+        some[k] = __uint_as_float(x[k][0]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = k ? 0 : 8; e < 32; e += 2)
-          some[e / 2 & 7] = most_of(some[e / 2 & 7], __uint_as_float(x[k][e]), __uint_as_float(x[k][e + 1]));
-      float most = most_of(most_of(some[0], some[1], some[2]), most_of(some[3], some[4], some[5]), most_of(some[6], some[7], some[7])) * c;
-      // The sums are scaled to a new maximum only where one of the unit's rows has grown by more than 2^8: probabilities beside the old one stay in
+        for (int e = 1; e < 31; e += 2) some[k] = most_of(some[k], __uint_as_float(x[k][e]), __uint_as_float(x[k][e + 1]));
+        some[k] = most_of(some[k], __uint_as_float(x[k][31]), __uint_as_float(x[k][31]));
+      }
+      const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
+      // The sums are scaled to a new maximum only where one of the warp's rows has grown by more than 2^8: probabilities beside the old one stay in
       // range. A NaN grows, too, and makes one of everything in its row.
-      if (any_of_256(1 + u, !(most <= top + 8.f))) {
-        told[half * ATT_TILE] = most;
-        meet_256(1 + u);
-        const float now = most_of(top, most, told[(half ^ 1) * ATT_TILE]);
+      if (__any_sync(0xffffffffu, !(most <= top + 8.f))) {
+        const float now = most_of(top, most, most);
         const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
         top = now;
         sum *= f;
-        if (turns) {
+        if (j) {
 #pragma unroll
-          for (int k = 0; k < HD / 32; ++k) {
+          for (int k = 0; k < HD / 16; ++k) {
             uint32_t o[16];
             tmem_ld_32x16(o_col + k * 16, o);
             tmem_ld_wait();
@@ -232,7 +225,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       const Pair ref = both(top == -INFINITY ? 0.f : -top);
       Pair part[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < 4; ++k) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
@@ -241,33 +234,30 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
           part[e / 2 & 3] = part[e / 2 & 3] + Pair(p0, p1);
           p[e / 2] = pack_bf16x2(p0, p1);
         }
-        tmem_st_32x16(s_col + k * 16, p);   // over this half's scores, which all are in registers
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + k));
+        tmem_st_32x16(s_col + k * 16, p);   // over scores that all are in registers
+        if (k & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + (k >> 1)));
+        }
       }
       float a, d;
       ((part[0] + part[1]) + (part[2] + part[3])).to(a, d);
       sum += a + d;
-      ++turns;
     }
     if (2 * pair + u < units) {
-      if (turns) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
+      if (ok && n) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
       tc_fence_after();
-      meet_256(1 + u);   // maxima told before have been read
-      told[half * ATT_TILE] = sum;
-      meet_256(1 + u);
-      sum = told[0] + told[ATT_TILE];   // in one order
       const bool mine = i < len;
-      if (half == 0)   // no probability behind the end
-        minus_lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
+      // no probability behind the end
+      minus_lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
       const float f = 1.f / sum;
-      uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD + half * (HD / 2));
+      uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD);
 #pragma unroll
-      for (int k = 0; k < HD / 64; ++k) {
+      for (int k = 0; k < HD / 32; ++k) {
         uint32_t o[32];
-        if (turns && ok) {
+        if (n && ok) {
           tmem_ld_32x32(o_col + k * 32, o);
           tmem_ld_wait();
         }
@@ -275,7 +265,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (mine && turns && ok) {
+            if (mine && n && ok) {
               auto two = [&](int at) { return pack_bf16x2(__uint_as_float(o[at]) * f, __uint_as_float(o[at + 1]) * f); };
               v = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
             }
@@ -285,7 +275,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       }
     }
   }
-  attn_end(cta);
+  attn_end<R>(cta);
 }
 
 // ------------------------------------------------------------------ backward
@@ -325,6 +315,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, 
 // overlap: with KEYS tensor memory is full with T1, T2 and two sums, P lies over T1 and dS over T2; dv's product and the next scores run while dS is
 // computed, dk's and the next T2 while the next probabilities are. dq leaves room for two tiles' scores, and dS lies over those. Every sum is made
 // in one order: gradients are the same bits in every run.
+using AttnBwdRoles = AttnRoles<16>;
 template <int HD, bool KEYS>
 struct AttnBwd {
   static constexpr int TILE = ATT_TILE * HD * 2;
@@ -350,13 +341,14 @@ struct AttnSplit {
 };
 
 template <int HD, bool KEYS>
-__global__ void __launch_bounds__(ATT_THREADS, 1)
+__global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const __grid_constant__ CUtensorMap tmD, const float* minus_lse, const float* minus_delta, bf16* grad1, bf16* grad2, AttnShape s,
                          AttnSplit split, int* err_word) {
   using L = AttnBwd<HD, KEYS>;
+  using R = AttnBwdRoles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const AttnCta cta = attn_begin<L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::READ && i < L::CLEAR1 ? ATT_COMPUTE : 1; });
+  const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::READ && i < L::CLEAR1 ? R::LOAD : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -406,7 +398,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
   auto pass2 = [&](int i) { return cta.smem + L::PASS2 + i % L::N2 * L::TILE; };
   auto stats = [&](int i) { return cta.smem + L::STAT + i % L::N1 * L::STATS; };
 
-  if (warp == ATT_LOAD) {
+  if (warp == R::LOAD) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync() && n > 0) {
       mbar_expect_tx(cta.bar(L::THERE), 2 * L::TILE);
@@ -432,7 +424,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
         }
       grid_release();
     }
-  } else if (warp == ATT_MMA) {
+  } else if (warp == R::MMA) {
     // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue
     if (elect_one_sync()) {
       bool ok = n > 0 && cta.wait(L::THERE, 0, DEV_ERR_FULL_BAR_TIMEOUT);
@@ -494,7 +486,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       }
       if (ok) umma_commit(cta.bar(L::DONE));
     }
-  } else if (warp == ATT_ZERO) {
+  } else if (warp == R::ZERO) {
     // ---------------------------------------------------------------- rows behind the sequence's end, in the last tile of each head
     if (clear_from < ATT_TILE)
       for (int i = per_head - 1, g = 0; i < n; i += per_head, ++g) {
@@ -631,7 +623,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
       }
     }
   }
-  attn_end(cta);
+  attn_end<R>(cta);
 }
 
 // The gradients of tiles whose walk was split: their parts' sums, one after the other.
@@ -699,7 +691,7 @@ static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = allow_smem<attention_fwd_kernel<HD>>(AttnFwd<HD>::SMEM)) return rc;
   const int units = s.rows / ATT_TILE * s.G;
-  launch_dependent(attention_fwd_kernel<HD>, s.B * s.nkv * ((units + 1) / 2), ATT_THREADS, AttnFwd<HD>::SMEM, stream, q, k, v,
+  launch_dependent(attention_fwd_kernel<HD>, s.B * s.nkv * ((units + 1) / 2), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v,
                    static_cast<bf16*>(a.out), a.lse, s, device_status_word());
   B200_CUDA_OK(cudaGetLastError());
   return 0;
@@ -737,7 +729,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   const int tiles = s.rows / ATT_TILE;
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
-    launch_dependent(keys, s.B * s.nkv * (tiles + split.tiles * split.parts), ATT_THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, a.lse, a.delta,
+    launch_dependent(keys, s.B * s.nkv * (tiles + split.tiles * split.parts), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, a.lse, a.delta,
                      static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, err);
     if (split.parts) {
       const int64_t n = static_cast<int64_t>(s.B) * s.nkv * split.tiles * 2 * (ATT_TILE * HD / 4);
@@ -746,7 +738,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
     }
   }
   if (a.dq)
-    launch_dependent(queries, s.B * s.nq * tiles, ATT_THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
+    launch_dependent(queries, s.B * s.nq * tiles, AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
                      static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, nullptr}, err);
   B200_CUDA_OK(cudaGetLastError());
   return 0;

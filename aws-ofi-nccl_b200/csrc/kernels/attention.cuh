@@ -13,10 +13,12 @@ using bf16 = __nv_bfloat16;
 
 constexpr int ATT_TILE = 128;                         // rows of a tile that stays, lanes of tensor memory
 constexpr int ATT_BOX = 64;                           // rows of one TMA box
-constexpr int ATT_COMPUTE = 16;                       // warps that compute: four for each quarter of a tile's rows
-constexpr int ATT_LOAD = 16, ATT_MMA = 17;            // the warps that load and issue products, one thread each
-constexpr int ATT_ZERO = 18;                          // the warp that clears what lies behind a sequence's end
-constexpr int ATT_THREADS = 608;
+// Warps of a CTA: COMPUTE of them compute, as many for each quarter of a tile's rows; behind them one that loads and one that issues products, a thread
+// each, and one that clears what lies behind a sequence's end.
+template <int COMPUTE>
+struct AttnRoles {
+  static constexpr int LOAD = COMPUTE, MMA = COMPUTE + 1, ZERO = COMPUTE + 2, THREADS = 32 * (COMPUTE + 3);
+};
 constexpr float ATT_LOG2E = 1.4426950408889634f;
 
 struct AttnShape {
@@ -175,23 +177,6 @@ __device__ __forceinline__ float most_of(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Whether `mine` is true for any thread of 256 that meet at barrier `id`
-__device__ __forceinline__ bool any_of_256(int id, bool mine) {
-  uint32_t r;
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.u32 p, %2, 0;\n"
-      "barrier.cta.red.or.pred q, %1, 256, p;\n"
-      "selp.u32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(r)
-      : "r"(id), "r"(static_cast<uint32_t>(mine))
-      : "memory");
-  return r;
-}
-__device__ __forceinline__ void meet_256(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
-
 // What all roles of a CTA share: barriers and the flag that one of its waits has given up. It has all of tensor memory, from column 0 on.
 struct AttnCta {
   uint32_t smem, bars;   // aligned tiles; barriers behind them
@@ -230,7 +215,7 @@ struct AttnCta {
 constexpr int ATT_BAR_BYTES = 256;   // barriers, the slot of tensor memory's address and the flag
 
 // Barrier i is completed by count(i) arrivals. Tensor memory is the issuing warp's. Every thread calls this.
-template <int TILE_BYTES, int BARS, class Count>
+template <class Roles, int TILE_BYTES, int BARS, class Count>
 __device__ __forceinline__ AttnCta attn_begin(uint8_t* smem_raw, int* err_word, Count count) {
   static_assert(BARS * 8 + 16 <= ATT_BAR_BYTES, "more barriers than room");
   AttnCta c;
@@ -244,7 +229,7 @@ __device__ __forceinline__ AttnCta attn_begin(uint8_t* smem_raw, int* err_word, 
     *c.abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x / 32 == ATT_MMA) {
+  if (threadIdx.x / 32 == Roles::MMA) {
     tmem_alloc(c.bars + BARS * 8, 512);
     tmem_relinquish();
   }
@@ -253,6 +238,7 @@ __device__ __forceinline__ AttnCta attn_begin(uint8_t* smem_raw, int* err_word, 
   tc_fence_after();
   return c;
 }
+template <class Roles>
 __device__ __forceinline__ void attn_end(const AttnCta& c) {
   tc_fence_before();
   __syncthreads();
@@ -260,7 +246,7 @@ __device__ __forceinline__ void attn_end(const AttnCta& c) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
   }
-  if (threadIdx.x / 32 == ATT_MMA) {
+  if (threadIdx.x / 32 == Roles::MMA) {
     tc_fence_after();
     tmem_dealloc(0, 512);
   }

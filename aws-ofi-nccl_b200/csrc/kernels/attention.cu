@@ -17,88 +17,105 @@
 
 namespace b200 {
 
+// Kernels stay: as many CTAs as SMs, each with several items of work (a tile and its walk over the other side), whose loads and first products run
+// beside the end of the item before. Items are ordered by their length, longest first, and dealt there and back, so that every CTA has about as much.
+__device__ __forceinline__ int dealt(int turn) {
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  return turn * ctas + (turn & 1 ? ctas - 1 - cta : cta);
+}
+
 // ------------------------------------------------------------------ forward
-// A CTA takes two units of 128 queries of one head each that share a head of k and v: two heads of a group for the same tokens, or where the number
+// An item are two units of 128 queries of one head each that share a head of k and v: two heads of a group for the same tokens, or where the number
 // of heads in a group is odd also neighbouring tokens. So a tile of k and v is loaded once for 256 rows.
 struct AttnUnit {
-  int head, i0, lo, hi;   // rows from i0; key tiles lo to hi of its window (none where lo > hi)
-  bool live;
+  int head, i0, lo, hi;   // rows from i0; key tiles lo to hi of its window
+  bool live, exists;      // has rows in front of the sequence's end, of the tensor's
 };
-__device__ __forceinline__ AttnUnit attn_unit(const AttnShape& s, int kv_head, int u, int len) {
-  AttnUnit r;
-  const int tile = u / s.G;
-  r.head = kv_head * s.G + (u - tile * s.G);
-  r.i0 = tile * ATT_TILE;
-  r.live = r.i0 < len;
-  r.hi = r.live ? (min(r.i0 + ATT_TILE, len) - 1) / ATT_TILE : -1;
-  r.lo = r.live ? (s.window ? max(0, r.i0 - s.window + 1) / ATT_TILE : 0) : 0;
-  return r;
-}
-// The key tiles of a pair of units: those that hold sinks, in front of the windows' tiles, and these.
-struct AttnWalk {
-  int far, lo, n;          // far sink tiles, then tiles from lo; n in all
-  int sink_tiles;
+struct AttnFwdItem {
+  int b, kv_head, len;
+  AttnUnit unit[2];
+  // the walk of both: `far` tiles of sinks, then tiles from lo; n in all
+  int far, lo, n, sink_tiles;
+  int clear_from;   // from which row on its last tile is not the sequence's: what TMA does not fill with zeros by itself
   __device__ __forceinline__ int tile(int j) const { return j < far ? j : lo + j - far; }
-  __device__ __forceinline__ bool uses(const AttnUnit& u, int t) const { return u.live && t <= u.hi && (t >= u.lo || t < sink_tiles); }
+  __device__ __forceinline__ bool uses(int u, int t) const { return unit[u].live && t <= unit[u].hi && (t >= unit[u].lo || t < sink_tiles); }
+
+  __device__ __forceinline__ AttnFwdItem(const AttnShape& s, int item) {
+    const int heads = s.B * s.nkv, units = s.rows / ATT_TILE * s.G;
+    const int nth = item / heads, pair = (units + 1) / 2 - 1 - nth, bh = item - nth * heads;
+    b = bh / s.nkv, kv_head = bh - b * s.nkv;
+    len = sequence_length(s, b);
+    sink_tiles = s.window ? (s.sinks + ATT_TILE - 1) / ATT_TILE : 0;
+    lo = 1 << 30;
+    int hi = -1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      AttnUnit& r = unit[u];
+      const int at = 2 * pair + u, rows = at / s.G;
+      r.head = kv_head * s.G + (at - rows * s.G);
+      r.i0 = rows * ATT_TILE;
+      r.exists = at < units;
+      r.live = r.exists && r.i0 < len;
+      r.hi = r.live ? (min(r.i0 + ATT_TILE, len) - 1) / ATT_TILE : -1;
+      r.lo = s.window ? max(0, r.i0 - s.window + 1) / ATT_TILE : 0;
+      if (r.live) lo = min(lo, r.lo);
+      hi = max(hi, r.hi);
+    }
+    far = hi < 0 ? 0 : min(sink_tiles, lo);
+    n = hi < 0 ? 0 : far + hi - lo + 1;
+    clear_from = n > 0 && len < s.S ? min(len - hi * ATT_TILE, ATT_TILE) : ATT_TILE;
+  }
 };
-__device__ __forceinline__ AttnWalk attn_walk(const AttnShape& s, const AttnUnit& a, const AttnUnit& b) {
-  AttnWalk w;
-  w.sink_tiles = s.window ? (s.sinks + ATT_TILE - 1) / ATT_TILE : 0;
-  w.lo = min(a.live ? a.lo : 1 << 30, b.live ? b.lo : 1 << 30);
-  const int hi = max(a.hi, b.hi);
-  w.far = hi < 0 ? 0 : min(w.sink_tiles, w.lo);
-  w.n = hi < 0 ? 0 : w.far + hi - w.lo + 1;
-  return w;
-}
 
 using AttnFwdRoles = AttnRoles<8>;
 template <int HD>
 struct AttnFwd {
   static constexpr int TILE = ATT_TILE * HD * 2;
   static constexpr int STAGES = 4;
-  static constexpr int TILES = (2 + STAGES) * TILE;
+  static constexpr int OUT = (2 + STAGES) * TILE;       // 32 rows of 64 elements of each warp on their way out
+  static constexpr int TILES = OUT + 8 * 4096;
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
-  // barriers: stages full and empty; q there; scores there, probabilities there (or their row scaled), sums of a unit done
-  static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, SCORES = Q + 2, PROBS = SCORES + 2, DONE = PROBS + 4, CLEAR = DONE + 2, CLEARED = CLEAR + 1, BARS = CLEARED + 1;
+  // barriers: stages full and empty; q there and read; scores there; probabilities there (or their row scaled), in two parts; sums of a unit done; rows behind
+  // a sequence's end to be cleared, cleared
+  static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, QREAD = Q + 2, SCORES = QREAD + 2, PROBS = SCORES + 2, DONE = PROBS + 4, CLEAR = DONE + 2,
+                       CLEARED = CLEAR + 1, BARS = CLEARED + 1;
   // tensor memory: scores of a unit (probabilities as bf16 over their first half), its sums
   static constexpr int S_COL = 0, O_COL = 256;
+  static constexpr int FIRST = 96;   // columns of probabilities that are handed over while the others are computed
 };
 
 template <int HD>
 __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         bf16* out, float* minus_lse, AttnShape s, int* err_word) {
+                         const __grid_constant__ CUtensorMap tmO, float* minus_lse, AttnShape s, int items, int* err_word) {
   using L = AttnFwd<HD>;
   using R = AttnFwdRoles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the longest walks first
-  const int heads = s.B * s.nkv, units = s.rows / ATT_TILE * s.G;
-  const int pair = (units + 1) / 2 - 1 - static_cast<int>(blockIdx.x) / heads, bh = static_cast<int>(blockIdx.x) % heads;
-  const int b = bh / s.nkv, kv_head = bh - b * s.nkv;
-  const int len = sequence_length(s, b);
-  AttnUnit unit[2] = {attn_unit(s, kv_head, 2 * pair, len), attn_unit(s, kv_head, 2 * pair + 1, len)};
-  if (2 * pair + 1 >= units) unit[1].live = false, unit[1].hi = -1;
-  const AttnWalk walk = attn_walk(s, unit[0], unit[1]);
   const uint32_t q_tile = cta.smem, stages = cta.smem + 2 * L::TILE;
-  // from which row on the last tile is not the sequence's: what TMA does not fill with zeros by itself
-  const int clear_from = walk.n > 0 && len < s.S ? len - walk.tile(walk.n - 1) * ATT_TILE : ATT_TILE;
+  auto stage = [&](uint32_t i) { return stages + i % L::STAGES * L::TILE; };
 
   if (warp == R::LOAD) {
     // ---------------------------------------------------------------- loads: q, then k and v in turn
     if (elect_one_sync()) {
-      for (int u = 0; u < 2; ++u)
-        if (unit[u].live) {
-          mbar_expect_tx(cta.bar(L::Q + u), L::TILE);
-          load_tile<HD, ATT_TILE>(q_tile + u * L::TILE, &tmQ, b, unit[u].head, unit[u].i0, cta.bar(L::Q + u));
+      uint32_t loaded = 0, q_loaded[2] = {0, 0};
+      bool ok = true;
+      for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+        const AttnFwdItem w(s, dealt(turn));
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (w.unit[u].live && (ok = ok && cta.wait(L::QREAD + u, (q_loaded[u]++ & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) {
+            mbar_expect_tx(cta.bar(L::Q + u), L::TILE);
+            load_tile<HD, ATT_TILE>(q_tile + u * L::TILE, &tmQ, w.b, w.unit[u].head, w.unit[u].i0, cta.bar(L::Q + u));
+          }
+        for (int i = 0; i < 2 * w.n && ok; ++i, ++loaded) {
+          const int st = loaded % L::STAGES;
+          if (!(ok = cta.wait(L::EMPTY + st, (loaded / L::STAGES & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
+          mbar_expect_tx(cta.bar(L::FULL + st), L::TILE);
+          load_tile<HD, ATT_TILE>(stage(loaded), i & 1 ? &tmV : &tmK, w.b, w.kv_head, w.tile(i >> 1) * ATT_TILE, cta.bar(L::FULL + st));
         }
-      for (int i = 0; i < 2 * walk.n; ++i) {
-        const int st = i % L::STAGES;
-        if (!cta.wait(L::EMPTY + st, (i / L::STAGES & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT)) break;
-        mbar_expect_tx(cta.bar(L::FULL + st), L::TILE);
-        load_tile<HD, ATT_TILE>(stages + st * L::TILE, i & 1 ? &tmV : &tmK, b, kv_head, walk.tile(i >> 1) * ATT_TILE, cta.bar(L::FULL + st));
       }
       grid_release();
     }
@@ -106,174 +123,217 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue: probabilities
     // are read before the next scores of their unit are written over them
     if (elect_one_sync()) {
-      auto full = [&](int i) { return cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
-      auto scores = [&](int u, int i) {
-        multiply_rows<HD>(L::S_COL + u * ATT_TILE, q_tile + u * L::TILE, stages + i % L::STAGES * L::TILE);
-        umma_commit(cta.bar(L::SCORES + u));
-      };
-      bool ok = walk.n > 0 && full(0);
-      bool first[2] = {true, true};   // a unit's sums are not begun
-      uint32_t turns[2] = {0, 0};     // tiles that a unit has taken
-      if (ok) {
-        for (int u = 0; u < 2 && ok; ++u)
-          if (unit[u].live) {
-            ok = cta.wait(L::Q + u, 0, DEV_ERR_FULL_BAR_TIMEOUT);
+      auto full = [&](uint32_t i) { return cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
+      uint32_t at = 0, q_used[2] = {0, 0}, turns[2] = {0, 0}, cleared = 0;   // loads, units and their tiles so far
+      bool ok = true;
+      for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+        const AttnFwdItem w(s, dealt(turn));
+        if (w.n == 0) continue;
+        auto scores = [&](int u, uint32_t i, int t) {
+          multiply_rows<HD>(L::S_COL + u * ATT_TILE, q_tile + u * L::TILE, stage(i));
+          umma_commit(cta.bar(L::SCORES + u));
+          if (t == w.unit[u].hi) umma_commit(cta.bar(L::QREAD + u));
+        };
+        bool begun[2] = {false, false};   // a unit's sums
+        if (!(ok = full(at))) break;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (w.unit[u].live) {
+            ok = ok && cta.wait(L::Q + u, q_used[u]++ & 1, DEV_ERR_FULL_BAR_TIMEOUT);
             tc_fence_after();
-            if (ok && walk.uses(unit[u], walk.tile(0))) scores(u, 0);
+            if (ok && w.uses(u, w.tile(0))) scores(u, at, w.tile(0));
           }
-        umma_commit(cta.bar(L::EMPTY));
-      }
-      for (int j = 0; j < walk.n && ok; ++j) {
-        const int t = walk.tile(j), next = walk.tile(j + 1);
-        const bool more = j + 1 < walk.n;
-        if (!(ok = full(2 * j + 1) && (!more || full(2 * j + 2)))) break;
-        if (!more && clear_from < ATT_TILE) {
-          mbar_arrive(cta.bar(L::CLEAR));
-          if (!(ok = cta.wait(L::CLEARED, 0, DEV_ERR_FULL_BAR_TIMEOUT))) break;
-        }
-        const uint32_t v_low = TileDesc<ATT_TILE, true>::low(stages + (2 * j + 1) % L::STAGES * L::TILE);
+        umma_commit(cta.bar(L::EMPTY + at % L::STAGES));
+        for (int j = 0; j < w.n && ok; ++j, at += 2) {
+          const int t = w.tile(j), next = w.tile(j + 1);
+          const bool more = j + 1 < w.n;
+          if (!(ok = full(at + 1) && (!more || full(at + 2)))) break;
+          if (!more && w.clear_from < ATT_TILE) {
+            mbar_arrive(cta.bar(L::CLEAR));
+            if (!(ok = cta.wait(L::CLEARED, cleared++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
+          }
+          const uint32_t v_low = TileDesc<ATT_TILE, true>::low(stage(at + 1));
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (walk.uses(unit[u], t)) {
-            // in two parts, as they are there
+          for (int u = 0; u < 2; ++u) {
+            if (w.uses(u, t)) {
+              // in two parts, as they are there
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
-              tc_fence_after();
-              multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 4, part || !first[u]);
+              for (int part = 0; part < 2; ++part) {
+                if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+                tc_fence_after();
+                if (part == 0) multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, 0, begun[u]);
 #pragma unroll
-              for (int k = 1; k < 4; ++k) multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 4 + k, true);
+                for (int k = part ? L::FIRST / 16 : 1; k < (part ? ATT_TILE : L::FIRST) / 16; ++k)
+                  multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, k, true);
+              }
+              if (!ok) break;
+              begun[u] = true;
+              ++turns[u];
+              if (t == w.unit[u].hi) umma_commit(cta.bar(L::DONE + u));
             }
-            if (!ok) break;
-            first[u] = false;
-            ++turns[u];
+            if (more && w.uses(u, next)) scores(u, at + 2, next);
           }
-          if (more && walk.uses(unit[u], next)) scores(u, 2 * j + 2);
-          if (!more) umma_commit(cta.bar(L::DONE + u));
+          if (!ok) break;
+          umma_commit(cta.bar(L::EMPTY + (at + 1) % L::STAGES));
+          if (more) umma_commit(cta.bar(L::EMPTY + (at + 2) % L::STAGES));
         }
-        if (!ok) break;
-        umma_commit(cta.bar(L::EMPTY + (2 * j + 1) % L::STAGES));
-        if (more) umma_commit(cta.bar(L::EMPTY + (2 * j + 2) % L::STAGES));
       }
     }
   } else if (warp == R::ZERO) {
-    // ---------------------------------------------------------------- v behind the sequence's end, in the last tile of the walk
-    const int i = 2 * walk.n - 1;
-    if (clear_from < ATT_TILE && cta.wait(L::CLEAR, 0, DEV_ERR_FULL_BAR_TIMEOUT) && cta.wait(L::FULL + i % L::STAGES, i / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT))
-      zero_rows<HD, ATT_TILE>(stages + i % L::STAGES * L::TILE, clear_from, cta.bar(L::CLEARED));
+    // ---------------------------------------------------------------- v behind a sequence's end, in the last tile of a walk
+    uint32_t at = 0, cleared = 0;
+    for (int turn = 0; s.lengths && dealt(turn) < items; ++turn) {
+      const AttnFwdItem w(s, dealt(turn));
+      at += 2 * w.n;
+      if (w.clear_from == ATT_TILE) continue;
+      if (!cta.wait(L::CLEAR, cleared++ & 1, DEV_ERR_FULL_BAR_TIMEOUT) || !cta.wait(L::FULL + (at - 1) % L::STAGES, (at - 1) / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT)) break;
+      zero_rows<HD, ATT_TILE>(stage(at - 1), w.clear_from, cta.bar(L::CLEARED));
+    }
   } else {
     // ---------------------------------------------------------------- softmax: a thread has a row
     const int u = warp >> 2;
-    AttnUnit me = attn_unit(s, kv_head, 2 * pair + u, len);
-    if (2 * pair + u >= units) me.live = false;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE, o_col = lanes + L::O_COL + u * 128;
-    const int i = me.i0 + (warp & 3) * 32 + lane;
     const float c = s.scale * ATT_LOG2E;
     const Pair c2 = both(c);
-    // this unit's own tiles of the walk
-    const int far = me.live ? min(walk.sink_tiles, me.lo) : 0, n = me.live ? far + me.hi - me.lo + 1 : 0;
-    float top = -INFINITY, sum = 0.f;   // of the scores times c, as far as the sums are scaled to it; relative to 2^top
+    const uint32_t slab = cta.smem + L::OUT + warp * 4096;
+    uint32_t turns = 0, done = 0;   // tiles and units so far
     bool ok = true;
 #pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int j0 = (j < far ? j : me.lo + j - far) * ATT_TILE;
-      if (!(ok = cta.wait(L::SCORES + u, j & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
-      tc_fence_after();
-      uint32_t x[4][32];
+    for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+      const AttnFwdItem w(s, dealt(turn));
+      AttnUnit me = w.unit[0];
+      if (u) me = w.unit[1];
+      if (!me.exists) continue;
+      const int i = me.i0 + (warp & 3) * 32 + lane;
+      // this unit's own tiles of the walk
+      const int far = min(w.sink_tiles, me.lo), n = me.live ? far + me.hi - me.lo + 1 : 0;
+      float top = -INFINITY, sum = 0.f;   // of the scores times c, as far as the sums are scaled to it; relative to 2^top
+#pragma unroll 1
+      for (int j = 0; j < n; ++j, ++turns) {
+        const int j0 = (j < far ? j : me.lo + j - far) * ATT_TILE;
+        if (!(ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+        tc_fence_after();
+        const bool whole = j0 + ATT_TILE - 1 <= me.i0 && (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks);
+        const int last = i - j0, first = s.window ? last - s.window + 1 : 0, sinks = s.window ? s.sinks - j0 : 0;
+        auto hide = [&](uint32_t(&x)[32], int k) {   // of columns from 32 k on
+          const uint32_t seen = columns_seen(first - k * 32, last - k * 32, sinks - k * 32);
+          if (__all_sync(0xffffffffu, seen == 0xffffffffu)) return;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) tmem_ld_32x32(s_col + k * 32, x[k]);
-      tmem_ld_wait();
-      if (!(j0 + ATT_TILE - 1 <= me.i0 && (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks))) {
-        const int last = i - j0, first = s.window ? last - s.window + 1 : -1, sinks = s.window ? s.sinks - j0 : 0;
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1)) x[e] = 0xFF800000u;   // -inf
+        };
+        // Scores are read twice, for their maximum and for the probabilities, half of a row at a time: a whole one with what else is needed is more than
+        // a thread has registers
+        uint32_t x[32], y[32];
+        float some[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; k += 2) {
+          tmem_ld_32x32(s_col + k * 32, x);
+          tmem_ld_32x32(s_col + k * 32 + 32, y);
+          tmem_ld_wait();
+          if (!whole) hide(x, k), hide(y, k + 1);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int at = k * 32 + e;
-            if (at > last || (at < first && at >= sinks)) x[k][e] = 0xFF800000u;   // -inf
-          }
-      }
-      float some[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        some[k] = __uint_as_float(x[k][0]);
-#pragma unroll
-        for (int e = 1; e < 31; e += 2) some[k] = most_of(some[k], __uint_as_float(x[k][e]), __uint_as_float(x[k][e + 1]));
-        some[k] = most_of(some[k], __uint_as_float(x[k][31]), __uint_as_float(x[k][31]));
-      }
-      const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
-      // The sums are scaled to a new maximum only where one of the warp's rows has grown by more than 2^8: probabilities beside the old one stay in
-      // range. A NaN grows, too, and makes one of everything in its row.
-      if (__any_sync(0xffffffffu, !(most <= top + 8.f))) {
-        const float now = most_of(top, most, most);
-        const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
-        top = now;
-        sum *= f;
-        if (j) {
-#pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            uint32_t o[16];
-            tmem_ld_32x16(o_col + k * 16, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st_32x16(o_col + k * 16, o);
+          for (int e = 0; e < 32; e += 4) {
+            some[0] = most_of(some[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            some[1] = most_of(some[1], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+            some[2] = most_of(some[2], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+            some[3] = most_of(some[3], __uint_as_float(y[e + 2]), __uint_as_float(y[e + 3]));
           }
         }
-      }
-      const Pair ref = both(top == -INFINITY ? 0.f : -top);
-      Pair part[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+        const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
+        // The sums are scaled to a new maximum only where one of the warp's rows has grown by more than 2^8: probabilities beside the old one stay in
+        // range. A NaN grows, too, and makes one of everything in its row.
+        if (__any_sync(0xffffffffu, !(most <= top + 8.f))) {
+          const float now = most_of(top, most, most);
+          const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
+          top = now;
+          sum *= f;
+          if (j) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t p[16];
+            for (int k = 0; k < HD / 16; ++k) {
+              uint32_t o[16];
+              tmem_ld_32x16(o_col + k * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float p0, p1;
-          exp2_pair(e, fma2(pair_of(x[k][e], x[k][e + 1]), c2, ref), p0, p1);
-          part[e / 2 & 3] = part[e / 2 & 3] + Pair(p0, p1);
-          p[e / 2] = pack_bf16x2(p0, p1);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st_32x16(o_col + k * 16, o);
+            }
+          }
         }
-        tmem_st_32x16(s_col + k * 16, p);   // over scores that all are in registers
-        if (k & 1) {
+        const Pair ref = both(top == -INFINITY ? 0.f : -top);
+        Pair part[2] = {both(0.f), both(0.f)};
+        auto probabilities = [&](const uint32_t(&x)[32], int k) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float p0, p1;
+            exp2_pair(e, fma2(pair_of(x[e], x[e + 1]), c2, ref), p0, p1);
+            part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
+            p[e / 2] = pack_bf16x2(p0, p1);
+          }
+          tmem_st_32x16(s_col + k * 16, p);
+        };
+        auto hand_over = [&](int which) {
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + (k >> 1)));
-        }
+          if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + which));
+        };
+        // probabilities of 32 columns come to lie over columns that have been read
+        tmem_ld_32x32(s_col, x);
+        tmem_ld_32x32(s_col + 32, y);
+        tmem_ld_wait();
+        if (!whole) hide(x, 0), hide(y, 1);
+        probabilities(x, 0);
+        tmem_ld_32x32(s_col + 64, x);
+        probabilities(y, 1);
+        tmem_ld_32x32(s_col + 96, y);
+        tmem_ld_wait();
+        if (!whole) hide(x, 2), hide(y, 3);
+        probabilities(x, 2);
+        static_assert(L::FIRST == 96, "three quarters of the columns");
+        hand_over(0);
+        probabilities(y, 3);
+        hand_over(1);
+        float a, d;
+        (part[0] + part[1]).to(a, d);
+        sum += a + d;
       }
-      float a, d;
-      ((part[0] + part[1]) + (part[2] + part[3])).to(a, d);
-      sum += a + d;
-    }
-    if (2 * pair + u < units) {
-      if (ok && n) ok = cta.wait(L::DONE + u, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
+      if (ok && n) ok = cta.wait(L::DONE + u, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
       tc_fence_after();
-      const bool mine = i < len;
+      const bool mine = i < w.len;
       // no probability behind the end
-      minus_lse[(static_cast<int64_t>(b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
+      minus_lse[(static_cast<int64_t>(w.b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
       const float f = 1.f / sum;
-      uint4* row = reinterpret_cast<uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + me.head) * HD);
+      const bool any = mine && n && ok;
 #pragma unroll
-      for (int k = 0; k < HD / 32; ++k) {
-        uint32_t o[32];
+      for (int k = 0; k < HD / 64; ++k) {
+        uint32_t o[2][32];
         if (n && ok) {
-          tmem_ld_32x32(o_col + k * 32, o);
+          tmem_ld_32x32(o_col + k * 64, o[0]);
+          tmem_ld_32x32(o_col + k * 64 + 32, o[1]);
           tmem_ld_wait();
         }
-        if (i < s.S) {
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (mine && n && ok) {
-              auto two = [&](int at) { return pack_bf16x2(__uint_as_float(o[at]) * f, __uint_as_float(o[at + 1]) * f); };
-              v = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
-            }
-            row[k * 4 + e / 8] = v;
-          }
+        for (int e = 0; e < 64; e += 8) {
+          auto two = [&](int at) {
+            return any ? pack_bf16x2(__uint_as_float(o[at >> 5][at & 31]) * f, __uint_as_float(o[at >> 5][(at & 31) + 1]) * f) : 0u;
+          };
+          st_shared_v4(slab + lane * 128 + ((e / 8 ^ (lane & 7)) << 4), two(e), two(e + 2), two(e + 4), two(e + 6));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(&tmO, slab, k * 64, me.head, me.i0 + (warp & 3) * 32, w.b);
+          tma_store_commit();
         }
       }
+      tc_fence_before();   // the sums are read: by the next handing over of probabilities they may be written
     }
+    if (lane == 0) tma_store_wait<0>();
   }
   attn_end<R>(cta);
 }
@@ -325,8 +385,8 @@ struct AttnBwd {
   static constexpr int TILES = STAT + (KEYS ? N1 * STATS : 0);
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
   static_assert(SMEM <= 232448, "more than a CTA's shared memory");
-  static constexpr int FULL1 = 0, EMPTY1 = FULL1 + N1, FULL2 = EMPTY1 + N1, EMPTY2 = FULL2 + N2, THERE = EMPTY2 + N2;
-  static constexpr int T1 = THERE + 1, T2 = T1 + (KEYS ? 1 : 2), DONE = T2 + 1;            // T1 and T2 there, sums done
+  static constexpr int FULL1 = 0, EMPTY1 = FULL1 + N1, FULL2 = EMPTY1 + N1, EMPTY2 = FULL2 + N2, THERE = EMPTY2 + N2, HELD_READ = THERE + 1;
+  static constexpr int T1 = HELD_READ + 1, T2 = T1 + (KEYS ? 1 : 2), DONE = T2 + 1;            // T1 and T2 there, sums done
   static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1;
   // rows behind a sequence's end are to be cleared, are zeros: of both passing tensors
   static constexpr int CLEAR1 = GRADS + 1, CLEARED1 = CLEAR1 + 1, CLEAR2 = CLEARED1 + 1, CLEARED2 = CLEAR2 + 1, BARS = CLEARED2 + 1;  // P and dS there: by all warps
@@ -340,182 +400,228 @@ struct AttnSplit {
   float* sums;   // [1 + parts][B * nkv * tiles][dv, dk][128][HD]
 };
 
+// An item: a held tile and its walk, `far` passing tiles from 0, then tiles from `lo` on, per_head in all; with KEYS for each head of the group.
+template <bool KEYS>
+struct AttnBwdItem {
+  int b, head, first_head, len, r0;   // first_head: of the passing tensors
+  int tile, part, far, lo, per_head, n;
+  int clear_from;   // from which row on a head's last tile is not the sequence's: what TMA does not fill with zeros by itself
+  bool joined;      // its sums are one part of several
+  __device__ __forceinline__ int row(int at) const { return (at < far ? at : lo + at - far) * ATT_TILE; }   // the first one of a head's at-th tile
+
+  __device__ __forceinline__ AttnBwdItem(const AttnShape& s, const AttnSplit& split, int item) {
+    const int heads = s.B * (KEYS ? s.nkv : s.nq), tiles = s.rows / ATT_TILE;
+    const int split_items = KEYS ? heads * split.tiles * split.parts : 0;
+    part = far = 0;
+    int index = item;
+    if (index < split_items) {
+      part = index / (heads * split.tiles);
+      index -= part * heads * split.tiles;
+      ++part;
+      tile = index / heads;
+      index -= tile * heads;
+    } else {
+      index -= split_items;
+      tile = index / heads;
+      index -= tile * heads;
+      if (!KEYS) tile = tiles - 1 - tile;   // the longest walks first
+    }
+    const int of_batch = KEYS ? s.nkv : s.nq;
+    b = index / of_batch;
+    head = index - b * of_batch;
+    first_head = KEYS ? head * s.G : head / s.G;
+    len = sequence_length(s, b), r0 = tile * ATT_TILE;
+    joined = KEYS && split.parts > 0 && tile < split.tiles;
+    if constexpr (KEYS) {
+      // queries of the window: up to the last key's; of the far parts: behind those
+      const int end = (len + ATT_TILE - 1) / ATT_TILE;
+      const int near = s.window ? min(end, (r0 + ATT_TILE - 1 + s.window - 1) / ATT_TILE + 1) : end;
+      lo = tile;
+      int hi = near;
+      if (part) {
+        lo = min(near + (part - 1) * split.part_tiles, end);
+        hi = min(lo + split.part_tiles, end);
+      } else if (s.window && !joined && r0 < s.sinks) {
+        hi = end;   // sinks whose walk is not split
+      }
+      per_head = r0 < len ? max(0, hi - lo) : 0;
+    } else {
+      const int last = min(r0 + ATT_TILE, len) - 1;
+      lo = s.window ? max(0, r0 - s.window + 1) / ATT_TILE : 0;
+      far = s.window ? min((s.sinks + ATT_TILE - 1) / ATT_TILE, lo) : 0;
+      per_head = r0 < len ? far + last / ATT_TILE - lo + 1 : 0;
+    }
+    n = (KEYS ? s.G : 1) * per_head;
+    clear_from = n > 0 && len < s.S ? min(len - row(per_head - 1), ATT_TILE) : ATT_TILE;
+  }
+};
+
 template <int HD, bool KEYS>
 __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const __grid_constant__ CUtensorMap tmD, const float* minus_lse, const float* minus_delta, bf16* grad1, bf16* grad2, AttnShape s,
-                         AttnSplit split, int* err_word) {
+                         AttnSplit split, int items, int* err_word) {
   using L = AttnBwd<HD, KEYS>;
   using R = AttnBwdRoles;
+  using Item = AttnBwdItem<KEYS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::READ && i < L::CLEAR1 ? R::LOAD : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // this CTA's tile and its walk: `far` tiles from 0, then tiles from `lo` on, `per_head` in all; with KEYS for each head of the group
-  int b, head, tile, part = 0, far = 0, lo = 0, per_head;
-  int index = blockIdx.x;
-  const int heads = s.B * (KEYS ? s.nkv : s.nq), tiles = s.rows / ATT_TILE;
-  const int split_ctas = KEYS ? heads * split.tiles * split.parts : 0;
-  if (index < split_ctas) {
-    part = 1 + index / (heads * split.tiles);
-    index %= heads * split.tiles;
-    tile = index / heads;
-  } else {
-    index -= split_ctas;
-    tile = KEYS ? index / heads : tiles - 1 - index / heads;   // the longest walks first
-  }
-  b = index % heads;
-  head = b % (KEYS ? s.nkv : s.nq);
-  b /= KEYS ? s.nkv : s.nq;
-  const int len = sequence_length(s, b), r0 = tile * ATT_TILE;
-  const bool joined = KEYS && split.parts > 0 && tile < split.tiles;
-  if constexpr (KEYS) {
-    // queries of the window: up to the last key's; of the far parts: behind those
-    const int end = (len + ATT_TILE - 1) / ATT_TILE;
-    const int near = s.window ? min(end, (r0 + ATT_TILE - 1 + s.window - 1) / ATT_TILE + 1) : end;
-    lo = tile;
-    int hi = near;
-    if (part) {
-      lo = min(near + (part - 1) * split.part_tiles, end);
-      hi = min(lo + split.part_tiles, end);
-    } else if (s.window && !joined && r0 < s.sinks) {
-      hi = end;   // sinks whose walk is not split
-    }
-    per_head = r0 < len ? max(0, hi - lo) : 0;
-  } else {
-    const int last = min(r0 + ATT_TILE, len) - 1;
-    lo = s.window ? max(0, r0 - s.window + 1) / ATT_TILE : 0;
-    far = s.window ? min((s.sinks + ATT_TILE - 1) / ATT_TILE, lo) : 0;
-    per_head = r0 < len ? far + last / ATT_TILE - lo + 1 : 0;
-  }
-  const int group = KEYS ? s.G : 1, n = group * per_head;
-  const int first_head = KEYS ? head * s.G : head / s.G;   // of the passing tensors
-  auto row_of = [&](int at) { return (at < far ? at : lo + at - far) * ATT_TILE; };   // the first row of a head's at-th tile
-  // from which row on a head's last tile is not the sequence's: what TMA does not fill with zeros by itself
-  const int clear_from = n > 0 && len < s.S ? len - row_of(per_head - 1) : ATT_TILE;
-  auto pass1 = [&](int i) { return cta.smem + L::PASS1 + i % L::N1 * L::TILE; };
-  auto pass2 = [&](int i) { return cta.smem + L::PASS2 + i % L::N2 * L::TILE; };
-  auto stats = [&](int i) { return cta.smem + L::STAT + i % L::N1 * L::STATS; };
+  // numbers of passing tiles count over all items
+  auto pass1 = [&](uint32_t i) { return cta.smem + L::PASS1 + i % L::N1 * L::TILE; };
+  auto pass2 = [&](uint32_t i) { return cta.smem + L::PASS2 + i % L::N2 * L::TILE; };
+  auto full1 = [&](uint32_t i) { return cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
+  auto full2 = [&](uint32_t i) { return cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT); };
 
   if (warp == R::LOAD) {
     // ---------------------------------------------------------------- loads
-    if (elect_one_sync() && n > 0) {
-      mbar_expect_tx(cta.bar(L::THERE), 2 * L::TILE);
-      load_tile<HD, ATT_TILE>(cta.smem, KEYS ? &tmK : &tmQ, b, head, r0, cta.bar(L::THERE));
-      load_tile<HD, ATT_TILE>(cta.smem + L::TILE, KEYS ? &tmV : &tmD, b, head, r0, cta.bar(L::THERE));
-      int i = 0;
+    if (elect_one_sync()) {
+      uint32_t i = 0, held = 0;
       bool ok = true;
-      for (int g = 0; g < group && ok; ++g)
-        for (int at = 0; at < per_head; ++at, ++i) {
-          const int row = row_of(at);
-          const uint32_t full1 = cta.bar(L::FULL1 + i % L::N1), full2 = cta.bar(L::FULL2 + i % L::N2);
+      for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+        const Item w(s, split, dealt(turn));
+        if (w.n == 0) continue;
+        if (!(ok = cta.wait(L::HELD_READ, (held++ & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
+        mbar_expect_tx(cta.bar(L::THERE), 2 * L::TILE);
+        load_tile<HD, ATT_TILE>(cta.smem, KEYS ? &tmK : &tmQ, w.b, w.head, w.r0, cta.bar(L::THERE));
+        load_tile<HD, ATT_TILE>(cta.smem + L::TILE, KEYS ? &tmV : &tmD, w.b, w.head, w.r0, cta.bar(L::THERE));
+        int at = 0, head = w.first_head;
+        for (int k = 0; k < w.n; ++k, ++i) {
+          const int row = w.row(at);
+          const uint32_t bar1 = cta.bar(L::FULL1 + i % L::N1), bar2 = cta.bar(L::FULL2 + i % L::N2);
           if (!(ok = cta.wait(L::EMPTY1 + i % L::N1, (i / L::N1 & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
-          mbar_expect_tx(full1, L::TILE + (KEYS ? L::STATS : 0));
-          load_tile<HD, ATT_TILE>(pass1(i), KEYS ? &tmQ : &tmK, b, first_head + g, row, full1);
+          mbar_expect_tx(bar1, L::TILE + (KEYS ? L::STATS : 0));
+          load_tile<HD, ATT_TILE>(pass1(i), KEYS ? &tmQ : &tmK, w.b, head, row, bar1);
           if constexpr (KEYS) {
-            const int64_t from = (static_cast<int64_t>(b) * s.nq + first_head + g) * s.rows + row;
-            bulk_load(stats(i), minus_lse + from, ATT_TILE * 4, full1);
-            bulk_load(stats(i) + ATT_TILE * 4, minus_delta + from, ATT_TILE * 4, full1);
+            const uint32_t stats = cta.smem + L::STAT + i % L::N1 * L::STATS;
+            const int64_t from = (static_cast<int64_t>(w.b) * s.nq + head) * s.rows + row;
+            bulk_load(stats, minus_lse + from, ATT_TILE * 4, bar1);
+            bulk_load(stats + ATT_TILE * 4, minus_delta + from, ATT_TILE * 4, bar1);
           }
           if (!(ok = cta.wait(L::EMPTY2 + i % L::N2, (i / L::N2 & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
-          mbar_expect_tx(full2, L::TILE);
-          load_tile<HD, ATT_TILE>(pass2(i), KEYS ? &tmD : &tmV, b, first_head + g, row, full2);
+          mbar_expect_tx(bar2, L::TILE);
+          load_tile<HD, ATT_TILE>(pass2(i), KEYS ? &tmD : &tmV, w.b, head, row, bar2);
+          if (++at == w.per_head) at = 0, ++head;
         }
+      }
       grid_release();
     }
   } else if (warp == R::MMA) {
     // ---------------------------------------------------------------- products. Of one thread they run in the order of their issue
     if (elect_one_sync()) {
-      bool ok = n > 0 && cta.wait(L::THERE, 0, DEV_ERR_FULL_BAR_TIMEOUT);
-      int left1 = per_head, left2 = per_head;   // tiles of a head that are to come, of each of the passing tensors
-      uint32_t cleared1 = 0, cleared2 = 0;
-      auto t1 = [&](int i) {
-        if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
-        if (--left1 == 0) {
-          left1 = per_head;
-          if (clear_from < ATT_TILE) {
-            mbar_arrive(cta.bar(L::CLEAR1));
-            if (!(ok = cta.wait(L::CLEARED1, cleared1++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+      uint32_t base = 0, held = 0, cleared1 = 0, cleared2 = 0;
+      bool ok = true;
+      for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+        const Item w(s, split, dealt(turn));
+        const int n = w.n;
+        if (n == 0) continue;
+        if (!(ok = cta.wait(L::THERE, held++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
+        int left1 = w.per_head, left2 = w.per_head;   // tiles of a head that are to come, of each of the passing tensors
+        auto t1 = [&](int k) {
+          const uint32_t i = base + k;
+          if (!(ok = full1(i))) return;
+          if (--left1 == 0) {
+            left1 = w.per_head;
+            if (w.clear_from < ATT_TILE) {
+              mbar_arrive(cta.bar(L::CLEAR1));
+              if (!(ok = cta.wait(L::CLEARED1, cleared1++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+            }
           }
-        }
-        tc_fence_after();
-        const int two = KEYS ? 0 : i & 1;
-        multiply_rows<HD>(L::T1_COL + two * 128, cta.smem, pass1(i));
-        umma_commit(cta.bar(L::T1 + two));
-      };
-      auto t2 = [&](int i) {
-        if (!(ok = cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
-        if (--left2 == 0) {
-          left2 = per_head;
-          if (clear_from < ATT_TILE) {
-            mbar_arrive(cta.bar(L::CLEAR2));
-            if (!(ok = cta.wait(L::CLEARED2, cleared2++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
-          }
-        }
-        tc_fence_after();
-        multiply_rows<HD>(L::T2_COL, cta.smem + L::TILE, pass2(i));
-        umma_commit(cta.bar(L::T2));
-        if constexpr (!KEYS) umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
-      };
-      // sum += operand tile; the operand of each group's 32 columns lies over those columns
-      auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, bool begun, int freed) {
-        const uint32_t low = TileDesc<ATT_TILE, true>::low(tile_at);
-        multiply_step<HD, 32>(acc, operand, low, 0, begun);
-#pragma unroll
-        for (int k = 1; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand, low, k, true);
-        umma_commit(cta.bar(freed));
-      };
-      if (ok) t1(0);
-      if (ok) t2(0);
-      if (!KEYS && ok && n > 1) t1(1);
-      for (int i = 0; i < n && ok; ++i) {
-        if constexpr (KEYS) {
-          if (!(ok = cta.wait(L::PROBS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
           tc_fence_after();
-          add(L::ACC1_COL, L::T1_COL, pass2(i), i > 0, L::EMPTY2 + i % L::N2);
-          if (i + 1 < n) t1(i + 1);
+          const int two = KEYS ? 0 : i & 1;
+          multiply_rows<HD>(L::T1_COL + two * 128, cta.smem, pass1(i));
+          umma_commit(cta.bar(L::T1 + two));
+        };
+        auto t2 = [&](int k) {
+          const uint32_t i = base + k;
+          if (!(ok = full2(i))) return;
+          if (--left2 == 0) {
+            left2 = w.per_head;
+            if (w.clear_from < ATT_TILE) {
+              mbar_arrive(cta.bar(L::CLEAR2));
+              if (!(ok = cta.wait(L::CLEARED2, cleared2++ & 1, DEV_ERR_FULL_BAR_TIMEOUT))) return;
+            }
+          }
+          tc_fence_after();
+          multiply_rows<HD>(L::T2_COL, cta.smem + L::TILE, pass2(i));
+          umma_commit(cta.bar(L::T2));
+          if constexpr (!KEYS) umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
+          if (k + 1 == n) umma_commit(cta.bar(L::HELD_READ));   // the last product with a held tile
+        };
+        // sum += operand tile; the operand of each group's 32 columns lies over those columns
+        auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, bool begun, int freed) {
+          const uint32_t low = TileDesc<ATT_TILE, true>::low(tile_at);
+          multiply_step<HD, 32>(acc, operand, low, 0, begun);
+#pragma unroll
+          for (int k = 1; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand, low, k, true);
+          umma_commit(cta.bar(freed));
+        };
+        t1(0);
+        if (ok) t2(0);
+        if (!KEYS && ok && n > 1) t1(1);
+        for (int k = 0; k < n && ok; ++k) {
+          const uint32_t i = base + k;
+          if constexpr (KEYS) {
+            if (!(ok = cta.wait(L::PROBS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+            tc_fence_after();
+            add(L::ACC1_COL, L::T1_COL, pass2(i), k > 0, L::EMPTY2 + i % L::N2);
+            if (k + 1 < n) t1(k + 1);
+          }
+          if (!ok || !(ok = cta.wait(L::GRADS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+          tc_fence_after();
+          if (!KEYS && k + 1 < n) t2(k + 1);
+          if (!ok) break;
+          add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), k > 0, L::EMPTY1 + i % L::N1);
+          if (k + 1 == n) umma_commit(cta.bar(L::DONE));
+          if (KEYS && k + 1 < n) t2(k + 1);
+          if (!KEYS && k + 2 < n) t1(k + 2);
         }
-        if (!ok || !(ok = cta.wait(L::GRADS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
-        tc_fence_after();
-        if (!KEYS && i + 1 < n) t2(i + 1);
-        if (!ok) break;
-        add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), i > 0, L::EMPTY1 + i % L::N1);
-        if (KEYS && i + 1 < n) t2(i + 1);
-        if (!KEYS && i + 2 < n) t1(i + 2);
+        base += n;
       }
-      if (ok) umma_commit(cta.bar(L::DONE));
     }
   } else if (warp == R::ZERO) {
-    // ---------------------------------------------------------------- rows behind the sequence's end, in the last tile of each head
-    if (clear_from < ATT_TILE)
-      for (int i = per_head - 1, g = 0; i < n; i += per_head, ++g) {
-        if (!cta.wait(L::CLEAR1, g & 1, DEV_ERR_FULL_BAR_TIMEOUT) || !cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT)) break;
-        zero_rows<HD, ATT_TILE>(pass1(i), clear_from, cta.bar(L::CLEARED1));
-        if (!cta.wait(L::CLEAR2, g & 1, DEV_ERR_FULL_BAR_TIMEOUT) || !cta.wait(L::FULL2 + i % L::N2, i / L::N2 & 1, DEV_ERR_FULL_BAR_TIMEOUT)) break;
-        zero_rows<HD, ATT_TILE>(pass2(i), clear_from, cta.bar(L::CLEARED2));
-      }
+    // ---------------------------------------------------------------- rows behind a sequence's end, in the last tile of each head
+    uint32_t base = 0, cleared = 0;
+    bool ok = true;
+    for (int turn = 0; s.lengths && ok && dealt(turn) < items; ++turn) {
+      const Item w(s, split, dealt(turn));
+      if (w.clear_from < ATT_TILE)
+        for (int k = w.per_head - 1; k < w.n && ok; k += w.per_head, ++cleared) {
+          const uint32_t i = base + k;
+          if (!(ok = cta.wait(L::CLEAR1, cleared & 1, DEV_ERR_FULL_BAR_TIMEOUT) && full1(i))) break;
+          zero_rows<HD, ATT_TILE>(pass1(i), w.clear_from, cta.bar(L::CLEARED1));
+          if (!(ok = cta.wait(L::CLEAR2, cleared & 1, DEV_ERR_FULL_BAR_TIMEOUT) && full2(i))) break;
+          zero_rows<HD, ATT_TILE>(pass2(i), w.clear_from, cta.bar(L::CLEARED2));
+        }
+      base += w.n;
+    }
   } else {
     // ---------------------------------------------------------------- probabilities: a thread has 32 columns of a row of the held tile
     const int w = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const int r = r0 + (warp & 3) * 32 + lane;
     const Pair c = both(s.scale * ATT_LOG2E);
+    const uint8_t* const stat_base = smem_raw + (cta.smem - smem_u32(smem_raw)) + L::STAT + w * 128;
+    uint32_t i = 0, done = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+    const Item it(s, split, dealt(turn));
+    const int r0 = it.r0, r = r0 + (warp & 3) * 32 + lane;
     Pair my_lse, my_delta;
     if constexpr (!KEYS) {
-      const int64_t from = (static_cast<int64_t>(b) * s.nq + head) * s.rows + r;
+      const int64_t from = (static_cast<int64_t>(it.b) * s.nq + it.head) * s.rows + r;
       my_lse = both(minus_lse[from]);
       my_delta = both(minus_delta[from]);
     }
-    const uint8_t* const stat_base = smem_raw + (cta.smem - smem_u32(smem_raw)) + L::STAT + w * 128;
-    bool ok = true;
     int at = 0;
-    for (int i = 0; i < n; ++i) {
-      const int c0 = row_of(at) + w * 32;
-      if (++at == per_head) at = 0;
+#pragma unroll 1
+    for (int k = 0; k < it.n; ++k, ++i) {
+      const int c0 = it.row(at) + w * 32;
+      if (++at == it.per_head) at = 0;
       const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
       if constexpr (KEYS) {   // lse and delta of the stage
-        if (!(ok = cta.wait(L::FULL1 + i % L::N1, i / L::N1 & 1, DEV_ERR_FULL_BAR_TIMEOUT))) break;
+        if (!(ok = full1(i))) break;
       }
       if (!(ok = cta.wait(KEYS ? L::T1 : L::T1 + (i & 1), KEYS ? i & 1 : i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
       tc_fence_after();
@@ -547,6 +653,16 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(cta.bar(barrier));
       };
+      auto hide = [&](uint32_t(&packed)[16]) {   // also what zero times is not finite
+        const uint32_t seen = columns_seen(first, last, sinks);
+        if (__any_sync(0xffffffffu, seen + 1 > 1)) {   // neither none nor all of a row
+#pragma unroll
+          for (int e = 0; e < 16; ++e) packed[e] = seen_pair(packed[e], seen, e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) packed[e] &= seen;
+        }
+      };
       uint32_t p[32], y[32], o[16];
       tmem_ld_32x32(t1, p);
       tmem_ld_wait();
@@ -560,14 +676,10 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
         p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
       }
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (e > last || (e < first && e >= sinks)) p[e] = 0;
-      }
       if constexpr (KEYS) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
+        if (!whole) hide(o);
         tmem_st_32x16(t1, o);   // over columns that this warp has read
         arrive(L::PROBS);
       }
@@ -581,29 +693,30 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         row_numbers(1, e, d0, d1);
         float a, d;
         (pair_of(p[e], p[e + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
-        if (!whole) a = p[e] ? a : 0.f, d = p[e + 1] ? d : 0.f;   // zero times what is not finite
         o[e / 2] = pack_bf16x2(a, d);
         (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
-        if (!whole) a = p[e + 2] ? a : 0.f, d = p[e + 3] ? d : 0.f;
         o[e / 2 + 1] = pack_bf16x2(a, d);
       }
+      if (!whole) hide(o);
       tmem_st_32x16(KEYS ? t2 : t1, o);
       arrive(L::GRADS);
     }
     // ---------------------------------------------------------------- what the sums became
-    if (ok && n > 0) ok = cta.wait(L::DONE, 0, DEV_ERR_TMEM_FULL_TIMEOUT);
+    if (ok && it.n > 0) ok = cta.wait(L::DONE, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
     tc_fence_after();
-    const bool full = ok && n > 0, mine = r < len;
+    const bool full = ok && it.n > 0, mine = r < it.len;
     // KEYS: the first two groups of warps have dv, the others dk, half of the columns each; dq's columns are shared by four
     constexpr int COLS = KEYS ? HD / 2 : HD / 4;
     const int which = KEYS ? w >> 1 : 1, col = (KEYS ? w & 1 : w) * COLS;
     const uint32_t acc = lanes + (which ? L::ACC2_COL : L::ACC1_COL) + col;
     const float f = which ? s.scale : 1.f;
     const int out_heads = KEYS ? s.nkv : s.nq;
-    bf16* row = (which ? grad2 : grad1) + ((static_cast<int64_t>(b) * s.S + r) * out_heads + head) * HD + col;
+    bf16* row = (which ? grad2 : grad1) + ((static_cast<int64_t>(it.b) * s.S + r) * out_heads + it.head) * HD + col;
     float* sums = nullptr;
-    if (joined) sums = split.sums + (((static_cast<int64_t>(part) * heads * split.tiles + static_cast<int64_t>(tile) * heads + b * s.nkv + head) * 2 + which) *
-                                      ATT_TILE + (r - r0)) * HD + col;
+    if (it.joined) {
+      const int64_t heads = static_cast<int64_t>(s.B) * s.nkv, place = (it.part * split.tiles + it.tile) * heads + it.b * s.nkv + it.head;
+      sums = split.sums + ((place * 2 + which) * ATT_TILE + (r - r0)) * HD + col;
+    }
 #pragma unroll
     for (int k = 0; k < COLS / 16; ++k) {
       uint32_t o[16];
@@ -613,7 +726,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
-      if (joined) {
+      if (it.joined) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) reinterpret_cast<uint4*>(sums)[k * 4 + e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       } else if (r < s.S) {
@@ -621,6 +734,8 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 16; e += 8) reinterpret_cast<uint4*>(row)[k * 2 + e / 8] = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
       }
+    }
+    tc_fence_before();   // the sums are read
     }
   }
   attn_end<R>(cta);
@@ -651,14 +766,14 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnSplit split, bf
   *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
 }
 
-// [B][S][heads][HD] with element strides {batch, token, head}, boxes of 64 rows x 64 elements of a head
-static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd) {
+// [B][S][heads][HD] with element strides {batch, token, head}, boxes of 64 (or `rows`) rows x 64 elements of a head
+static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd, int rows = ATT_BOX) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) return B200_ERR_NO_DRIVER;
   auto pitch = [&](int size, long long stride) { return static_cast<cuuint64_t>(size == 1 ? hd : stride) * 2; };   // of a single one any will do
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(B)};
   const cuuint64_t strides[3] = {pitch(heads, t.head), pitch(S, t.token), pitch(B, t.batch)};
-  const cuuint32_t box[4] = {64, 1, ATT_BOX, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return 0;
@@ -685,14 +800,16 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
 
 template <int HD>
 static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, o;
+  const long long row = static_cast<long long>(s.nq) * HD;
+  if (int rc = attn_map(&o, {a.out, s.S * row, row, HD}, s.B, s.S, s.nq, HD, 32)) return rc;
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = allow_smem<attention_fwd_kernel<HD>>(AttnFwd<HD>::SMEM)) return rc;
-  const int units = s.rows / ATT_TILE * s.G;
-  launch_dependent(attention_fwd_kernel<HD>, s.B * s.nkv * ((units + 1) / 2), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v,
-                   static_cast<bf16*>(a.out), a.lse, s, device_status_word());
+  const int items = s.B * s.nkv * ((s.rows / ATT_TILE * s.G + 1) / 2);
+  launch_dependent(attention_fwd_kernel<HD>, std::min(items, sm_count()), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v, o,
+                   a.lse, s, items, device_status_word());
   B200_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -729,17 +846,20 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   const int tiles = s.rows / ATT_TILE;
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
-    launch_dependent(keys, s.B * s.nkv * (tiles + split.tiles * split.parts), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, a.lse, a.delta,
-                     static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, err);
+    const int items = s.B * s.nkv * (tiles + split.tiles * split.parts);
+    launch_dependent(keys, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, a.lse, a.delta,
+                     static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, items, err);
     if (split.parts) {
       const int64_t n = static_cast<int64_t>(s.B) * s.nkv * split.tiles * 2 * (ATT_TILE * HD / 4);
       launch_dependent(attention_join_kernel<HD>, static_cast<int>((n + 255) / 256), 256, 0, stream, split, static_cast<bf16*>(a.dv),
                        static_cast<bf16*>(a.dk), s);
     }
   }
-  if (a.dq)
-    launch_dependent(queries, s.B * s.nq * tiles, AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
-                     static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, nullptr}, err);
+  if (a.dq) {
+    const int items = s.B * s.nq * tiles;
+    launch_dependent(queries, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
+                     static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, nullptr}, items, err);
+  }
   B200_CUDA_OK(cudaGetLastError());
   return 0;
 }

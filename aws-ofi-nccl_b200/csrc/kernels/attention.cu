@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "attention.cuh"
 #include "b200ops.h"
@@ -22,6 +23,12 @@ namespace b200 {
 __device__ __forceinline__ int dealt(int turn) {
   const int ctas = gridDim.x, cta = blockIdx.x;
   return turn * ctas + (turn & 1 ? ctas - 1 - cta : cta);
+}
+
+// A number that the compiler takes for a new one: an item made of it again behind its walk costs less than the registers that keep it along the walk.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+r"(x));
+  return x;
 }
 
 // ------------------------------------------------------------------ forward
@@ -42,8 +49,8 @@ struct AttnFwdItem {
 
   __device__ __forceinline__ AttnFwdItem(const AttnShape& s, int item) {
     const int heads = s.B * s.nkv, units = s.rows / ATT_TILE * s.G;
-    const int nth = item / heads, pair = (units + 1) / 2 - 1 - nth, bh = item - nth * heads;
-    b = bh / s.nkv, kv_head = bh - b * s.nkv;
+    const int nth = s.by_heads_kv.quotient(item), pair = (units + 1) / 2 - 1 - nth, bh = item - nth * heads;
+    b = s.by_nkv.quotient(bh), kv_head = bh - b * s.nkv;
     len = sequence_length(s, b);
     sink_tiles = s.window ? (s.sinks + ATT_TILE - 1) / ATT_TILE : 0;
     lo = 1 << 30;
@@ -51,7 +58,7 @@ struct AttnFwdItem {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       AttnUnit& r = unit[u];
-      const int at = 2 * pair + u, rows = at / s.G;
+      const int at = 2 * pair + u, rows = s.by_G.quotient(at);
       r.head = kv_head * s.G + (at - rows * s.G);
       r.i0 = rows * ATT_TILE;
       r.exists = at < units;
@@ -201,20 +208,17 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     bool ok = true;
 #pragma unroll 1
     for (int turn = 0; ok && dealt(turn) < items; ++turn) {
-      const AttnFwdItem w(s, dealt(turn));
-      AttnUnit me = w.unit[0];
-      if (u) me = w.unit[1];
-      if (!me.exists) continue;
-      const int i = me.i0 + (warp & 3) * 32 + lane;
+      const AttnFwdItem walk(s, dealt(turn));
+      const int i0 = u ? walk.unit[1].i0 : walk.unit[0].i0, i = i0 + (warp & 3) * 32 + lane, lo = u ? walk.unit[1].lo : walk.unit[0].lo;
       // this unit's own tiles of the walk
-      const int far = min(w.sink_tiles, me.lo), n = me.live ? far + me.hi - me.lo + 1 : 0;
+      const int far = min(walk.sink_tiles, lo), n = (u ? walk.unit[1].live : walk.unit[0].live) ? far + (u ? walk.unit[1].hi : walk.unit[0].hi) - lo + 1 : 0;
       float top = -INFINITY, sum = 0.f;   // of the scores times c, as far as the sums are scaled to it; relative to 2^top
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++turns) {
-        const int j0 = (j < far ? j : me.lo + j - far) * ATT_TILE;
+        const int j0 = (j < far ? j : lo + j - far) * ATT_TILE;
         if (!(ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
         tc_fence_after();
-        const bool whole = j0 + ATT_TILE - 1 <= me.i0 && (s.window == 0 || me.i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks);
+        const bool whole = j0 + ATT_TILE - 1 <= i0 && (s.window == 0 || i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks);
         const int last = i - j0, first = s.window ? last - s.window + 1 : 0, sinks = s.window ? s.sinks - j0 : 0;
         auto hide = [&](uint32_t(&x)[32], int k) {   // of columns from 32 k on
           const uint32_t seen = columns_seen(first - k * 32, last - k * 32, sinks - k * 32);
@@ -268,7 +272,8 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float p0, p1;
-            exp2_pair(e, fma2(pair_of(x[e], x[e + 1]), c2, ref), p0, p1);
+            fma2(pair_of(x[e], x[e + 1]), c2, ref).to(p0, p1);
+            p0 = exp2_unit(p0), p1 = exp2_unit(p1);
             part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
             p[e / 2] = pack_bf16x2(p0, p1);
           }
@@ -300,6 +305,9 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         (part[0] + part[1]).to(a, d);
         sum += a + d;
       }
+      const AttnFwdItem w(s, dealt(anew(turn)));
+      const AttnUnit me = u ? w.unit[1] : w.unit[0];
+      if (!me.exists) continue;
       if (ok && n) ok = cta.wait(L::DONE + u, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
       tc_fence_after();
       const bool mine = i < w.len;
@@ -339,32 +347,45 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
 }
 
 // ------------------------------------------------------------------ backward
-// minus_delta[b][head][i] = -(sum over a row of dout * out), 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes.
+// minus_delta[b][head][i] = -(sum over a row of dout * out), 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes, two rows of a
+// thread at once.
+constexpr int DELTA_ROWS = 2;
 template <int HD>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, float* minus_delta, AttnShape s) {
+__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, float* minus_delta,
+                                                              AttnShape s, int blocks) {
+  constexpr int LANES = HD / 8, STEP = 256 / LANES;
+  const int b = blockIdx.x / blocks, v = threadIdx.x % LANES;
+  const int64_t first = static_cast<int64_t>(blockIdx.x - b * blocks) * (STEP * DELTA_ROWS);   // over [rows][nq]
+  const int token = first < INT_MAX ? s.by_nq.quotient(static_cast<int>(first)) : static_cast<int>(first / s.nq);
+  const int rest = static_cast<int>(first - static_cast<int64_t>(token) * s.nq) + threadIdx.x / LANES;
   grid_wait();
   grid_release();
-  constexpr int LANES = HD / 8;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;   // over [B][rows][nq]
-  const int v = threadIdx.x % LANES;
-  const bool there = row < static_cast<int64_t>(s.B) * s.rows * s.nq;
-  const int h = there ? static_cast<int>(row % s.nq) : 0;
-  const int64_t bt = there ? row / s.nq : 0;
-  const int b = static_cast<int>(bt / s.rows), i = static_cast<int>(bt % s.rows);
-  float sum = 0.f;
-  if (there && i < sequence_length(s, b)) {
-    const uint4 a = reinterpret_cast<const uint4*>(dout + b * db + i * dt + h * dh)[v];
-    const uint4 o = reinterpret_cast<const uint4*>(out + ((static_cast<int64_t>(b) * s.S + i) * s.nq + h) * HD)[v];
-    const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162*>(&a), *y = reinterpret_cast<const __nv_bfloat162*>(&o);
+  const int len = sequence_length(s, b);
+  uint4 a[DELTA_ROWS], o[DELTA_ROWS];
+  int h[DELTA_ROWS], i[DELTA_ROWS];
+#pragma unroll
+  for (int k = 0; k < DELTA_ROWS; ++k) {
+    const int more = s.by_nq.quotient(rest + k * STEP);
+    i[k] = token + more, h[k] = rest + k * STEP - more * s.nq;
+    a[k] = o[k] = make_uint4(0, 0, 0, 0);
+    if (i[k] < len) {
+      a[k] = reinterpret_cast<const uint4*>(dout + b * db + i[k] * dt + h[k] * dh)[v];
+      o[k] = reinterpret_cast<const uint4*>(out + ((static_cast<int64_t>(b) * s.S + i[k]) * s.nq + h[k]) * HD)[v];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < DELTA_ROWS; ++k) {
+    const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162*>(&a[k]), *y = reinterpret_cast<const __nv_bfloat162*>(&o[k]);
+    float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       sum = fmaf(__low2float(x[e]), __low2float(y[e]), sum);
       sum = fmaf(__high2float(x[e]), __high2float(y[e]), sum);
     }
-  }
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (there && v == 0) minus_delta[(static_cast<int64_t>(b) * s.nq + h) * s.rows + i] = -sum;
+    for (int d = LANES / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (v == 0 && i[k] < s.rows) minus_delta[(static_cast<int64_t>(b) * s.nq + h[k]) * s.rows + i[k]] = -sum;
+  }
 }
 
 // Both gradient kernels hold a tile of 128 rows and walk over tiles of 128 rows of the other side:
@@ -397,6 +418,7 @@ struct AttnBwd {
 // head, and their sums and those of the tile's own window are joined in order. parts 0: no tile has any.
 struct AttnSplit {
   int tiles, parts, part_tiles;
+  Divisor by_part;   // items of a part
   float* sums;   // [1 + parts][B * nkv * tiles][dv, dk][128][HD]
 };
 
@@ -414,22 +436,22 @@ struct AttnBwdItem {
     const int split_items = KEYS ? heads * split.tiles * split.parts : 0;
     part = far = 0;
     int index = item;
+    const Divisor &by_heads = KEYS ? s.by_heads_kv : s.by_heads_q, &by_head = KEYS ? s.by_nkv : s.by_nq;
     if (index < split_items) {
-      part = index / (heads * split.tiles);
+      part = split.by_part.quotient(index);
       index -= part * heads * split.tiles;
       ++part;
-      tile = index / heads;
+      tile = by_heads.quotient(index);
       index -= tile * heads;
     } else {
       index -= split_items;
-      tile = index / heads;
+      tile = by_heads.quotient(index);
       index -= tile * heads;
       if (!KEYS) tile = tiles - 1 - tile;   // the longest walks first
     }
-    const int of_batch = KEYS ? s.nkv : s.nq;
-    b = index / of_batch;
-    head = index - b * of_batch;
-    first_head = KEYS ? head * s.G : head / s.G;
+    b = by_head.quotient(index);
+    head = index - b * by_head.d;
+    first_head = KEYS ? head * s.G : s.by_G.quotient(head);
     len = sequence_length(s, b), r0 = tile * ATT_TILE;
     joined = KEYS && split.parts > 0 && tile < split.tiles;
     if constexpr (KEYS) {
@@ -604,21 +626,24 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     const uint8_t* const stat_base = smem_raw + (cta.smem - smem_u32(smem_raw)) + L::STAT + w * 128;
     uint32_t i = 0, done = 0;
     bool ok = true;
+    float my_lse = 0.f, my_delta = 0.f;
+    auto fetch = [&](const Item& of) {   // lse and delta of a row
+      if constexpr (!KEYS) {
+        const int64_t from = (static_cast<int64_t>(of.b) * s.nq + of.head) * s.rows + of.r0 + (warp & 3) * 32 + lane;
+        my_lse = minus_lse[from];
+        my_delta = minus_delta[from];
+      }
+    };
+    if (dealt(0) < items) fetch(Item(s, split, dealt(0)));
 #pragma unroll 1
     for (int turn = 0; ok && dealt(turn) < items; ++turn) {
-    const Item it(s, split, dealt(turn));
-    const int r0 = it.r0, r = r0 + (warp & 3) * 32 + lane;
-    Pair my_lse, my_delta;
-    if constexpr (!KEYS) {
-      const int64_t from = (static_cast<int64_t>(it.b) * s.nq + it.head) * s.rows + r;
-      my_lse = both(minus_lse[from]);
-      my_delta = both(minus_delta[from]);
-    }
+    const Item walk(s, split, dealt(turn));
+    const int r0 = walk.r0, r = r0 + (warp & 3) * 32 + lane, n = walk.n;
     int at = 0;
 #pragma unroll 1
-    for (int k = 0; k < it.n; ++k, ++i) {
-      const int c0 = it.row(at) + w * 32;
-      if (++at == it.per_head) at = 0;
+    for (int k = 0; k < n; ++k, ++i) {
+      const int c0 = walk.row(at) + w * 32;
+      if (++at == walk.per_head) at = 0;
       const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
       if constexpr (KEYS) {   // lse and delta of the stage
         if (!(ok = full1(i))) break;
@@ -644,7 +669,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           const ulonglong2 v = stat[of * (ATT_TILE / 4) + e / 4];
           p0.bits = v.x, p1.bits = v.y;
         } else {
-          p0 = p1 = of ? my_delta : my_lse;
+          p0 = p1 = both(of ? my_delta : my_lse);
         }
       };
       auto arrive = [&](int barrier) {
@@ -702,37 +727,61 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
       arrive(L::GRADS);
     }
     // ---------------------------------------------------------------- what the sums became
+    // while the last products run
+    if (!KEYS && dealt(turn + 1) < items) fetch(Item(s, split, dealt(turn + 1)));
+    const Item it(s, split, dealt(anew(turn)));
     if (ok && it.n > 0) ok = cta.wait(L::DONE, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
     tc_fence_after();
-    const bool full = ok && it.n > 0, mine = r < it.len;
+    const bool full = ok && it.n > 0, mine = it.r0 + (warp & 3) * 32 + lane < it.len;
     // KEYS: the first two groups of warps have dv, the others dk, half of the columns each; dq's columns are shared by four
     constexpr int COLS = KEYS ? HD / 2 : HD / 4;
     const int which = KEYS ? w >> 1 : 1, col = (KEYS ? w & 1 : w) * COLS;
     const uint32_t acc = lanes + (which ? L::ACC2_COL : L::ACC1_COL) + col;
     const float f = which ? s.scale : 1.f;
     const int out_heads = KEYS ? s.nkv : s.nq;
-    bf16* row = (which ? grad2 : grad1) + ((static_cast<int64_t>(it.b) * s.S + r) * out_heads + it.head) * HD + col;
+    const int row0 = it.r0 + (warp & 3) * 32;   // the warp's
+    bf16* const grad = (which ? grad2 : grad1) + ((static_cast<int64_t>(it.b) * s.S + row0) * out_heads + it.head) * HD + col;
+    const int64_t pitch = static_cast<int64_t>(out_heads) * HD;
     float* sums = nullptr;
     if (it.joined) {
       const int64_t heads = static_cast<int64_t>(s.B) * s.nkv, place = (it.part * split.tiles + it.tile) * heads + it.b * s.nkv + it.head;
-      sums = split.sums + ((place * 2 + which) * ATT_TILE + (r - r0)) * HD + col;
+      sums = split.sums + ((place * 2 + which) * ATT_TILE + (warp & 3) * 32) * HD + col;
     }
-#pragma unroll
-    for (int k = 0; k < COLS / 16; ++k) {
-      uint32_t o[16];
+    auto load = [&](int c, uint32_t(&o)[16]) {   // 16 columns, scaled
       if (full) {
-        tmem_ld_32x16(acc + k * 16, o);
+        tmem_ld_32x16(acc + c, o);
         tmem_ld_wait();
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
-      if (it.joined) {
+    };
+    auto two = [](const uint32_t(&o)[16], int e) { return pack_bf16x2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])); };
+    if constexpr (!KEYS && COLS % 32 == 0) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) reinterpret_cast<uint4*>(sums)[k * 4 + e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-      } else if (r < s.S) {
-        auto two = [&](int a) { return pack_bf16x2(__uint_as_float(o[a]), __uint_as_float(o[a + 1])); };
+      for (int c = 0; c < COLS; c += 32) {
+        uint32_t o[16], packed[16];
 #pragma unroll
-        for (int e = 0; e < 16; e += 8) reinterpret_cast<uint4*>(row)[k * 2 + e / 8] = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
+        for (int k = 0; k < 2; ++k) {
+          load(c + k * 16, o);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) packed[k * 8 + e] = two(o, e);
+        }
+        store_rows64(packed, [&](int at) { return row0 + at < s.S ? reinterpret_cast<uint4*>(grad + at * pitch + c) : nullptr; });
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < COLS; c += 16) {
+        uint32_t o[16];
+        load(c, o);
+        if (it.joined) {
+          uint4* const at = reinterpret_cast<uint4*>(sums + lane * HD + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) at[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        } else if (row0 + lane < s.S) {
+          uint4* const at = reinterpret_cast<uint4*>(grad + lane * pitch + c);
+          at[0] = make_uint4(two(o, 0), two(o, 1), two(o, 2), two(o, 3));
+          at[1] = make_uint4(two(o, 4), two(o, 5), two(o, 6), two(o, 7));
+        }
       }
     }
     tc_fence_before();   // the sums are read
@@ -794,6 +843,7 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
   s.sinks = s.window ? a.sinks : 0;
   s.lengths = a.lengths;
   s.scale = a.scale;
+  s.by_G = Divisor(s.G), s.by_nq = Divisor(s.nq), s.by_nkv = Divisor(s.nkv), s.by_heads_q = Divisor(s.B * s.nq), s.by_heads_kv = Divisor(s.B * s.nkv);
   // a CTA for each tile and head
   return static_cast<int64_t>(s.B) * s.nq * (s.rows / ATT_TILE) < (1ll << 30);
 }
@@ -816,7 +866,7 @@ static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
 
 // The walk of a sink's tile is split where there is a window: parts as long as a window's walk, but no more CTAs than some waves.
 static AttnSplit attn_split(const AttnShape& s, float* sums) {
-  AttnSplit p{0, 0, 0, sums};
+  AttnSplit p{0, 0, 0, Divisor(), sums};
   if (s.sinks == 0) return p;
   const int near = s.window / ATT_TILE + 2, all = s.rows / ATT_TILE;
   if (all <= 2 * near) return p;
@@ -824,6 +874,7 @@ static AttnSplit attn_split(const AttnShape& s, float* sums) {
   const int64_t most = std::max<int64_t>(1, 4 * 148 / (static_cast<int64_t>(s.B) * s.nkv * p.tiles));
   p.parts = static_cast<int>(std::min<int64_t>(most, (all - 1) / near));
   p.part_tiles = (all + p.parts - 1) / p.parts;
+  p.by_part = Divisor(s.B * s.nkv * p.tiles);
   return p;
 }
 
@@ -839,10 +890,11 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (int rc = allow_smem<attention_bwd_kernel<HD, true>>(AttnBwd<HD, true>::SMEM)) return rc;
   if (int rc = allow_smem<attention_bwd_kernel<HD, false>>(AttnBwd<HD, false>::SMEM)) return rc;
   int* err = device_status_word();
-  const int64_t vecs = static_cast<int64_t>(s.B) * s.rows * s.nq * (HD / 8);
+  const int per_block = 256 / (HD / 8) * DELTA_ROWS;
+  const int blocks = static_cast<int>((static_cast<int64_t>(s.rows) * s.nq + per_block - 1) / per_block);   // of a sequence
   auto stride = [](int size, long long x) { return size == 1 ? 0 : x; };
-  launch_dependent(attention_delta_kernel<HD>, static_cast<int>((vecs + 255) / 256), 256, 0, stream, static_cast<const bf16*>(a.dout.data),
-                   stride(s.B, a.dout.batch), stride(s.S, a.dout.token), stride(s.nq, a.dout.head), static_cast<const bf16*>(a.out), a.delta, s);
+  launch_dependent(attention_delta_kernel<HD>, s.B * blocks, 256, 0, stream, static_cast<const bf16*>(a.dout.data),
+                   stride(s.B, a.dout.batch), stride(s.S, a.dout.token), stride(s.nq, a.dout.head), static_cast<const bf16*>(a.out), a.delta, s, blocks);
   const int tiles = s.rows / ATT_TILE;
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
@@ -858,7 +910,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (a.dq) {
     const int items = s.B * s.nq * tiles;
     launch_dependent(queries, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
-                     static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, nullptr}, items, err);
+                     static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, Divisor(), nullptr}, items, err);
   }
   B200_CUDA_OK(cudaGetLastError());
   return 0;

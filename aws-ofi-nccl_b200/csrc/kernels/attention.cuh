@@ -21,6 +21,28 @@ struct AttnRoles {
 };
 constexpr float ATT_LOG2E = 1.4426950408889634f;
 
+// Quotients by a number that the host knows: floor(n / d) = floor(n m / 2^(32 + s)) for 0 <= n < 2^31 with 2^s >= d and m the least integer from 2^(32 + s) / d on,
+// where that is less than 2^32 (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divisor {
+  int d = 1;
+  uint32_t m = 0;
+  int s = -1;   // -1: d is one
+  Divisor() = default;
+  __host__ explicit Divisor(int by) : d(by) {
+    if (by == 1) return;
+    s = 0;
+    while ((1ll << (s + 1)) < by) ++s;   // 2^s < d <= 2^(s + 1): the quotient of 2^(32 + s) has 32 bits
+    m = static_cast<uint32_t>(((1ull << (32 + s)) + by - 1) / by);
+  }
+  __host__ __device__ __forceinline__ int quotient(int n) const {
+#ifdef __CUDA_ARCH__
+    return s < 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), m) >> s);
+#else
+    return s < 0 ? n : static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * m >> 32 >> s);
+#endif
+  }
+};
+
 struct AttnShape {
   int B, S, nq, nkv;   // batch, tokens, heads of q, heads of k and v
   int G;               // heads of q that share one of k and v
@@ -28,6 +50,7 @@ struct AttnShape {
   int window, sinks;   // window 0: all keys up to the query (then sinks is 0)
   const int* lengths;  // [B], or null: all sequences have S tokens
   float scale;
+  Divisor by_G, by_nq, by_nkv, by_heads_q, by_heads_kv;   // heads_q: B * nq
 };
 
 __device__ __forceinline__ int sequence_length(const AttnShape& s, int b) { return s.lengths ? min(max(s.lengths[b], 0), s.S) : s.S; }
@@ -168,7 +191,8 @@ __device__ __forceinline__ Pair exp2_cubic(Pair x) {
   t.to(a, b);
   return p * pair_of((__float_as_uint(a) << 23) + 0x3F800000u, (__float_as_uint(b) << 23) + 0x3F800000u);
 }
-// The same of x by the unit, or of every fourth pair of a row (number e / 2) in float units: both then have the same to do.
+// The same of x by the unit, or of every fourth pair of a row (number e / 2) in float units, where the unit bounds a phase: the gradients' kernels take
+// 239 and 173 us for 247 and 180 over 4096 tokens of 32 heads; with every second pair 239 and 179. The forward pass gains nothing by it.
 __device__ __forceinline__ void exp2_pair(int e, Pair x, float& a, float& b) {
   if (e / 2 % 4 == 3) {
     exp2_cubic(x).to(a, b);
@@ -196,6 +220,33 @@ __device__ __forceinline__ uint32_t columns_seen(int first, int last, int sinks)
 // Two packed bf16, those of columns 2 k and 2 k + 1, where they are seen, else zeros
 __device__ __forceinline__ uint32_t seen_pair(uint32_t packed, uint32_t seen, int k) {
   return packed & ((seen >> (2 * k) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * k + 1) & 1 ? 0xFFFF0000u : 0u));
+}
+
+// 64 bytes of each of a warp's rows, a lane holding its own row's, to `row_at(r)` + 16 bytes times a lane's number among four (null: left out). Four lanes exchange
+// their vectors first, so that a store covers 64 bytes of eight rows: 16 of each of 32 rows take the memory pipeline four times as long (of dk and dv 6000 clocks a tile).
+template <class Row>
+__device__ __forceinline__ void store_rows64(uint32_t (&w)[16], Row row_at) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int step = 1; step <= 2; ++step) {
+    const bool upper = lane & step;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k & step) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t &a = w[k * 4 + e], &b = w[(k + step) * 4 + e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? a : b, step);
+        if (upper)
+          a = got;
+        else
+          b = got;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (uint4* at = row_at((lane & ~3) + k)) at[lane & 3] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
 }
 
 // What all roles of a CTA share: barriers and the flag that one of its waits has given up. It has all of tensor memory, from column 0 on.

@@ -4,6 +4,7 @@
 // Query i sees key j where j <= i, and with a window also i - j < window or j < sinks; a sequence of the batch has length[b] tokens,
 // and rows behind them are zeros, in the output and in the gradients. Since j <= i, a query in front of the length sees no key behind it.
 #pragma once
+#include "divisor.h"
 #include "gemm_tcgen05.cuh"
 #include "pair_math.cuh"
 
@@ -20,28 +21,6 @@ struct AttnRoles {
   static constexpr int LOAD = COMPUTE, MMA = COMPUTE + 1, ZERO = COMPUTE + 2, THREADS = 32 * (COMPUTE + 3);
 };
 constexpr float ATT_LOG2E = 1.4426950408889634f;
-
-// Quotients by a number that the host knows: floor(n / d) = floor(n m / 2^(32 + s)) for 0 <= n < 2^31 with 2^s >= d and m the least integer from 2^(32 + s) / d on,
-// where that is less than 2^32 (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
-struct Divisor {
-  int d = 1;
-  uint32_t m = 0;
-  int s = -1;   // -1: d is one
-  Divisor() = default;
-  __host__ explicit Divisor(int by) : d(by) {
-    if (by == 1) return;
-    s = 0;
-    while ((1ll << (s + 1)) < by) ++s;   // 2^s < d <= 2^(s + 1): the quotient of 2^(32 + s) has 32 bits
-    m = static_cast<uint32_t>(((1ull << (32 + s)) + by - 1) / by);
-  }
-  __host__ __device__ __forceinline__ int quotient(int n) const {
-#ifdef __CUDA_ARCH__
-    return s < 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), m) >> s);
-#else
-    return s < 0 ? n : static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * m >> 32 >> s);
-#endif
-  }
-};
 
 struct AttnShape {
   int B, S, nq, nkv;   // batch, tokens, heads of q, heads of k and v

@@ -60,6 +60,14 @@ struct B200AdamwTensor {
 int b200_adamw_many(const B200AdamwTensor* list, int count, int bits, double lr, double beta1, double beta2, double eps, long long step, double grad_scale,
                     int zero_grad, int* launches, void* stream);
 
+// Activations in 8 bits, codes [rows][width] and a byte for every 32 of a row (or what is left of it), and SwiGLU with gate and up kept so, as rows 2t and
+// 2t + 1 of F; see kept8.cu. width and F are multiples of 8. swiglu_kept8 makes gate|up of what is kept, and act unless that is null.
+int b200_keep8(const void* x, long long pitch, void* codes, void* powers, long long rows, int width, void* stream);
+int b200_kept8(const void* codes, const void* powers, void* x, long long rows, int width, void* stream);
+int b200_swiglu_keep8(const void* gu, void* act, void* codes, void* powers, long long T, int F, void* stream);
+int b200_swiglu_bwd8(const void* dout, const void* codes, const void* powers, void* dgu, long long T, int F, void* stream);
+int b200_swiglu_kept8(const void* codes, const void* powers, void* gu, void* act, long long T, int F, void* stream);
+
 // Attention with a window and sinks, and its gradients; see attention.cu. Tensors are [batch][token][head][hd] bf16 with element strides (multiples of
 // eight; any for a dimension of one) and contiguous heads; out, dq, dk and dv are contiguous. lse and delta are [B][nq][S rounded up to 128] floats.
 // dq, or dk and dv together, may be null; sums are b200_attention_bwd_workspace's number of floats.

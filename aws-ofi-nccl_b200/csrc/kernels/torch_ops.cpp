@@ -109,6 +109,40 @@ Tensor write_param_grad(const Tensor& weight, Produce produce) {
   return {};
 }
 
+// x in 8 bits, for layers that keep it so: codes and a byte for every 32 of a row
+struct Kept {
+  Tensor codes, powers;
+};
+constexpr const char* KEPT_NO_TANGENTS = "layers that keep activations in 8 bits have no forward-mode derivative";
+constexpr const char* KEPT_NO_SECOND = "layers that keep activations in 8 bits have no second derivative";
+Tensor powers_like(const Tensor& codes, int64_t rows, int64_t width) { return fresh({rows, (width + 31) / 32}, at::kByte, codes); }
+Kept keep8(const Tensor& x) {   // a matrix with contiguous rows
+  const int64_t rows = x.size(0), width = x.size(1);
+  const CUDAGuard guard(x.device());
+  const bool fits = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (rows == 1 || x.stride(0) % 8 == 0);
+  const Tensor rows_at = fits ? x : x.clone(at::MemoryFormat::Contiguous);
+  Kept k;
+  k.codes = fresh({rows, width}, at::kFloat8_e4m3fn, x);
+  k.powers = powers_like(k.codes, rows, width);
+  if (rows) launched();
+  check(b200_keep8(rows_at.data_ptr(), rows == 1 ? width : rows_at.stride(0), k.codes.data_ptr(), k.powers.data_ptr(), rows, static_cast<int>(width), stream()),
+        "b200_keep8");
+  return k;
+}
+Tensor kept8(const Tensor& codes, const Tensor& powers) {
+  const CUDAGuard guard(codes.device());
+  const Tensor x = fresh(codes.sizes(), at::kBFloat16, codes);
+  const int64_t width = codes.size(-1), rows = rows_of(codes, width);
+  if (rows) launched();
+  check(b200_kept8(codes.data_ptr(), powers.data_ptr(), x.data_ptr(), rows, static_cast<int>(width), stream()), "b200_kept8");
+  return x;
+}
+// What the backward pass of a layer that keeps 8 bits refuses
+void refuse_second(const Tensor& dy) {
+  refuse_tangents({&dy}, KEPT_NO_TANGENTS);
+  if (at::GradMode::is_enabled()) raise(PyExc_RuntimeError, KEPT_NO_SECOND);
+}
+
 // y = x W^T
 struct Linear : public Function<Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight) {
@@ -141,6 +175,46 @@ struct Linear : public Function<Linear> {
       else if (want_dx)
         gemm(dy, weight, false, true, dx, false);
       return {want_dx ? dx.view(x.sizes()) : dx, dw};
+    });
+  }
+};
+
+// The same with x kept in 8 bits, from which the weight's gradient is made
+struct Linear8 : public Function<Linear8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight) {
+    const CUDAGuard guard(x.device());
+    auto shape = x.sizes().vec();
+    const Tensor x2 = x.reshape({-1, x.size(-1)});
+    shape.back() = weight.size(0);
+    const Tensor y = at::empty(shape, x.options().dtype(at::kBFloat16));
+    gemm(x2, weight, false, false, y.view({-1, weight.size(0)}), false);
+    const Kept k = weight.requires_grad() ? keep8(x2) : Kept();
+    ctx->save_for_backward({weight, k.codes, k.powers});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return on_engine_thread([&]() -> variable_list {
+      refuse_second(grads[0]);
+      const auto saved = ctx->get_saved_variables();
+      const Tensor &weight = saved[0], &codes = saved[1], &powers = saved[2];
+      const CUDAGuard guard(weight.device());
+      const Tensor dy = rows16(grads[0].reshape({-1, grads[0].size(-1)}));
+      Tensor dx, dw;
+      const bool want_dx = ctx->needs_input_grad(0);
+      if (want_dx) dx = fresh({dy.size(0), weight.size(1)}, at::kBFloat16, dy);
+      if (ctx->needs_input_grad(1)) {
+        const Tensor x = kept8(codes, powers);
+        dw = write_param_grad(weight, [&](const Tensor& out, bool accumulate) {
+          if (want_dx)
+            linear_grads(dy, x, weight, dx, out, accumulate);
+          else
+            gemm(dy, x, true, true, out, accumulate);
+        });
+      } else if (want_dx) {
+        gemm(dy, weight, false, true, dx, false);
+      }
+      return {want_dx ? dx.view(ctx->saved_data["shape"].toIntVector()) : dx, dw};
     });
   }
 };
@@ -254,62 +328,132 @@ struct SwiGLU : public Function<SwiGLU> {
   }
 };
 
+// The same with gate and up kept in 8 bits
+struct SwiGLU8 : public Function<SwiGLU8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& gu) {
+    const CUDAGuard guard(gu.device());
+    const int64_t F = gu.size(-1) / 2, T = rows_of(gu, 2 * F);
+    auto shape = gu.sizes().vec();
+    const Tensor codes = fresh(shape, at::kFloat8_e4m3fn, gu), powers = powers_like(codes, 2 * T, F);
+    shape.back() = F;
+    const Tensor out = fresh(shape, at::kBFloat16, gu), rows = rows16(gu);
+    if (T) launched();
+    check(b200_swiglu_keep8(rows.data_ptr(), out.data_ptr(), codes.data_ptr(), powers.data_ptr(), T, static_cast<int>(F), stream()), "b200_swiglu_keep8");
+    ctx->save_for_backward({codes, powers});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return on_engine_thread([&]() -> variable_list {
+      refuse_second(grads[0]);
+      const auto saved = ctx->get_saved_variables();
+      const Tensor &codes = saved[0], &powers = saved[1];
+      const CUDAGuard guard(codes.device());
+      const int64_t F = codes.size(-1) / 2, T = rows_of(codes, 2 * F);
+      const Tensor dout = rows16(grads[0]), dgu = fresh(codes.sizes(), at::kBFloat16, codes);
+      if (T) launched();
+      check(b200_swiglu_bwd8(dout.data_ptr(), codes.data_ptr(), powers.data_ptr(), dgu.data_ptr(), T, static_cast<int>(F), stream()), "b200_swiglu_bwd8");
+      return {dgu};
+    });
+  }
+};
+
+// y, with gate|up and the activation for the backward pass
+Tensor swiglu_mlp_of(const Tensor& x, const Tensor& w_gu, const Tensor& w_down, Tensor& gu, Tensor& act) {
+  require(bf16_cuda(x) && bf16_cuda(w_gu) && bf16_cuda(w_down), "x and the weights are bfloat16 CUDA tensors");
+  require(x.dim() >= 1 && w_gu.dim() == 2 && w_down.dim() == 2 && w_gu.is_contiguous() && w_down.is_contiguous(),
+          "x has a last dimension and the weights are contiguous matrices");
+  const int64_t F = w_down.size(1), K = w_gu.size(1);
+  require(w_gu.size(0) == 2 * F && x.size(-1) == K, "the weights are [2F, hidden] and [out, F]");
+  const Tensor x2 = x.reshape({-1, K});
+  require(x2.stride(1) == 1, "x has contiguous rows");
+  const int T = static_cast<int>(x2.size(0));
+  gu = at::empty({T, 2 * F}, x.options()), act = at::empty({T, F}, x.options());
+  g_launches.fetch_add(b200_gemm_swiglu_launches(x2.data_ptr(), w_gu.data_ptr(), T, static_cast<int>(F), static_cast<int>(K), x2.stride(0)),
+                       std::memory_order_relaxed);
+  check(b200_gemm_swiglu(x2.data_ptr(), w_gu.data_ptr(), gu.data_ptr(), act.data_ptr(), T, static_cast<int>(F), static_cast<int>(K),
+                         x2.stride(0), stream()),
+        "b200_gemm_swiglu");
+  auto shape = x.sizes().vec();
+  shape.back() = w_down.size(0);
+  Tensor y = at::empty(shape, x.options());
+  gemm(act, w_down, false, false, y.view({-1, w_down.size(0)}), false);
+  return y;
+}
+// Gradients from x as rows, gate|up and the activation (x and the activation where their weights' gradients are asked for)
+variable_list swiglu_mlp_grads(AutogradContext* ctx, const Tensor& dout, const Tensor& x2, const Tensor& w_gu, const Tensor& w_down, const Tensor& gu,
+                               const Tensor& act, at::IntArrayRef shape) {
+  const Tensor dy = rows16(dout.reshape({-1, dout.size(-1)}));
+  const int T = static_cast<int>(dy.size(0)), F = static_cast<int>(gu.size(1) / 2), H = static_cast<int>(dy.size(1));
+  Tensor dgu, dx, dw_gu, dw_down;
+  if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
+    const int launches = b200_gemm_swiglu_bwd_launches(dy.data_ptr(), w_down.data_ptr(), T, F, H, dy.stride(0));
+    const Tensor scratch = launches == 1 ? Tensor() : at::empty({T, F}, gu.options());
+    dgu = at::empty_like(gu);
+    g_launches.fetch_add(launches, std::memory_order_relaxed);
+    check(b200_gemm_swiglu_bwd(dy.data_ptr(), w_down.data_ptr(), gu.data_ptr(), dgu.data_ptr(),
+                               scratch.defined() ? scratch.data_ptr() : nullptr, T, F, H, dy.stride(0), stream()),
+          "b200_gemm_swiglu_bwd");
+  }
+  if (ctx->needs_input_grad(2))
+    dw_down = write_param_grad(w_down, [&](const Tensor& out, bool accumulate) { gemm(dy, act, true, true, out, accumulate); });
+  const bool want_dx = ctx->needs_input_grad(0);
+  if (want_dx) dx = at::empty({T, w_gu.size(1)}, dy.options());
+  if (ctx->needs_input_grad(1))
+    dw_gu = write_param_grad(w_gu, [&](const Tensor& out, bool accumulate) {
+      if (want_dx)
+        linear_grads(dgu, x2, w_gu, dx, out, accumulate);
+      else
+        gemm(dgu, x2, true, true, out, accumulate);
+    });
+  else if (want_dx)
+    gemm(dgu, w_gu, false, true, dx, false);
+  return {want_dx ? dx.view(shape) : dx, dw_gu, dw_down};
+}
+
 // The SwiGLU MLP of a decoder layer, gate over up in w_gu. One layer instead of three, so that the activation and its
 // gradient ride in the products beside them.
 struct SwiGLUMLP : public Function<SwiGLUMLP> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gu, const Tensor& w_down) {
-    require(bf16_cuda(x) && bf16_cuda(w_gu) && bf16_cuda(w_down), "x and the weights are bfloat16 CUDA tensors");
-    require(x.dim() >= 1 && w_gu.dim() == 2 && w_down.dim() == 2 && w_gu.is_contiguous() && w_down.is_contiguous(),
-            "x has a last dimension and the weights are contiguous matrices");
-    const int64_t F = w_down.size(1), K = w_gu.size(1);
-    require(w_gu.size(0) == 2 * F && x.size(-1) == K, "the weights are [2F, hidden] and [out, F]");
-    const Tensor x2 = x.reshape({-1, K});
-    require(x2.stride(1) == 1, "x has contiguous rows");
-    const int T = static_cast<int>(x2.size(0));
-    const Tensor gu = at::empty({T, 2 * F}, x.options()), act = at::empty({T, F}, x.options());
-    g_launches.fetch_add(b200_gemm_swiglu_launches(x2.data_ptr(), w_gu.data_ptr(), T, static_cast<int>(F), static_cast<int>(K), x2.stride(0)),
-                         std::memory_order_relaxed);
-    check(b200_gemm_swiglu(x2.data_ptr(), w_gu.data_ptr(), gu.data_ptr(), act.data_ptr(), T, static_cast<int>(F), static_cast<int>(K),
-                           x2.stride(0), stream()),
-          "b200_gemm_swiglu");
-    auto shape = x.sizes().vec();
-    shape.back() = w_down.size(0);
-    Tensor y = at::empty(shape, x.options());
-    gemm(act, w_down, false, false, y.view({-1, w_down.size(0)}), false);
+    Tensor gu, act;
+    const Tensor y = swiglu_mlp_of(x, w_gu, w_down, gu, act);
     ctx->save_for_backward({x, w_gu, w_down, gu, act});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return on_engine_thread([&]() -> variable_list {
       const auto saved = ctx->get_saved_variables();
-      const Tensor &x = saved[0], &w_gu = saved[1], &w_down = saved[2], &gu = saved[3], &act = saved[4];
-      const Tensor dy = rows16(grads[0].reshape({-1, grads[0].size(-1)}));
-      const int T = static_cast<int>(dy.size(0)), F = static_cast<int>(act.size(1)), H = static_cast<int>(dy.size(1));
-      Tensor dgu, dx, dw_gu, dw_down;
-      if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) {
-        const int launches = b200_gemm_swiglu_bwd_launches(dy.data_ptr(), w_down.data_ptr(), T, F, H, dy.stride(0));
-        const Tensor scratch = launches == 1 ? Tensor() : at::empty_like(act);
-        dgu = at::empty_like(gu);
-        g_launches.fetch_add(launches, std::memory_order_relaxed);
-        check(b200_gemm_swiglu_bwd(dy.data_ptr(), w_down.data_ptr(), gu.data_ptr(), dgu.data_ptr(),
-                                   scratch.defined() ? scratch.data_ptr() : nullptr, T, F, H, dy.stride(0), stream()),
-              "b200_gemm_swiglu_bwd");
-      }
-      if (ctx->needs_input_grad(2))
-        dw_down = write_param_grad(w_down, [&](const Tensor& out, bool accumulate) { gemm(dy, act, true, true, out, accumulate); });
-      const Tensor x2 = x.reshape({-1, x.size(-1)});
-      const bool want_dx = ctx->needs_input_grad(0);
-      if (want_dx) dx = at::empty_like(x2, x2.options(), at::MemoryFormat::Contiguous);
-      if (ctx->needs_input_grad(1))
-        dw_gu = write_param_grad(w_gu, [&](const Tensor& out, bool accumulate) {
-          if (want_dx)
-            linear_grads(dgu, x2, w_gu, dx, out, accumulate);
-          else
-            gemm(dgu, x2, true, true, out, accumulate);
-        });
-      else if (want_dx)
-        gemm(dgu, w_gu, false, true, dx, false);
-      return {want_dx ? dx.view(x.sizes()) : dx, dw_gu, dw_down};
+      return swiglu_mlp_grads(ctx, grads[0], saved[0].reshape({-1, saved[0].size(-1)}), saved[1], saved[2], saved[3], saved[4], saved[0].sizes());
+    });
+  }
+};
+
+// The same with x, gate and up kept in 8 bits; the activation is made of these again, so that the gradients are those of what is kept
+struct SwiGLUMLP8 : public Function<SwiGLUMLP8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gu, const Tensor& w_down) {
+    const CUDAGuard guard(x.device());
+    Tensor gu, act;
+    const Tensor x2 = x.reshape({-1, x.size(-1)}), y = swiglu_mlp_of(x, w_gu, w_down, gu, act);
+    const int64_t F = act.size(1);
+    const bool any = x.requires_grad() || w_gu.requires_grad() || w_down.requires_grad();
+    const Kept in = w_gu.requires_grad() ? keep8(x2) : Kept(), halves = any ? keep8(gu.view({-1, F})) : Kept();
+    ctx->save_for_backward({w_gu, w_down, in.codes, in.powers, halves.codes, halves.powers});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return on_engine_thread([&]() -> variable_list {
+      refuse_second(grads[0]);
+      const auto saved = ctx->get_saved_variables();
+      const Tensor &w_gu = saved[0], &w_down = saved[1], &codes = saved[4], &powers = saved[5];
+      const CUDAGuard guard(w_gu.device());
+      const int64_t F = codes.size(1), T = codes.size(0) / 2;
+      const Tensor x = saved[2].defined() ? kept8(saved[2], saved[3]) : Tensor();
+      const Tensor gu = fresh({T, 2 * F}, at::kBFloat16, codes), act = ctx->needs_input_grad(2) ? fresh({T, F}, at::kBFloat16, codes) : Tensor();
+      if (T) launched();
+      check(b200_swiglu_kept8(codes.data_ptr(), powers.data_ptr(), gu.data_ptr(), act.defined() ? act.data_ptr() : nullptr, T, static_cast<int>(F), stream()),
+            "b200_swiglu_kept8");
+      const auto shape = ctx->saved_data["shape"].toIntVector();
+      return swiglu_mlp_grads(ctx, grads[0], x, w_gu, w_down, gu, act, shape);
     });
   }
 };
@@ -410,6 +554,49 @@ struct RopeQKV : public Function<RopeQKV> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w) { return Linear::apply(x, w); }
+void check_kept_width(const Tensor& x, int64_t width) { require(bf16_cuda(x) && width > 0 && width % 8 == 0, "what is kept in 8 bits are bfloat16 CUDA rows of a multiple of 8 elements"); }
+Tensor linear8(const Tensor& x, const Tensor& w) {
+  require(x.dim() >= 1 && w.dim() == 2, "x has a last dimension and the weight is a matrix");
+  check_kept_width(x, x.size(-1));
+  refuse_tangents({&x, &w}, KEPT_NO_TANGENTS);
+  return at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()) ? Linear8::apply(x, w) : Linear::apply(x, w);
+}
+Tensor swiglu8(const Tensor& gu) {
+  require(gu.dim() >= 1 && gu.size(-1) % 2 == 0 && gu.is_contiguous(), "gate_up is contiguous and has two halves");
+  check_kept_width(gu, gu.size(-1) / 2);
+  refuse_tangents({&gu}, KEPT_NO_TANGENTS);
+  return at::GradMode::is_enabled() && gu.requires_grad() ? SwiGLU8::apply(gu) : SwiGLU::apply(gu);
+}
+Tensor swiglu_mlp8(const Tensor& x, const Tensor& w_gu, const Tensor& w_down) {
+  require(x.dim() >= 1 && w_gu.dim() == 2 && w_down.dim() == 2, "x has a last dimension and the weights are matrices");
+  check_kept_width(x, x.size(-1));
+  check_kept_width(w_down, w_down.size(1));
+  refuse_tangents({&x, &w_gu, &w_down}, KEPT_NO_TANGENTS);
+  return at::GradMode::is_enabled() && (x.requires_grad() || w_gu.requires_grad() || w_down.requires_grad()) ? SwiGLUMLP8::apply(x, w_gu, w_down)
+                                                                                                             : SwiGLUMLP::apply(x, w_gu, w_down);
+}
+variable_list keep_rows8(const Tensor& x) {
+  require(x.dim() >= 1, "x has a last dimension");
+  check_kept_width(x, x.size(-1));
+  refuse_tangents({&x}, KEPT_NO_TANGENTS);
+  require(!at::GradMode::is_enabled() || !x.requires_grad(), "keep_rows8 has no gradient: call it under torch.no_grad()");
+  const Tensor x2 = x.reshape({-1, x.size(-1)});
+  const Kept k = keep8(x2.stride(1) == 1 ? x2 : x2.contiguous());
+  auto shape = x.sizes().vec();
+  const Tensor codes = k.codes.view(shape);
+  shape.back() = k.powers.size(1);
+  return {codes, k.powers.view(shape)};
+}
+Tensor kept_rows8(const Tensor& codes, const Tensor& powers) {
+  require(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() >= 1 && codes.is_contiguous() && codes.size(-1) > 0 && codes.size(-1) % 8 == 0,
+          "codes are contiguous float8_e4m3fn CUDA rows of a multiple of 8 elements");
+  auto shape = codes.sizes().vec();
+  shape.back() = (shape.back() + 31) / 32;
+  require(same_device(powers, codes) && powers.scalar_type() == at::kByte && powers.is_contiguous() && powers.sizes() == at::IntArrayRef(shape),
+          "powers are contiguous bytes, one for every 32 of a row");
+  require(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 8 == 0, "codes lie on a boundary of 8 bytes");
+  return kept8(codes, powers);
+}
 variable_list rmsnorm(const Tensor& x, const c10::optional<Tensor>& res, const Tensor& w, double eps) {
   return RMSNorm::apply(x, res, w, eps);
 }
@@ -426,6 +613,11 @@ variable_list rope_qkv(const Tensor& qkv, const Tensor& cos, const Tensor& sin, 
 
 TORCH_LIBRARY(b200ops, m) {
   m.def("linear(Tensor x, Tensor weight) -> Tensor", linear);
+  m.def("linear8(Tensor x, Tensor weight) -> Tensor", linear8);
+  m.def("swiglu8(Tensor gate_up) -> Tensor", swiglu8);
+  m.def("swiglu_mlp8(Tensor x, Tensor w_gate_up, Tensor w_down) -> Tensor", swiglu_mlp8);
+  m.def("keep_rows8(Tensor x) -> Tensor[]", keep_rows8);
+  m.def("kept_rows8(Tensor codes, Tensor powers) -> Tensor", kept_rows8);
   m.def("embedding(Tensor ids, Tensor table) -> Tensor", embedding);
   m.def("rmsnorm(Tensor x, Tensor? res, Tensor weight, float eps) -> Tensor[]", rmsnorm);
   m.def("swiglu(Tensor gate_up) -> Tensor", swiglu);
@@ -456,6 +648,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                                           int64_t nq, int64_t nkv, int64_t hd) {
           return traced_or_direct("b200ops::rope_qkv", rope_qkv, qkv, cos, sin, B, S, nq, nkv, hd);
         }));
+  m.def("linear8", torch::wrap_pybind_function_no_gil(
+                       [](const Tensor& x, const Tensor& w) { return traced_or_direct("b200ops::linear8", linear8, x, w); }));
+  m.def("swiglu8", torch::wrap_pybind_function_no_gil([](const Tensor& gu) { return traced_or_direct("b200ops::swiglu8", swiglu8, gu); }));
+  m.def("swiglu_mlp8", torch::wrap_pybind_function_no_gil([](const Tensor& x, const Tensor& w_gu, const Tensor& w_down) {
+          return traced_or_direct("b200ops::swiglu_mlp8", swiglu_mlp8, x, w_gu, w_down);
+        }));
+  m.def("keep_rows8", torch::wrap_pybind_function_no_gil([](const Tensor& x) { return traced_or_direct("b200ops::keep_rows8", keep_rows8, x); }));
+  m.def("kept_rows8", torch::wrap_pybind_function_no_gil(
+                          [](const Tensor& codes, const Tensor& powers) { return traced_or_direct("b200ops::kept_rows8", kept_rows8, codes, powers); }));
   m.def("cross_entropy", torch::wrap_pybind_function_no_gil(cross_entropy));
   bind_moe(m);
   bind_attention(m);

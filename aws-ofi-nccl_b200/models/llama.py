@@ -1,5 +1,6 @@
 """Llama-3 decoder for training on B200: every GEMM runs on the tcgen05 kernel, every bandwidth
-op on the kernels of llm_ops.cu; attention uses torch SDPA (a library kernel).
+op on the kernels of llm_ops.cu; attention over all keys uses torch SDPA (a library kernel), attention with a window the
+kernels of attention.cu.
 
 Parameters live in ONE flat bf16 buffer and their gradients in ONE flat bf16 buffer
 (``weight.main_grad`` views), so the optimizer is a single fused launch and a data-parallel
@@ -13,6 +14,7 @@ import math
 import torch
 import torch.nn.functional as F
 
+from ..ops import attention as attention_ops
 from ..ops import gemm as gemm_ops
 from ..ops import llm as llm_ops
 
@@ -28,6 +30,15 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     rms_eps: float = 1e-5
     max_seq: int = 4096
+    window: int = 0      # keys that a query sees, itself among them; 0: all up to itself
+    sinks: int = 0       # first tokens that every query sees beside its window
+    keep_bits: int = 16  # of the activations that the projections in front of attention and the MLP keep for the backward pass: 16 or 8
+
+    def __post_init__(self):
+        if self.window < 0 or self.sinks < 0 or (self.sinks and not self.window):
+            raise ValueError("a window is no negative number, and sinks go with one")
+        if self.keep_bits not in (8, 16):
+            raise ValueError(f"activations are kept in 8 or 16 bits, not {self.keep_bits}")
 
     @property
     def head_dim(self) -> int:
@@ -111,6 +122,8 @@ class Llama:
         cfg = self.cfg
         hd, nq, nkv = cfg.head_dim, cfg.n_heads, cfg.n_kv_heads
         q, k, v = llm_ops.rope_qkv(qkv, self.cos, self.sin, B, S, nq, nkv, hd)
+        if cfg.window:
+            return attention_ops.attention(q, k, v, window=cfg.window, sinks=cfg.sinks).reshape(B * S, nq * hd)
         q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=(nq != nkv))
         return o.transpose(1, 2).reshape(B * S, nq * hd)
@@ -125,11 +138,11 @@ class Llama:
         for i in range(cfg.n_layers):
             n1, h = llm_ops.rmsnorm(h if delta is None else delta, P[f"l{i}.norm1"], cfg.rms_eps,
                                     residual=None if delta is None else h)
-            qkv = gemm_ops.linear(n1, P[f"l{i}.wqkv"])
+            qkv = gemm_ops.linear(n1, P[f"l{i}.wqkv"], keep_bits=cfg.keep_bits)
             attn = self._attention(qkv, B, S)
             o = gemm_ops.linear(attn, P[f"l{i}.wo"])
             n2, h = llm_ops.rmsnorm(o, P[f"l{i}.norm2"], cfg.rms_eps, residual=h)
-            delta = llm_ops.swiglu_mlp(n2, P[f"l{i}.wgu"], P[f"l{i}.wdown"])
+            delta = llm_ops.swiglu_mlp(n2, P[f"l{i}.wgu"], P[f"l{i}.wdown"], keep_bits=cfg.keep_bits)
         nf, _ = llm_ops.rmsnorm(delta, P["normf"], cfg.rms_eps, residual=h)
         logits = gemm_ops.linear(nf, P["lm_head"])
         return llm_ops.cross_entropy(logits, labels.reshape(-1))
@@ -151,6 +164,9 @@ def reference_forward_loss(model: Llama, ids: torch.Tensor, labels: torch.Tensor
         a, b = t[..., : hd // 2], t[..., hd // 2:]
         return torch.cat([a * c - b * s, b * c + a * s], -1)
 
+    i, j = torch.arange(S, device=model.device)[:, None], torch.arange(S, device=model.device)[None]
+    sees = (j <= i) & ((i - j < cfg.window) | (j < cfg.sinks)) if cfg.window else None
+
     h = P["embed"][ids]
     for i in range(cfg.n_layers):
         n1 = norm(h, P[f"l{i}.norm1"])
@@ -160,7 +176,7 @@ def reference_forward_loss(model: Llama, ids: torch.Tensor, labels: torch.Tensor
         v = qkv[..., (nq + nkv) * hd:].view(B, S, nkv, hd).transpose(1, 2)
         k = k.repeat_interleave(nq // nkv, 1)
         v = v.repeat_interleave(nq // nkv, 1)
-        o = F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2).reshape(B, S, nq * hd)
+        o = F.scaled_dot_product_attention(q, k, v, attn_mask=sees, is_causal=sees is None).transpose(1, 2).reshape(B, S, nq * hd)
         h = h + o @ P[f"l{i}.wo"].T
         n2 = norm(h, P[f"l{i}.norm2"])
         gu = n2 @ P[f"l{i}.wgu"].T

@@ -70,8 +70,13 @@ def gemm_fp8(a8: torch.Tensor, b8: torch.Tensor, a_scale: torch.Tensor, b_scale:
     return out
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+def linear(x: torch.Tensor, weight: torch.Tensor, *, keep_bits: int = 16) -> torch.Tensor:
     """y = x W^T.  The weight gradient is written straight into ``weight.main_grad`` when the
     parameter has one (a view of the flat gradient buffer), and the ``grad_ready`` hook of the
-    parameter is called so a data-parallel engine can start reducing that bucket at once."""
-    return _lib.native().linear(x, weight)
+    parameter is called so a data-parallel engine can start reducing that bucket at once.
+
+    ``keep_bits`` 8 keeps x for the weight's gradient in 8 bits, as ``llm.keep_rows8`` does, instead of the tensor itself: y and x's gradient are the
+    same, the weight's is made of the rounded x.  Rows of x hold a multiple of 8 elements then, and there is no second derivative."""
+    if keep_bits not in (8, 16):
+        raise ValueError(f"activations are kept in 8 or 16 bits, not {keep_bits}")
+    return _lib.native().linear8(x, weight) if keep_bits == 8 else _lib.native().linear(x, weight)

@@ -25,16 +25,39 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residu
     return tuple(_lib.native().rmsnorm_fp8(x, residual, weight, eps, group))
 
 
-def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
-    """silu(gate) * up for a fused [..., 2F] tensor laid out as gate | up."""
-    return _lib.native().swiglu(gate_up)
+def _kept(bits: int) -> bool:
+    if bits not in (8, 16):
+        raise ValueError(f"activations are kept in 8 or 16 bits, not {bits}")
+    return bits == 8
 
 
-def swiglu_mlp(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
+def swiglu(gate_up: torch.Tensor, *, keep_bits: int = 16) -> torch.Tensor:
+    """silu(gate) * up for a fused [..., 2F] tensor laid out as gate | up.  ``keep_bits`` 8 keeps both for the backward pass in 8 bits, as
+    ``keep_rows8`` does with rows of F, instead of the tensor itself: the gradient is that at the rounded gate and up.  F is a multiple of 8."""
+    return _lib.native().swiglu8(gate_up) if _kept(keep_bits) else _lib.native().swiglu(gate_up)
+
+
+def swiglu_mlp(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, *, keep_bits: int = 16) -> torch.Tensor:
     """``linear(swiglu(linear(x, w_gate_up)), w_down)`` as one layer: the activation and its gradient are part of
     the products beside them.  w_gate_up [2F, hidden] (gate over up) and w_down [out, F] are contiguous; their
-    gradients go where those of ``linear`` go."""
+    gradients go where those of ``linear`` go.  ``keep_bits`` 8 keeps x, gate and up in 8 bits (hidden + 2F bytes a token and a 32nd of that, where 16
+    bits and the activation are 2 hidden + 6F) and makes the activation of these again: its output is the same, its gradients are those at the rounded values."""
+    if _kept(keep_bits):
+        return _lib.native().swiglu_mlp8(x, w_gate_up, w_down)
     return _lib.native().swiglu_mlp(x, w_gate_up, w_down)
+
+
+def keep_rows8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, powers): x (bf16, rows of a multiple of 8 elements) as the layers with ``keep_bits`` 8 keep it, for layers of a program's own. Every 32
+    elements of a row (or what is left of it) share a power of two, the least with which their largest is no more than 448: codes are e4m3 of x's shape, powers
+    bytes e that stand for 2^(e - 127).  Only the rounding to e4m3 is lost, half a step: 2^-4 of a value, or 2^-10 of the power below 2^-6 of it.
+    What is not finite becomes NaN and counts for no power.  There is no gradient."""
+    return tuple(_lib.native().keep_rows8(x))
+
+
+def kept_rows8(codes: torch.Tensor, powers: torch.Tensor) -> torch.Tensor:
+    """What ``keep_rows8`` kept, in bf16."""
+    return _lib.native().kept_rows8(codes, powers)
 
 
 def rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int,

@@ -20,6 +20,10 @@ namespace b200 {
 using bf16 = __nv_bfloat16;
 
 constexpr int KEPT_THREADS = 256;
+// Vectors of a thread. Two loads ahead where a lane has 16 bytes of one tensor to read: 4096 x 4096 13.8 us to be kept (3.8 TB/s) and 8.5 back, 17.8 and 10.9
+// with one each (before the loads' turn came the search for values that are not finite out of the way: 16.9 with two); SwiGLU of 4096 x 14336 84.6 us (5.6 TB/s) for 106.
+// Where three and more tensors are read one vector is as fast: its gradient 82.6 (5.7 TB/s), 82.3 with two, 87.7 with four.
+constexpr int KEEP_VECS = 2, KEPT_VECS = 2, SWIGLU_KEEP_VECS = 2, SWIGLU_KEPT_VECS = 1;
 
 // Rows of `width` elements as vectors: `vecs` for each, of which the last may lie behind the row's end.
 struct KeptRows {
@@ -61,86 +65,123 @@ __device__ __forceinline__ void store_kept(const KeptRows& s, const KeptPlace& p
   if ((p.col & (KEPT_GROUP - 8)) == 0) powers[p.row * s.groups + p.col / KEPT_GROUP] = static_cast<uint8_t>(power);
 }
 
-// Rows are numbered from the launch's first; k counts a launch's vectors. All threads of a warp have the same number of turns.
-template <class F>
-__device__ __forceinline__ void for_vectors(const KeptRows& s, F f) {
-  const int64_t total = static_cast<int64_t>(s.rows) * s.by_vecs.d, step = static_cast<int64_t>(gridDim.x) * KEPT_THREADS;
-  for (int64_t k = static_cast<int64_t>(blockIdx.x) * KEPT_THREADS; k < total; k += step) f(static_cast<int>(k) + static_cast<int>(threadIdx.x));
+// A CTA's vectors, VECS for a thread, whose loads are all under way before the first is worked on. k counts a launch's vectors.
+template <int VECS>
+__device__ __forceinline__ int kept_vector(int i) {
+  return (static_cast<int>(blockIdx.x) * VECS + i) * KEPT_THREADS + static_cast<int>(threadIdx.x);
 }
 
+template <int VECS>
 __global__ void __launch_bounds__(KEPT_THREADS) keep8_kernel(const bf16* x, int64_t pitch, uint8_t* codes, uint8_t* powers, KeptRows s) {
   grid_wait();
   grid_release();
-  for_vectors(s, [&](int k) {
-    const KeptPlace p = kept_place(s, k);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (p.there) v = *reinterpret_cast<const uint4*>(x + p.row * pitch + p.col);
+  KeptPlace p[VECS];
+  uint4 v[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    p[i] = kept_place(s, kept_vector<VECS>(i));
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (p[i].there) v[i] = *reinterpret_cast<const uint4*>(x + p[i].row * pitch + p[i].col);
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
     uint32_t power;
-    const uint2 c = keep8(v, power);
-    store_kept(s, p, c, power, codes, powers);
-  });
+    const uint2 c = keep8(v[i], power);
+    store_kept(s, p[i], c, power, codes, powers);
+  }
 }
 
+template <int VECS>
 __global__ void __launch_bounds__(KEPT_THREADS) kept8_kernel(const uint8_t* codes, const uint8_t* powers, bf16* x, KeptRows s) {
   grid_wait();
   grid_release();
-  for_vectors(s, [&](int k) {
-    const KeptPlace p = kept_place(s, k);
-    if (!p.there) return;
+  KeptPlace p[VECS];
+  uint2 c[VECS];
+  uint32_t power[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    p[i] = kept_place(s, kept_vector<VECS>(i));
+    c[i] = make_uint2(0, 0);
+    power[i] = 0;
+    if (!p[i].there) continue;
+    c[i] = *reinterpret_cast<const uint2*>(codes + p[i].row * s.width + p[i].col);
+    power[i] = powers[p[i].row * s.groups + p[i].col / KEPT_GROUP];
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    if (!p[i].there) continue;
     float f[8];
-    kept8(*reinterpret_cast<const uint2*>(codes + p.row * s.width + p.col), powers[p.row * s.groups + p.col / KEPT_GROUP], f);
-    *reinterpret_cast<uint4*>(x + p.row * s.width + p.col) = pack8(f);
-  });
+    kept8(c[i], power[i], f);
+    *reinterpret_cast<uint4*>(x + p[i].row * s.width + p[i].col) = pack8(f);
+  }
 }
 
 // gate|up [T][2F] -> act = silu(gate) * up, of the values as they come, and both halves as they are kept: rows 2t and 2t + 1 of F elements. s: T rows of F.
+template <int VECS>
 __global__ void __launch_bounds__(KEPT_THREADS) swiglu_keep8_kernel(const bf16* gu, bf16* act, uint8_t* codes, uint8_t* powers, KeptRows s) {
   grid_wait();
   grid_release();
-  for_vectors(s, [&](int k) {
-    KeptPlace p = kept_place(s, k);
-    uint4 g = make_uint4(0, 0, 0, 0), u = g;
-    if (p.there) {
-      const bf16* at = gu + p.row * 2 * s.width + p.col;
-      g = load_once(at);
-      u = load_once(at + s.width);
+  KeptPlace p[VECS];
+  uint4 g[VECS], u[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    p[i] = kept_place(s, kept_vector<VECS>(i));
+    g[i] = u[i] = make_uint4(0, 0, 0, 0);
+    if (!p[i].there) continue;
+    const bf16* at = gu + p[i].row * 2 * s.width + p[i].col;
+    g[i] = load_once(at);
+    u[i] = load_once(at + s.width);
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    if (p[i].there) {
       float a[8], b[8];
-      unpack8(g, a);
-      unpack8(u, b);
+      unpack8(g[i], a);
+      unpack8(u[i], b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) a[e] = silu(a[e]) * b[e];
-      *reinterpret_cast<uint4*>(act + p.row * s.width + p.col) = pack8(a);
+      *reinterpret_cast<uint4*>(act + p[i].row * s.width + p[i].col) = pack8(a);
     }
     uint32_t g_power, u_power;
-    const uint2 g_codes = keep8(g, g_power), u_codes = keep8(u, u_power);
-    p.row *= 2;
-    store_kept(s, p, g_codes, g_power, codes, powers);
-    p.row += 1;
-    store_kept(s, p, u_codes, u_power, codes, powers);
-  });
+    const uint2 g_codes = keep8(g[i], g_power), u_codes = keep8(u[i], u_power);
+    KeptPlace half = p[i];
+    half.row *= 2;
+    store_kept(s, half, g_codes, g_power, codes, powers);
+    half.row += 1;
+    store_kept(s, half, u_codes, u_power, codes, powers);
+  }
 }
 
 // What the backward pass makes of kept halves. GRAD: their gradients [T][2F] from that of act; else the halves themselves (and act, unless null).
-template <bool GRAD>
+template <bool GRAD, int VECS>
 __global__ void __launch_bounds__(KEPT_THREADS)
     swiglu_kept8_kernel(const uint8_t* codes, const uint8_t* powers, const bf16* dout, bf16* to, bf16* act, KeptRows s) {
   grid_wait();
   grid_release();
-  for_vectors(s, [&](int k) {
-    const KeptPlace p = kept_place(s, k);
-    if (!p.there) return;
-    const uint8_t* at = codes + p.row * 2 * s.width + p.col;
-    const uint8_t* power = powers + p.row * 2 * s.groups + p.col / KEPT_GROUP;
-    const uint2 gc = *reinterpret_cast<const uint2*>(at), uc = *reinterpret_cast<const uint2*>(at + s.width);
-    uint4 d4;
-    if constexpr (GRAD) d4 = load_once(dout + p.row * s.width + p.col);
+  KeptPlace p[VECS];
+  uint2 gc[VECS], uc[VECS];
+  uint32_t gp[VECS], up[VECS];
+  uint4 d4[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    p[i] = kept_place(s, kept_vector<VECS>(i));
+    if (!p[i].there) continue;
+    const uint8_t* at = codes + p[i].row * 2 * s.width + p[i].col;
+    const uint8_t* power = powers + p[i].row * 2 * s.groups + p[i].col / KEPT_GROUP;
+    gc[i] = *reinterpret_cast<const uint2*>(at), uc[i] = *reinterpret_cast<const uint2*>(at + s.width);
+    gp[i] = power[0], up[i] = power[s.groups];
+    if constexpr (GRAD) d4[i] = load_once(dout + p[i].row * s.width + p[i].col);
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    if (!p[i].there) continue;
     float g[8], u[8];
-    kept8(gc, power[0], g);
-    kept8(uc, power[s.groups], u);
-    bf16* row = to + p.row * 2 * s.width + p.col;
+    kept8(gc[i], gp[i], g);
+    kept8(uc[i], up[i], u);
+    bf16* row = to + p[i].row * 2 * s.width + p[i].col;
     if constexpr (GRAD) {
       float d[8];
-      unpack8(d4, d);
+      unpack8(d4[i], d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float l = logistic(g[e]), a = g[e] * l;
@@ -152,22 +193,21 @@ __global__ void __launch_bounds__(KEPT_THREADS)
       float a[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) a[e] = silu(g[e]) * u[e];
-      *reinterpret_cast<uint4*>(act + p.row * s.width + p.col) = pack8(a);
+      *reinterpret_cast<uint4*>(act + p[i].row * s.width + p[i].col) = pack8(a);
     }
     __stcs(reinterpret_cast<uint4*>(row), pack8(g));
     __stcs(reinterpret_cast<uint4*>(row + s.width), pack8(u));
-  });
+  }
 }
 
-// Calls launch(first row, rows) for slices of less than 2^30 vectors, so that their numbers have 32 bits.
+// Calls launch(first row, rows, CTAs of so many vectors a thread) for slices of less than 2^30 vectors, so that their numbers have 32 bits.
 template <class F>
-static int in_slices(long long rows, int width, F launch) {
-  const int vecs = (width + KEPT_GROUP - 1) / KEPT_GROUP * 4;
+static int in_slices(long long rows, int width, int vecs_of_thread, F launch) {
+  const int vecs = (width + KEPT_GROUP - 1) / KEPT_GROUP * 4, of_cta = KEPT_THREADS * vecs_of_thread;
   const long long most = std::max(1ll, (1ll << 30) / vecs);
   for (long long at = 0; at < rows; at += most) {
     const KeptRows s(static_cast<int>(std::min(most, rows - at)), width);
-    const int64_t blocks = (static_cast<int64_t>(s.rows) * vecs + KEPT_THREADS - 1) / KEPT_THREADS;
-    launch(at, s, static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(sm_count()) * 64)));
+    launch(at, s, static_cast<int>((static_cast<int64_t>(s.rows) * vecs + of_cta - 1) / of_cta));
   }
   B200_CUDA_OK(cudaGetLastError());
   return 0;
@@ -191,8 +231,8 @@ int b200_keep8(const void* x, long long pitch, void* codes, void* powers, long l
   if (rows == 0) return 0;
   ensure_context();
   if (!kept_ok(rows, width, {x}, {codes}) || !powers || (rows > 1 && pitch % 8)) return B200_ERR_BAD_ARG;
-  return in_slices(rows, width, [&](long long at, const KeptRows& s, int grid) {
-    launch_dependent(keep8_kernel, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const bf16*>(x) + at * pitch, pitch,
+  return in_slices(rows, width, KEEP_VECS, [&](long long at, const KeptRows& s, int grid) {
+    launch_dependent(keep8_kernel<KEEP_VECS>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const bf16*>(x) + at * pitch, pitch,
                      static_cast<uint8_t*>(codes) + at * width, static_cast<uint8_t*>(powers) + at * s.groups, s);
   });
 }
@@ -201,8 +241,8 @@ int b200_kept8(const void* codes, const void* powers, void* x, long long rows, i
   if (rows == 0) return 0;
   ensure_context();
   if (!kept_ok(rows, width, {x}, {codes}) || !powers) return B200_ERR_BAD_ARG;
-  return in_slices(rows, width, [&](long long at, const KeptRows& s, int grid) {
-    launch_dependent(kept8_kernel, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes) + at * width,
+  return in_slices(rows, width, KEPT_VECS, [&](long long at, const KeptRows& s, int grid) {
+    launch_dependent(kept8_kernel<KEPT_VECS>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes) + at * width,
                      static_cast<const uint8_t*>(powers) + at * s.groups, static_cast<bf16*>(x) + at * width, s);
   });
 }
@@ -211,8 +251,8 @@ int b200_swiglu_keep8(const void* gu, void* act, void* codes, void* powers, long
   if (T == 0) return 0;
   ensure_context();
   if (!kept_ok(T, F, {gu, act}, {codes}) || !powers) return B200_ERR_BAD_ARG;
-  return in_slices(T, F, [&](long long at, const KeptRows& s, int grid) {
-    launch_dependent(swiglu_keep8_kernel, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const bf16*>(gu) + at * 2 * F,
+  return in_slices(T, F, SWIGLU_KEEP_VECS, [&](long long at, const KeptRows& s, int grid) {
+    launch_dependent(swiglu_keep8_kernel<SWIGLU_KEEP_VECS>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const bf16*>(gu) + at * 2 * F,
                      static_cast<bf16*>(act) + at * F, static_cast<uint8_t*>(codes) + at * 2 * F, static_cast<uint8_t*>(powers) + at * 2 * s.groups, s);
   });
 }
@@ -221,8 +261,8 @@ int b200_swiglu_bwd8(const void* dout, const void* codes, const void* powers, vo
   if (T == 0) return 0;
   ensure_context();
   if (!kept_ok(T, F, {dout, dgu}, {codes}) || !powers) return B200_ERR_BAD_ARG;
-  return in_slices(T, F, [&](long long at, const KeptRows& s, int grid) {
-    launch_dependent(swiglu_kept8_kernel<true>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes) + at * 2 * F,
+  return in_slices(T, F, SWIGLU_KEPT_VECS, [&](long long at, const KeptRows& s, int grid) {
+    launch_dependent(swiglu_kept8_kernel<true, SWIGLU_KEPT_VECS>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes) + at * 2 * F,
                      static_cast<const uint8_t*>(powers) + at * 2 * s.groups, static_cast<const bf16*>(dout) + at * F, static_cast<bf16*>(dgu) + at * 2 * F,
                      static_cast<bf16*>(nullptr), s);
   });
@@ -232,8 +272,8 @@ int b200_swiglu_kept8(const void* codes, const void* powers, void* gu, void* act
   if (T == 0) return 0;
   ensure_context();
   if (!kept_ok(T, F, {gu}, {codes}) || !powers || reinterpret_cast<uintptr_t>(act) % 16) return B200_ERR_BAD_ARG;
-  return in_slices(T, F, [&](long long at, const KeptRows& s, int grid) {
-    launch_dependent(swiglu_kept8_kernel<false>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes) + at * 2 * F,
+  return in_slices(T, F, SWIGLU_KEPT_VECS, [&](long long at, const KeptRows& s, int grid) {
+    launch_dependent(swiglu_kept8_kernel<false, SWIGLU_KEPT_VECS>, grid, KEPT_THREADS, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes) + at * 2 * F,
                      static_cast<const uint8_t*>(powers) + at * 2 * s.groups, static_cast<const bf16*>(nullptr), static_cast<bf16*>(gu) + at * 2 * F,
                      act ? static_cast<bf16*>(act) + at * F : nullptr, s);
   });

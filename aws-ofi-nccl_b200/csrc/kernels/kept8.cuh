@@ -16,20 +16,25 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t finite_or_zero(uint32_t magnitude) { return magnitude >= 0x7F80u ? 0u : magnitude; }
 
 // Eight bf16 of a lane -> their codes and, in all four lanes of the group, the byte of its power. A whole warp calls it.
 __device__ __forceinline__ uint2 keep8(const uint4& v, uint32_t& power) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t most = max_u16x2(max_u16x2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), max_u16x2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
-  bool finite = true;
-  if (max(most >> 16, most & 0xFFFFu) >= 0x7F80u) {
-    finite = false;
+  most = max(most >> 16, most & 0xFFFFu);
+  if (most >= 0x7F80u) {   // rare: such values become NaN, and the largest of the others is looked for
     most = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) most = max(most, max(finite_or_zero(w[k] >> 16 & 0x7FFFu), finite_or_zero(w[k] & 0x7FFFu)));
-  } else {
-    most = max(most >> 16, most & 0xFFFFu);
+#pragma unroll 1
+    for (int k = 0; k < 8; ++k) {
+      const int at = k >> 1, shift = (k & 1) * 16;
+      const uint32_t word = at == 0 ? w[0] : at == 1 ? w[1] : at == 2 ? w[2] : w[3], m = word >> shift & 0x7FFFu;
+      if (m < 0x7F80u) {
+        most = max(most, m);
+        continue;
+      }
+      const uint32_t nan = 0x7FFFu << shift;
+      w[0] |= at == 0 ? nan : 0, w[1] |= at == 1 ? nan : 0, w[2] |= at == 2 ? nan : 0, w[3] |= at == 3 ? nan : 0;
+    }
   }
   most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
   most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -41,11 +46,7 @@ __device__ __forceinline__ uint2 keep8(const uint4& v, uint32_t& power) {
   for (int k = 0; k < 2; ++k) {
     float f[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t bits = e & 1 ? w[2 * k + e / 2] & 0xFFFF0000u : w[2 * k + e / 2] << 16;
-      f[e] = __uint_as_float(bits) * scale;
-      if (!finite && (bits & 0x7F800000u) == 0x7F800000u) f[e] = __uint_as_float(0x7FFFFFFFu);
-    }
+    for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(e & 1 ? w[2 * k + e / 2] & 0xFFFF0000u : w[2 * k + e / 2] << 16) * scale;
     codes[k] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3)) |
                (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3)) << 16);
   }

@@ -115,9 +115,13 @@ class Trainer:
 
     def launches_per_step(self) -> int:
         """Number of this library's kernels launched by one step (GEMMs + bandwidth kernels)."""
-        L = self.cfg.n_layers
+        L, cfg = self.cfg.n_layers, self.cfg
         fwd = 1 + L * (2 + 4 + 1 + 1) + 1 + 1 + 1  # embed; per layer 2 norms, 4 GEMMs, rope, swiglu; final norm, lm_head, CE
         bwd = 1 + L * (2 * 2 + 8 + 1 + 1) + 2 + 2  # embed bwd; per layer norm bwd(2 kernels each), 8 GEMMs, rope, swiglu
+        if cfg.window:   # forward; row sums, gradients of keys and of queries (and where sinks are seen from far away their parts' sums)
+            fwd, bwd = fwd + L, bwd + 3 * L
+        if cfg.keep_bits == 8:   # x of two layers, gate|up there; x twice and gate|up back
+            fwd, bwd = fwd + 3 * L, bwd + 3 * L
         opt = 1
         dp = self.dp.launches_per_step() if self.dp is not None else 0
         return fwd + bwd + opt + dp

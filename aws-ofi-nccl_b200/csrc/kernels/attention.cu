@@ -74,21 +74,22 @@ struct AttnFwdItem {
   }
 };
 
-using AttnFwdRoles = AttnRoles<8>;
+using AttnFwdRoles = AttnRoles<16>;
 template <int HD>
 struct AttnFwd {
   static constexpr int TILE = ATT_TILE * HD * 2;
   static constexpr int STAGES = 4;
-  static constexpr int OUT = (2 + STAGES) * TILE;       // 32 rows of 64 elements of each warp on their way out
-  static constexpr int TILES = OUT + 8 * 4096;
+  static constexpr int OUT = (2 + STAGES) * TILE;       // 32 rows of 32 elements of each warp on their way out
+  static constexpr int TOLD = OUT + 16 * 2048;          // a number for each row, from one of its threads to the other
+  static constexpr int TILES = TOLD + 2 * ATT_TILE * 4;
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
   // barriers: stages full and empty; q there and read; scores there; probabilities there (or their row scaled), in two parts; sums of a unit done; rows behind
   // a sequence's end to be cleared, cleared
   static constexpr int FULL = 0, EMPTY = STAGES, Q = 2 * STAGES, QREAD = Q + 2, SCORES = QREAD + 2, PROBS = SCORES + 2, DONE = PROBS + 4, CLEAR = DONE + 2,
                        CLEARED = CLEAR + 1, BARS = CLEARED + 1;
-  // tensor memory: scores of a unit (probabilities as bf16 over their first half), its sums
+  // tensor memory: scores of a unit (probabilities as bf16 over the first columns of each half), its sums
   static constexpr int S_COL = 0, O_COL = 256;
-  static constexpr int FIRST = 96;   // columns of probabilities that are handed over while the others are computed
+  static_assert(SMEM <= 232448, "more than a CTA's shared memory");
 };
 
 template <int HD>
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
   using L = AttnFwd<HD>;
   using R = AttnFwdRoles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 4 : 1; });
+  const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 8 : 1; });
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t q_tile = cta.smem, stages = cta.smem + 2 * L::TILE;
@@ -163,15 +164,15 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             if (w.uses(u, t)) {
-              // in two parts, as they are there
+              // in two parts, of 32 columns of both halves, as they are there
 #pragma unroll
               for (int part = 0; part < 2; ++part) {
                 if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
                 tc_fence_after();
-                if (part == 0) multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, 0, begun[u]);
-#pragma unroll
-                for (int k = part ? L::FIRST / 16 : 1; k < (part ? ATT_TILE : L::FIRST) / 16; ++k)
-                  multiply_step<HD, 128>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, k, true);
+                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2, part || begun[u]);
+                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 1, true);
+                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 4, true);
+                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 5, true);
               }
               if (!ok) break;
               begun[u] = true;
@@ -197,65 +198,65 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
       zero_rows<HD, ATT_TILE>(stage(at - 1), w.clear_from, cta.bar(L::CLEARED));
     }
   } else {
-    // ---------------------------------------------------------------- softmax: a thread has a row
-    const int u = warp >> 2;
+    // ---------------------------------------------------------------- softmax: a thread has half of a row
+    const int u = warp >> 3, half = warp >> 2 & 1, place = (warp & 3) * 32 + lane, meeting = 1 + u;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE, o_col = lanes + L::O_COL + u * 128;
+    const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE + half * 64, o_col = lanes + L::O_COL + u * 128 + half * (HD / 2);
+    volatile float* const told = reinterpret_cast<volatile float*>(smem_raw + (cta.smem - smem_u32(smem_raw)) + L::TOLD) + u * ATT_TILE + place;
     const float c = s.scale * ATT_LOG2E;
     const Pair c2 = both(c);
-    const uint32_t slab = cta.smem + L::OUT + warp * 4096;
+    const uint32_t slab = cta.smem + L::OUT + warp * 2048;
     uint32_t turns = 0, done = 0;   // tiles and units so far
-    bool ok = true;
+    bool ok = true;                 // where a wait gives up the walks go on without its scores: all threads of a unit meet as often
 #pragma unroll 1
-    for (int turn = 0; ok && dealt(turn) < items; ++turn) {
+    for (int turn = 0; dealt(turn) < items; ++turn) {
       const AttnFwdItem walk(s, dealt(turn));
-      const int i0 = u ? walk.unit[1].i0 : walk.unit[0].i0, i = i0 + (warp & 3) * 32 + lane, lo = u ? walk.unit[1].lo : walk.unit[0].lo;
+      const int i0 = u ? walk.unit[1].i0 : walk.unit[0].i0, lo = u ? walk.unit[1].lo : walk.unit[0].lo;
       // this unit's own tiles of the walk
       const int far = min(walk.sink_tiles, lo), n = (u ? walk.unit[1].live : walk.unit[0].live) ? far + (u ? walk.unit[1].hi : walk.unit[0].hi) - lo + 1 : 0;
-      float top = -INFINITY, sum = 0.f;   // of the scores times c, as far as the sums are scaled to it; relative to 2^top
+      float top = -INFINITY;   // of the scores times c, as far as the sums are scaled to it
+      float sum = 0.f;         // of this half's probabilities, relative to 2^top
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++turns) {
-        const int j0 = (j < far ? j : lo + j - far) * ATT_TILE;
-        if (!(ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+        const int j0 = (j < far ? j : lo + j - far) * ATT_TILE + half * 64;
+        ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
         tc_fence_after();
-        const bool whole = j0 + ATT_TILE - 1 <= i0 && (s.window == 0 || i0 + ATT_TILE - 1 - j0 < s.window || j0 + ATT_TILE <= s.sinks);
-        const int last = i - j0, first = s.window ? last - s.window + 1 : 0, sinks = s.window ? s.sinks - j0 : 0;
+        const bool whole = j0 + 63 <= i0 && (s.window == 0 || i0 + ATT_TILE - 1 - j0 < s.window || j0 + 64 <= s.sinks);
         auto hide = [&](uint32_t(&x)[32], int k) {   // of columns from 32 k on
-          const uint32_t seen = columns_seen(first - k * 32, last - k * 32, sinks - k * 32);
+          const int last = i0 + place - j0 - k * 32, first = s.window ? last - s.window + 1 : 0, sinks = s.window ? s.sinks - j0 - k * 32 : 0;
+          const uint32_t seen = columns_seen(first, last, sinks);
           if (__all_sync(0xffffffffu, seen == 0xffffffffu)) return;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!(seen >> e & 1)) x[e] = 0xFF800000u;   // -inf
         };
-        // Scores are read twice, for their maximum and for the probabilities, half of a row at a time: a whole one with what else is needed is more than
-        // a thread has registers
-        uint32_t x[32], y[32];
+        // Scores are read twice, for their maximum and for the probabilities: all of them with what else is needed are more than a thread has registers
+        uint32_t x[32];
         float some[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
+        for (int k = 0; k < 2; ++k) {
           tmem_ld_32x32(s_col + k * 32, x);
-          tmem_ld_32x32(s_col + k * 32 + 32, y);
           tmem_ld_wait();
-          if (!whole) hide(x, k), hide(y, k + 1);
+          if (!whole) hide(x, k);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            some[0] = most_of(some[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-            some[1] = most_of(some[1], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
-            some[2] = most_of(some[2], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-            some[3] = most_of(some[3], __uint_as_float(y[e + 2]), __uint_as_float(y[e + 3]));
-          }
+          for (int e = 0; e < 32; e += 2) some[e / 2 & 3] = most_of(some[e / 2 & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
         }
         const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
-        // The sums are scaled to a new maximum only where one of the warp's rows has grown by more than 2^8: probabilities beside the old one stay in
+        // The sums are scaled to a new maximum only where one of the unit's rows has grown by more than 2^8: probabilities beside the old one stay in
         // range. A NaN grows, too, and makes one of everything in its row.
-        if (__any_sync(0xffffffffu, !(most <= top + 8.f))) {
-          const float now = most_of(top, most, most);
+        if (any_of_256(meeting, !(most <= top + 8.f))) {
+          if (half) *told = most;
+          meet_256(meeting);
+          float now = 0.f;
+          if (!half) *told = now = most_of(top, most, *told);
+          meet_256(meeting);
+          if (half) now = *told;
           const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
           top = now;
           sum *= f;
           if (j) {
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
+            for (int k = 0; k < HD / 32; ++k) {
               uint32_t o[16];
               tmem_ld_32x16(o_col + k * 16, o);
               tmem_ld_wait();
@@ -267,7 +268,12 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         }
         const Pair ref = both(top == -INFINITY ? 0.f : -top);
         Pair part[2] = {both(0.f), both(0.f)};
-        auto probabilities = [&](const uint32_t(&x)[32], int k) {
+        // probabilities of 32 columns come to lie over columns that have been read
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          tmem_ld_32x32(s_col + k * 32, x);
+          tmem_ld_wait();
+          if (!whole) hide(x, k);
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -278,29 +284,11 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
             p[e / 2] = pack_bf16x2(p0, p1);
           }
           tmem_st_32x16(s_col + k * 16, p);
-        };
-        auto hand_over = [&](int which) {
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + which));
-        };
-        // probabilities of 32 columns come to lie over columns that have been read
-        tmem_ld_32x32(s_col, x);
-        tmem_ld_32x32(s_col + 32, y);
-        tmem_ld_wait();
-        if (!whole) hide(x, 0), hide(y, 1);
-        probabilities(x, 0);
-        tmem_ld_32x32(s_col + 64, x);
-        probabilities(y, 1);
-        tmem_ld_32x32(s_col + 96, y);
-        tmem_ld_wait();
-        if (!whole) hide(x, 2), hide(y, 3);
-        probabilities(x, 2);
-        static_assert(L::FIRST == 96, "three quarters of the columns");
-        hand_over(0);
-        probabilities(y, 3);
-        hand_over(1);
+          if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + k));
+        }
         float a, d;
         (part[0] + part[1]).to(a, d);
         sum += a + d;
@@ -308,34 +296,37 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
       const AttnFwdItem w(s, dealt(anew(turn)));
       const AttnUnit me = u ? w.unit[1] : w.unit[0];
       if (!me.exists) continue;
-      if (ok && n) ok = cta.wait(L::DONE + u, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
+      if (half) *told = sum;
+      meet_256(meeting);
+      if (!half) *told = sum = sum + *told;
+      meet_256(meeting);
+      if (half) sum = *told;
+      if (n) ok = cta.wait(L::DONE + u, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
       tc_fence_after();
+      const int i = me.i0 + place;
       const bool mine = i < w.len;
-      // no probability behind the end
-      minus_lse[(static_cast<int64_t>(w.b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
+      if (!half)   // no probability behind the end
+        minus_lse[(static_cast<int64_t>(w.b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
       const float f = 1.f / sum;
       const bool any = mine && n && ok;
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k) {
-        uint32_t o[2][32];
+        uint32_t o[32];
         if (n && ok) {
-          tmem_ld_32x32(o_col + k * 64, o[0]);
-          tmem_ld_32x32(o_col + k * 64 + 32, o[1]);
+          tmem_ld_32x32(o_col + k * 32, o);
           tmem_ld_wait();
         }
         if (lane == 0) tma_store_wait_read<0>();
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 64; e += 8) {
-          auto two = [&](int at) {
-            return any ? pack_bf16x2(__uint_as_float(o[at >> 5][at & 31]) * f, __uint_as_float(o[at >> 5][(at & 31) + 1]) * f) : 0u;
-          };
-          st_shared_v4(slab + lane * 128 + ((e / 8 ^ (lane & 7)) << 4), two(e), two(e + 2), two(e + 4), two(e + 6));
+        for (int e = 0; e < 32; e += 8) {
+          auto two = [&](int at) { return any ? pack_bf16x2(__uint_as_float(o[at]) * f, __uint_as_float(o[at + 1]) * f) : 0u; };
+          st_shared_v4(slab + lane * 64 + ((e / 8 ^ (lane >> 1 & 3)) << 4), two(e), two(e + 2), two(e + 4), two(e + 6));   // 64-byte swizzle
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_4d(&tmO, slab, k * 64, me.head, me.i0 + (warp & 3) * 32, w.b);
+          tma_store_4d(&tmO, slab, half * (HD / 2) + k * 32, me.head, me.i0 + (warp & 3) * 32, w.b);
           tma_store_commit();
         }
       }
@@ -815,16 +806,16 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnSplit split, bf
   *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
 }
 
-// [B][S][heads][HD] with element strides {batch, token, head}, boxes of 64 (or `rows`) rows x 64 elements of a head
-static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd, int rows = ATT_BOX) {
+// [B][S][heads][HD] with element strides {batch, token, head}, boxes of 64 rows x 64 elements of a head, or to be stored 32 x 32
+static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd, bool store = false) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) return B200_ERR_NO_DRIVER;
   auto pitch = [&](int size, long long stride) { return static_cast<cuuint64_t>(size == 1 ? hd : stride) * 2; };   // of a single one any will do
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(B)};
   const cuuint64_t strides[3] = {pitch(heads, t.head), pitch(S, t.token), pitch(B, t.batch)};
-  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {store ? 32u : 64u, 1, store ? 32u : static_cast<cuuint32_t>(ATT_BOX), 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return 0;
   fprintf(stderr, "[b200ops] cuTensorMapEncodeTiled failed: %d (base=%p, %d x %d x %d x %d)\n", static_cast<int>(r), t.data, B, S, heads, hd);
   return B200_ERR_TENSORMAP;
@@ -852,7 +843,7 @@ template <int HD>
 static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
   CUtensorMap q, k, v, o;
   const long long row = static_cast<long long>(s.nq) * HD;
-  if (int rc = attn_map(&o, {a.out, s.S * row, row, HD}, s.B, s.S, s.nq, HD, 32)) return rc;
+  if (int rc = attn_map(&o, {a.out, s.S * row, row, HD}, s.B, s.S, s.nq, HD, true)) return rc;
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;

@@ -165,7 +165,7 @@ def test_mlp_is_its_parts(t, hidden, f):
 
 @pytest.mark.gpu
 def test_a_layer_holds_no_more_than_it_keeps():
-    """Bytes that live between the passes."""
+    """Bytes asked for that live between the passes (the allocator may hand out up to a megabyte more)."""
     from aws_ofi_nccl_b200.ops import llm
 
     t, hidden, f = 4096, 512, 1024
@@ -174,10 +174,11 @@ def test_a_layer_holds_no_more_than_it_keeps():
     for bits in (8, 16):
         x = torch.randn(t, hidden, device="cuda").to(BF)
         torch.cuda.synchronize()
-        before = torch.cuda.memory_allocated()
+        asked = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]   # noqa: E731
+        before = asked()
         y = llm.swiglu_mlp(x, wgu, wd, keep_bits=bits)
         del x
-        held[bits] = torch.cuda.memory_allocated() - before - y.numel() * 2 + t * hidden * 2
+        held[bits] = asked() - before - y.numel() * 2 + t * hidden * 2
         del y
     assert held[8] <= t * (hidden + 2 * f) * 33 // 32 + 8192 and held[16] >= t * (2 * hidden + 6 * f)
 

@@ -212,6 +212,8 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     for (int turn = 0; dealt(turn) < items; ++turn) {
       const AttnFwdItem walk(s, dealt(turn));
       const int i0 = u ? walk.unit[1].i0 : walk.unit[0].i0, lo = u ? walk.unit[1].lo : walk.unit[0].lo;
+      const bool exists = u ? walk.unit[1].exists : walk.unit[0].exists;
+      const int head_of_all = walk.b * s.nq + (u ? walk.unit[1].head : walk.unit[0].head);
       // this unit's own tiles of the walk
       const int far = min(walk.sink_tiles, lo), n = (u ? walk.unit[1].live : walk.unit[0].live) ? far + (u ? walk.unit[1].hi : walk.unit[0].hi) - lo + 1 : 0;
       float top = -INFINITY;   // of the scores times c, as far as the sums are scaled to it
@@ -293,9 +295,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         (part[0] + part[1]).to(a, d);
         sum += a + d;
       }
-      const AttnFwdItem w(s, dealt(anew(turn)));
-      const AttnUnit me = u ? w.unit[1] : w.unit[0];
-      if (!me.exists) continue;
+      if (!exists) continue;
       if (half) *told = sum;
       meet_256(meeting);
       if (!half) *told = sum = sum + *told;
@@ -303,10 +303,10 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
       if (half) sum = *told;
       if (n) ok = cta.wait(L::DONE + u, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
       tc_fence_after();
-      const int i = me.i0 + place;
-      const bool mine = i < w.len;
+      const int b = s.by_nq.quotient(head_of_all), head = head_of_all - b * s.nq, i = i0 + place;
+      const bool mine = i < sequence_length(s, b);
       if (!half)   // no probability behind the end
-        minus_lse[(static_cast<int64_t>(w.b) * s.nq + me.head) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
+        minus_lse[static_cast<int64_t>(head_of_all) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
       const float f = 1.f / sum;
       const bool any = mine && n && ok;
 #pragma unroll
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_4d(&tmO, slab, half * (HD / 2) + k * 32, me.head, me.i0 + (warp & 3) * 32, w.b);
+          tma_store_4d(&tmO, slab, half * (HD / 2) + k * 32, head, i0 + (warp & 3) * 32, b);
           tma_store_commit();
         }
       }
@@ -618,14 +618,15 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     uint32_t i = 0, done = 0;
     bool ok = true;
     float my_lse = 0.f, my_delta = 0.f;
-    auto fetch = [&](const Item& of) {   // lse and delta of a row
-      if constexpr (!KEYS) {
-        const int64_t from = (static_cast<int64_t>(of.b) * s.nq + of.head) * s.rows + of.r0 + (warp & 3) * 32 + lane;
-        my_lse = minus_lse[from];
-        my_delta = minus_delta[from];
-      }
+    auto fetch = [&](int turn) {   // lse and delta of a row of dq's items
+      const int index = dealt(turn);
+      if (KEYS || index >= items) return;
+      const int nth = s.by_heads_q.quotient(index), of_all = index - nth * s.by_heads_q.d;
+      const int64_t from = static_cast<int64_t>(of_all) * s.rows + s.rows - (nth + 1) * ATT_TILE + (warp & 3) * 32 + lane;
+      my_lse = minus_lse[from];
+      my_delta = minus_delta[from];
     };
-    if (dealt(0) < items) fetch(Item(s, split, dealt(0)));
+    fetch(0);
 #pragma unroll 1
     for (int turn = 0; ok && dealt(turn) < items; ++turn) {
     const Item walk(s, split, dealt(turn));
@@ -718,9 +719,8 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
       arrive(L::GRADS);
     }
     // ---------------------------------------------------------------- what the sums became
-    // while the last products run
-    if (!KEYS && dealt(turn + 1) < items) fetch(Item(s, split, dealt(turn + 1)));
-    const Item it(s, split, dealt(anew(turn)));
+    fetch(turn + 1);   // while the last products run
+    const Item it(s, split, dealt(KEYS ? anew(turn) : turn));
     if (ok && it.n > 0) ok = cta.wait(L::DONE, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
     tc_fence_after();
     const bool full = ok && it.n > 0, mine = it.r0 + (warp & 3) * 32 + lane < it.len;

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "b200ops.h"
@@ -224,76 +225,95 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
         tc_fence_after();
         const bool whole = j0 + 63 <= i0 && (s.window == 0 || i0 + ATT_TILE - 1 - j0 < s.window || j0 + 64 <= s.sinks);
-        auto hide = [&](uint32_t(&x)[32], int k) {   // of columns from 32 k on
-          const int last = i0 + place - j0 - k * 32, first = s.window ? last - s.window + 1 : 0, sinks = s.window ? s.sinks - j0 - k * 32 : 0;
-          const uint32_t seen = columns_seen(first, last, sinks);
-          if (__all_sync(0xffffffffu, seen == 0xffffffffu)) return;
+        auto take = [&](auto is_whole) {   // a tile on no border without any of what a border takes
+          constexpr bool WHOLE = decltype(is_whole)::value;
+          // what a row sees of each 32 columns; blocks of 32 rows and columns of which none is seen are zeros without their scores being looked at
+          uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+          if constexpr (!WHOLE) {
+            const int last = i0 + place - j0, first = s.window ? last - s.window + 1 : 0, sinks = s.window ? s.sinks - j0 : 0;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(seen >> e & 1)) x[e] = 0xFF800000u;   // -inf
-        };
-        // Scores are read twice, for their maximum and for the probabilities: all of them with what else is needed are more than a thread has registers
-        uint32_t x[32];
-        float some[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int k = 0; k < 2; ++k) seen[k] = columns_seen(first - k * 32, last - k * 32, sinks - k * 32);
+          }
+          const bool some_seen[2] = {WHOLE || __any_sync(0xffffffffu, seen[0]), WHOLE || __any_sync(0xffffffffu, seen[1])};
+          auto hide = [&](uint32_t(&x)[32], int k) {
+            if (WHOLE || __all_sync(0xffffffffu, seen[k] == 0xffffffffu)) return;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          tmem_ld_32x32(s_col + k * 32, x);
-          tmem_ld_wait();
-          if (!whole) hide(x, k);
+            for (int e = 0; e < 32; ++e)
+              if (!(seen[k] >> e & 1)) x[e] = 0xFF800000u;   // -inf
+          };
+          // Scores are read twice, for their maximum and for the probabilities: all of them with what else is needed are more than a thread has registers
+          uint32_t x[32];
+          float some[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) some[e / 2 & 3] = most_of(some[e / 2 & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-        }
-        const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
-        // The sums are scaled to a new maximum only where one of the unit's rows has grown by more than 2^8: probabilities beside the old one stay in
-        // range. A NaN grows, too, and makes one of everything in its row.
-        if (any_of_256(meeting, !(most <= top + 8.f))) {
-          if (half) *told = most;
-          meet_256(meeting);
-          float now = 0.f;
-          if (!half) *told = now = most_of(top, most, *told);
-          meet_256(meeting);
-          if (half) now = *told;
-          const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
-          top = now;
-          sum *= f;
-          if (j) {
+          for (int k = 0; k < 2; ++k) {
+            if (!some_seen[k]) continue;
+            tmem_ld_32x32(s_col + k * 32, x);
+            tmem_ld_wait();
+            hide(x, k);
 #pragma unroll
-            for (int k = 0; k < HD / 32; ++k) {
-              uint32_t o[16];
-              tmem_ld_32x16(o_col + k * 16, o);
-              tmem_ld_wait();
+            for (int e = 0; e < 32; e += 2) some[e / 2 & 3] = most_of(some[e / 2 & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          }
+          const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
+          // The sums are scaled to a new maximum only where one of the unit's rows has grown by more than 2^8: probabilities beside the old one stay in
+          // range. A NaN grows, too, and makes one of everything in its row.
+          if (any_of_256(meeting, !(most <= top + 8.f))) {
+            if (half) *told = most;
+            meet_256(meeting);
+            float now = 0.f;
+            if (!half) *told = now = most_of(top, most, *told);
+            meet_256(meeting);
+            if (half) now = *told;
+            const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
+            top = now;
+            sum *= f;
+            if (j) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st_32x16(o_col + k * 16, o);
+              for (int k = 0; k < HD / 32; ++k) {
+                uint32_t o[16];
+                tmem_ld_32x16(o_col + k * 16, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st_32x16(o_col + k * 16, o);
+              }
             }
           }
-        }
-        const Pair ref = both(top == -INFINITY ? 0.f : -top);
-        Pair part[2] = {both(0.f), both(0.f)};
-        // probabilities of 32 columns come to lie over columns that have been read
+          const Pair ref = both(top == -INFINITY ? 0.f : -top);
+          Pair part[2] = {both(0.f), both(0.f)};
+          // probabilities of 32 columns come to lie over columns that have been read
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          tmem_ld_32x32(s_col + k * 32, x);
-          tmem_ld_wait();
-          if (!whole) hide(x, k);
-          uint32_t p[16];
+          for (int k = 0; k < 2; ++k) {
+            uint32_t p[16];
+            if (some_seen[k]) {
+              tmem_ld_32x32(s_col + k * 32, x);
+              tmem_ld_wait();
+              hide(x, k);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float p0, p1;
-            fma2(pair_of(x[e], x[e + 1]), c2, ref).to(p0, p1);
-            p0 = exp2_unit(p0), p1 = exp2_unit(p1);
-            part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
-            p[e / 2] = pack_bf16x2(p0, p1);
+              for (int e = 0; e < 32; e += 2) {
+                float p0, p1;
+                fma2(pair_of(x[e], x[e + 1]), c2, ref).to(p0, p1);
+                p0 = exp2_unit(p0), p1 = exp2_unit(p1);
+                part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
+                p[e / 2] = pack_bf16x2(p0, p1);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) p[e] = 0;
+            }
+            tmem_st_32x16(s_col + k * 16, p);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + k));
           }
-          tmem_st_32x16(s_col + k * 16, p);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 2 * u + k));
-        }
-        float a, d;
-        (part[0] + part[1]).to(a, d);
-        sum += a + d;
+          float a, d;
+          (part[0] + part[1]).to(a, d);
+          sum += a + d;
+        };
+        if (whole)
+          take(std::true_type());
+        else
+          take(std::false_type());
       }
       if (!exists) continue;
       if (half) *told = sum;
@@ -399,9 +419,9 @@ struct AttnBwd {
   static_assert(SMEM <= 232448, "more than a CTA's shared memory");
   static constexpr int FULL1 = 0, EMPTY1 = FULL1 + N1, FULL2 = EMPTY1 + N1, EMPTY2 = FULL2 + N2, THERE = EMPTY2 + N2, HELD_READ = THERE + 1;
   static constexpr int T1 = HELD_READ + 1, T2 = T1 + (KEYS ? 1 : 2), DONE = T2 + 1;            // T1 and T2 there, sums done
-  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1;
+  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1;   // P and dS there: by all warps
   // rows behind a sequence's end are to be cleared, are zeros: of both passing tensors
-  static constexpr int CLEAR1 = GRADS + 1, CLEARED1 = CLEAR1 + 1, CLEAR2 = CLEARED1 + 1, CLEARED2 = CLEAR2 + 1, BARS = CLEARED2 + 1;  // P and dS there: by all warps
+  static constexpr int CLEAR1 = GRADS + 1, CLEARED1 = CLEAR1 + 1, CLEAR2 = CLEARED1 + 1, CLEARED2 = CLEAR2 + 1, BARS = CLEARED2 + 1;
   // tensor memory: scores (dq: of two tiles), dout v^T, sums
   static constexpr int T1_COL = 0, T2_COL = KEYS ? 128 : 256, ACC1_COL = 256, ACC2_COL = 384;
 };
@@ -629,153 +649,153 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     fetch(0);
 #pragma unroll 1
     for (int turn = 0; ok && dealt(turn) < items; ++turn) {
-    const Item walk(s, split, dealt(turn));
-    const int r0 = walk.r0, r = r0 + (warp & 3) * 32 + lane, n = walk.n;
-    int at = 0;
+      const Item walk(s, split, dealt(turn));
+      const int r0 = walk.r0, r = r0 + (warp & 3) * 32 + lane, n = walk.n;
+      int at = 0;
 #pragma unroll 1
-    for (int k = 0; k < n; ++k, ++i) {
-      const int c0 = walk.row(at) + w * 32;
-      if (++at == walk.per_head) at = 0;
-      const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
-      if constexpr (KEYS) {   // lse and delta of the stage
-        if (!(ok = full1(i))) break;
-      }
-      if (!(ok = cta.wait(KEYS ? L::T1 : L::T1 + (i & 1), KEYS ? i & 1 : i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
-      tc_fence_after();
-      // which columns this row's partner sees: those from first to last, and those in front of `sinks`
-      bool whole;
-      int first, last, sinks = 0;
-      if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
-        whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + 31 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
-        first = r - c0;
-        last = s.window == 0 || r < s.sinks ? 32 : first + s.window - 1;
-      } else {                // columns are keys
-        whole = c0 + 31 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + 32 <= s.sinks);
-        last = r - c0;
-        first = s.window ? last - s.window + 1 : 0;
-        sinks = s.window ? s.sinks - c0 : 0;
-      }
-      const ulonglong2* const stat = reinterpret_cast<const ulonglong2*>(stat_base + i % L::N1 * L::STATS);
-      auto row_numbers = [&](int of, int e, Pair& p0, Pair& p1) {   // of columns e to e + 3: lse (0), delta (1)
-        if constexpr (KEYS) {
-          const ulonglong2 v = stat[of * (ATT_TILE / 4) + e / 4];
-          p0.bits = v.x, p1.bits = v.y;
-        } else {
-          p0 = p1 = both(of ? my_delta : my_lse);
+      for (int k = 0; k < n; ++k, ++i) {
+        const int c0 = walk.row(at) + w * 32;
+        if (++at == walk.per_head) at = 0;
+        const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
+        if constexpr (KEYS) {   // lse and delta of the stage
+          if (!(ok = full1(i))) break;
         }
-      };
-      auto arrive = [&](int barrier) {
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(cta.bar(barrier));
-      };
-      auto hide = [&](uint32_t(&packed)[16]) {   // also what zero times is not finite
-        const uint32_t seen = columns_seen(first, last, sinks);
-        if (__any_sync(0xffffffffu, seen + 1 > 1)) {   // neither none nor all of a row
-#pragma unroll
-          for (int e = 0; e < 16; ++e) packed[e] = seen_pair(packed[e], seen, e);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) packed[e] &= seen;
+        if (!(ok = cta.wait(KEYS ? L::T1 : L::T1 + (i & 1), KEYS ? i & 1 : i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+        tc_fence_after();
+        // which columns this row's partner sees: those from first to last, and those in front of `sinks`
+        bool whole;
+        int first, last, sinks = 0;
+        if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
+          whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + 31 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
+          first = r - c0;
+          last = s.window == 0 || r < s.sinks ? 32 : first + s.window - 1;
+        } else {                // columns are keys
+          whole = c0 + 31 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + 32 <= s.sinks);
+          last = r - c0;
+          first = s.window ? last - s.window + 1 : 0;
+          sinks = s.window ? s.sinks - c0 : 0;
         }
-      };
-      uint32_t p[32], y[32], o[16];
-      tmem_ld_32x32(t1, p);
-      tmem_ld_wait();
+        const ulonglong2* const stat = reinterpret_cast<const ulonglong2*>(stat_base + i % L::N1 * L::STATS);
+        auto row_numbers = [&](int of, int e, Pair& p0, Pair& p1) {   // of columns e to e + 3: lse (0), delta (1)
+          if constexpr (KEYS) {
+            const ulonglong2 v = stat[of * (ATT_TILE / 4) + e / 4];
+            p0.bits = v.x, p1.bits = v.y;
+          } else {
+            p0 = p1 = both(of ? my_delta : my_lse);
+          }
+        };
+        auto arrive = [&](int barrier) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(cta.bar(barrier));
+        };
+        auto hide = [&](uint32_t(&packed)[16]) {   // also what zero times is not finite
+          const uint32_t seen = columns_seen(first, last, sinks);
+          if (__any_sync(0xffffffffu, seen + 1 > 1)) {   // neither none nor all of a row
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        Pair l0, l1;
-        row_numbers(0, e, l0, l1);
-        float a, d;
-        exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
-        p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
-        exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
-        p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
-      }
-      if constexpr (KEYS) {
+            for (int e = 0; e < 16; ++e) packed[e] = seen_pair(packed[e], seen, e);
+          } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
-        if (!whole) hide(o);
-        tmem_st_32x16(t1, o);   // over columns that this warp has read
-        arrive(L::PROBS);
-      }
-      if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
-      tc_fence_after();
-      tmem_ld_32x32(t2, y);
-      tmem_ld_wait();
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        Pair d0, d1;
-        row_numbers(1, e, d0, d1);
-        float a, d;
-        (pair_of(p[e], p[e + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
-        o[e / 2] = pack_bf16x2(a, d);
-        (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
-        o[e / 2 + 1] = pack_bf16x2(a, d);
-      }
-      if (!whole) hide(o);
-      tmem_st_32x16(KEYS ? t2 : t1, o);
-      arrive(L::GRADS);
-    }
-    // ---------------------------------------------------------------- what the sums became
-    fetch(turn + 1);   // while the last products run
-    const Item it(s, split, dealt(KEYS ? anew(turn) : turn));
-    if (ok && it.n > 0) ok = cta.wait(L::DONE, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
-    tc_fence_after();
-    const bool full = ok && it.n > 0, mine = it.r0 + (warp & 3) * 32 + lane < it.len;
-    // KEYS: the first two groups of warps have dv, the others dk, half of the columns each; dq's columns are shared by four
-    constexpr int COLS = KEYS ? HD / 2 : HD / 4;
-    const int which = KEYS ? w >> 1 : 1, col = (KEYS ? w & 1 : w) * COLS;
-    const uint32_t acc = lanes + (which ? L::ACC2_COL : L::ACC1_COL) + col;
-    const float f = which ? s.scale : 1.f;
-    const int out_heads = KEYS ? s.nkv : s.nq;
-    const int row0 = it.r0 + (warp & 3) * 32;   // the warp's
-    bf16* const grad = (which ? grad2 : grad1) + ((static_cast<int64_t>(it.b) * s.S + row0) * out_heads + it.head) * HD + col;
-    const int64_t pitch = static_cast<int64_t>(out_heads) * HD;
-    float* sums = nullptr;
-    if (it.joined) {
-      const int64_t heads = static_cast<int64_t>(s.B) * s.nkv, place = (it.part * split.tiles + it.tile) * heads + it.b * s.nkv + it.head;
-      sums = split.sums + ((place * 2 + which) * ATT_TILE + (warp & 3) * 32) * HD + col;
-    }
-    auto load = [&](int c, uint32_t(&o)[16]) {   // 16 columns, scaled
-      if (full) {
-        tmem_ld_32x16(acc + c, o);
+            for (int e = 0; e < 16; ++e) packed[e] &= seen;
+          }
+        };
+        uint32_t p[32], y[32], o[16];
+        tmem_ld_32x32(t1, p);
         tmem_ld_wait();
-      }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
-    };
-    auto two = [](const uint32_t(&o)[16], int e) { return pack_bf16x2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])); };
-    if constexpr (!KEYS && COLS % 32 == 0) {
-#pragma unroll
-      for (int c = 0; c < COLS; c += 32) {
-        uint32_t o[16], packed[16];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          load(c + k * 16, o);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) packed[k * 8 + e] = two(o, e);
+        for (int e = 0; e < 32; e += 4) {
+          Pair l0, l1;
+          row_numbers(0, e, l0, l1);
+          float a, d;
+          exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
+          p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
+          exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
+          p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
         }
-        store_rows64(packed, [&](int at) { return row0 + at < s.S ? reinterpret_cast<uint4*>(grad + at * pitch + c) : nullptr; });
+        if constexpr (KEYS) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
+          if (!whole) hide(o);
+          tmem_st_32x16(t1, o);   // over columns that this warp has read
+          arrive(L::PROBS);
+        }
+        if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+        tc_fence_after();
+        tmem_ld_32x32(t2, y);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          Pair d0, d1;
+          row_numbers(1, e, d0, d1);
+          float a, d;
+          (pair_of(p[e], p[e + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
+          o[e / 2] = pack_bf16x2(a, d);
+          (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
+          o[e / 2 + 1] = pack_bf16x2(a, d);
+        }
+        if (!whole) hide(o);
+        tmem_st_32x16(KEYS ? t2 : t1, o);
+        arrive(L::GRADS);
       }
-    } else {
+      // ---------------------------------------------------------------- what the sums became
+      fetch(turn + 1);   // while the last products run
+      const Item it(s, split, dealt(KEYS ? anew(turn) : turn));
+      if (ok && it.n > 0) ok = cta.wait(L::DONE, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
+      tc_fence_after();
+      const bool full = ok && it.n > 0, mine = it.r0 + (warp & 3) * 32 + lane < it.len;
+      // KEYS: the first two groups of warps have dv, the others dk, half of the columns each; dq's columns are shared by four
+      constexpr int COLS = KEYS ? HD / 2 : HD / 4;
+      const int which = KEYS ? w >> 1 : 1, col = (KEYS ? w & 1 : w) * COLS;
+      const uint32_t acc = lanes + (which ? L::ACC2_COL : L::ACC1_COL) + col;
+      const float f = which ? s.scale : 1.f;
+      const int out_heads = KEYS ? s.nkv : s.nq;
+      const int row0 = it.r0 + (warp & 3) * 32;   // the warp's
+      bf16* const grad = (which ? grad2 : grad1) + ((static_cast<int64_t>(it.b) * s.S + row0) * out_heads + it.head) * HD + col;
+      const int64_t pitch = static_cast<int64_t>(out_heads) * HD;
+      float* sums = nullptr;
+      if (it.joined) {
+        const int64_t heads = static_cast<int64_t>(s.B) * s.nkv, place = (it.part * split.tiles + it.tile) * heads + it.b * s.nkv + it.head;
+        sums = split.sums + ((place * 2 + which) * ATT_TILE + (warp & 3) * 32) * HD + col;
+      }
+      auto load = [&](int c, uint32_t(&o)[16]) {   // 16 columns, scaled
+        if (full) {
+          tmem_ld_32x16(acc + c, o);
+          tmem_ld_wait();
+        }
 #pragma unroll
-      for (int c = 0; c < COLS; c += 16) {
-        uint32_t o[16];
-        load(c, o);
-        if (it.joined) {
-          uint4* const at = reinterpret_cast<uint4*>(sums + lane * HD + c);
+        for (int e = 0; e < 16; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+      };
+      auto two = [](const uint32_t(&o)[16], int e) { return pack_bf16x2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])); };
+      if constexpr (!KEYS && COLS % 32 == 0) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) at[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        } else if (row0 + lane < s.S) {
-          uint4* const at = reinterpret_cast<uint4*>(grad + lane * pitch + c);
-          at[0] = make_uint4(two(o, 0), two(o, 1), two(o, 2), two(o, 3));
-          at[1] = make_uint4(two(o, 4), two(o, 5), two(o, 6), two(o, 7));
+        for (int c = 0; c < COLS; c += 32) {
+          uint32_t o[16], packed[16];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            load(c + k * 16, o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) packed[k * 8 + e] = two(o, e);
+          }
+          store_rows64(packed, [&](int at) { return row0 + at < s.S ? reinterpret_cast<uint4*>(grad + at * pitch + c) : nullptr; });
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < COLS; c += 16) {
+          uint32_t o[16];
+          load(c, o);
+          if (it.joined) {
+            uint4* const at = reinterpret_cast<uint4*>(sums + lane * HD + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) at[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else if (row0 + lane < s.S) {
+            uint4* const at = reinterpret_cast<uint4*>(grad + lane * pitch + c);
+            at[0] = make_uint4(two(o, 0), two(o, 1), two(o, 2), two(o, 3));
+            at[1] = make_uint4(two(o, 4), two(o, 5), two(o, 6), two(o, 7));
+          }
         }
       }
-    }
-    tc_fence_before();   // the sums are read
+      tc_fence_before();   // the sums are read
     }
   }
   attn_end<R>(cta);

@@ -419,7 +419,7 @@ struct AttnBwd {
   static_assert(SMEM <= 232448, "more than a CTA's shared memory");
   static constexpr int FULL1 = 0, EMPTY1 = FULL1 + N1, FULL2 = EMPTY1 + N1, EMPTY2 = FULL2 + N2, THERE = EMPTY2 + N2, HELD_READ = THERE + 1;
   static constexpr int T1 = HELD_READ + 1, T2 = T1 + (KEYS ? 1 : 2), DONE = T2 + 1;            // T1 and T2 there, sums done
-  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 1;   // P and dS there: by all warps
+  static constexpr int READ = DONE + 1, PROBS = READ, GRADS = PROBS + 2;   // P, in two parts, and dS there: by all warps
   // rows behind a sequence's end are to be cleared, are zeros: of both passing tensors
   static constexpr int CLEAR1 = GRADS + 1, CLEARED1 = CLEAR1 + 1, CLEAR2 = CLEARED1 + 1, CLEARED2 = CLEAR2 + 1, BARS = CLEARED2 + 1;
   // tensor memory: scores (dq: of two tiles), dout v^T, sums
@@ -596,9 +596,18 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         for (int k = 0; k < n && ok; ++k) {
           const uint32_t i = base + k;
           if constexpr (KEYS) {
-            if (!(ok = cta.wait(L::PROBS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
-            tc_fence_after();
-            add(L::ACC1_COL, L::T1_COL, pass2(i), k > 0, L::EMPTY2 + i % L::N2);
+            // in two parts, of 16 columns of every group, as they are there
+            const uint32_t low = TileDesc<ATT_TILE, true>::low(pass2(i));
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              if (!(ok = ok && cta.wait(L::PROBS + part, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
+              tc_fence_after();
+              multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL, low, part, part || k > 0);
+#pragma unroll
+              for (int step = 2; step < ATT_TILE / 16; step += 2) multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL, low, step + part, true);
+            }
+            if (!ok) break;
+            umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
             if (k + 1 < n) t1(k + 1);
           }
           if (!ok || !(ok = cta.wait(L::GRADS, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
@@ -704,21 +713,29 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         tmem_ld_32x32(t1, p);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          Pair l0, l1;
-          row_numbers(0, e, l0, l1);
-          float a, d;
-          exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
-          p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
-          exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
-          p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
-        }
-        if constexpr (KEYS) {
+        for (int part = 0; part < 2; ++part) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = pack_bf16x2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
-          if (!whole) hide(o);
-          tmem_st_32x16(t1, o);   // over columns that this warp has read
-          arrive(L::PROBS);
+          for (int e = part * 16; e < part * 16 + 16; e += 4) {
+            Pair l0, l1;
+            row_numbers(0, e, l0, l1);
+            float a, d;
+            exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
+            p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
+            exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
+            p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
+          }
+          if constexpr (KEYS) {
+            uint32_t q[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = pack_bf16x2(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]));
+            if (!whole) {
+              const uint32_t seen = columns_seen(first, last, sinks) >> (part * 16);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) q[e] = seen_pair(q[e], seen, e);
+            }
+            tmem_st_32x8(t1 + part * 8, q);   // over columns that this warp has read
+            arrive(L::PROBS + part);
+          }
         }
         if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
         tc_fence_after();

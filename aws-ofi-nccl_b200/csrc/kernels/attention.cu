@@ -190,13 +190,17 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     }
   } else if (warp == R::ZERO) {
     // ---------------------------------------------------------------- v behind a sequence's end, in the last tile of a walk
-    uint32_t at = 0, cleared = 0;
-    for (int turn = 0; s.lengths && dealt(turn) < items; ++turn) {
+    uint32_t at = 0, cleared = 0, before = 0;   // before: loads at the last one
+    bool ok = true;
+    for (int turn = 0; s.lengths && ok && dealt(turn) < items; ++turn) {
       const AttnFwdItem w(s, dealt(turn));
       at += 2 * w.n;
       if (w.clear_from == ATT_TILE) continue;
-      if (!cta.wait(L::CLEAR, cleared++ & 1, DEV_ERR_FULL_BAR_TIMEOUT) || !cta.wait(L::FULL + (at - 1) % L::STAGES, (at - 1) / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT)) break;
-      zero_rows<HD, ATT_TILE>(stage(at - 1), w.clear_from, cta.bar(L::CLEARED));
+      const uint32_t last = at - 1;
+      ok = cta.wait(L::CLEAR, cleared++ & 1, DEV_ERR_FULL_BAR_TIMEOUT, at - before) &&
+           cta.wait(L::FULL + last % L::STAGES, last / L::STAGES & 1, DEV_ERR_FULL_BAR_TIMEOUT);
+      if (ok) zero_rows<HD, ATT_TILE>(stage(last), w.clear_from, cta.bar(L::CLEARED));
+      before = at;
     }
   } else {
     // ---------------------------------------------------------------- softmax: a thread has half of a row
@@ -624,17 +628,18 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     }
   } else if (warp == R::ZERO) {
     // ---------------------------------------------------------------- rows behind a sequence's end, in the last tile of each head
-    uint32_t base = 0, cleared = 0;
+    uint32_t base = 0, cleared = 0, before = 0;   // before: tiles at the last one
     bool ok = true;
     for (int turn = 0; s.lengths && ok && dealt(turn) < items; ++turn) {
       const Item w(s, split, dealt(turn));
       if (w.clear_from < ATT_TILE)
         for (int k = w.per_head - 1; k < w.n && ok; k += w.per_head, ++cleared) {
           const uint32_t i = base + k;
-          if (!(ok = cta.wait(L::CLEAR1, cleared & 1, DEV_ERR_FULL_BAR_TIMEOUT) && full1(i))) break;
+          if (!(ok = cta.wait(L::CLEAR1, cleared & 1, DEV_ERR_FULL_BAR_TIMEOUT, i + 1 - before) && full1(i))) break;
           zero_rows<HD, ATT_TILE>(pass1(i), w.clear_from, cta.bar(L::CLEARED1));
-          if (!(ok = cta.wait(L::CLEAR2, cleared & 1, DEV_ERR_FULL_BAR_TIMEOUT) && full2(i))) break;
+          if (!(ok = cta.wait(L::CLEAR2, cleared & 1, DEV_ERR_FULL_BAR_TIMEOUT, 2) && full2(i))) break;
           zero_rows<HD, ATT_TILE>(pass2(i), w.clear_from, cta.bar(L::CLEARED2));
+          before = i;
         }
       base += w.n;
     }

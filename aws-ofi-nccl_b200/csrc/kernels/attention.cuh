@@ -256,7 +256,9 @@ struct AttnCta {
   volatile int* abort_flag;
   int* err_word;
   __device__ __forceinline__ uint32_t bar(int i) const { return bars + 8u * i; }
-  __device__ __forceinline__ bool wait(int i, uint32_t parity, int code) const {
+  // `steps`: of a walk that may pass meanwhile, each of which has the limit that a wait for one has (who waits for a single one of them ends with a stuck CTA
+  // all the same, by the flag)
+  __device__ __forceinline__ bool wait(int i, uint32_t parity, int code, uint32_t steps = 1) const {
     // Polled: a thread that is suspended for a time comes back later, 5 % of the forward pass and of the gradients
     const uint32_t at = bar(i);
     uint64_t t0 = 0;
@@ -276,7 +278,7 @@ struct AttnCta {
         if (*abort_flag) return false;
         const uint64_t t = globaltimer_ns();
         if (!t0) t0 = t;
-        if (t - t0 > GEMM_WAIT_LIMIT_NS) {
+        if (t - t0 > GEMM_WAIT_LIMIT_NS * steps) {
           *abort_flag = 1;
           if (err_word) atomicCAS(err_word, 0, code);
           return false;

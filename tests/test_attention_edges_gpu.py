@@ -238,3 +238,34 @@ def test_trainer_steps_with_a_window():
     before = tr.model.flat_params.clone()
     losses = [tr.step(ids, labels) for _ in range(2)]
     assert all(x == x and x < 20 for x in losses) and tr.model.flat_params.isfinite().all() and not torch.equal(before, tr.model.flat_params)
+
+
+@pytest.mark.gpu
+def test_traced():
+    """The tracer records the operators of the native layers, attention and those that keep 8 bits among them."""
+    from aws_ofi_nccl_b200.ops import gemm, llm
+    from aws_ofi_nccl_b200.ops.attention import attention
+
+    q, k, v, _ = _inputs(1, 130, 2, 1, 64, seed=8)
+    w = torch.randn(256, 128, device="cuda").to(BF)
+
+    def step(q, k, v):
+        o = attention(q, k, v, window=30, sinks=1).reshape(130, 128)
+        return llm.swiglu(gemm.linear(o, w, keep_bits=8), keep_bits=8)
+
+    traced = torch.jit.trace(step, (q, k, v), check_trace=False)
+    other = _inputs(1, 130, 2, 1, 64, seed=9)[:3]
+    assert torch.equal(traced(*other), step(*other))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b, s, nq, nkv, window, sinks", [(1, 1100, 8, 8, 130, 3), (3, 2100, 3, 3, 0, 0), (5, 640, 8, 2, 64, 1), (40, 64, 8, 4, 20, 2), (1, 6000, 5, 1, 700, 40)])
+def test_more_tiles_than_ctas(b, s, nq, nkv, window, sinks):
+    """CTAs that take several tiles, of ragged sequences and of full ones, empty ones among them."""
+    q, k, v, do = _inputs(b, s, nq, nkv, 64, seed=s)
+    _check(q, k, v, do, window=window, sinks=sinks)
+    n = torch.tensor([(s * (3 * i + 1) // (2 * b + 1)) % (s + 1) if i % 4 != 2 else 0 for i in range(b)], dtype=torch.int32, device="cuda")
+    for t in (q, k, v, do):
+        for i, at in enumerate(n.tolist()):
+            t[i, at:] = float("nan")
+    _check(q, k, v, do, window=window, sinks=sinks, lengths=n)

@@ -808,8 +808,9 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           load(c, o);
           if (it.joined) {
             uint4* const at = reinterpret_cast<uint4*>(sums + lane * HD + c);
+            if (it.part == 0 || row0 + lane < s.sinks)   // from far away only sinks are seen
 #pragma unroll
-            for (int e = 0; e < 4; ++e) at[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              for (int e = 0; e < 4; ++e) at[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else if (row0 + lane < s.S) {
             uint4* const at = reinterpret_cast<uint4*>(grad + lane * pitch + c);
             at[0] = make_uint4(two(o, 0), two(o, 1), two(o, 2), two(o, 3));
@@ -839,8 +840,9 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnSplit split, bf
   if (row >= s.S) return;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   const float4* from = reinterpret_cast<const float4*>(split.sums) + at;
-#pragma unroll 4
-  for (int p = 0; p <= split.parts; ++p) {
+  const int parts = row < s.sinks ? split.parts : 0;   // beside the window's, which all rows have
+#pragma unroll 8
+  for (int p = 0; p <= parts; ++p) {
     const float4 x = from[p * tiles * 2 * VECS];
     sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
   }

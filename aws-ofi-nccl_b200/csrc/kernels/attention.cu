@@ -96,7 +96,7 @@ struct AttnFwd {
 template <int HD>
 __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         const __grid_constant__ CUtensorMap tmO, float* minus_lse, AttnShape s, int items, int* err_word) {
+                         const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmR, int with_rest, float* minus_lse, AttnShape s, int items, int* err_word) {
   using L = AttnFwd<HD>;
   using R = AttnFwdRoles;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -333,6 +333,19 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         minus_lse[static_cast<int64_t>(head_of_all) * s.rows + i] = mine ? -top - log2f(sum) : -INFINITY;
       const float f = 1.f / sum;
       const bool any = mine && n && ok;
+      uint32_t rest[HD / 8];   // of this thread's half of a row
+      auto slab_free = [&] {
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+      };
+      auto slab_out = [&](const CUtensorMap* m, int col) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(m, slab, col, head, i0 + (warp & 3) * 32, b);
+          tma_store_commit();
+        }
+      };
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k) {
         uint32_t o[32];
@@ -340,19 +353,27 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           tmem_ld_32x32(o_col + k * 32, o);
           tmem_ld_wait();
         }
-        if (lane == 0) tma_store_wait_read<0>();
-        __syncwarp();
+        slab_free();
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
-          auto two = [&](int at) { return any ? pack_bf16x2(__uint_as_float(o[at]) * f, __uint_as_float(o[at + 1]) * f) : 0u; };
-          st_shared_v4(slab + lane * 64 + ((e / 8 ^ (lane >> 1 & 3)) << 4), two(e), two(e + 2), two(e + 4), two(e + 6));   // 64-byte swizzle
+          uint32_t two[4];
+#pragma unroll
+          for (int q = 0; q < 8; q += 4) {
+            float f4[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) f4[r] = any ? __uint_as_float(o[e + q + r]) * f : 0.f;
+            two[q / 2] = pack_bf16x2(f4[0], f4[1]), two[q / 2 + 1] = pack_bf16x2(f4[2], f4[3]);
+            rest[k * 8 + (e + q) / 4] = rest_of(f4, two[q / 2], two[q / 2 + 1]);
+          }
+          st_shared_v4(slab + lane * 64 + ((e / 8 ^ (lane >> 1 & 3)) << 4), two[0], two[1], two[2], two[3]);   // 64-byte swizzle
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_4d(&tmO, slab, half * (HD / 2) + k * 32, head, i0 + (warp & 3) * 32, b);
-          tma_store_commit();
-        }
+        slab_out(&tmO, half * (HD / 2) + k * 32);
+      }
+      if (with_rest) {
+        slab_free();
+#pragma unroll
+        for (int e = 0; e < HD / 8; e += 4) st_shared_v4(slab + lane * (HD / 2) + e * 4, rest[e], rest[e + 1], rest[e + 2], rest[e + 3]);
+        slab_out(&tmR, half * (HD / 2));
       }
       tc_fence_before();   // the sums are read: by the next handing over of probabilities they may be written
     }
@@ -362,30 +383,34 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
 }
 
 // ------------------------------------------------------------------ backward
-// minus_delta[b][head][i] = -(sum over a row of dout * out), 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes, two rows of a
+// minus_delta[b][head][i] = -(sum over a row of dout * (out + what its rounding left, unless rest is null)), 0 behind a sequence's end. 16-byte vectors of a row in neighbouring lanes, two rows of a
 // thread at once.
 constexpr int DELTA_ROWS = 2;
 template <int HD>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, float* minus_delta,
+__global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, int64_t db, int64_t dt, int64_t dh, const bf16* out, const uint8_t* rest, float* minus_delta,
                                                               AttnShape s, int blocks) {
   constexpr int LANES = HD / 8, STEP = 256 / LANES;
   const int b = blockIdx.x / blocks, v = threadIdx.x % LANES;
   const int64_t first = static_cast<int64_t>(blockIdx.x - b * blocks) * (STEP * DELTA_ROWS);   // over [rows][nq]
   const int token = first < INT_MAX ? s.by_nq.quotient(static_cast<int>(first)) : static_cast<int>(first / s.nq);
-  const int rest = static_cast<int>(first - static_cast<int64_t>(token) * s.nq) + threadIdx.x / LANES;
+  const int beyond = static_cast<int>(first - static_cast<int64_t>(token) * s.nq) + threadIdx.x / LANES;
   grid_wait();
   grid_release();
   const int len = sequence_length(s, b);
   uint4 a[DELTA_ROWS], o[DELTA_ROWS];
+  uint2 more_of[DELTA_ROWS];
   int h[DELTA_ROWS], i[DELTA_ROWS];
 #pragma unroll
   for (int k = 0; k < DELTA_ROWS; ++k) {
-    const int more = s.by_nq.quotient(rest + k * STEP);
-    i[k] = token + more, h[k] = rest + k * STEP - more * s.nq;
+    const int more = s.by_nq.quotient(beyond + k * STEP);
+    i[k] = token + more, h[k] = beyond + k * STEP - more * s.nq;
     a[k] = o[k] = make_uint4(0, 0, 0, 0);
+    more_of[k] = make_uint2(0, 0);
     if (i[k] < len) {
       a[k] = reinterpret_cast<const uint4*>(dout + b * db + i[k] * dt + h[k] * dh)[v];
-      o[k] = reinterpret_cast<const uint4*>(out + ((static_cast<int64_t>(b) * s.S + i[k]) * s.nq + h[k]) * HD)[v];
+      const int64_t at = ((static_cast<int64_t>(b) * s.S + i[k]) * s.nq + h[k]) * HD + v * 8;
+      o[k] = *reinterpret_cast<const uint4*>(out + at);
+      if (rest) more_of[k] = *reinterpret_cast<const uint2*>(rest + at);
     }
   }
 #pragma unroll
@@ -394,8 +419,9 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const bf16* dout, 
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      sum = fmaf(__low2float(x[e]), __low2float(y[e]), sum);
-      sum = fmaf(__high2float(x[e]), __high2float(y[e]), sum);
+      const float2 r = rest_pair((e < 2 ? more_of[k].x : more_of[k].y) >> (16 * (e & 1)));
+      sum = fmaf(__low2float(x[e]), __low2float(y[e]) + r.x, sum);
+      sum = fmaf(__high2float(x[e]), __high2float(y[e]) + r.y, sum);
     }
 #pragma unroll
     for (int d = LANES / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -850,16 +876,19 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnSplit split, bf
   *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
 }
 
-// [B][S][heads][HD] with element strides {batch, token, head}, boxes of 64 rows x 64 elements of a head, or to be stored 32 x 32
-static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd, bool store = false) {
+// [B][S][heads][hd] with element strides {batch, token, head}. Boxes to load: 64 rows x 64 elements of a head; to store: 32 rows x `store` elements of
+// `bytes` bytes, bf16 in the 64-byte swizzle.
+static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd, int store = 0, int bytes = 2) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) return B200_ERR_NO_DRIVER;
-  auto pitch = [&](int size, long long stride) { return static_cast<cuuint64_t>(size == 1 ? hd : stride) * 2; };   // of a single one any will do
+  auto pitch = [&](int size, long long stride) { return static_cast<cuuint64_t>(size == 1 ? hd : stride) * bytes; };   // of a single one any will do
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(B)};
   const cuuint64_t strides[3] = {pitch(heads, t.head), pitch(S, t.token), pitch(B, t.batch)};
-  const cuuint32_t box[4] = {store ? 32u : 64u, 1, store ? 32u : static_cast<cuuint32_t>(ATT_BOX), 1}, one[4] = {1, 1, 1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t box[4] = {store ? static_cast<cuuint32_t>(store) : 64u, 1, store ? 32u : static_cast<cuuint32_t>(ATT_BOX), 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(t.data), dims, strides, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         bytes == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return 0;
   fprintf(stderr, "[b200ops] cuTensorMapEncodeTiled failed: %d (base=%p, %d x %d x %d x %d)\n", static_cast<int>(r), t.data, B, S, heads, hd);
   return B200_ERR_TENSORMAP;
@@ -885,16 +914,21 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
 
 template <int HD>
 static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-  CUtensorMap q, k, v, o;
+  CUtensorMap q, k, v, o, r;
   const long long row = static_cast<long long>(s.nq) * HD;
-  if (int rc = attn_map(&o, {a.out, s.S * row, row, HD}, s.B, s.S, s.nq, HD, true)) return rc;
+  if (int rc = attn_map(&o, {a.out, s.S * row, row, HD}, s.B, s.S, s.nq, HD, 32)) return rc;
+  if (a.rest) {
+    if (int rc = attn_map(&r, {a.rest, s.S * row, row, HD}, s.B, s.S, s.nq, HD, HD / 2, 1)) return rc;
+  } else {
+    r = o;
+  }
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = allow_smem<attention_fwd_kernel<HD>>(AttnFwd<HD>::SMEM)) return rc;
   const int items = s.B * s.nkv * ((s.rows / ATT_TILE * s.G + 1) / 2);
   launch_dependent(attention_fwd_kernel<HD>, std::min(items, sm_count()), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v, o,
-                   a.lse, s, items, device_status_word());
+                   r, a.rest != nullptr, a.lse, s, items, device_status_word());
   B200_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -929,7 +963,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   const int blocks = static_cast<int>((static_cast<int64_t>(s.rows) * s.nq + per_block - 1) / per_block);   // of a sequence
   auto stride = [](int size, long long x) { return size == 1 ? 0 : x; };
   launch_dependent(attention_delta_kernel<HD>, s.B * blocks, 256, 0, stream, static_cast<const bf16*>(a.dout.data),
-                   stride(s.B, a.dout.batch), stride(s.S, a.dout.token), stride(s.nq, a.dout.head), static_cast<const bf16*>(a.out), a.delta, s, blocks);
+                   stride(s.B, a.dout.batch), stride(s.S, a.dout.token), stride(s.nq, a.dout.head), static_cast<const bf16*>(a.out), static_cast<const uint8_t*>(a.rest), a.delta, s, blocks);
   const int tiles = s.rows / ATT_TILE;
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
@@ -962,7 +996,7 @@ int b200_attention_fwd(const B200AttnArgs* args, void* stream) {
   const B200AttnArgs& a = *args;
   AttnShape s;
   if (!attn_shape(s, a) || !attn_tensor_ok(a.q, a.B, a.S, a.nq) || !attn_tensor_ok(a.k, a.B, a.S, a.nkv) || !attn_tensor_ok(a.v, a.B, a.S, a.nkv) || !a.out ||
-      reinterpret_cast<uintptr_t>(a.out) % 16 || !a.lse)
+      reinterpret_cast<uintptr_t>(a.out) % 16 || reinterpret_cast<uintptr_t>(a.rest) % 16 || !a.lse)
     return B200_ERR_BAD_ARG;
   return a.hd == 128 ? attn_fwd<128>(a, s, static_cast<cudaStream_t>(stream)) : attn_fwd<64>(a, s, static_cast<cudaStream_t>(stream));
 }
@@ -980,7 +1014,7 @@ int b200_attention_bwd(const B200AttnArgs* args, int* launches, void* stream) {
   AttnShape s;
   if (!attn_shape(s, a) || !attn_tensor_ok(a.q, a.B, a.S, a.nq) || !attn_tensor_ok(a.k, a.B, a.S, a.nkv) || !attn_tensor_ok(a.v, a.B, a.S, a.nkv) ||
       !attn_tensor_ok(a.dout, a.B, a.S, a.nq) || !a.out || reinterpret_cast<uintptr_t>(a.out) % 16 || !a.lse || reinterpret_cast<uintptr_t>(a.lse) % 16 ||
-      !a.delta || reinterpret_cast<uintptr_t>(a.delta) % 16 || !a.dk != !a.dv || reinterpret_cast<uintptr_t>(a.dq) % 16 ||
+      !a.delta || reinterpret_cast<uintptr_t>(a.delta) % 16 || !a.dk != !a.dv || reinterpret_cast<uintptr_t>(a.rest) % 16 || reinterpret_cast<uintptr_t>(a.dq) % 16 ||
       reinterpret_cast<uintptr_t>(a.dk) % 16 || reinterpret_cast<uintptr_t>(a.dv) % 16)
     return B200_ERR_BAD_ARG;
   const AttnSplit p = attn_split(s, nullptr);

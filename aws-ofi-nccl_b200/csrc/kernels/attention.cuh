@@ -4,6 +4,8 @@
 // Query i sees key j where j <= i, and with a window also i - j < window or j < sinks; a sequence of the batch has length[b] tokens,
 // and rows behind them are zeros, in the output and in the gradients. Since j <= i, a query in front of the length sees no key behind it.
 #pragma once
+#include <cuda_fp8.h>
+
 #include "divisor.h"
 #include "gemm_tcgen05.cuh"
 #include "pair_math.cuh"
@@ -204,6 +206,20 @@ __device__ __forceinline__ uint32_t columns_seen(int first, int last, int sinks)
 // Two packed bf16, those of columns 2 k and 2 k + 1, where they are seen, else zeros
 __device__ __forceinline__ uint32_t seen_pair(uint32_t packed, uint32_t seen, int k) {
   return packed & ((seen >> (2 * k) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * k + 1) & 1 ? 0xFFFF0000u : 0u));
+}
+
+// What the rounding of out to bf16 leaves, as e5m2 of 2^12 times it: delta, a sum over out that the gradients of scores lie beside, is made of both. Of out
+// alone it is off by 2^-9 of its terms, as much as the gradients' own rounding, and dq and dk of a few keys a row by 2^-8.2 in the mean instead of 2^-8.7.
+constexpr float REST_SCALE = 4096.f;
+__device__ __forceinline__ uint32_t rest_of(const float (&f)[4], uint32_t packed01, uint32_t packed23) {
+  const float2 a = make_float2((f[0] - __uint_as_float(packed01 << 16)) * REST_SCALE, (f[1] - __uint_as_float(packed01 & 0xFFFF0000u)) * REST_SCALE);
+  const float2 b = make_float2((f[2] - __uint_as_float(packed23 << 16)) * REST_SCALE, (f[3] - __uint_as_float(packed23 & 0xFFFF0000u)) * REST_SCALE);
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E5M2)) | (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E5M2)) << 16);
+}
+__device__ __forceinline__ float2 rest_pair(uint32_t codes) {   // of the low two bytes
+  const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E5M2);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+  return make_float2(f.x * (1.f / REST_SCALE), f.y * (1.f / REST_SCALE));
 }
 
 // 64 bytes of each of a warp's rows, a lane holding its own row's, to `row_at(r)` + 16 bytes times a lane's number among four (null: left out). Four lanes exchange

@@ -77,7 +77,7 @@ struct B200AttnTensor {
 };
 struct B200AttnArgs {
   B200AttnTensor q, k, v, dout;
-  void* out;
+  void *out, *rest;   // rest: null, or a byte for each element of out, written beside it and read for delta
   float *lse, *delta, *sums;
   void *dq, *dk, *dv;
   const int* lengths;   // [B] or null

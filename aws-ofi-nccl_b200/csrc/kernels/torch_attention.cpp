@@ -37,14 +37,15 @@ B200AttnArgs arguments(const Tensor& q, const Tensor& k, const Tensor& v, const 
 Tensor row_numbers(const Tensor& q) {   // a number for every row of every head, in whole tiles
   return fresh({q.size(0), q.size(2), (q.size(1) + 127) / 128 * 128}, at::kFloat, q);
 }
-// out, and lse where the caller keeps it
-Tensor forward_of(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Window& w, Tensor& lse) {
+// out, and what a backward pass needs of it: lse, and with `rest` what its rounding left
+Tensor forward_of(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Window& w, Tensor& lse, Tensor* rest) {
   const CUDAGuard guard(q.device());
   Tensor out = fresh(q.sizes(), at::kBFloat16, q);
   lse = row_numbers(q);
+  if (rest) *rest = fresh(q.sizes(), at::kByte, q);
   if (q.numel() == 0) return out;
   B200AttnArgs a = arguments(q, k, v, lengths, w);
-  a.out = out.data_ptr(), a.lse = lse.data_ptr<float>();
+  a.out = out.data_ptr(), a.rest = rest ? rest->data_ptr() : nullptr, a.lse = lse.data_ptr<float>();
   launched();
   check(b200_attention_fwd(&a, stream()), "b200_attention_fwd");
   return out;
@@ -54,15 +55,15 @@ struct Attention : public Function<Attention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& lengths, int64_t window,
                         int64_t sinks, double scale) {
     const Tensor qb = boxed(q), kb = boxed(k), vb = boxed(v), n = lengths ? *lengths : Tensor();
-    Tensor lse, out = forward_of(qb, kb, vb, n, {window, sinks, scale}, lse);
-    ctx->save_for_backward({qb, kb, vb, n, out, lse});
+    Tensor lse, rest, out = forward_of(qb, kb, vb, n, {window, sinks, scale}, lse, &rest);
+    ctx->save_for_backward({qb, kb, vb, n, out, lse, rest});
     ctx->saved_data["window"] = window, ctx->saved_data["sinks"] = sinks, ctx->saved_data["scale"] = scale;
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return on_engine_thread([&]() -> variable_list {
       const auto saved = ctx->get_saved_variables();
-      const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lengths = saved[3], &out = saved[4], &lse = saved[5];
+      const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lengths = saved[3], &out = saved[4], &lse = saved[5], &rest = saved[6];
       refuse_tangents({&grads[0], &q, &k, &v}, NO_TANGENTS);
       if (at::GradMode::is_enabled()) raise(PyExc_RuntimeError, "attention has no second derivative");
       const CUDAGuard guard(q.device());
@@ -74,7 +75,7 @@ struct Attention : public Function<Attention> {
         B200AttnArgs a =
             arguments(q, k, v, lengths, {ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble()});
         const Tensor delta = row_numbers(q);
-        a.dout = described(dout), a.out = out.data_ptr(), a.lse = lse.data_ptr<float>(), a.delta = delta.data_ptr<float>();
+        a.dout = described(dout), a.out = out.data_ptr(), a.rest = rest.data_ptr(), a.lse = lse.data_ptr<float>(), a.delta = delta.data_ptr<float>();
         a.dq = dq.defined() ? dq.data_ptr() : nullptr;
         Tensor sums;
         if (dk.defined()) {
@@ -112,7 +113,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::o
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return Attention::apply(q, k, v, lengths, window, sinks, factor);
   Tensor lse;
-  return forward_of(boxed(q), boxed(k), boxed(v), lengths ? *lengths : Tensor(), {window, sinks, factor}, lse);
+  return forward_of(boxed(q), boxed(k), boxed(v), lengths ? *lengths : Tensor(), {window, sinks, factor}, lse, nullptr);
 }
 
 }  // namespace

@@ -18,7 +18,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int 
     itself.  ``lengths`` (int32 [batch], on the device; numbers beyond [0, tokens] count as the nearest of these) says how many tokens each sequence has: rows behind them are
     zeros in the output and in all gradients, whatever they hold.  ``scale`` is head_dim ** -0.5 unless given.
 
-    Scores, probabilities and sums are computed in 32 bits; probabilities and their gradients are rounded to bf16 as operands of the products.
+    Scores, probabilities and sums are computed in 32 bits; probabilities and their gradients are rounded to bf16 as operands of the products.  For a
+    backward pass the inputs, the output, a byte for each of its elements (what rounding it left) and a number for each row are kept.
     Results and gradients are the same bits in every run.  A value in front of a sequence's end that is not finite makes NaN of rows
     that see it, and may of rows in the same 128 that do not.  Tensors may be strided with contiguous heads; where strides or
     addresses are no multiples of 16 bytes they are copied first.  Gradients are of the first order and the reverse mode."""

@@ -20,9 +20,10 @@ namespace b200 {
 using bf16 = __nv_bfloat16;
 
 constexpr int KEPT_THREADS = 256;
-// Vectors of a thread. Two loads ahead where a lane has 16 bytes of one tensor to read: 4096 x 4096 13.8 us to be kept (3.8 TB/s) and 8.5 back, 17.8 and 10.9
-// with one each (before the loads' turn came the search for values that are not finite out of the way: 16.9 with two); SwiGLU of 4096 x 14336 84.6 us (5.6 TB/s) for 106.
-// Where three and more tensors are read one vector is as fast: its gradient 82.6 (5.7 TB/s), 82.3 with two, 87.7 with four.
+// Vectors of a thread, all of whose loads are under way at once. 4096 x 4096 is kept in 13.4 us (3.8 TB/s) and comes back in 8.2, SwiGLU of 4096 x 14336 keeps its
+// halves in 83 (5.7 TB/s; issue slots 85 % busy: 30 instructions an element) and makes its gradient of them in 82 to 85 (5.6). With one vector each the first three took
+// 17.8, 10.9 and 106 us, before the search for values that are not finite came out of the way of the others; with four 16.9, 9.7 and 101. The gradient, which reads
+// three tensors, took 82.2 with one, 82.3 with two and 87.7 with four.
 constexpr int KEEP_VECS = 2, KEPT_VECS = 2, SWIGLU_KEEP_VECS = 2, SWIGLU_KEPT_VECS = 1;
 
 // Rows of `width` elements as vectors: `vecs` for each, of which the last may lie behind the row's end.
@@ -45,11 +46,6 @@ __device__ __forceinline__ KeptPlace kept_place(const KeptRows& s, int k) {
   return p;
 }
 __device__ __forceinline__ uint4 load_once(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
-__device__ __forceinline__ void unpack8(const uint4& q, float (&f)[8]) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) f[2 * k] = __uint_as_float(w[k] << 16), f[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-}
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   uint32_t w[4];
 #pragma unroll
@@ -86,7 +82,9 @@ __global__ void __launch_bounds__(KEPT_THREADS) keep8_kernel(const bf16* x, int6
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     uint32_t power;
-    const uint2 c = keep8(v[i], power);
+    float f[8];
+    unpack8(v[i], f);
+    const uint2 c = keep8(v[i], f, power);
     store_kept(s, p[i], c, power, codes, powers);
   }
 }
@@ -134,16 +132,17 @@ __global__ void __launch_bounds__(KEPT_THREADS) swiglu_keep8_kernel(const bf16* 
   }
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
+    float a[8], b[8];
+    unpack8(g[i], a);
+    unpack8(u[i], b);
     if (p[i].there) {
-      float a[8], b[8];
-      unpack8(g[i], a);
-      unpack8(u[i], b);
+      float o[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] = silu(a[e]) * b[e];
-      *reinterpret_cast<uint4*>(act + p[i].row * s.width + p[i].col) = pack8(a);
+      for (int e = 0; e < 8; e += 2) (Pair(silu(a[e]), silu(a[e + 1])) * Pair(b[e], b[e + 1])).to(o[e], o[e + 1]);
+      *reinterpret_cast<uint4*>(act + p[i].row * s.width + p[i].col) = pack8(o);
     }
     uint32_t g_power, u_power;
-    const uint2 g_codes = keep8(g[i], g_power), u_codes = keep8(u[i], u_power);
+    const uint2 g_codes = keep8(g[i], a, g_power), u_codes = keep8(u[i], b, u_power);
     KeptPlace half = p[i];
     half.row *= 2;
     store_kept(s, half, g_codes, g_power, codes, powers);
@@ -183,11 +182,11 @@ __global__ void __launch_bounds__(KEPT_THREADS)
       float d[8];
       unpack8(d4[i], d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float l = logistic(g[e]), a = g[e] * l;
-        const float dg = d[e] * u[e] * (l + a * (1.f - l));
-        u[e] = d[e] * a;
-        g[e] = dg;
+      for (int e = 0; e < 8; e += 2) {
+        const Pair l(logistic(g[e]), logistic(g[e + 1])), d2(d[e], d[e + 1]), a = Pair(g[e], g[e + 1]) * l;
+        const Pair slope = fma2(a, fma2(l, both(-1.f), both(1.f)), l);
+        (d2 * Pair(u[e], u[e + 1]) * slope).to(g[e], g[e + 1]);
+        (d2 * a).to(u[e], u[e + 1]);
       }
     } else if (act) {
       float a[8];

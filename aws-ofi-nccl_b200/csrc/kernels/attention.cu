@@ -240,10 +240,12 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           }
           const bool some_seen[2] = {WHOLE || __any_sync(0xffffffffu, seen[0]), WHOLE || __any_sync(0xffffffffu, seen[1])};
           auto hide = [&](uint32_t(&x)[32], int k) {
-            if (WHOLE || __all_sync(0xffffffffu, seen[k] == 0xffffffffu)) return;
+            if constexpr (!WHOLE) {
+              if (__all_sync(0xffffffffu, seen[k] == 0xffffffffu)) return;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen[k] >> e & 1)) x[e] = 0xFF800000u;   // -inf
+              for (int e = 0; e < 32; ++e)
+                if (!(seen[k] >> e & 1)) x[e] = 0xFF800000u;   // -inf
+            }
           };
           // Scores are read twice, for their maximum and for the probabilities: all of them with what else is needed are more than a thread has registers
           uint32_t x[32];
@@ -902,14 +904,15 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
   if (static_cast<int64_t>(a.S) > (1 << 30)) return false;
   s.B = a.B, s.S = a.S, s.nq = a.nq, s.nkv = a.nkv, s.G = a.nq / a.nkv;
   s.rows = (a.S + ATT_TILE - 1) / ATT_TILE * ATT_TILE;
+  // items' numbers have 32 bits
+  if (static_cast<int64_t>(s.B) * s.nq >= (1 << 30) || static_cast<int64_t>(s.B) * s.nq * (s.rows / ATT_TILE) >= (1 << 30)) return false;
   // a window that holds every key, or sinks that are, is none
   s.window = a.window >= a.S || (a.window > 0 && a.sinks >= a.S) ? 0 : a.window;
   s.sinks = s.window ? a.sinks : 0;
   s.lengths = a.lengths;
   s.scale = a.scale;
   s.by_G = Divisor(s.G), s.by_nq = Divisor(s.nq), s.by_nkv = Divisor(s.nkv), s.by_heads_q = Divisor(s.B * s.nq), s.by_heads_kv = Divisor(s.B * s.nkv);
-  // a CTA for each tile and head
-  return static_cast<int64_t>(s.B) * s.nq * (s.rows / ATT_TILE) < (1ll << 30);
+  return true;
 }
 
 template <int HD>
@@ -933,17 +936,23 @@ static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   return 0;
 }
 
-// The walk of a sink's tile is split where there is a window: parts as long as a window's walk, but no more CTAs than some waves.
+// The walk of a sink's tile is split where it is more than twice as long as a window's: into parts as long as that, but into no more than make some waves.
+// Where such tiles alone make two waves they are whole items, the first to be dealt.
 static AttnSplit attn_split(const AttnShape& s, float* sums) {
   AttnSplit p{0, 0, 0, Divisor(), sums};
   if (s.sinks == 0) return p;
   const int near = s.window / ATT_TILE + 2, all = s.rows / ATT_TILE;
   if (all <= 2 * near) return p;
   p.tiles = (s.sinks + ATT_TILE - 1) / ATT_TILE;
-  const int64_t most = std::max<int64_t>(1, 4 * 148 / (static_cast<int64_t>(s.B) * s.nkv * p.tiles));
+  const int64_t items = static_cast<int64_t>(s.B) * s.nkv * p.tiles, sms = sm_count();
+  if (items >= 2 * sms) {
+    p.tiles = 0;
+    return p;
+  }
+  const int64_t most = 4 * sms / items;
   p.parts = static_cast<int>(std::min<int64_t>(most, (all - 1) / near));
   p.part_tiles = (all + p.parts - 1) / p.parts;
-  p.by_part = Divisor(s.B * s.nkv * p.tiles);
+  p.by_part = Divisor(static_cast<int>(items));
   return p;
 }
 

@@ -259,7 +259,8 @@ def test_traced():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("b, s, nq, nkv, window, sinks", [(1, 1100, 8, 8, 130, 3), (3, 2100, 3, 3, 0, 0), (5, 640, 8, 2, 64, 1), (40, 64, 8, 4, 20, 2), (1, 6000, 5, 1, 700, 40)])
+@pytest.mark.parametrize("b, s, nq, nkv, window, sinks", [(1, 1100, 8, 8, 130, 3), (3, 2100, 3, 3, 0, 0), (5, 640, 8, 2, 64, 1), (40, 64, 8, 4, 20, 2), (1, 6000, 5, 1, 700, 40), (40, 700, 8, 8, 20, 2),
+                                                           (1, 2000, 1, 1, 1, 1900)])
 def test_more_tiles_than_ctas(b, s, nq, nkv, window, sinks):
     """CTAs that take several tiles, of ragged sequences and of full ones, empty ones among them."""
     q, k, v, do = _inputs(b, s, nq, nkv, 64, seed=s)
@@ -269,3 +270,55 @@ def test_more_tiles_than_ctas(b, s, nq, nkv, window, sinks):
         for i, at in enumerate(n.tolist()):
             t[i, at:] = float("nan")
     _check(q, k, v, do, window=window, sinks=sinks, lengths=n)
+
+
+def test_c_entries_refuse_what_they_cannot_number(built):
+    """Sizes whose products pass 32 bits, null and unaligned pointers, strides off 16 bytes: the code for a bad argument in front of any launch, with addresses
+    that nothing may touch."""
+    import ctypes as C
+
+    from aws_ofi_nccl_b200.ops import _lib
+
+    class Part(C.Structure):
+        _fields_ = [("data", C.c_void_p), ("batch", C.c_longlong), ("token", C.c_longlong), ("head", C.c_longlong)]
+
+    class Args(C.Structure):
+        _fields_ = ([(n, Part) for n in ("q", "k", "v", "dout")] + [(n, C.c_void_p) for n in ("out", "rest", "lse", "delta", "sums", "dq", "dk", "dv", "lengths")] +
+                    [(n, C.c_int) for n in ("B", "S", "nq", "nkv", "hd", "window", "sinks")] + [("scale", C.c_float)])
+
+    lib, bad, at = _lib.load(), 10001, 1 << 20
+
+    def args(**kw):
+        a = Args(B=1, S=16, nq=2, nkv=1, hd=64, scale=0.125)
+        for n in ("q", "k", "v", "dout"):
+            setattr(a, n, Part(at, 16 * 128, 128, 64))
+        for n in ("out", "lse", "delta", "dq", "dk", "dv"):
+            setattr(a, n, at)
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return a
+
+    for kw in (dict(B=1 << 20, nq=1 << 12, nkv=1 << 12), dict(B=1 << 16, nq=1 << 16, nkv=1), dict(B=1 << 15, nq=1 << 15), dict(B=1 << 10, nq=1 << 10, S=1 << 18), dict(S=0),
+               dict(S=(1 << 30) + 1), dict(B=0), dict(nkv=0), dict(nq=0), dict(nq=3, nkv=2), dict(hd=96), dict(window=-1), dict(sinks=-1), dict(scale=0.0),
+               dict(scale=float("nan")), dict(out=None), dict(lse=None), dict(out=at + 2), dict(rest=at + 8), dict(q=Part(None, 2048, 128, 64)),
+               dict(k=Part(at + 8, 2048, 128, 64)), dict(v=Part(at, 2048, 100, 64)), dict(v=Part(at, 2048, 0, 64))):
+        a = args(**kw)
+        assert lib.b200_attention_fwd(C.byref(a), None) == bad, kw
+        assert lib.b200_attention_bwd(C.byref(a), None, None) == bad, kw
+    for kw in (dict(delta=None), dict(dv=None), dict(dq=at + 8), dict(dout=Part(at, 2048, 128, 60))):
+        a = args(**kw)
+        assert lib.b200_attention_bwd(C.byref(a), None, None) == bad, kw
+    vp, ll, i = C.c_void_p, C.c_longlong, C.c_int
+    p, odd = vp(at), vp(at + 2)
+    for rows, width in ((-1, 64), (4, 0), (4, 12), (4, -8), (4, (1 << 29) + 8)):
+        assert lib.b200_keep8(p, ll(width), p, p, ll(rows), i(width), None) == bad
+        for call in (lib.b200_kept8,):
+            assert call(p, p, p, ll(rows), i(width), None) == bad
+        for call in (lib.b200_swiglu_keep8, lib.b200_swiglu_bwd8, lib.b200_swiglu_kept8):
+            assert call(p, p, p, p, ll(rows), i(width), None) == bad
+    assert lib.b200_keep8(None, ll(64), p, p, ll(4), i(64), None) == bad
+    assert lib.b200_keep8(p, ll(60), p, p, ll(4), i(64), None) == bad
+    assert lib.b200_keep8(p, ll(64), odd, p, ll(4), i(64), None) == bad
+    assert lib.b200_kept8(p, None, p, ll(4), i(64), None) == bad
+    assert lib.b200_swiglu_keep8(p, odd, p, p, ll(4), i(64), None) == bad
+    assert lib.b200_swiglu_bwd8(odd, p, p, p, ll(4), i(64), None) == bad

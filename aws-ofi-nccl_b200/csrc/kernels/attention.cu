@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax: a thread has half of a row
-    const int u = warp >> 3, half = warp >> 2 & 1, place = (warp & 3) * 32 + lane, meeting = 1 + u;
+    const int u = warp >> 3, half = warp >> 2 & 1, place = (warp & 3) * 32 + lane;
+    const int meeting = 1 + u * 4 + (warp & 3);   // of the two warps that have the same rows
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_col = lanes + L::S_COL + u * ATT_TILE + half * 64, o_col = lanes + L::O_COL + u * 128 + half * (HD / 2);
     volatile float* const told = reinterpret_cast<volatile float*>(smem_raw + (cta.smem - smem_u32(smem_raw)) + L::TOLD) + u * ATT_TILE + place;
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     const Pair c2 = both(c);
     const uint32_t slab = cta.smem + L::OUT + warp * 2048;
     uint32_t turns = 0, done = 0;   // tiles and units so far
-    bool ok = true;                 // where a wait gives up the walks go on without its scores: all threads of a unit meet as often
+    bool ok = true;                 // where a wait gives up the walks go on without its scores: both warps of some rows meet as often
 #pragma unroll 1
     for (int turn = 0; dealt(turn) < items; ++turn) {
       const AttnFwdItem walk(s, dealt(turn));
@@ -260,14 +261,14 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
             for (int e = 0; e < 32; e += 2) some[e / 2 & 3] = most_of(some[e / 2 & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
           }
           const float most = most_of(most_of(some[0], some[1], some[2]), some[3], some[3]) * c;
-          // The sums are scaled to a new maximum only where one of the unit's rows has grown by more than 2^8: probabilities beside the old one stay in
-          // range. A NaN grows, too, and makes one of everything in its row.
-          if (any_of_256(meeting, !(most <= top + 8.f))) {
+          // The sums are scaled to a new maximum only where one of the two warps' rows has grown by more than 2^8: probabilities beside the old one
+          // stay in range. A NaN grows, too, and makes one of everything in its row.
+          if (any_of_64(meeting, !(most <= top + 8.f))) {
             if (half) *told = most;
-            meet_256(meeting);
+            meet_64(meeting);
             float now = 0.f;
             if (!half) *told = now = most_of(top, most, *told);
-            meet_256(meeting);
+            meet_64(meeting);
             if (half) now = *told;
             const float f = now == -INFINITY ? 1.f : exp2_unit(top - now);
             top = now;
@@ -323,9 +324,9 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
       }
       if (!exists) continue;
       if (half) *told = sum;
-      meet_256(meeting);
+      meet_64(meeting);
       if (!half) *told = sum = sum + *told;
-      meet_256(meeting);
+      meet_64(meeting);
       if (half) sum = *told;
       if (n) ok = cta.wait(L::DONE + u, done++ & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
       tc_fence_after();

@@ -249,14 +249,14 @@ __device__ __forceinline__ void store_rows64(uint32_t (&w)[16], Row row_at) {
     if (uint4* at = row_at((lane & ~3) + k)) at[lane & 3] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
 }
 
-// Whether `mine` is true for any thread of 256 that meet at barrier `id`
-__device__ __forceinline__ bool any_of_256(int id, bool mine) {
+// Whether `mine` is true for any thread of two warps that meet at barrier `id`
+__device__ __forceinline__ bool any_of_64(int id, bool mine) {
   uint32_t r;
   asm volatile(
       "{\n"
       ".reg .pred p, q;\n"
       "setp.ne.u32 p, %2, 0;\n"
-      "barrier.cta.red.or.pred q, %1, 256, p;\n"
+      "barrier.cta.red.or.pred q, %1, 64, p;\n"
       "selp.u32 %0, 1, 0, q;\n"
       "}\n"
       : "=r"(r)
@@ -264,7 +264,7 @@ __device__ __forceinline__ bool any_of_256(int id, bool mine) {
       : "memory");
   return r;
 }
-__device__ __forceinline__ void meet_256(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void meet_64(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // What all roles of a CTA share: barriers and the flag that one of its waits has given up. It has all of tensor memory, from column 0 on.
 struct AttnCta {

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     volatile float* const told = reinterpret_cast<volatile float*>(smem_raw + (cta.smem - smem_u32(smem_raw)) + L::TOLD) + u * ATT_TILE + place;
     const float c = s.scale * ATT_LOG2E;
     const Pair c2 = both(c);
-    const uint32_t slab = cta.smem + L::OUT + warp * 2048;
+    const RowsOut slab{cta.smem + L::OUT + warp * 2048};
     uint32_t turns = 0, done = 0;   // tiles and units so far
     bool ok = true;                 // where a wait gives up the walks go on without its scores: both warps of some rows meet as often
 #pragma unroll 1
@@ -337,18 +337,6 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
       const float f = 1.f / sum;
       const bool any = mine && n && ok;
       uint32_t rest[HD / 8];   // of this thread's half of a row
-      auto slab_free = [&] {
-        if (lane == 0) tma_store_wait_read<0>();
-        __syncwarp();
-      };
-      auto slab_out = [&](const CUtensorMap* m, int col) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_4d(m, slab, col, head, i0 + (warp & 3) * 32, b);
-          tma_store_commit();
-        }
-      };
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k) {
         uint32_t o[32];
@@ -356,27 +344,24 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           tmem_ld_32x32(o_col + k * 32, o);
           tmem_ld_wait();
         }
-        slab_free();
+        uint32_t two[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint32_t two[4];
+        for (int e = 0; e < 32; e += 4) {
+          float f4[4];
 #pragma unroll
-          for (int q = 0; q < 8; q += 4) {
-            float f4[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) f4[r] = any ? __uint_as_float(o[e + q + r]) * f : 0.f;
-            two[q / 2] = pack_bf16x2(f4[0], f4[1]), two[q / 2 + 1] = pack_bf16x2(f4[2], f4[3]);
-            rest[k * 8 + (e + q) / 4] = rest_of(f4, two[q / 2], two[q / 2 + 1]);
-          }
-          st_shared_v4(slab + lane * 64 + ((e / 8 ^ (lane >> 1 & 3)) << 4), two[0], two[1], two[2], two[3]);   // 64-byte swizzle
+          for (int r = 0; r < 4; ++r) f4[r] = any ? __uint_as_float(o[e + r]) * f : 0.f;
+          two[e / 2] = pack_bf16x2(f4[0], f4[1]), two[e / 2 + 1] = pack_bf16x2(f4[2], f4[3]);
+          rest[k * 8 + e / 4] = rest_of(f4, two[e / 2], two[e / 2 + 1]);
         }
-        slab_out(&tmO, half * (HD / 2) + k * 32);
+        slab.free();
+        slab.put(two);
+        slab.out(&tmO, half * (HD / 2) + k * 32, head, i0 + (warp & 3) * 32, b);
       }
       if (with_rest) {
-        slab_free();
+        slab.free();
 #pragma unroll
-        for (int e = 0; e < HD / 8; e += 4) st_shared_v4(slab + lane * (HD / 2) + e * 4, rest[e], rest[e + 1], rest[e + 2], rest[e + 3]);
-        slab_out(&tmR, half * (HD / 2));
+        for (int e = 0; e < HD / 8; e += 4) st_shared_v4(slab.slab + lane * (HD / 2) + e * 4, rest[e], rest[e + 1], rest[e + 2], rest[e + 3]);
+        slab.out(&tmR, half * (HD / 2), head, i0 + (warp & 3) * 32, b);
       }
       tc_fence_before();   // the sums are read: by the next handing over of probabilities they may be written
     }
@@ -444,9 +429,11 @@ using AttnBwdRoles = AttnRoles<16>;
 template <int HD, bool KEYS>
 struct AttnBwd {
   static constexpr int TILE = ATT_TILE * HD * 2;
-  static constexpr int N1 = HD == 64 || !KEYS ? 3 : 2, N2 = 2;   // stages of the passing tensors
+  // stages of the passing tensors. dq's first one is wanted two tiles ahead, its second one is free again as soon as T2 is there
+  static constexpr int N1 = HD == 64 || !KEYS ? 3 : 2, N2 = KEYS ? 2 : 1;
   static constexpr int STATS = 2 * ATT_TILE * 4;                 // lse and delta of a stage's rows
-  static constexpr int PASS1 = 2 * TILE, PASS2 = PASS1 + N1 * TILE, STAT = PASS2 + N2 * TILE;
+  static constexpr int PASS1 = 2 * TILE, PASS2 = PASS1 + N1 * TILE, OUT = PASS2 + N2 * TILE;
+  static constexpr int STAT = OUT + (KEYS ? 0 : 16 * 2048);      // behind each warp's rows on their way out
   static constexpr int TILES = STAT + (KEYS ? N1 * STATS : 0);
   static constexpr int SMEM = 1024 + TILES + ATT_BAR_BYTES;
   static_assert(SMEM <= 232448, "more than a CTA's shared memory");
@@ -525,7 +512,8 @@ struct AttnBwdItem {
 template <int HD, bool KEYS>
 __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         const __grid_constant__ CUtensorMap tmD, const float* minus_lse, const float* minus_delta, bf16* grad1, bf16* grad2, AttnShape s,
+                         const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmG, const float* minus_lse, const float* minus_delta,
+                         bf16* dv, bf16* dk, AttnShape s,
                          AttnSplit split, int items, int* err_word) {
   using L = AttnBwd<HD, KEYS>;
   using R = AttnBwdRoles;
@@ -677,6 +665,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     const int w = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const Pair c = both(s.scale * ATT_LOG2E);
+    const RowsOut slab{cta.smem + L::OUT + warp * 2048};
     const uint8_t* const stat_base = smem_raw + (cta.smem - smem_u32(smem_raw)) + L::STAT + w * 128;
     uint32_t i = 0, done = 0;
     bool ok = true;
@@ -800,15 +789,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
       const int which = KEYS ? w >> 1 : 1, col = (KEYS ? w & 1 : w) * COLS;
       const uint32_t acc = lanes + (which ? L::ACC2_COL : L::ACC1_COL) + col;
       const float f = which ? s.scale : 1.f;
-      const int out_heads = KEYS ? s.nkv : s.nq;
       const int row0 = it.r0 + (warp & 3) * 32;   // the warp's
-      bf16* const grad = (which ? grad2 : grad1) + ((static_cast<int64_t>(it.b) * s.S + row0) * out_heads + it.head) * HD + col;
-      const int64_t pitch = static_cast<int64_t>(out_heads) * HD;
-      float* sums = nullptr;
-      if (it.joined) {
-        const int64_t heads = static_cast<int64_t>(s.B) * s.nkv, place = (it.part * split.tiles + it.tile) * heads + it.b * s.nkv + it.head;
-        sums = split.sums + ((place * 2 + which) * ATT_TILE + (warp & 3) * 32) * HD + col;
-      }
       auto load = [&](int c, uint32_t(&o)[16]) {   // 16 columns, scaled
         if (full) {
           tmem_ld_32x16(acc + c, o);
@@ -818,37 +799,43 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         for (int e = 0; e < 16; ++e) o[e] = full && mine ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
       };
       auto two = [](const uint32_t(&o)[16], int e) { return pack_bf16x2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])); };
-      if constexpr (!KEYS && COLS % 32 == 0) {
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          uint32_t o[16], packed[16];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            load(c + k * 16, o);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) packed[k * 8 + e] = two(o, e);
-          }
-          store_rows64(packed, [&](int at) { return row0 + at < s.S ? reinterpret_cast<uint4*>(grad + at * pitch + c) : nullptr; });
+      if constexpr (KEYS) {
+        // from registers, 6000 clocks of a tile's 110000: through shared memory the walk's loop is left too few registers (226 -> 284 us)
+        bf16* const grad = (which ? dk : dv) + ((static_cast<int64_t>(it.b) * s.S + row0 + lane) * s.nkv + it.head) * HD + col;
+        float* sums = nullptr;
+        if (it.joined) {
+          const int64_t heads = static_cast<int64_t>(s.B) * s.nkv, place = (it.part * split.tiles + it.tile) * heads + it.b * s.nkv + it.head;
+          sums = split.sums + ((place * 2 + which) * ATT_TILE + (warp & 3) * 32 + lane) * HD + col;
         }
-      } else {
 #pragma unroll
         for (int c = 0; c < COLS; c += 16) {
           uint32_t o[16];
           load(c, o);
           if (it.joined) {
-            uint4* const at = reinterpret_cast<uint4*>(sums + lane * HD + c);
             if (it.part == 0 || row0 + lane < s.sinks)   // from far away only sinks are seen
 #pragma unroll
-              for (int e = 0; e < 4; ++e) at[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(sums + c)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else if (row0 + lane < s.S) {
-            uint4* const at = reinterpret_cast<uint4*>(grad + lane * pitch + c);
+            uint4* const at = reinterpret_cast<uint4*>(grad + c);
             at[0] = make_uint4(two(o, 0), two(o, 1), two(o, 2), two(o, 3));
             at[1] = make_uint4(two(o, 4), two(o, 5), two(o, 6), two(o, 7));
           }
         }
+      } else {
+        uint32_t o[16], packed[COLS / 2];
+#pragma unroll
+        for (int c = 0; c < COLS; c += 16) {
+          load(c, o);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) packed[c / 2 + e] = two(o, e);
+        }
+        slab.free();
+        slab.put(packed);
+        slab.out(&tmG, col, it.head, row0, it.b);
       }
       tc_fence_before();   // the sums are read
     }
+    if (!KEYS && lane == 0) tma_store_wait<0>();
   }
   attn_end<R>(cta);
 }
@@ -880,7 +867,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnSplit split, bf
 }
 
 // [B][S][heads][hd] with element strides {batch, token, head}. Boxes to load: 64 rows x 64 elements of a head; to store: 32 rows x `store` elements of
-// `bytes` bytes, bf16 in the 64-byte swizzle.
+// `bytes` bytes, 32 of bf16 in the 64-byte swizzle.
 static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int heads, int hd, int store = 0, int bytes = 2) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) return B200_ERR_NO_DRIVER;
@@ -890,7 +877,7 @@ static int attn_map(CUtensorMap* m, const B200AttnTensor& t, int B, int S, int h
   const cuuint32_t box[4] = {store ? static_cast<cuuint32_t>(store) : 64u, 1, store ? 32u : static_cast<cuuint32_t>(ATT_BOX), 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(t.data), dims, strides, box, one,
                          CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         bytes == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         store * bytes == 64 && bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : store ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return 0;
   fprintf(stderr, "[b200ops] cuTensorMapEncodeTiled failed: %d (base=%p, %d x %d x %d x %d)\n", static_cast<int>(r), t.data, B, S, heads, hd);
@@ -959,7 +946,7 @@ static AttnSplit attn_split(const AttnShape& s, float* sums) {
 
 template <int HD>
 static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-  CUtensorMap q, k, v, d;
+  CUtensorMap q, k, v, d, g;
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
@@ -978,7 +965,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
     const int items = s.B * s.nkv * (tiles + split.tiles * split.parts);
-    launch_dependent(keys, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, a.lse, a.delta,
+    launch_dependent(keys, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, d, a.lse, a.delta,
                      static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, items, err);
     if (split.parts) {
       const int64_t n = static_cast<int64_t>(s.B) * s.nkv * split.tiles * 2 * (ATT_TILE * HD / 4);
@@ -987,9 +974,11 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
     }
   }
   if (a.dq) {
+    const long long row = static_cast<long long>(s.nq) * HD;
+    if (int rc = attn_map(&g, {a.dq, s.S * row, row, HD}, s.B, s.S, s.nq, HD, HD / 4)) return rc;
     const int items = s.B * s.nq * tiles;
-    launch_dependent(queries, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, a.lse, a.delta, static_cast<bf16*>(nullptr),
-                     static_cast<bf16*>(a.dq), s, AttnSplit{0, 0, 0, Divisor(), nullptr}, items, err);
+    launch_dependent(queries, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, g, a.lse, a.delta,
+                     static_cast<bf16*>(nullptr), static_cast<bf16*>(nullptr), s, AttnSplit{0, 0, 0, Divisor(), nullptr}, items, err);
   }
   B200_CUDA_OK(cudaGetLastError());
   return 0;

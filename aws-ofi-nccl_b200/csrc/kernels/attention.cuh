@@ -222,33 +222,6 @@ __device__ __forceinline__ float2 rest_pair(uint32_t codes) {   // of the low tw
   return make_float2(f.x * (1.f / REST_SCALE), f.y * (1.f / REST_SCALE));
 }
 
-// 64 bytes of each of a warp's rows, a lane holding its own row's, to `row_at(r)` + 16 bytes times a lane's number among four (null: left out). Four lanes exchange
-// their vectors first, so that a store covers 64 bytes of eight rows: 16 of each of 32 rows take the memory pipeline four times as long (of dk and dv 6000 clocks a tile).
-template <class Row>
-__device__ __forceinline__ void store_rows64(uint32_t (&w)[16], Row row_at) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int step = 1; step <= 2; ++step) {
-    const bool upper = lane & step;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (k & step) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t &a = w[k * 4 + e], &b = w[(k + step) * 4 + e];
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? a : b, step);
-        if (upper)
-          a = got;
-        else
-          b = got;
-      }
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (uint4* at = row_at((lane & ~3) + k)) at[lane & 3] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-}
-
 // Whether `mine` is true for any thread of two warps that meet at barrier `id`
 __device__ __forceinline__ bool any_of_64(int id, bool mine) {
   uint32_t r;
@@ -265,6 +238,31 @@ __device__ __forceinline__ bool any_of_64(int id, bool mine) {
   return r;
 }
 __device__ __forceinline__ void meet_64(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// A warp's way out: 32 rows of 32 elements (or 16) in shared memory (in the 64-byte swizzle, or plain), from there to the tensor by TMA. From registers 16 bytes of
+// each of 32 rows take the memory pipeline 32 turns a store, of a tile of dk and dv 6000 clocks, and what is spilled waits behind them.
+struct RowsOut {
+  uint32_t slab;
+  __device__ __forceinline__ void free() const {   // of the store before
+    if ((threadIdx.x & 31) == 0) tma_store_wait_read<0>();
+    __syncwarp();
+  }
+  template <int WORDS>   // of this lane's row
+  __device__ __forceinline__ void put(const uint32_t (&w)[WORDS]) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int e = 0; e < WORDS; e += 4)
+      st_shared_v4(slab + lane * WORDS * 4 + ((WORDS == 16 ? e / 4 ^ (lane >> 1 & 3) : e / 4) << 4), w[e], w[e + 1], w[e + 2], w[e + 3]);
+  }
+  __device__ __forceinline__ void out(const CUtensorMap* m, int x, int head, int row, int b) const {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      tma_store_4d(m, slab, x, head, row, b);
+      tma_store_commit();
+    }
+  }
+};
 
 // What all roles of a CTA share: barriers and the flag that one of its waits has given up. It has all of tensor memory, from column 0 on.
 struct AttnCta {

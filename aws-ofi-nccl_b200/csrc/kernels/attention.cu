@@ -687,6 +687,8 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
 #pragma unroll 1
       for (int k = 0; k < n; ++k, ++i) {
         const int c0 = walk.row(at) + w * 32;
+        // blocks far from the window of which no sink is part are zeros without a look at the scores
+        const bool nothing = KEYS ? walk.part > 0 && r0 + (warp & 3) * 32 >= s.sinks : at < walk.far && c0 >= s.sinks;
         if (++at == walk.per_head) at = 0;
         const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
         if constexpr (KEYS) {   // lse and delta of the stage
@@ -694,6 +696,27 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         }
         if (!(ok = cta.wait(KEYS ? L::T1 : L::T1 + (i & 1), KEYS ? i & 1 : i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
         tc_fence_after();
+        auto arrive = [&](int barrier) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(cta.bar(barrier));
+        };
+        if (nothing) {
+          uint32_t zeros[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) zeros[e] = 0;
+          tmem_st_32x16(t1, zeros);
+          if constexpr (KEYS) {
+            arrive(L::PROBS);
+            if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 1));
+            if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+            tc_fence_after();
+            tmem_st_32x16(t2, zeros);
+          }
+          arrive(L::GRADS);
+          continue;
+        }
         // which columns this row's partner sees: those from first to last, and those in front of `sinks`
         bool whole;
         int first, last, sinks = 0;
@@ -715,12 +738,6 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           } else {
             p0 = p1 = both(of ? my_delta : my_lse);
           }
-        };
-        auto arrive = [&](int barrier) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(cta.bar(barrier));
         };
         auto hide = [&](uint32_t(&packed)[16]) {   // also what zero times is not finite
           const uint32_t seen = columns_seen(first, last, sinks);

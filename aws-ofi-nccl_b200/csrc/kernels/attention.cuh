@@ -159,9 +159,6 @@ __device__ __forceinline__ float exp2_unit(float x) {
 }
 
 __device__ __forceinline__ Pair pair_of(uint32_t a, uint32_t b) { return Pair(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ void ld_shared_pairs(uint32_t addr, Pair& a, Pair& b) {
-  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a.bits), "=l"(b.bits) : "r"(addr) : "memory");
-}
 
 // 2^x of both where x <= 120, in float units beside the one for exponentials, which has a quarter of their rate: 2^n p(f) with n the integer nearest to
 // x, f = x - n and p the cubic whose largest relative error on [-1/2, 1/2] is the least (7.5e-5, by Remez' exchange; probabilities are rounded to bf16

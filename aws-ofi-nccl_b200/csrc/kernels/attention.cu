@@ -93,12 +93,13 @@ struct AttnFwd {
   static_assert(SMEM <= 232448, "more than a CTA's shared memory");
 };
 
-template <int HD>
+template <int HD, bool FINE>
 __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmR, int with_rest, float* minus_lse, AttnShape s, int items, int* err_word) {
   using L = AttnFwd<HD>;
   using R = AttnFwdRoles;
+  constexpr int GROUP = FINE ? 32 : 64;   // columns of scores in whose first ones probabilities lie; FINE: behind them what their rounding left
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 8 : 1; });
   grid_wait();
@@ -170,10 +171,13 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
               for (int part = 0; part < 2; ++part) {
                 if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
                 tc_fence_after();
-                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2, part || begun[u]);
-                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 1, true);
-                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 4, true);
-                multiply_step<HD, 64>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 5, true);
+                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2, part || begun[u]);
+                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 1, true);
+                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 4, true);
+                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 5, true);
+                if constexpr (FINE)
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE + 16, v_low, part * 2 + k + (k & 2), true);
               }
               if (!ok) break;
               begun[u] = true;
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           // probabilities of 32 columns come to lie over columns that have been read
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            uint32_t p[16];
+            uint32_t p[16], left[16];
             if (some_seen[k]) {
               tmem_ld_32x32(s_col + k * 32, x);
               tmem_ld_wait();
@@ -302,12 +306,14 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
                 p0 = exp2_unit(p0), p1 = exp2_unit(p1);
                 part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
                 p[e / 2] = pack_bf16x2(p0, p1);
+                if constexpr (FINE) left[e / 2] = left_of(p0, p1, p[e / 2]);
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) p[e] = 0;
+              for (int e = 0; e < 16; ++e) p[e] = left[e] = 0;
             }
-            tmem_st_32x16(s_col + k * 16, p);
+            tmem_st_32x16(s_col + k * (FINE ? 32 : 16), p);
+            if constexpr (FINE) tmem_st_32x16(s_col + k * 32 + 16, left);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -509,7 +515,7 @@ struct AttnBwdItem {
   }
 };
 
-template <int HD, bool KEYS>
+template <int HD, bool KEYS, bool FINE>
 __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmG, const float* minus_lse, const float* minus_delta,
@@ -609,6 +615,9 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           multiply_step<HD, 32>(acc, operand, low, 0, begun);
 #pragma unroll
           for (int k = 1; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand, low, k, true);
+          if constexpr (FINE)
+#pragma unroll
+            for (int k = 0; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand + 16, low, k, true);
           umma_commit(cta.bar(freed));
         };
         t1(0);
@@ -626,6 +635,9 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
               multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL, low, part, part || k > 0);
 #pragma unroll
               for (int step = 2; step < ATT_TILE / 16; step += 2) multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL, low, step + part, true);
+              if constexpr (FINE)
+#pragma unroll
+                for (int step = 0; step < ATT_TILE / 16; step += 2) multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL + 16, low, step + part, true);
             }
             if (!ok) break;
             umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
@@ -702,17 +714,19 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(cta.bar(barrier));
         };
-        if (nothing) {
+        if (nothing) {   // dq: T1 of the next tile comes behind this T2, so that its barrier is found in the phase that others find
           uint32_t zeros[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) zeros[e] = 0;
           tmem_st_32x16(t1, zeros);
+          if constexpr (FINE) tmem_st_32x16(t1 + 16, zeros);
           if constexpr (KEYS) {
             arrive(L::PROBS);
             if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 1));
             if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
             tc_fence_after();
             tmem_st_32x16(t2, zeros);
+            if constexpr (FINE) tmem_st_32x16(t2 + 16, zeros);
           }
           arrive(L::GRADS);
           continue;
@@ -749,7 +763,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
             for (int e = 0; e < 16; ++e) packed[e] &= seen;
           }
         };
-        uint32_t p[32], y[32], o[16];
+        uint32_t p[32], y[32], o[16], left[16];
         tmem_ld_32x32(t1, p);
         tmem_ld_wait();
 #pragma unroll
@@ -768,8 +782,14 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
             uint32_t q[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) q[e] = pack_bf16x2(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]));
+            const uint32_t seen = whole ? 0xffffffffu : columns_seen(first, last, sinks) >> (part * 16);
+            if constexpr (FINE) {
+              uint32_t left[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) left[e] = seen_pair(left_of(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]), q[e]), seen, e);
+              tmem_st_32x8(t1 + 16 + part * 8, left);
+            }
             if (!whole) {
-              const uint32_t seen = columns_seen(first, last, sinks) >> (part * 16);
 #pragma unroll
               for (int e = 0; e < 8; ++e) q[e] = seen_pair(q[e], seen, e);
             }
@@ -788,11 +808,17 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           float a, d;
           (pair_of(p[e], p[e + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
           o[e / 2] = pack_bf16x2(a, d);
+          if constexpr (FINE) left[e / 2] = left_of(a, d, o[e / 2]);
           (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
           o[e / 2 + 1] = pack_bf16x2(a, d);
+          if constexpr (FINE) left[e / 2 + 1] = left_of(a, d, o[e / 2 + 1]);
         }
         if (!whole) hide(o);
         tmem_st_32x16(KEYS ? t2 : t1, o);
+        if constexpr (FINE) {
+          if (!whole) hide(left);
+          tmem_st_32x16((KEYS ? t2 : t1) + 16, left);
+        }
         arrive(L::GRADS);
       }
       // ---------------------------------------------------------------- what the sums became
@@ -920,7 +946,13 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
   return true;
 }
 
-template <int HD>
+// Rows of at most 64 keys (FINE): probabilities and the gradients of scores go into their products as two operands, what they are rounded to and what that
+// left. One rounding of an operand is up to 2^-8; many keys make 2^-9.3 in the mean of it, few do not, and in delta, of the output, it comes once more: over 3 to 8 tokens
+// dq and dk were off by 2.6e-3 to 3.4e-3, from 33 to 64 keys by 2.5e-3, now by 1.7e-3, which is their own rounding. It costs a third: 16384 tokens of 32 heads take
+// 145 instead of 101 us forward, 398 instead of 296 for dk, dv and dq.
+static bool few_keys(const AttnShape& s) { return (s.window ? std::min(s.S, s.window + s.sinks) : s.S) <= 64; }
+
+template <int HD, bool FINE>
 static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
   CUtensorMap q, k, v, o, r;
   const long long row = static_cast<long long>(s.nq) * HD;
@@ -933,9 +965,9 @@ static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
-  if (int rc = allow_smem<attention_fwd_kernel<HD>>(AttnFwd<HD>::SMEM)) return rc;
+  if (int rc = allow_smem<attention_fwd_kernel<HD, FINE>>(AttnFwd<HD>::SMEM)) return rc;
   const int items = s.B * s.nkv * ((s.rows / ATT_TILE * s.G + 1) / 2);
-  launch_dependent(attention_fwd_kernel<HD>, std::min(items, sm_count()), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v, o,
+  launch_dependent(attention_fwd_kernel<HD, FINE>, std::min(items, sm_count()), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v, o,
                    r, a.rest != nullptr, a.lse, s, items, device_status_word());
   B200_CUDA_OK(cudaGetLastError());
   return 0;
@@ -961,17 +993,17 @@ static AttnSplit attn_split(const AttnShape& s, float* sums) {
   return p;
 }
 
-template <int HD>
+template <int HD, bool FINE>
 static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
   CUtensorMap q, k, v, d, g;
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&d, a.dout, s.B, s.S, s.nq, HD)) return rc;
-  auto keys = attention_bwd_kernel<HD, true>;
-  auto queries = attention_bwd_kernel<HD, false>;
-  if (int rc = allow_smem<attention_bwd_kernel<HD, true>>(AttnBwd<HD, true>::SMEM)) return rc;
-  if (int rc = allow_smem<attention_bwd_kernel<HD, false>>(AttnBwd<HD, false>::SMEM)) return rc;
+  auto keys = attention_bwd_kernel<HD, true, FINE>;
+  auto queries = attention_bwd_kernel<HD, false, FINE>;
+  if (int rc = allow_smem<attention_bwd_kernel<HD, true, FINE>>(AttnBwd<HD, true>::SMEM)) return rc;
+  if (int rc = allow_smem<attention_bwd_kernel<HD, false, FINE>>(AttnBwd<HD, false>::SMEM)) return rc;
   int* err = device_status_word();
   const int per_block = 256 / (HD / 8) * DELTA_ROWS;
   const int blocks = static_cast<int>((static_cast<int64_t>(s.rows) * s.nq + per_block - 1) / per_block);   // of a sequence
@@ -1014,7 +1046,8 @@ int b200_attention_fwd(const B200AttnArgs* args, void* stream) {
   if (!attn_shape(s, a) || !attn_tensor_ok(a.q, a.B, a.S, a.nq) || !attn_tensor_ok(a.k, a.B, a.S, a.nkv) || !attn_tensor_ok(a.v, a.B, a.S, a.nkv) || !a.out ||
       reinterpret_cast<uintptr_t>(a.out) % 16 || reinterpret_cast<uintptr_t>(a.rest) % 16 || !a.lse)
     return B200_ERR_BAD_ARG;
-  return a.hd == 128 ? attn_fwd<128>(a, s, static_cast<cudaStream_t>(stream)) : attn_fwd<64>(a, s, static_cast<cudaStream_t>(stream));
+  const auto run = few_keys(s) ? a.hd == 128 ? attn_fwd<128, true> : attn_fwd<64, true> : a.hd == 128 ? attn_fwd<128, false> : attn_fwd<64, false>;
+  return run(a, s, static_cast<cudaStream_t>(stream));
 }
 
 long long b200_attention_bwd_workspace(const B200AttnArgs* args) {
@@ -1036,7 +1069,8 @@ int b200_attention_bwd(const B200AttnArgs* args, int* launches, void* stream) {
   const AttnSplit p = attn_split(s, nullptr);
   if (a.dk && p.parts && (!a.sums || reinterpret_cast<uintptr_t>(a.sums) % 16)) return B200_ERR_BAD_ARG;
   if (launches) *launches = 1 + (a.dk ? 1 + (p.parts > 0) : 0) + (a.dq ? 1 : 0);
-  return a.hd == 128 ? attn_bwd<128>(a, s, static_cast<cudaStream_t>(stream)) : attn_bwd<64>(a, s, static_cast<cudaStream_t>(stream));
+  const auto run = few_keys(s) ? a.hd == 128 ? attn_bwd<128, true> : attn_bwd<64, true> : a.hd == 128 ? attn_bwd<128, false> : attn_bwd<64, false>;
+  return run(a, s, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -219,6 +219,12 @@ __device__ __forceinline__ float2 rest_pair(uint32_t codes) {   // of the low tw
   return make_float2(f.x * (1.f / REST_SCALE), f.y * (1.f / REST_SCALE));
 }
 
+// What the rounding of two numbers to bf16 left, in bf16; nothing of an infinity
+__device__ __forceinline__ uint32_t left_of(float a, float b, uint32_t packed) {
+  const float x = __uint_as_float(packed << 16), y = __uint_as_float(packed & 0xFFFF0000u);
+  return pack_bf16x2(x == a ? 0.f : a - x, y == b ? 0.f : b - y);
+}
+
 // Whether `mine` is true for any thread of two warps that meet at barrier `id`
 __device__ __forceinline__ bool any_of_64(int id, bool mine) {
   uint32_t r;

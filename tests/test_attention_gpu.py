@@ -21,8 +21,8 @@ def _inputs(b, s, nq, nkv, hd, seed=0, std=1.0):
     return make(nq), make(nkv), make(nkv), make(nq)
 
 
-def _expected(q, k, v, do, window, sinks, lengths, scale=None):
-    """name -> (value, bound) in 64 bits; rows behind a sequence's end do not take part."""
+def _expected(q, k, v, do, window, sinks, lengths, scale=None, inner=None):
+    """name -> (value, bound) in 64 bits; rows behind a sequence's end do not take part. inner: what operands and delta are off by instead of u."""
     B, S, nq, hd = q.shape
     nkv, scale = k.shape[2], scale or hd ** -0.5
     i, j = torch.arange(S, device="cuda")[:, None], torch.arange(S, device="cuda")[None]
@@ -40,13 +40,15 @@ def _expected(q, k, v, do, window, sinks, lengths, scale=None):
     p = torch.where(sees, torch.exp(x - x.amax(-1, keepdim=True).clamp_min(-1e300)), 0.0)
     p = p / p.sum(-1, keepdim=True).clamp_min(1e-300)
     out = p @ V
-    err_out = U * (p @ V.abs()) + U * out.abs()
+    w = inner or U
+    err_out = w * (p @ V.abs()) + U * out.abs()
+    err_delta = (D.abs() * (w * (p @ V.abs()) if inner else err_out)).sum(-1, keepdim=True)
     dp = D @ V.transpose(2, 3)
     ds = p * (dp - (D * out).sum(-1, keepdim=True)) * scale
-    err_ds = U * ds.abs() + scale * p * (D.abs() * err_out).sum(-1, keepdim=True)
+    err_ds = w * ds.abs() + scale * p * err_delta
     group = lambda x: x.view(B, nkv, G, S, hd).sum(2)   # noqa: E731
     dv, dk, dq = group(p.transpose(2, 3) @ D), group(ds.transpose(2, 3) @ Q), ds @ K
-    bounds = dict(out=err_out, dv=U * group(p.transpose(2, 3) @ D.abs()) + U * dv.abs(),
+    bounds = dict(out=err_out, dv=w * group(p.transpose(2, 3) @ D.abs()) + U * dv.abs(),
                   dk=group(err_ds.transpose(2, 3) @ Q.abs()) + U * dk.abs(), dq=err_ds @ K.abs() + U * dq.abs())
     return {name: (value.transpose(1, 2), bounds[name].transpose(1, 2) * MORE + TINY) for name, value in dict(out=out, dq=dq, dk=dk, dv=dv).items()}
 
@@ -59,9 +61,9 @@ def _run(q, k, v, do, **kw):
     return dict(zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, do))))
 
 
-def _check(q, k, v, do, window=0, sinks=0, lengths=None, scale=None):
+def _check(q, k, v, do, window=0, sinks=0, lengths=None, scale=None, inner=None):
     got = _run(q, k, v, do, window=window, sinks=sinks, lengths=lengths, scale=scale)
-    for name, (value, bound) in _expected(q, k, v, do, window, sinks, lengths, scale).items():
+    for name, (value, bound) in _expected(q, k, v, do, window, sinks, lengths, scale, inner).items():
         assert got[name].dtype == BF and got[name].shape == value.shape
         off = (got[name].double() - value).abs()
         worst = (off / bound).max().item()
@@ -125,3 +127,14 @@ def test_a_key_that_is_minus_infinity_weighs_nothing():
     # the same probabilities, summed in another order: each side is off by its own rounding and its operands'
     p_v = v.abs().double().amax()
     assert ((out[:, 151:].double() - want[:, 150:].double()).abs() <= 4 * U * p_v).all() and out[:, :150].isfinite().all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("b, s, nq, nkv, window, sinks", [(1, 2, 1, 1, 0, 0), (2, 3, 4, 2, 0, 0), (3, 32, 6, 2, 0, 0), (1, 700, 4, 4, 1, 0), (2, 700, 4, 2, 1, 1),
+                                                          (1, 1000, 2, 1, 20, 12), (4, 300, 3, 3, 2, 30), (40, 130, 8, 8, 3, 0), (2, 64, 2, 1, 0, 0), (1, 600, 4, 2, 33, 31)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_rows_of_few_keys_are_rounded_once(b, s, nq, nkv, window, sinks, hd, ragged):
+    """Up to 64 keys a row, probabilities and gradients of scores are operands of 16 bits of mantissa (2^-17): what is left beside the results' rounding are
+    exponentials by a cubic (2^-13.7) and delta, of the output and five bits of its rest (2^-8 of it, off by at most 2^-3: 2^-11). Together below 2^-10."""
+    lengths = torch.tensor([s - n * s // 3 % s for n in range(b)], dtype=torch.int32, device="cuda") if ragged else None
+    _check(*_inputs(b, s, nq, nkv, hd, seed=s), window=window, sinks=sinks, lengths=lengths, inner=2.0 ** -10)

@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(cta.bar(barrier));
         };
-        if (nothing) {   // dq: T1 of the next tile comes behind this T2, so that its barrier is found in the phase that others find
+        if (nothing) {
           uint32_t zeros[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) zeros[e] = 0;
@@ -723,8 +723,11 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           if constexpr (KEYS) {
             arrive(L::PROBS);
             if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 1));
-            if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
-            tc_fence_after();
+          }
+          // T2 comes behind the tile before, whose gradients all warps have handed over then: dq's T1 may be there before that
+          if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
+          tc_fence_after();
+          if constexpr (KEYS) {
             tmem_st_32x16(t2, zeros);
             if constexpr (FINE) tmem_st_32x16(t2 + 16, zeros);
           }

@@ -322,3 +322,17 @@ def test_c_entries_refuse_what_they_cannot_number(built):
     assert lib.b200_kept8(p, None, p, ll(4), i(64), None) == bad
     assert lib.b200_swiglu_keep8(p, odd, p, p, ll(4), i(64), None) == bad
     assert lib.b200_swiglu_bwd8(odd, p, p, p, ll(4), i(64), None) == bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window, sinks", [(150, 3), (150, 40), (20, 17), (300, 150)])
+def test_what_is_not_finite_stays_in_its_sequence(window, sinks, hd):
+    """CTAs take items of several sequences one after the other: nothing of one whose keys, values or gradients are NaN is left for the next."""
+    q, k, v, do = _inputs(24, 900, 4, 2, hd, seed=3)
+    want = _run(q, k, v, do, window=window, sinks=sinks)
+    for t in (q, k, v, do):
+        t[::3] = float("nan")
+    got = _run(q, k, v, do, window=window, sinks=sinks)
+    for name in want:
+        assert all(torch.equal(got[name][n::3], want[name][n::3]) for n in (1, 2)) and got[name][::3].isnan().all()

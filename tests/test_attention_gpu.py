@@ -138,3 +138,11 @@ def test_rows_of_few_keys_are_rounded_once(b, s, nq, nkv, window, sinks, hd, rag
     exponentials by a cubic (2^-13.7) and delta, of the output and five bits of its rest (2^-8 of it, off by at most 2^-3: 2^-11). Together below 2^-10."""
     lengths = torch.tensor([s - n * s // 3 % s for n in range(b)], dtype=torch.int32, device="cuda") if ragged else None
     _check(*_inputs(b, s, nq, nkv, hd, seed=s), window=window, sinks=sinks, lengths=lengths, inner=2.0 ** -10)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window, sinks", [(40, 150), (300, 161), (130, 290), (10, 400), (500, 130)])
+def test_sinks_of_several_tiles(window, sinks, hd):
+    """Walks with several tiles far from the window, of which some of the last one's columns are sinks."""
+    lengths = torch.tensor([1700, 0, 1031], dtype=torch.int32, device="cuda")
+    _check(*_inputs(3, 1700, 6, 2, hd, seed=window), window=window, sinks=sinks, lengths=lengths)

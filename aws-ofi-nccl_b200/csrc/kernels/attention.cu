@@ -949,11 +949,11 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
   return true;
 }
 
-// Rows of at most 64 keys (FINE): probabilities and the gradients of scores go into their products as two operands, what they are rounded to and what that
+// Rows of at most 128 keys (FINE): probabilities and the gradients of scores go into their products as two operands, what they are rounded to and what that
 // left. One rounding of an operand is up to 2^-8; many keys make 2^-9.3 in the mean of it, few do not, and in delta, of the output, it comes once more: over 3 to 8 tokens
-// dq and dk were off by 2.6e-3 to 3.4e-3, from 33 to 64 keys by 2.5e-3, now by 1.7e-3, which is their own rounding. It costs a third: 16384 tokens of 32 heads take
+// dq and dk were off by 2.6e-3 to 3.4e-3, from 33 to 90 keys by 2.5e-3, now by 1.7e-3, which is their own rounding. It costs a third: 16384 tokens of 32 heads take
 // 145 instead of 101 us forward, 398 instead of 296 for dk, dv and dq.
-static bool few_keys(const AttnShape& s) { return (s.window ? std::min(s.S, s.window + s.sinks) : s.S) <= 64; }
+static bool few_keys(const AttnShape& s) { return (s.window ? std::min(s.S, s.window + s.sinks) : s.S) <= ATT_TILE; }
 
 template <int HD, bool FINE>
 static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {

@@ -131,10 +131,10 @@ def test_a_key_that_is_minus_infinity_weighs_nothing():
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("b, s, nq, nkv, window, sinks", [(1, 2, 1, 1, 0, 0), (2, 3, 4, 2, 0, 0), (3, 32, 6, 2, 0, 0), (1, 700, 4, 4, 1, 0), (2, 700, 4, 2, 1, 1),
-                                                          (1, 1000, 2, 1, 20, 12), (4, 300, 3, 3, 2, 30), (40, 130, 8, 8, 3, 0), (2, 64, 2, 1, 0, 0), (1, 600, 4, 2, 33, 31)])
+                                                          (1, 1000, 2, 1, 20, 12), (4, 300, 3, 3, 2, 30), (40, 130, 8, 8, 3, 0), (2, 64, 2, 1, 0, 0), (1, 600, 4, 2, 33, 31), (2, 128, 3, 1, 0, 0), (1, 900, 4, 4, 100, 28)])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_rows_of_few_keys_are_rounded_once(b, s, nq, nkv, window, sinks, hd, ragged):
-    """Up to 64 keys a row, probabilities and gradients of scores are operands of 16 bits of mantissa (2^-17): what is left beside the results' rounding are
+    """Up to 128 keys a row, probabilities and gradients of scores are operands of 16 bits of mantissa (2^-17): what is left beside the results' rounding are
     exponentials by a cubic (2^-13.7) and delta, of the output and five bits of its rest (2^-8 of it, off by at most 2^-3: 2^-11). Together below 2^-10."""
     lengths = torch.tensor([s - n * s // 3 % s for n in range(b)], dtype=torch.int32, device="cuda") if ragged else None
     _check(*_inputs(b, s, nq, nkv, hd, seed=s), window=window, sinks=sinks, lengths=lengths, inner=2.0 ** -10)

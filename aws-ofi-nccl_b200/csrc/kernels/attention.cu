@@ -96,7 +96,8 @@ struct AttnFwd {
 template <int HD, bool FINE>
 __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmR, int with_rest, float* minus_lse, AttnShape s, int items, int* err_word) {
+                         const __grid_constant__ CUtensorMap tmSinks, const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmR, int with_rest,
+                         float* minus_lse, AttnShape s, int items, int* err_word) {
   using L = AttnFwd<HD>;
   using R = AttnFwdRoles;
   constexpr int GROUP = FINE ? 32 : 64;   // columns of scores in whose first ones probabilities lie; FINE: behind them what their rounding left
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           const int st = loaded % L::STAGES;
           if (!(ok = cta.wait(L::EMPTY + st, (loaded / L::STAGES & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
           mbar_expect_tx(cta.bar(L::FULL + st), L::TILE);
-          load_tile<HD, ATT_TILE>(stage(loaded), i & 1 ? &tmV : &tmK, w.b, w.kv_head, w.tile(i >> 1) * ATT_TILE, cta.bar(L::FULL + st));
+          load_tile<HD, ATT_TILE>(stage(loaded), i & 1 ? i >> 1 < w.far ? &tmSinks : &tmV : &tmK, w.b, w.kv_head, w.tile(i >> 1) * ATT_TILE, cta.bar(L::FULL + st));
         }
       }
       grid_release();
@@ -518,7 +519,8 @@ struct AttnBwdItem {
 template <int HD, bool KEYS, bool FINE>
 __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmG, const float* minus_lse, const float* minus_delta,
+                         const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmSinks, const __grid_constant__ CUtensorMap tmG,
+                         const float* minus_lse, const float* minus_delta,
                          bf16* dv, bf16* dk, AttnShape s,
                          AttnSplit split, int items, int* err_word) {
   using L = AttnBwd<HD, KEYS>;
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           const uint32_t bar1 = cta.bar(L::FULL1 + i % L::N1), bar2 = cta.bar(L::FULL2 + i % L::N2);
           if (!(ok = cta.wait(L::EMPTY1 + i % L::N1, (i / L::N1 & 1) ^ 1, DEV_ERR_EMPTY_BAR_TIMEOUT))) break;
           mbar_expect_tx(bar1, L::TILE + (KEYS ? L::STATS : 0));
-          load_tile<HD, ATT_TILE>(pass1(i), KEYS ? &tmQ : &tmK, w.b, head, row, bar1);
+          load_tile<HD, ATT_TILE>(pass1(i), KEYS ? &tmQ : at < w.far ? &tmSinks : &tmK, w.b, head, row, bar1);
           if constexpr (KEYS) {
             const uint32_t stats = cta.smem + L::STAT + i % L::N1 * L::STATS;
             const int64_t from = (static_cast<int64_t>(w.b) * s.nq + head) * s.rows + row;
@@ -955,9 +957,17 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
 // 145 instead of 101 us forward, 398 instead of 296 for dk, dv and dq.
 static bool few_keys(const AttnShape& s) { return (s.window ? std::min(s.S, s.window + s.sinks) : s.S) <= ATT_TILE; }
 
+// k or v with no tokens but its sinks, of which tiles far from a window are made: what lies behind the sinks would reach every later row where it is not finite, since
+// its products with zero are not zero. TMA fills those rows with zeros. The tensor's own map where no tile is far, or sinks end with a tile.
+static int sinks_map(CUtensorMap* m, const CUtensorMap& all, const B200AttnTensor& t, const AttnShape& s, int hd) {
+  if (s.sinks % ATT_TILE && s.rows - ATT_TILE - s.window + 1 >= ATT_TILE) return attn_map(m, t, s.B, s.sinks, s.nkv, hd);
+  *m = all;
+  return 0;
+}
+
 template <int HD, bool FINE>
 static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-  CUtensorMap q, k, v, o, r;
+  CUtensorMap q, k, v, sinks, o, r;
   const long long row = static_cast<long long>(s.nq) * HD;
   if (int rc = attn_map(&o, {a.out, s.S * row, row, HD}, s.B, s.S, s.nq, HD, 32)) return rc;
   if (a.rest) {
@@ -968,9 +978,10 @@ static int attn_fwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (int rc = attn_map(&q, a.q, s.B, s.S, s.nq, HD)) return rc;
   if (int rc = attn_map(&k, a.k, s.B, s.S, s.nkv, HD)) return rc;
   if (int rc = attn_map(&v, a.v, s.B, s.S, s.nkv, HD)) return rc;
+  if (int rc = sinks_map(&sinks, v, a.v, s, HD)) return rc;
   if (int rc = allow_smem<attention_fwd_kernel<HD, FINE>>(AttnFwd<HD>::SMEM)) return rc;
   const int items = s.B * s.nkv * ((s.rows / ATT_TILE * s.G + 1) / 2);
-  launch_dependent(attention_fwd_kernel<HD, FINE>, std::min(items, sm_count()), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v, o,
+  launch_dependent(attention_fwd_kernel<HD, FINE>, std::min(items, sm_count()), AttnFwdRoles::THREADS, AttnFwd<HD>::SMEM, stream, q, k, v, sinks, o,
                    r, a.rest != nullptr, a.lse, s, items, device_status_word());
   B200_CUDA_OK(cudaGetLastError());
   return 0;
@@ -1017,7 +1028,7 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (a.dk) {
     const AttnSplit split = attn_split(s, a.sums);
     const int items = s.B * s.nkv * (tiles + split.tiles * split.parts);
-    launch_dependent(keys, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, d, a.lse, a.delta,
+    launch_dependent(keys, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, true>::SMEM, stream, q, k, v, d, k, d, a.lse, a.delta,
                      static_cast<bf16*>(a.dv), static_cast<bf16*>(a.dk), s, split, items, err);
     if (split.parts) {
       const int64_t n = static_cast<int64_t>(s.B) * s.nkv * split.tiles * 2 * (ATT_TILE * HD / 4);
@@ -1028,8 +1039,10 @@ static int attn_bwd(const B200AttnArgs& a, const AttnShape& s, cudaStream_t stre
   if (a.dq) {
     const long long row = static_cast<long long>(s.nq) * HD;
     if (int rc = attn_map(&g, {a.dq, s.S * row, row, HD}, s.B, s.S, s.nq, HD, HD / 4)) return rc;
+    CUtensorMap sinks;
+    if (int rc = sinks_map(&sinks, k, a.k, s, HD)) return rc;
     const int items = s.B * s.nq * tiles;
-    launch_dependent(queries, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, g, a.lse, a.delta,
+    launch_dependent(queries, std::min(items, sm_count()), AttnBwdRoles::THREADS, AttnBwd<HD, false>::SMEM, stream, q, k, v, d, sinks, g, a.lse, a.delta,
                      static_cast<bf16*>(nullptr), static_cast<bf16*>(nullptr), s, AttnSplit{0, 0, 0, Divisor(), nullptr}, items, err);
   }
   B200_CUDA_OK(cudaGetLastError());

@@ -32,6 +32,22 @@ __device__ __forceinline__ int anew(int x) {
   return x;
 }
 
+// Rows of at most 128 keys take probabilities and the gradients of scores into their products as two operands, what they are rounded to and what that left (of few keys
+// one rounding of an operand does not average out). These are all rows of a launch with FINE, and the first 128 of every sequence: those that begin in front of row
+// 128, whatever the batch is padded to. With a window and its sinks beyond 128 keys no other row sees so few.
+__device__ __forceinline__ bool few_keys_from(int row) { return row < ATT_TILE; }
+// An operand lies as packed pairs over the first half of each 32 columns of scores that it came from, the second one over the other half.
+constexpr int OP_GROUP = 32, OP_SECOND = 16;
+
+// The products of second operands, those steps of which STEPS has a bit. Called, not part of the loops over tiles: there its instructions, hardly ever run, cost 2 to 5 % of
+// the time.
+template <int HD, uint32_t STEPS>
+__device__ __noinline__ void multiply_second(uint32_t d, uint32_t operand, uint32_t b_low) {
+#pragma unroll
+  for (int k = 0; k < ATT_TILE / 16; ++k)
+    if (STEPS >> k & 1) multiply_step<HD, OP_GROUP>(d, operand + OP_SECOND, b_low, k, true);
+}
+
 // ------------------------------------------------------------------ forward
 // An item are two units of 128 queries of one head each that share a head of k and v: two heads of a group for the same tokens, or where the number
 // of heads in a group is odd also neighbouring tokens. So a tile of k and v is loaded once for 256 rows.
@@ -100,7 +116,6 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
                          float* minus_lse, AttnShape s, int items, int* err_word) {
   using L = AttnFwd<HD>;
   using R = AttnFwdRoles;
-  constexpr int GROUP = FINE ? 32 : 64;   // columns of scores in whose first ones probabilities lie; FINE: behind them what their rounding left
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const AttnCta cta = attn_begin<R, L::TILES, L::BARS>(smem_raw, err_word, [](int i) { return i >= L::PROBS && i < L::DONE ? 8 : 1; });
   grid_wait();
@@ -172,13 +187,18 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
               for (int part = 0; part < 2; ++part) {
                 if (!(ok = ok && cta.wait(L::PROBS + 2 * u + part, turns[u] & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
                 tc_fence_after();
-                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2, part || begun[u]);
-                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 1, true);
-                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 4, true);
-                multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE, v_low, part * 2 + 5, true);
-                if constexpr (FINE)
+                auto step = [&](int operand, int k, bool add) {
+                  multiply_step<HD, OP_GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE + operand, v_low, part * 2 + k + (k & 2), add);
+                };
+                step(0, 0, part || begun[u]);
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) multiply_step<HD, GROUP>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE + 16, v_low, part * 2 + k + (k & 2), true);
+                for (int k = 1; k < 4; ++k) step(0, k, true);
+                if constexpr (FINE) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) step(OP_SECOND, k, true);
+                } else if (few_keys_from(w.unit[u].i0)) {
+                  multiply_second<HD, 0x33>(L::O_COL + u * 128, L::S_COL + u * ATT_TILE + part * OP_GROUP, v_low + part * TileDesc<ATT_TILE, true>::step(2));
+                }
               }
               if (!ok) break;
               begun[u] = true;
@@ -235,8 +255,8 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
         ok = cta.wait(L::SCORES + u, turns & 1, DEV_ERR_TMEM_FULL_TIMEOUT) && ok;
         tc_fence_after();
         const bool whole = j0 + 63 <= i0 && (s.window == 0 || i0 + ATT_TILE - 1 - j0 < s.window || j0 + 64 <= s.sinks);
-        auto take = [&](auto is_whole) {   // a tile on no border without any of what a border takes
-          constexpr bool WHOLE = decltype(is_whole)::value;
+        auto take = [&](auto is_whole, auto in_two) {   // a tile on no border without any of what a border takes
+          constexpr bool WHOLE = decltype(is_whole)::value, TWO = decltype(in_two)::value;
           // what a row sees of each 32 columns; blocks of 32 rows and columns of which none is seen are zeros without their scores being looked at
           uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
           if constexpr (!WHOLE) {
@@ -245,23 +265,23 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
             for (int k = 0; k < 2; ++k) seen[k] = columns_seen(first - k * 32, last - k * 32, sinks - k * 32);
           }
           const bool some_seen[2] = {WHOLE || __any_sync(0xffffffffu, seen[0]), WHOLE || __any_sync(0xffffffffu, seen[1])};
-          auto hide = [&](uint32_t(&x)[32], int k) {
+          auto hide = [&](auto& x, int k, int from) {   // columns `from` on of 32
             if constexpr (!WHOLE) {
               if (__all_sync(0xffffffffu, seen[k] == 0xffffffffu)) return;
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(seen[k] >> e & 1)) x[e] = 0xFF800000u;   // -inf
+              for (int e = 0; e < static_cast<int>(sizeof(x) / 4); ++e)
+                if (!(seen[k] >> (from + e) & 1)) x[e] = 0xFF800000u;   // -inf
             }
           };
           // Scores are read twice, for their maximum and for the probabilities: all of them with what else is needed are more than a thread has registers
-          uint32_t x[32];
           float some[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             if (!some_seen[k]) continue;
+            uint32_t x[32];
             tmem_ld_32x32(s_col + k * 32, x);
             tmem_ld_wait();
-            hide(x, k);
+            hide(x, k, 0);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) some[e / 2 & 3] = most_of(some[e / 2 & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
           }
@@ -295,26 +315,34 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           // probabilities of 32 columns come to lie over columns that have been read
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            uint32_t p[16], left[16];
-            if (some_seen[k]) {
-              tmem_ld_32x32(s_col + k * 32, x);
-              tmem_ld_wait();
-              hide(x, k);
+            constexpr int COLS = TWO ? 16 : 32;   // at a time: with 32 the path of one operand spills what two take
+            uint32_t left[COLS / 2];
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                float p0, p1;
-                fma2(pair_of(x[e], x[e + 1]), c2, ref).to(p0, p1);
-                p0 = exp2_unit(p0), p1 = exp2_unit(p1);
-                part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
-                p[e / 2] = pack_bf16x2(p0, p1);
-                if constexpr (FINE) left[e / 2] = left_of(p0, p1, p[e / 2]);
+            for (int from = 0; from < 32; from += COLS) {
+              uint32_t p[COLS / 2];
+              if (some_seen[k]) {
+                uint32_t x[COLS];
+                tmem_ld_cols(s_col + k * 32 + from, x);
+                tmem_ld_wait();
+                if (TWO && from) tmem_st_cols(s_col + k * OP_GROUP + OP_SECOND, left);   // where scores of these columns were
+                hide(x, k, from);
+#pragma unroll
+                for (int e = 0; e < COLS; e += 2) {
+                  float p0, p1;
+                  fma2(pair_of(x[e], x[e + 1]), c2, ref).to(p0, p1);
+                  p0 = exp2_unit(p0), p1 = exp2_unit(p1);
+                  part[e / 2 & 1] = part[e / 2 & 1] + Pair(p0, p1);
+                  p[e / 2] = pack_bf16x2(p0, p1);
+                  if constexpr (TWO) left[e / 2] = left_of(p0, p1, p[e / 2]);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < COLS / 2; ++e) p[e] = left[e] = 0;
+                if (TWO && from) tmem_st_cols(s_col + k * OP_GROUP + OP_SECOND, left);
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) p[e] = left[e] = 0;
+              tmem_st_cols(s_col + k * OP_GROUP + from / 2, p);
             }
-            tmem_st_32x16(s_col + k * (FINE ? 32 : 16), p);
-            if constexpr (FINE) tmem_st_32x16(s_col + k * 32 + 16, left);
+            if constexpr (TWO) tmem_st_cols(s_col + k * OP_GROUP + OP_SECOND + 8, left);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -324,10 +352,13 @@ __global__ void __launch_bounds__(AttnFwdRoles::THREADS, 1)
           (part[0] + part[1]).to(a, d);
           sum += a + d;
         };
+        using Two = std::bool_constant<FINE>;
         if (whole)
-          take(std::true_type());
+          take(std::true_type(), Two());
+        else if (!FINE && few_keys_from(i0))   // never whole
+          take(std::false_type(), std::true_type());
         else
-          take(std::false_type());
+          take(std::false_type(), Two());
       }
       if (!exists) continue;
       if (half) *told = sum;
@@ -516,6 +547,122 @@ struct AttnBwdItem {
   }
 };
 
+// A warp's values in tensor memory are there for the products behind a barrier.
+__device__ __forceinline__ void hand_over(const AttnCta& cta, int barrier) {
+  tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(cta.bar(barrier));
+}
+// A warp's part of a tile, 32 columns from c0 on of rows from r0 on of which this thread has row r: from scores and dout v^T to the operands of the second products, with
+// TWO both. lse and delta are those of columns (stat) with KEYS, else of the row. False: a wait gave up.
+template <class L, bool KEYS, bool TWO>
+__device__ __forceinline__ bool tile_gradients(const AttnCta& cta, uint32_t i, uint32_t t1, uint32_t t2, int r, int r0, int c0, int window, int all_sinks, Pair c,
+                                               const ulonglong2* stat, float my_lse, float my_delta) {
+  // which columns this row's partner sees: those from first to last, and those in front of `sinks`
+  bool whole;
+  int first, last, sinks = 0;
+  if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
+    whole = c0 >= r0 + ATT_TILE - 1 && (window == 0 || c0 + 31 - r0 < window || r0 + ATT_TILE <= all_sinks);
+    first = r - c0;
+    last = window == 0 || r < all_sinks ? 32 : first + window - 1;
+  } else {                // columns are keys
+    whole = c0 + 31 <= r0 && (window == 0 || r0 + ATT_TILE - 1 - c0 < window || c0 + 32 <= all_sinks);
+    last = r - c0;
+    first = window ? last - window + 1 : 0;
+    sinks = window ? all_sinks - c0 : 0;
+  }
+  auto row_numbers = [&](int of, int e, Pair& p0, Pair& p1) {   // of columns e to e + 3: lse (0), delta (1)
+    if constexpr (KEYS) {
+      const ulonglong2 v = stat[of * (ATT_TILE / 4) + e / 4];
+      p0.bits = v.x, p1.bits = v.y;
+    } else {
+      p0 = p1 = both(of ? my_delta : my_lse);
+    }
+  };
+  auto hide = [&](uint32_t(&packed)[16]) {   // also what zero times is not finite
+    const uint32_t seen = columns_seen(first, last, sinks);
+    if (__any_sync(0xffffffffu, seen + 1 > 1)) {   // neither none nor all of a row
+#pragma unroll
+      for (int e = 0; e < 16; ++e) packed[e] = seen_pair(packed[e], seen, e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) packed[e] &= seen;
+    }
+  };
+  uint32_t p[32];
+  tmem_ld_32x32(t1, p);
+  tmem_ld_wait();
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+#pragma unroll
+    for (int e = part * 16; e < part * 16 + 16; e += 4) {
+      Pair l0, l1;
+      row_numbers(0, e, l0, l1);
+      float a, d;
+      exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
+      p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
+      exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
+      p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
+    }
+    if constexpr (KEYS) {
+      uint32_t q[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = pack_bf16x2(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]));
+      const uint32_t seen = whole ? 0xffffffffu : columns_seen(first, last, sinks) >> (part * 16);
+      if constexpr (TWO) {
+        uint32_t left[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) left[e] = seen_pair(left_of(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]), q[e]), seen, e);
+        tmem_st_32x8(t1 + OP_SECOND + part * 8, left);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = seen_pair(q[e], seen, e);
+      }
+      tmem_st_32x8(t1 + part * 8, q);   // over columns that this warp has read
+      hand_over(cta, L::PROBS + part);
+    }
+  }
+  if (!cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT)) return false;
+  tc_fence_after();
+  uint32_t o[16], left[16];
+  constexpr int COLS = TWO ? 16 : 32;   // at a time, as in the forward pass
+#pragma unroll
+  for (int from = 0; from < 32; from += COLS) {
+    uint32_t y[COLS];
+    tmem_ld_cols(t2 + from, y);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = from; e < from + COLS; e += 4) {
+      Pair d0, d1;
+      row_numbers(1, e, d0, d1);
+      float a, d;
+      (pair_of(p[e], p[e + 1]) * (pair_of(y[e - from], y[e - from + 1]) + d0)).to(a, d);
+      o[e / 2] = pack_bf16x2(a, d);
+      if constexpr (TWO) left[e / 2] = left_of(a, d, o[e / 2]);
+      (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e - from + 2], y[e - from + 3]) + d1)).to(a, d);
+      o[e / 2 + 1] = pack_bf16x2(a, d);
+      if constexpr (TWO) left[e / 2 + 1] = left_of(a, d, o[e / 2 + 1]);
+    }
+  }
+  if (!whole) hide(o);
+  tmem_st_32x16(KEYS ? t2 : t1, o);
+  if constexpr (TWO) {
+    if (!whole) hide(left);
+    tmem_st_32x16((KEYS ? t2 : t1) + OP_SECOND, left);
+  }
+  hand_over(cta, L::GRADS);
+  return true;
+}
+// The same of a sequence's first tile, whose rows see few keys, in a launch with one operand. Called, too: as part of the loop it cost the other tiles 5 to 9 %, as it is 1 %
+// over 16384 tokens with a window of 1024 (dk and dv 543 -> 553 us, dq as before) and 5 % over 4096 without (227 -> 239, where such tiles are in the longest walks).
+template <class L, bool KEYS>
+__device__ __noinline__ bool first_tile_gradients(AttnCta cta, uint32_t i, uint32_t t1, uint32_t t2, int r, int c0, int window, int all_sinks, Pair c, const ulonglong2* stat,
+                                                  float my_lse, float my_delta) {
+  return tile_gradients<L, KEYS, true>(cta, i, t1, t2, r, 0, c0, window, all_sinks, c, stat, my_lse, my_delta);
+}
+
 template <int HD, bool KEYS, bool FINE>
 __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     attention_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -612,21 +759,28 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           if (k + 1 == n) umma_commit(cta.bar(L::HELD_READ));   // the last product with a held tile
         };
         // sum += operand tile; the operand of each group's 32 columns lies over those columns
-        auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, bool begun, int freed) {
+        auto add = [&](uint32_t acc, uint32_t operand, uint32_t tile_at, bool begun, bool two, int freed) {
           const uint32_t low = TileDesc<ATT_TILE, true>::low(tile_at);
-          multiply_step<HD, 32>(acc, operand, low, 0, begun);
+          multiply_step<HD, OP_GROUP>(acc, operand, low, 0, begun);
 #pragma unroll
-          for (int k = 1; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand, low, k, true);
-          if constexpr (FINE)
+          for (int k = 1; k < ATT_TILE / 16; ++k) multiply_step<HD, OP_GROUP>(acc, operand, low, k, true);
+          if constexpr (FINE) {
 #pragma unroll
-            for (int k = 0; k < ATT_TILE / 16; ++k) multiply_step<HD, 32>(acc, operand + 16, low, k, true);
+            for (int k = 0; k < ATT_TILE / 16; ++k) multiply_step<HD, OP_GROUP>(acc, operand + OP_SECOND, low, k, true);
+          } else if (two) {
+            multiply_second<HD, 0xFF>(acc, operand, low);
+          }
           umma_commit(cta.bar(freed));
         };
         t1(0);
         if (ok) t2(0);
         if (!KEYS && ok && n > 1) t1(1);
+        // of a sequence's first tile of queries: with KEYS the one that each head begins with, by what t2 has left of a head then
+        const bool first = !FINE && few_keys_from(w.r0) && w.part == 0;
+        const int left_at_first = !first ? -1 : w.per_head == 1 ? 1 : w.per_head - 1;
         for (int k = 0; k < n && ok; ++k) {
           const uint32_t i = base + k;
+          const bool two = KEYS ? left2 == left_at_first : first;
           if constexpr (KEYS) {
             // in two parts, of 16 columns of every group, as they are there
             const uint32_t low = TileDesc<ATT_TILE, true>::low(pass2(i));
@@ -634,12 +788,15 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
             for (int part = 0; part < 2; ++part) {
               if (!(ok = ok && cta.wait(L::PROBS + part, i & 1, DEV_ERR_TMEM_EMPTY_TIMEOUT))) break;
               tc_fence_after();
-              multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL, low, part, part || k > 0);
+              multiply_step<HD, OP_GROUP>(L::ACC1_COL, L::T1_COL, low, part, part || k > 0);
 #pragma unroll
-              for (int step = 2; step < ATT_TILE / 16; step += 2) multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL, low, step + part, true);
-              if constexpr (FINE)
+              for (int step = 2; step < ATT_TILE / 16; step += 2) multiply_step<HD, OP_GROUP>(L::ACC1_COL, L::T1_COL, low, step + part, true);
+              if constexpr (FINE) {
 #pragma unroll
-                for (int step = 0; step < ATT_TILE / 16; step += 2) multiply_step<HD, 32>(L::ACC1_COL, L::T1_COL + 16, low, step + part, true);
+                for (int step = 0; step < ATT_TILE / 16; step += 2) multiply_step<HD, OP_GROUP>(L::ACC1_COL, L::T1_COL + OP_SECOND, low, step + part, true);
+              } else if (two) {
+                multiply_second<HD, 0x55>(L::ACC1_COL, L::T1_COL + part * 8, low + part * TileDesc<ATT_TILE, true>::step(1));
+              }
             }
             if (!ok) break;
             umma_commit(cta.bar(L::EMPTY2 + i % L::N2));
@@ -649,7 +806,7 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           tc_fence_after();
           if (!KEYS && k + 1 < n) t2(k + 1);
           if (!ok) break;
-          add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), k > 0, L::EMPTY1 + i % L::N1);
+          add(L::ACC2_COL, KEYS ? L::T2_COL : L::T1_COL + (i & 1) * 128, pass1(i), k > 0, two, L::EMPTY1 + i % L::N1);
           if (k + 1 == n) umma_commit(cta.bar(L::DONE));
           if (KEYS && k + 1 < n) t2(k + 1);
           if (!KEYS && k + 2 < n) t1(k + 2);
@@ -697,12 +854,22 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
     for (int turn = 0; ok && dealt(turn) < items; ++turn) {
       const Item walk(s, split, dealt(turn));
       const int r0 = walk.r0, r = r0 + (warp & 3) * 32 + lane, n = walk.n;
-      int at = 0;
+      int at = 0, k = 0;
+      if (!FINE && !KEYS && few_keys_from(r0) && n > 0) {   // its only one
+        const uint32_t t1 = lanes + L::T1_COL + (i & 1) * 128 + w * 32, t2 = lanes + L::T2_COL + w * 32;
+        ok = cta.wait(L::T1 + (i & 1), i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT);
+        if (ok) {
+          tc_fence_after();
+          ok = first_tile_gradients<L, KEYS>(cta, i, t1, t2, r, w * 32, s.window, s.sinks, c, nullptr, my_lse, my_delta);
+        }
+        k = 1, ++i;
+      }
 #pragma unroll 1
-      for (int k = 0; k < n; ++k, ++i) {
+      for (; k < n; ++k, ++i) {
         const int c0 = walk.row(at) + w * 32;
         // blocks far from the window of which no sink is part are zeros without a look at the scores
         const bool nothing = KEYS ? walk.part > 0 && r0 + (warp & 3) * 32 >= s.sinks : at < walk.far && c0 >= s.sinks;
+        const bool first = few_keys_from(KEYS ? c0 - w * 32 : r0);
         if (++at == walk.per_head) at = 0;
         const uint32_t t1 = lanes + L::T1_COL + (KEYS ? 0 : (i & 1) * 128) + w * 32, t2 = lanes + L::T2_COL + w * 32;
         if constexpr (KEYS) {   // lse and delta of the stage
@@ -710,20 +877,14 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
         }
         if (!(ok = cta.wait(KEYS ? L::T1 : L::T1 + (i & 1), KEYS ? i & 1 : i >> 1 & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
         tc_fence_after();
-        auto arrive = [&](int barrier) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(cta.bar(barrier));
-        };
         if (nothing) {
           uint32_t zeros[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) zeros[e] = 0;
           tmem_st_32x16(t1, zeros);
-          if constexpr (FINE) tmem_st_32x16(t1 + 16, zeros);
+          if constexpr (FINE) tmem_st_32x16(t1 + OP_SECOND, zeros);
           if constexpr (KEYS) {
-            arrive(L::PROBS);
+            hand_over(cta, L::PROBS);
             if (lane == 0) mbar_arrive(cta.bar(L::PROBS + 1));
           }
           // T2 comes behind the tile before, whose gradients all warps have handed over then: dq's T1 may be there before that
@@ -731,100 +892,17 @@ __global__ void __launch_bounds__(AttnBwdRoles::THREADS, 1)
           tc_fence_after();
           if constexpr (KEYS) {
             tmem_st_32x16(t2, zeros);
-            if constexpr (FINE) tmem_st_32x16(t2 + 16, zeros);
+            if constexpr (FINE) tmem_st_32x16(t2 + OP_SECOND, zeros);
           }
-          arrive(L::GRADS);
+          hand_over(cta, L::GRADS);
           continue;
         }
-        // which columns this row's partner sees: those from first to last, and those in front of `sinks`
-        bool whole;
-        int first, last, sinks = 0;
-        if constexpr (KEYS) {   // columns are queries: from the key itself on, up to its window's end
-          whole = c0 >= r0 + ATT_TILE - 1 && (s.window == 0 || c0 + 31 - r0 < s.window || r0 + ATT_TILE <= s.sinks);
-          first = r - c0;
-          last = s.window == 0 || r < s.sinks ? 32 : first + s.window - 1;
-        } else {                // columns are keys
-          whole = c0 + 31 <= r0 && (s.window == 0 || r0 + ATT_TILE - 1 - c0 < s.window || c0 + 32 <= s.sinks);
-          last = r - c0;
-          first = s.window ? last - s.window + 1 : 0;
-          sinks = s.window ? s.sinks - c0 : 0;
-        }
         const ulonglong2* const stat = reinterpret_cast<const ulonglong2*>(stat_base + i % L::N1 * L::STATS);
-        auto row_numbers = [&](int of, int e, Pair& p0, Pair& p1) {   // of columns e to e + 3: lse (0), delta (1)
-          if constexpr (KEYS) {
-            const ulonglong2 v = stat[of * (ATT_TILE / 4) + e / 4];
-            p0.bits = v.x, p1.bits = v.y;
-          } else {
-            p0 = p1 = both(of ? my_delta : my_lse);
-          }
-        };
-        auto hide = [&](uint32_t(&packed)[16]) {   // also what zero times is not finite
-          const uint32_t seen = columns_seen(first, last, sinks);
-          if (__any_sync(0xffffffffu, seen + 1 > 1)) {   // neither none nor all of a row
-#pragma unroll
-            for (int e = 0; e < 16; ++e) packed[e] = seen_pair(packed[e], seen, e);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) packed[e] &= seen;
-          }
-        };
-        uint32_t p[32], y[32], o[16], left[16];
-        tmem_ld_32x32(t1, p);
-        tmem_ld_wait();
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-#pragma unroll
-          for (int e = part * 16; e < part * 16 + 16; e += 4) {
-            Pair l0, l1;
-            row_numbers(0, e, l0, l1);
-            float a, d;
-            exp2_pair(e, fma2(pair_of(p[e], p[e + 1]), c, l0), a, d);
-            p[e] = __float_as_uint(a), p[e + 1] = __float_as_uint(d);
-            exp2_pair(e + 2, fma2(pair_of(p[e + 2], p[e + 3]), c, l1), a, d);
-            p[e + 2] = __float_as_uint(a), p[e + 3] = __float_as_uint(d);
-          }
-          if constexpr (KEYS) {
-            uint32_t q[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q[e] = pack_bf16x2(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]));
-            const uint32_t seen = whole ? 0xffffffffu : columns_seen(first, last, sinks) >> (part * 16);
-            if constexpr (FINE) {
-              uint32_t left[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) left[e] = seen_pair(left_of(__uint_as_float(p[part * 16 + 2 * e]), __uint_as_float(p[part * 16 + 2 * e + 1]), q[e]), seen, e);
-              tmem_st_32x8(t1 + 16 + part * 8, left);
-            }
-            if (!whole) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) q[e] = seen_pair(q[e], seen, e);
-            }
-            tmem_st_32x8(t1 + part * 8, q);   // over columns that this warp has read
-            arrive(L::PROBS + part);
-          }
-        }
-        if (!(ok = cta.wait(L::T2, i & 1, DEV_ERR_TMEM_FULL_TIMEOUT))) break;
-        tc_fence_after();
-        tmem_ld_32x32(t2, y);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          Pair d0, d1;
-          row_numbers(1, e, d0, d1);
-          float a, d;
-          (pair_of(p[e], p[e + 1]) * (pair_of(y[e], y[e + 1]) + d0)).to(a, d);
-          o[e / 2] = pack_bf16x2(a, d);
-          if constexpr (FINE) left[e / 2] = left_of(a, d, o[e / 2]);
-          (pair_of(p[e + 2], p[e + 3]) * (pair_of(y[e + 2], y[e + 3]) + d1)).to(a, d);
-          o[e / 2 + 1] = pack_bf16x2(a, d);
-          if constexpr (FINE) left[e / 2 + 1] = left_of(a, d, o[e / 2 + 1]);
-        }
-        if (!whole) hide(o);
-        tmem_st_32x16(KEYS ? t2 : t1, o);
-        if constexpr (FINE) {
-          if (!whole) hide(left);
-          tmem_st_32x16((KEYS ? t2 : t1) + 16, left);
-        }
-        arrive(L::GRADS);
+        if (!FINE && KEYS && first)
+          ok = first_tile_gradients<L, KEYS>(cta, i, t1, t2, r, c0, s.window, s.sinks, c, stat, my_lse, my_delta);
+        else
+          ok = tile_gradients<L, KEYS, FINE>(cta, i, t1, t2, r, r0, c0, s.window, s.sinks, c, stat, my_lse, my_delta);
+        if (!ok) break;
       }
       // ---------------------------------------------------------------- what the sums became
       fetch(turn + 1);   // while the last products run
@@ -951,10 +1029,10 @@ static bool attn_shape(AttnShape& s, const B200AttnArgs& a) {
   return true;
 }
 
-// Rows of at most 128 keys (FINE): probabilities and the gradients of scores go into their products as two operands, what they are rounded to and what that
-// left. One rounding of an operand is up to 2^-8; many keys make 2^-9.3 in the mean of it, few do not, and in delta, of the output, it comes once more: over 3 to 8 tokens
-// dq and dk were off by 2.6e-3 to 3.4e-3, from 33 to 90 keys by 2.5e-3, now by 1.7e-3, which is their own rounding. It costs a third: 16384 tokens of 32 heads take
-// 145 instead of 101 us forward, 398 instead of 296 for dk, dv and dq.
+// Launches all of whose rows see at most 128 keys (FINE) take two operands in every tile; in others the first tile of each sequence does. One rounding of an operand is up
+// to 2^-8; many keys make 2^-9.3 in the mean of it, few do not, and in delta, of the output, it comes once more: over 3 to 8 tokens dq and dk were off by 2.6e-3 to 3.4e-3, from 33
+// to 128 keys by 2.5e-3, now by 1.7e-3, which is their own rounding. Rows of more keys stay at 2.4e-3: with two
+// operands 16384 tokens of 32 heads and a window of 128 take 130 us forward and 396 for dk, dv and dq, with one and a window of 129 97 and 314.
 static bool few_keys(const AttnShape& s) { return (s.window ? std::min(s.S, s.window + s.sinks) : s.S) <= ATT_TILE; }
 
 // k or v with no tokens but its sinks, of which tiles far from a window are made: what lies behind the sinks would reach every later row where it is not finite, since

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_attention_gpu import _inputs, _run
+from test_attention_gpu import _check, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,36 @@ def test_a_value_that_is_not_finite_stays_within_reach(window, sinks, at, hd, nq
                 assert got[n][:, row != at].isfinite().all() and _same(got[n][:, row // 32 != at // 32], want[n][:, row // 32 != at // 32]), (which, n)
         for n in ("dk", "dv"):
             assert _same(got[n][:, beyond & no_sinks], want[n][:, beyond & no_sinks]), (which, n)
+
+
+@pytest.mark.parametrize("hd, nq, nkv", [(64, 4, 2), (128, 3, 1)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (200, 20), (129, 0), (90, 60), (300, 3)])
+def test_a_sequence_is_the_same_alone_and_in_a_padded_batch(window, sinks, hd, nq, nkv):
+    """However far its batch is padded: output and gradients of a short sequence are the same bits."""
+    lengths = (3, 40, 90, 128, 1, 127)
+    ts = _inputs(len(lengths), 128, nq, nkv, hd, seed=window + hd)
+    for s in (128, 129, 700, 1400):
+        padded = [torch.nn.functional.pad(t, (0, 0, 0, 0, 0, s - 128)) for t in ts]
+        got = _run(*padded, window=window, sinks=sinks, lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+        for b, n in enumerate(lengths):
+            alone = _run(*(t[b:b + 1, :n] for t in ts), window=window, sinks=sinks)
+            for name in alone:
+                assert torch.equal(alone[name][0], got[name][b, :n]), (s, n, name)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (200, 20), (120, 30)])
+def test_short_sequences_of_a_long_batch_are_rounded_once(window, sinks, hd):
+    """Every row of at most 128 keys, whatever its batch is padded to: probabilities and gradients of scores have 16 bits of mantissa, and beside the results' own
+    rounding 2^-10 is left (test_rows_of_few_keys_are_rounded_once says of what)."""
+    lengths = torch.tensor([3, 40, 90, 128], dtype=torch.int32, device="cuda")
+    _check(*_inputs(4, 700, 4, 2, hd, seed=window), window=window, sinks=sinks, lengths=lengths, inner=2.0 ** -10)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (300, 20)])
+def test_first_rows_of_a_long_sequence_are_those_of_a_short_one(window, sinks, hd):
+    ts = _inputs(2, 900, 4, 2, hd, seed=11)
+    whole, part = _run(*ts, window=window, sinks=sinks), _run(*(t[:, :128] for t in ts), window=window, sinks=sinks)
+    for name in ("out", "dq"):
+        assert torch.equal(whole[name][:, :128], part[name]), name

@@ -554,7 +554,10 @@ struct RopeQKV : public Function<RopeQKV> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w) { return Linear::apply(x, w); }
-void check_kept_width(const Tensor& x, int64_t width) { require(bf16_cuda(x) && width > 0 && width % 8 == 0, "what is kept in 8 bits are bfloat16 CUDA rows of a multiple of 8 elements"); }
+constexpr int64_t KEPT_MOST = int64_t{1} << 29;   // what the kernels number a row's vectors in; checked in front of any cast
+void check_kept_width(const Tensor& x, int64_t width) {
+  require(bf16_cuda(x) && width > 0 && width % 8 == 0 && width <= KEPT_MOST, "what is kept in 8 bits are bfloat16 CUDA rows of a multiple of 8 elements, of 2^29 at most");
+}
 Tensor linear8(const Tensor& x, const Tensor& w) {
   require(x.dim() >= 1 && w.dim() == 2, "x has a last dimension and the weight is a matrix");
   check_kept_width(x, x.size(-1));
@@ -588,8 +591,9 @@ variable_list keep_rows8(const Tensor& x) {
   return {codes, k.powers.view(shape)};
 }
 Tensor kept_rows8(const Tensor& codes, const Tensor& powers) {
-  require(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() >= 1 && codes.is_contiguous() && codes.size(-1) > 0 && codes.size(-1) % 8 == 0,
-          "codes are contiguous float8_e4m3fn CUDA rows of a multiple of 8 elements");
+  require(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() >= 1 && codes.is_contiguous() && codes.size(-1) > 0 && codes.size(-1) % 8 == 0 &&
+              codes.size(-1) <= KEPT_MOST,
+          "codes are contiguous float8_e4m3fn CUDA rows of a multiple of 8 elements, of 2^29 at most");
   auto shape = codes.sizes().vec();
   shape.back() = (shape.back() + 31) / 32;
   require(same_device(powers, codes) && powers.scalar_type() == at::kByte && powers.is_contiguous() && powers.sizes() == at::IntArrayRef(shape),

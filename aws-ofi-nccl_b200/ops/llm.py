@@ -51,7 +51,7 @@ def keep_rows8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, powers): x (bf16, rows of a multiple of 8 elements) as the layers with ``keep_bits`` 8 keep it, for layers of a program's own. Every 32
     elements of a row (or what is left of it) share a power of two, the least with which their largest is no more than 448: codes are e4m3 of x's shape, powers
     bytes e that stand for 2^(e - 127).  Only the rounding to e4m3 is lost, half a step: 2^-4 of a value, or 2^-10 of the power below 2^-6 of it.
-    What is not finite becomes NaN and counts for no power.  There is no gradient."""
+    What is not finite becomes NaN and counts for no power.  Rows are of at most 2^29 elements.  There is no gradient."""
     return tuple(_lib.native().keep_rows8(x))
 
 

@@ -1,0 +1,27 @@
+"""Training on long sequences beside the operators' values: sizes that layers with 8 bits refuse, and what the model and the trainer make of their options."""
+import pytest
+import torch
+
+BF, F8 = torch.bfloat16, torch.float8_e4m3fn
+
+
+def _refused(fn, *args, error=(AssertionError, RuntimeError, ValueError), **kw):
+    with pytest.raises(error):
+        fn(*args, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [(1 << 29) + 8, (1 << 31) + 64, (1 << 32) + 64])
+def test_rows_that_are_too_long_are_refused(width):
+    """Also those whose number has the low 32 bits of a short row's; no row is there, so that none needs memory."""
+    from aws_ofi_nccl_b200.ops import gemm, llm
+
+    rows = lambda n, t=BF: torch.empty(0, n, device="cuda", dtype=t)   # noqa: E731
+    x = rows(width)
+    _refused(llm.keep_rows8, x)
+    _refused(llm.kept_rows8, rows(width, F8), rows((width + 31) // 32, torch.uint8))
+    for grad in (False, True):
+        _refused(llm.swiglu, rows(2 * width).requires_grad_(grad), keep_bits=8)
+        _refused(gemm.linear, rows(width).requires_grad_(grad), rows(width), keep_bits=8)
+        _refused(llm.swiglu_mlp, rows(width).requires_grad_(grad), rows(width), rows(64), keep_bits=8)
+        _refused(llm.swiglu_mlp, rows(64).requires_grad_(grad), rows(64), rows(width), keep_bits=8)

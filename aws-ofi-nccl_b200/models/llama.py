@@ -37,6 +37,8 @@ class LlamaConfig:
     def __post_init__(self):
         if self.window < 0 or self.sinks < 0 or (self.sinks and not self.window):
             raise ValueError("a window is no negative number, and sinks go with one")
+        if self.window and (self.head_dim not in (64, 128) or self.n_heads % self.n_kv_heads):
+            raise ValueError(f"a window takes heads of 64 or 128 elements, a multiple of those of k and v: not {self.n_heads} of {self.head_dim} on {self.n_kv_heads}")
         if self.keep_bits not in (8, 16):
             raise ValueError(f"activations are kept in 8 or 16 bits, not {self.keep_bits}")
 

@@ -25,3 +25,16 @@ def test_rows_that_are_too_long_are_refused(width):
         _refused(gemm.linear, rows(width).requires_grad_(grad), rows(width), keep_bits=8)
         _refused(llm.swiglu_mlp, rows(width).requires_grad_(grad), rows(width), rows(64), keep_bits=8)
         _refused(llm.swiglu_mlp, rows(64).requires_grad_(grad), rows(64), rows(width), keep_bits=8)
+
+
+def test_a_configuration_with_heads_that_a_window_cannot_have():
+    from aws_ofi_nccl_b200.models.llama import LlamaConfig
+
+    narrow = dict(hidden=256, n_heads=8, n_kv_heads=2)    # heads of 32
+    odd = dict(hidden=448, n_heads=7, n_kv_heads=2)       # seven heads of q on two of k and v
+    for kw in (narrow, odd, dict(hidden=200, n_heads=3, n_kv_heads=1)):
+        LlamaConfig(**kw)
+        _refused(LlamaConfig, **kw, window=64, error=ValueError)
+        _refused(LlamaConfig, **kw, window=64, sinks=2, error=ValueError)
+    for kw in (dict(), dict(hidden=256, n_heads=4, n_kv_heads=2), dict(hidden=384, n_heads=3, n_kv_heads=3)):
+        assert LlamaConfig(**kw, window=64).head_dim in (64, 128)

@@ -76,6 +76,7 @@ class Trainer:
     # ------------------------------------------------------------------ one optimizer step, device tensors in
     def step_device(self, ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         model, oc = self.model, self.optim
+        launched = _lib.launch_count
         model.reset_grad_flags()
         if self.dp is not None:
             self.dp.begin_step()
@@ -98,6 +99,7 @@ class Trainer:
             if hi < model.numel:
                 model.flat_grads[hi:].zero_()
             self.dp.gather_params(model.flat_params)
+        self.kernel_launches = _lib.launch_count - launched
         return loss.detach()
 
     # ------------------------------------------------------------------ end to end: pinned host batch in, float out
@@ -114,17 +116,9 @@ class Trainer:
         return loss
 
     def launches_per_step(self) -> int:
-        """Number of this library's kernels launched by one step (GEMMs + bandwidth kernels)."""
-        L, cfg = self.cfg.n_layers, self.cfg
-        fwd = 1 + L * (2 + 4 + 1 + 1) + 1 + 1 + 1  # embed; per layer 2 norms, 4 GEMMs, rope, swiglu; final norm, lm_head, CE
-        bwd = 1 + L * (2 * 2 + 8 + 1 + 1) + 2 + 2  # embed bwd; per layer norm bwd(2 kernels each), 8 GEMMs, rope, swiglu
-        if cfg.window:   # forward; row sums, gradients of keys and of queries (and where sinks are seen from far away their parts' sums)
-            fwd, bwd = fwd + L, bwd + 3 * L
-        if cfg.keep_bits == 8:   # x of two layers, gate|up there; x twice and gate|up back
-            fwd, bwd = fwd + 3 * L, bwd + 3 * L
-        opt = 1
-        dp = self.dp.launches_per_step() if self.dp is not None else 0
-        return fwd + bwd + opt + dp
+        """Number of this library's kernels that the last step launched (0 in front of the first), by their counter: how many products share a launch, and whether attention
+        joins the sums of sinks, depends on the batch's shape."""
+        return self.kernel_launches
 
     # ------------------------------------------------------------------ checkpoint / resume
     def state_dict(self) -> dict:

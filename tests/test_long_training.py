@@ -38,3 +38,34 @@ def test_a_configuration_with_heads_that_a_window_cannot_have():
         _refused(LlamaConfig, **kw, window=64, sinks=2, error=ValueError)
     for kw in (dict(), dict(hidden=256, n_heads=4, n_kv_heads=2), dict(hidden=384, n_heads=3, n_kv_heads=3)):
         assert LlamaConfig(**kw, window=64).head_dim in (64, 128)
+
+
+def _config(**kw):
+    from aws_ofi_nccl_b200.models.llama import LlamaConfig
+
+    return LlamaConfig(**dict(dict(vocab_size=1024, hidden=256, n_layers=2, n_heads=4, n_kv_heads=2, ffn=512, max_seq=128), **kw))
+
+
+@pytest.mark.gpu
+def test_launches_of_a_step_are_those_that_the_counter_saw():
+    """Per layer beside a model without: three kernels of a window's backward pass and one forward, a fourth where its sinks are seen from far away; three each way
+    of activations in 8 bits."""
+    from aws_ofi_nccl_b200.ops import _lib
+    from aws_ofi_nccl_b200.parallel.engine import Trainer
+
+    def launches(seq, **kw):
+        trainer = Trainer(_config(max_seq=seq, **kw))
+        assert trainer.launches_per_step() == 0
+        for _ in range(2):
+            ids, labels = (torch.randint(0, 1024, (2, seq)).pin_memory() for _ in range(2))
+            before = _lib.launch_count
+            trainer.step(ids, labels)
+            assert trainer.launches_per_step() == _lib.launch_count - before
+        return trainer.launches_per_step()
+
+    plain = launches(128)
+    assert launches(1024) == plain
+    assert launches(128, window=64, sinks=2) == launches(1024, window=64) == plain + 4 * 2
+    assert launches(1024, window=64, sinks=2) == plain + 5 * 2
+    assert launches(128, keep_bits=8) == plain + 6 * 2
+    assert launches(1024, window=64, sinks=2, keep_bits=8) == plain + 11 * 2

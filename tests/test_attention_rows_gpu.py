@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_attention_gpu import _check, _inputs, _run
+from test_attention_gpu import _check, _expected, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,18 @@ def test_first_rows_of_a_long_sequence_are_those_of_a_short_one(window, sinks, h
     whole, part = _run(*ts, window=window, sinks=sinks), _run(*(t[:, :128] for t in ts), window=window, sinks=sinks)
     for name in ("out", "dq"):
         assert torch.equal(whole[name][:, :128], part[name]), name
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("s, window, sinks", [(1100, 0, 0), (1500, 300, 4), (1500, 140, 150), (129, 0, 0)])
+def test_two_roundings_in_the_mean(s, window, sinks, hd):
+    """Rows of many keys: one rounding of an operand (P or dS) and the result's own, in the Frobenius norm.
+
+    Rounding a value m 2^e, 1 <= m < 2, to 8 bits of mantissa is off by at most half a step of 2^(e-7) and, over values whose further bits are even, by its root mean
+    square, 2^(e-7) / sqrt(12): relative to the value at most 2^-7 / sqrt(12) = 2.26e-3. An operand's errors are independent of each other and of what it is multiplied with, whose signs are
+    random here, so a product's relative norm is off by as much as the operand is. Two of them make sqrt(2) 2.26e-3 at most."""
+    ts = _inputs(2, s, 4, 2, hd, seed=s + hd)
+    got = _run(*ts, window=window, sinks=sinks)
+    for name, (want, _) in _expected(*ts, window, sinks, None).items():
+        off = ((got[name].double() - want).norm() / want.norm()).item()
+        assert off <= (2 / 12) ** 0.5 * 2.0 ** -7, (name, off)

@@ -3,8 +3,8 @@
 //   S = scale q k^T over visible keys, P = softmax(S), out = P v
 //   delta = sum(dout * out), dS = P * (dout v^T - delta), dq = scale dS k, dk = scale dS^T q, dv = P^T dout
 //
-// Scores never leave the SM: the forward pass keeps a running maximum and sum of each row, the backward pass computes P again from the
-// rows' log-sum (in base 2), whose negative the forward pass stores.
+// Scores never leave the SM: the forward pass keeps a running maximum and sum of each row (Milakov and Gimelshein, "Online normalizer calculation for
+// softmax", 2018), the backward pass computes P again from the rows' log-sum (in base 2), whose negative the forward pass stores.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -18,11 +18,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int 
     itself.  ``lengths`` (int32 [batch], on the device; numbers beyond [0, tokens] count as the nearest of these) says how many tokens each sequence has: rows behind them are
     zeros in the output and in all gradients, whatever they hold.  ``scale`` is head_dim ** -0.5 unless given.
 
-    Scores, probabilities and sums are computed in 32 bits; probabilities and their gradients are rounded to bf16 as operands of the products, in rows of at most
-    128 keys to two bf16 each (16 bits together).  For a
-    backward pass the inputs, the output, a byte for each of its elements (what rounding it left) and a number for each row are kept.
+    Scores, probabilities and sums are computed in 32 bits, the backward pass' probabilities to 7.5e-5; probabilities and their gradients are rounded to bf16 as
+    operands of the products, in rows of at most 128 keys to two bf16 each (16 bits together).  For a backward pass the inputs, the output, a byte for each of
+    its elements (what rounding it left) and four bytes for each row of a head, in whole 128 rows, are kept.
     Results and gradients are the same bits in every run.  A value in front of a sequence's end that is not finite makes NaN of rows
     that see it.  Products are made of blocks of 128 tokens, in which zero times it is NaN, so it may also of rows up to 512 tokens beyond the window's reach on either
-    side, and a query's value of dk and dv of blocks that hold sinks.  Tensors may be strided with contiguous heads; where strides or
+    side, and in dk and dv of blocks that hold sinks.  Tensors may be strided with contiguous heads; where strides or
     addresses are no multiples of 16 bytes they are copied first.  Gradients are of the first order and the reverse mode."""
     return _lib.native().attention(q, k, v, lengths, window, sinks, scale)
